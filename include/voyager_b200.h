@@ -394,7 +394,8 @@ int vq_linear_mxf8_noalloc_status(int32_t* code, void* stream);
  * on the current device: *code (host) = 0, or the first code any launch
  * recorded since the last clear -- GEMM 1-4, bf16 GEMM 11-14, W4A8 21-23,
  * tensor-parallel barrier
- * 100 + rank, attention 200 + its code.  The per-call error words report to
+ * 100 + rank, attention 200 + its code, key / value cache 301-303 and
+ * 311-314, E4M3 linear 321-324.  The per-call error words report to
  * one caller; this one lets the host ask, after a batch of work, whether any
  * launch gave up.  clear != 0 resets the word.  Synchronises `stream`.  The
  * reference raises on the host and has no device waits; this has no
@@ -671,6 +672,90 @@ int vq_slice_csr(const vq_tensor* data, const int32_t* indices, const int32_t* i
  * integers 0..k-1. */
 int vq_codebook_lookup(const vq_tensor* input, const int64_t* counts, int32_t ncounts,
                        const void* tables, int64_t nregions, vq_tensor* out, void* stream);
+
+/* ---- Decoding against a key / value cache in E4M3 ---------------------------
+ * No counterpart in the reference, whose graphs hold no cache: the operators a
+ * decoder layer runs per step next to the quantized ops above, on E4M3 codes
+ * (bytes, the float8_e4m3fn encoding) with float32 scales per block. */
+
+/* y = rms_norm(x + residual) * weight in float32 (mean of squares over the
+ * row, + eps), quantized per 128 columns: scale = max|y| / 448 (1 where the
+ * maximum is 0), code = E4M3(y / scale), nearest even, saturating.
+ *   x         VQ_BF16 or VQ_F32 [rows, cols], rows ldx elements apart
+ *   residual  the same type, rows ldr apart, or NULL
+ *   weight    the same type [cols], or NULL: no norm, y = x (+ residual)
+ *   codes     [rows, cols] bytes; scale float32 [rows, ceil(cols / 128)]
+ *   hidden    [rows, cols] x + residual in x's type (NULL without residual);
+ *             the norm is that of the unrounded sum
+ * A NaN makes its block's scale and codes NaN. */
+int vq_norm_quantize_fp8(const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                         const void* weight, int32_t dtype, int64_t rows, int64_t cols, float eps,
+                         void* codes, float* scale, void* hidden, void* stream);
+
+/* out[m, n] = bf16(bias[n] + sum_kb x_scale[m, kb] * w_scale[n / 128, kb] *
+ *             sum_{k in kb} x[m, k] w[n, k]), kb the blocks of 128 along K.
+ *   x [M, K], w [N, K] E4M3 bytes, 16-byte aligned, K a multiple of 16
+ *   x_scale float32 [M, nkb], w_scale float32 [ceil(N / 128), nkb], nkb = ceil(K / 128)
+ *   bias bf16 [N] or NULL; out bf16, rows ldo >= N elements apart
+ * Any M and N.  Waits are bounded; one that gives up sets the device's sticky
+ * word (vq_device_errors, 321-324). */
+int vq_linear_fp8_block(const void* x, const float* x_scale, const void* w, const float* w_scale,
+                        const void* bias, int64_t M, int64_t N, int64_t K, void* out, int64_t ldo,
+                        void* stream);
+
+/* Rotary positions of the query and key heads, and the new keys and values
+ * appended to a paged cache.
+ *   q [batch, tokens, heads, head_dim], k and v [batch, tokens, kv_heads,
+ *   head_dim]: VQ_BF16 or VQ_F32; strides: batch, token, head element strides
+ *   of q, k, v (nine), each a multiple of 16 bytes, the last dim dense
+ *   table float32 [positions, rot / 2, 2]: cos and sin of each pair's angle at
+ *   each position; positions >= table_width * page.  rot (a multiple of 16, at
+ *   most head_dim) columns of a head turn, as pairs (i, i + rot / 2) or, when
+ *   interleaved, (2i, 2i + 1); the others stay.
+ *   block_table int32 [batch, table_width]: the cache page of each page of a
+ *   sequence; lengths int32 [batch]: tokens the cache holds before the call;
+ *   counts int32 [batch]: new tokens (NULL: all `tokens`); token t of sequence
+ *   b gets position lengths[b] + t.
+ *   k_codes, v_codes E4M3 [pages, kv_heads, page, head_dim]; k_scale, v_scale
+ *   float32 [pages, kv_heads].  page 32, 64 or 128; head_dim 64 or 128.
+ *   q_out [batch, tokens, heads, head_dim] in q's type; 0 for tokens past counts.
+ * Scales are powers of two, the least with max|value| / scale <= 448 over a
+ * block's tokens, within [2^-100, 2^120]; a block that holds tokens keeps its
+ * scale unless the new ones need a larger one, and its codes are then brought
+ * to it.  A block is fresh when its first slot is written.  No two sequences
+ * of a call may append to the same page.  A plan that does not fit (a count
+ * outside 0..tokens, a negative length, tokens past table_width * page, a page
+ * outside the cache) leaves the tokens concerned out and sets the device's
+ * sticky word (301-303). */
+int vq_rope_append_kv8(const void* q, const void* k, const void* v, const int64_t* strides,
+                       int32_t dtype, const float* table, int64_t positions, int32_t rot,
+                       int32_t interleaved, int64_t batch, int64_t tokens, int32_t heads,
+                       int32_t kv_heads, int32_t head_dim, const void* block_table,
+                       int64_t table_width, const void* lengths, const void* counts, int64_t pages,
+                       int32_t page, void* q_out, void* k_codes, void* v_codes, float* k_scale,
+                       float* v_scale, void* stream);
+
+/* Causal attention of the newest tokens over that cache, which already holds
+ * their keys and values (lengths and counts as vq_rope_append_kv8 got them):
+ *   out[b, t, h] = sum_j softmax_j(sm_scale q . k_j) v_j, j <= lengths[b] + t;
+ * query heads in groups of heads / kv_heads share a kv head; tokens past
+ * counts[b] and rows that see no key get 0.
+ *   q bf16 [batch, tokens, heads, head_dim], q_strides: batch, token, head
+ *   (multiples of 8); out bf16 [batch, tokens, heads, head_dim]
+ *   workspace float32 (16-byte aligned) and counters int32 of the sizes that
+ *   vq_attn_kv8_workspace gives; the counters are 0 before the first call and
+ *   left 0 by each; calls that can overlap on the GPU need their own.
+ * Slots past a sequence's last token may hold anything.  Plans that do not fit
+ * and waits that give up set the device's sticky word (311-314). */
+int vq_attn_kv8_workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_heads,
+                          int32_t head_dim, int32_t page, int64_t table_width, int64_t* floats,
+                          int64_t* counters);
+int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t tokens,
+                int32_t heads, int32_t kv_heads, int32_t head_dim, const void* k_codes,
+                const void* v_codes, const float* k_scale, const float* v_scale, int64_t pages,
+                int32_t page, const void* block_table, int64_t table_width, const void* lengths,
+                const void* counts, float sm_scale, float* workspace, int64_t workspace_floats,
+                int32_t* counters, int64_t counters_len, void* out, void* stream);
 
 /* dst [..., C, R] = src [..., R, C] transposed (2- or 4-byte elements). */
 int vq_transpose(const vq_tensor* src, vq_tensor* dst, void* stream);

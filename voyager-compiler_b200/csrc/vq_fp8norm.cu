@@ -1,0 +1,231 @@
+// RMSNorm (with the residual's addition) and E4M3 quantization with one
+// float32 scale per 128 columns of a row:
+//
+//   h = x + r                          (float32; hidden = h in x's type)
+//   y = h * rsqrt(mean(h^2) + eps) * w (float32; without w: y = h)
+//   s = max|y| / 448 per 128 columns   (1 where the maximum is 0)
+//   code = E4M3(y / s)
+//
+// Everything between the loads and the stores is float32: the norm is that
+// of the unrounded sum, and each output is rounded once.  A NaN in a block
+// makes its scale and codes NaN (maxima are taken on magnitude bits, where
+// NaN sorts above infinity).
+//
+// Bound by HBM: x, r read once, hidden and codes written once (7 bytes per
+// bf16 element with the residual).  A row stays in its threads' registers
+// between the sum of squares and the quantization.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "voyager_b200.h"
+#include "vq_e4m3.cuh"
+
+namespace vq {
+namespace fp8n {
+
+using namespace vq::e4;
+
+struct Args {
+  const void* x;
+  const void* r;  // or null
+  const void* w;  // or null: no norm
+  int64_t ldx, ldr;
+  int64_t rows;
+  int cols, nblk;  // nblk = ceil(cols / 128)
+  float eps;
+  uint8_t* codes;  // [rows, cols]
+  float* scale;    // [rows, nblk]
+  void* hidden;    // [rows, cols], with r only
+};
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(FULL, v, d);
+  return v;
+}
+__device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+// The sum of v over the CTA's threads, in every thread; `part` holds one
+// float per warp.
+__device__ __forceinline__ float block_sum(float v, float* part) {
+  v = warp_sum(v);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = blockDim.x >> 5;
+  if (lane == 0) part[warp] = v;
+  __syncthreads();
+  return warp_sum(lane < n ? part[lane] : 0.0f);
+}
+
+__device__ __forceinline__ float block_scale(uint32_t m) {
+  return m ? __fdiv_rn(__uint_as_float(m), QMAX) : 1.0f;
+}
+
+// One CTA per row, NV groups of 8 consecutive elements per thread; columns a
+// multiple of 8, rows 16-byte aligned.  A block of 128 columns is 16
+// neighbouring lanes.
+template <typename T, int NV>
+__global__ void __launch_bounds__(1024) k_norm_vec(const Args a) {
+  using E = typename T::type;
+  __shared__ float part[32];
+  const int64_t row = blockIdx.x;
+  const E* x = reinterpret_cast<const E*>(a.x) + row * a.ldx;
+  const E* r = reinterpret_cast<const E*>(a.r) + row * a.ldr;
+  const E* w = reinterpret_cast<const E*>(a.w);
+  E* hid = reinterpret_cast<E*>(a.hidden) + row * a.cols;
+  float h[NV][8];
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * blockDim.x + threadIdx.x) * 8;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) h[i][k] = 0.0f;
+    if (c < a.cols) {
+      T::load8(x + c, h[i]);
+      if (a.r) {
+        float q[8];
+        T::load8(r + c, q);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) h[i][k] += q[k];
+        T::store8(hid + c, h[i]);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) ss = fmaf(h[i][k], h[i][k], ss);
+    }
+  }
+  float inv = 1.0f;
+  if (a.w) inv = rsqrtf(__fdiv_rn(block_sum(ss, part), (float)a.cols) + a.eps);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * blockDim.x + threadIdx.x) * 8;
+    if (a.w && c < a.cols) {
+      float g[8];
+      T::load8(w + c, g);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) h[i][k] = h[i][k] * inv * g[k];
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = max(m, mag(h[i][k]));
+#pragma unroll
+    for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(FULL, m, d));
+    if (c < a.cols) {
+      const float s = block_scale(m);
+      float q[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) q[k] = __fdiv_rn(h[i][k], s);
+      *reinterpret_cast<uint2*>(a.codes + row * a.cols + c) =
+          make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+      if ((threadIdx.x & 15) == 0) a.scale[row * a.nblk + (c >> 7)] = s;
+    }
+  }
+}
+
+// Any number of columns and any alignment: one CTA per row, one warp per 128
+// columns, element loads; the row is read again for the quantization.
+template <typename T>
+__global__ void __launch_bounds__(1024) k_norm_any(const Args a) {
+  using E = typename T::type;
+  __shared__ float part[32];
+  const int64_t row = blockIdx.x;
+  const E* x = reinterpret_cast<const E*>(a.x) + row * a.ldx;
+  const E* r = a.r ? reinterpret_cast<const E*>(a.r) + row * a.ldr : nullptr;
+  const E* w = reinterpret_cast<const E*>(a.w);
+  float inv = 1.0f;
+  if (a.w) {
+    float ss = 0.0f;
+    for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
+      const float h = T::load(x + c) + (r ? T::load(r + c) : 0.0f);
+      ss = fmaf(h, h, ss);
+    }
+    inv = rsqrtf(__fdiv_rn(block_sum(ss, part), (float)a.cols) + a.eps);
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+  for (int b = warp; b < a.nblk; b += nw) {
+    float y[4];
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = b * 128 + j * 32 + lane;
+      y[j] = 0.0f;
+      if (c < a.cols) {
+        float h = T::load(x + c);
+        if (r) {
+          h += T::load(r + c);
+          T::store(reinterpret_cast<E*>(a.hidden) + row * a.cols + c, h);
+        }
+        y[j] = a.w ? h * inv * T::load(w + c) : h;
+      }
+      m = max(m, mag(y[j]));
+    }
+    m = __reduce_max_sync(FULL, m);
+    const float s = block_scale(m);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = b * 128 + j * 32 + lane;
+      if (c < a.cols) a.codes[row * a.cols + c] = (uint8_t)pack2(__fdiv_rn(y[j], s), 0.0f);
+    }
+    if (lane == 0) a.scale[row * a.nblk + b] = s;
+  }
+}
+
+template <typename T>
+void launch(const Args& a, bool vec, cudaStream_t st) {
+  const int groups = (a.cols + 7) / 8;
+  if (!vec || groups > 4096) {
+    k_norm_any<T><<<(unsigned)a.rows, std::min(1024, std::max(32, a.nblk * 32)), 0, st>>>(a);
+    return;
+  }
+  int nv = 1;
+  while (groups > nv * 256 && nv < 4) nv *= 2;
+  const int threads = std::min(1024, ((groups + nv - 1) / nv + 31) / 32 * 32);
+  if (nv == 1)
+    k_norm_vec<T, 1><<<(unsigned)a.rows, threads, 0, st>>>(a);
+  else if (nv == 2)
+    k_norm_vec<T, 2><<<(unsigned)a.rows, threads, 0, st>>>(a);
+  else
+    k_norm_vec<T, 4><<<(unsigned)a.rows, threads, 0, st>>>(a);
+}
+
+}  // namespace fp8n
+}  // namespace vq
+
+using namespace vq::fp8n;
+
+extern "C" int vq_norm_quantize_fp8(const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                                    const void* weight, int32_t dtype, int64_t rows, int64_t cols,
+                                    float eps, void* codes, float* scale, void* hidden,
+                                    void* stream) {
+  if (rows < 0 || cols <= 0 || cols > (1 << 24) || rows >= (1ll << 31)) return VQ_ERR_INVALID;
+  if (dtype != VQ_BF16 && dtype != VQ_F32) return VQ_ERR_UNSUPPORTED;
+  if (rows == 0) return VQ_OK;
+  if (!x || !codes || !scale || (residual && !hidden)) return VQ_ERR_NULL;
+  if (ldx < cols || (residual && ldr < cols)) return VQ_ERR_SHAPE;
+  const int eb = dtype == VQ_BF16 ? 2 : 4;
+  auto aligned = [](const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; };
+  if (!aligned(x, eb) || !aligned(residual, eb) || !aligned(weight, eb) || !aligned(hidden, eb) ||
+      !aligned(scale, 4))
+    return VQ_ERR_ALIGNMENT;
+  Args a;
+  a.x = x;
+  a.r = residual;
+  a.w = weight;
+  a.ldx = ldx;
+  a.ldr = residual ? ldr : 0;
+  a.rows = rows;
+  a.cols = (int)cols;
+  a.nblk = (int)((cols + 127) / 128);
+  a.eps = eps;
+  a.codes = reinterpret_cast<uint8_t*>(codes);
+  a.scale = scale;
+  a.hidden = residual ? hidden : nullptr;
+  const bool vec = cols % 8 == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(weight, 16) &&
+                   aligned(a.hidden, 16) && aligned(codes, 8) && ldx * eb % 16 == 0 &&
+                   a.ldr * eb % 16 == 0;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == VQ_BF16)
+    launch<BF16>(a, vec, st);
+  else
+    launch<F32>(a, vec, st);
+  return cudaGetLastError() == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
+}

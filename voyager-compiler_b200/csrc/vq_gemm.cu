@@ -1087,6 +1087,20 @@ bool make_map_plain(CUtensorMap* m, const void* base, uint64_t rows, uint64_t co
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_map_box(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols_bytes,
+                  uint32_t box_cols, uint32_t box_rows, uint32_t swizzle) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[2] = {cols_bytes, rows};
+  cuuint64_t strides[1] = {cols_bytes};
+  cuuint32_t box[2] = {box_cols, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE,
+            swizzle == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int sm_count() {
   int dev = 0, n = 148;
   cudaGetDevice(&dev);
@@ -1240,6 +1254,15 @@ int sticky_dq(int* out, int clear, cudaStream_t st);
 }
 namespace w4 {
 int sticky_w4(int* out, int clear, cudaStream_t st);
+}
+namespace kv {
+int sticky_kv(int* out, int clear, cudaStream_t st);
+}
+namespace kva {
+int sticky_kva(int* out, int clear, cudaStream_t st);
+}
+namespace f8 {
+int sticky_f8(int* out, int clear, cudaStream_t st);
 }
 }  // namespace vq
 
@@ -1519,14 +1542,18 @@ int vq_linear_mxf8_noalloc_status(int32_t* code, void* stream) {
 int vq_device_errors(int32_t* code, int32_t clear, void* stream) {
   if (!code) return VQ_ERR_NULL;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  int v[5] = {0, 0, 0, 0, 0};
+  int v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (vq::tc::sticky_read(&v[0], clear, s) || vq::dq::sticky_dq(&v[1], clear, s) ||
       vq::tp::sticky_tp(&v[2], clear, s) || vq::attn::sticky_attn(&v[3], clear, s) ||
-      vq::w4::sticky_w4(&v[4], clear, s))
+      vq::w4::sticky_w4(&v[4], clear, s) || vq::kv::sticky_kv(&v[5], clear, s) ||
+      vq::kva::sticky_kva(&v[6], clear, s) || vq::f8::sticky_f8(&v[7], clear, s))
     return VQ_ERR_CUDA;
   // the first nonzero word: MXFP8 GEMM 1-4, bf16 GEMM 11-14, W4A8 21-23,
-  // tensor-parallel barrier 100 + rank, attention 200 + its code
+  // tensor-parallel barrier 100 + rank, attention 200 + its code, key / value
+  // cache 301-303 and 311-314, E4M3 linear 321-324
   *code = v[0] ? v[0] : (v[1] ? v[1] : (v[4] ? v[4] : (v[2] ? v[2] : (v[3] ? 200 + v[3] : 0))));
+  for (int i = 5; i < 8; ++i)
+    if (!*code) *code = v[i];
   return VQ_OK;
 }
 

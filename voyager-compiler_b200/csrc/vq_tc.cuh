@@ -270,6 +270,9 @@ bool make_map(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols_byt
 // Same without swizzle and with a box of box_cols bytes x box_rows rows.
 bool make_map_plain(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols_bytes,
                     uint32_t box_cols, uint32_t box_rows);
+// With SWIZZLE_128B or SWIZZLE_64B (swizzle = 128 or 64: the box's bytes per row).
+bool make_map_box(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols_bytes,
+                  uint32_t box_cols, uint32_t box_rows, uint32_t swizzle);
 int sm_count();
 }  // namespace mx
 }  // namespace vq

@@ -38,5 +38,7 @@ def check_errors(device=None, clear: bool = True) -> None:
         _lib.check(lib.vq_device_errors(ctypes.byref(code), 1 if clear else 0, _stream(dev)),
                    "vq_device_errors")
     if code.value:
-        raise _lib.VqError(f"a bounded device wait gave up on {dev} (code {code.value}): "
+        what = ("a key / value cache plan did not fit (a length, count or page out of range)"
+                if code.value in (301, 302, 303, 312, 313, 314) else "a bounded device wait gave up")
+        raise _lib.VqError(f"{what} on {dev} (code {code.value}): "
                            "the results of that launch are incomplete")

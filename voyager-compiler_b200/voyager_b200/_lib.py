@@ -237,6 +237,27 @@ _SIGNATURES = {
                                     ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                     ctypes.c_void_p, ctypes.c_void_p]),
     "vq_transpose": (ctypes.c_int, [P(VqTensor), P(VqTensor), ctypes.c_void_p]),
+    "vq_norm_quantize_fp8": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                            ctypes.c_int64, ctypes.c_void_p, ctypes.c_int32,
+                                            ctypes.c_int64, ctypes.c_int64, ctypes.c_float]
+                             + [ctypes.c_void_p] * 4),
+    "vq_linear_fp8_block": (ctypes.c_int, [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 3
+                            + [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
+    "vq_rope_append_kv8": (ctypes.c_int, [ctypes.c_void_p] * 3
+                           + [P(ctypes.c_int64), ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64,
+                              ctypes.c_int32, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64,
+                              ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+                              ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                              ctypes.c_int32] + [ctypes.c_void_p] * 6),
+    "vq_attn_kv8_workspace": (ctypes.c_int, [ctypes.c_int64] * 2 + [ctypes.c_int32] * 4
+                              + [ctypes.c_int64, P(ctypes.c_int64), P(ctypes.c_int64)]),
+    "vq_attn_kv8": (ctypes.c_int, [ctypes.c_void_p, P(ctypes.c_int64), ctypes.c_int64,
+                                   ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]
+                    + [ctypes.c_void_p] * 4 + [ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p,
+                                               ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+                                               ctypes.c_float, ctypes.c_void_p, ctypes.c_int64,
+                                               ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                               ctypes.c_void_p]),
     "vq_codebook_lookup": (ctypes.c_int, [P(VqTensor), P(ctypes.c_int64), ctypes.c_int32,
                                           ctypes.c_void_p, ctypes.c_int64, P(VqTensor),
                                           ctypes.c_void_p]),
