@@ -554,8 +554,7 @@ template <int D, int NT>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, cudaStream_t st) {
   using C = Cfg<D, NT>;
   static_assert(WARPS * C::STAGES * 8 <= 256, "barrier area");
-  if (cudaFuncSetAttribute(k_attn_kv8<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) !=
-      cudaSuccess)
+  if (!allow_smem<k_attn_kv8<D, NT>>(C::SMEM))
     return VQ_ERR_CUDA;
   k_attn_kv8<D, NT><<<dim3(a.chunks, a.Hkv * a.groups, a.B), THREADS, C::SMEM, st>>>(mk, mv, a);
   return cudaGetLastError() == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;

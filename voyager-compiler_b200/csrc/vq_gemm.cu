@@ -1102,10 +1102,14 @@ bool make_map_box(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols
 }
 
 int sm_count() {
+  static int known[64] = {};  // a device's count does not change
   int dev = 0, n = 148;
   cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && known[dev] > 0) return known[dev];
   cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-  return n > 0 ? n : 148;
+  n = n > 0 ? n : 148;
+  if (dev >= 0 && dev < 64) known[dev] = n;
+  return n;
 }
 
 // The CTA-pair kernel is used unless VQ_GEMM_PAIR=0 is set in the environment.

@@ -11,8 +11,10 @@
 // The MMAs of the next blocks run meanwhile: one multiply-add per output and
 // block on the CUDA cores against 128 on the tensor cores.
 //
-// k_fp8_wide  many tokens: tiles of 128 tokens (TMEM lanes) x BN weight rows
-//             (columns), persistent; a thread's scale is one scalar per block.
+// k_fp8_pair  many tokens: tiles of 256 tokens (TMEM lanes) x 256 weight rows
+//             (columns) on CTA pairs, persistent; k_fp8_one the same with
+//             128 x 128 tiles on single CTAs.  A thread's scale is one scalar
+//             per block.
 // k_fp8_few   few tokens: tiles of 128 weight rows (lanes) x BN tokens, so
 //             that no lane is idle when the weight is all there is to read;
 //             K is split over a cluster of CTAs, whose float32 sums are added
@@ -49,7 +51,7 @@ struct Args {
   int M, N, nk;        // nk = ceil(K / 128)
   int mt, nt, tiles;   // tiles of this kernel's shape
   int splits;          // k_fp8_few: CTAs of a cluster
-  int vec;             // out rows take 16-byte stores
+  int vec, vec4;       // out rows take 4-byte, 8-byte stores
 };
 
 // Instruction descriptor, kind::f8f6f4: E4M3 x E4M3, float32 sums, K-major
@@ -72,6 +74,43 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
 }
+// The loads so far have landed; r is named so that no use of it moves above.
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                 "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
+               :
+               : "memory");
+  asm volatile("" : "+r"(r[30]), "+r"(r[31]));
+}
+
+// acc += r * s for two neighbouring columns in one instruction (each lane's
+// product and sum rounded as fmaf rounds them).
+__device__ __forceinline__ void fma2(uint64_t& acc, uint32_t r0, uint32_t r1, uint64_t s) {
+  asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tfma.rn.f32x2 %0, t, %3, %0;\n\t}"
+      : "+l"(acc) : "r"(r0), "r"(r1), "l"(s));
+}
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
 
 // The four K = 32 MMAs of one stage (SWIZZLE_128B operands) into TMEM columns d.
 __device__ __forceinline__ void mma_stage(uint32_t d, uint64_t da, uint64_t db, uint32_t id) {
@@ -90,15 +129,110 @@ __device__ __forceinline__ void drain_loads(uint32_t full0, int stage, uint32_t 
 }
 
 // ---------------------------------------------------------------------------
-template <int BN>
-struct Wide {
-  static constexpr int STAGES = BN == 256 ? 4 : 6;
-  static constexpr int A_BYTES = 128 * BK, B_BYTES = BN * BK, STAGE = A_BYTES + B_BYTES;
-  static constexpr int BUFS = 512 / BN;
-  static constexpr int THREADS = 320;
-  static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
-  static constexpr int COLS = BN / 2;  // columns per promotion warp
-};
+// Promotion, shared by the two kernels for many tokens: one warp takes 32
+// token rows (a TMEM lane quarter) x COLS columns of each tile.
+constexpr int OUT_BYTES = 33 * 32 * 4;  // its staging: 32 rows x 64 columns of bf16, padded by a word
+
+// Adds the tile's nk blocks: the TMEM loads run one 32-column chunk ahead of
+// the multiply-adds, across the blocks too, so that the wait for a block's
+// MMAs hides behind the last chunk of the block before.  full(buf) waits for
+// a buffer (false: gave up), done(buf) gives it back; buffers are `bstep`
+// TMEM columns apart.
+template <int COLS, int BUFS, typename Full, typename Done>
+__device__ __forceinline__ bool promote(uint64_t (&acc)[COLS / 2], const float* sa, const float* sw, int nk,
+                                        uint32_t tbase, uint32_t bstep, int& buf, uint32_t& phase, Full full,
+                                        Done done) {
+  constexpr int CH = COLS / 32;
+  static_assert(CH % 2 == 0, "the chunk buffers alternate");
+  uint32_t r[2][32];
+  bool ok = full(buf, phase);
+  if (!ok) return false;
+  float s = __ldg(sa) * __ldg(sw);
+  tc_fence_after();
+  tmem_ld32(tbase + buf * bstep, r[0]);
+  for (int kt = 0; kt < nk; ++kt) {
+    const int kn = min(kt + 1, nk - 1);
+    const float na = __ldg(sa + kn), nw = __ldg(sw + kn);
+    const uint64_t s2 = pair(s, s);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      tmem_wait(r[c & 1]);
+      if (c + 1 < CH) {
+        tmem_ld32(tbase + buf * bstep + (c + 1) * 32, r[(c + 1) & 1]);
+      } else {
+        tc_fence_before();
+        done(buf);
+        if (++buf == BUFS) buf = 0, phase ^= 1;
+        if (kt + 1 < nk) {
+          if (ok) ok = full(buf, phase);
+          tc_fence_after();
+          tmem_ld32(tbase + buf * bstep, r[0]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], r[c & 1][2 * i], r[c & 1][2 * i + 1], s2);
+    }
+    s = na * nw;
+    if (!ok) {
+      tmem_wait(r[0]);
+      return false;
+    }
+  }
+  return true;
+}
+
+// This warp's columns of the bias into its staging, ahead of the tile.
+template <int COLS>
+__device__ __forceinline__ void fetch_bias(const Args& a, uint32_t* stage, int col0, int lane) {
+  if (!a.bias) return;
+  float* sb = reinterpret_cast<float*>(stage);
+  __syncwarp();
+#pragma unroll
+  for (int c = 0; c < COLS; c += 32)
+    sb[c + lane] = col0 + c + lane < a.N ? BF16::load(a.bias + col0 + c + lane) : 0.0f;
+}
+
+// Sums (+ bias) to bf16 rows through the staging, so that a warp's stores run
+// along the rows.
+template <int COLS>
+__device__ __forceinline__ void store_rows(const Args& a, uint64_t (&acc)[COLS / 2], uint32_t* stage, int r0,
+                                           int col0, int lane) {
+  if (a.bias) {
+    __syncwarp();
+    const float4* sb = reinterpret_cast<const float4*>(stage);
+#pragma unroll
+    for (int c = 0; c < COLS / 4; ++c) {
+      const float4 v = sb[c];
+      const float2 x = unpair(acc[2 * c]), y = unpair(acc[2 * c + 1]);
+      acc[2 * c] = pair(x.x + v.x, x.y + v.y);
+      acc[2 * c + 1] = pair(y.x + v.z, y.y + v.w);
+    }
+  }
+  const int rows = min(32, a.M - r0);
+#pragma unroll
+  for (int c = 0; c < COLS; c += 64) {
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const float2 v = unpair(acc[c / 2 + j]);
+      stage[lane * 33 + j] = bf_pack(v.x, v.y);
+    }
+    __syncwarp();
+    const int col = col0 + c + 2 * lane;
+    uint16_t* o = a.out + (int64_t)r0 * a.ldo + col;
+    if (a.vec && col + 2 <= a.N) {
+#pragma unroll 8
+      for (int i = 0; i < rows; ++i) *reinterpret_cast<uint32_t*>(o + (int64_t)i * a.ldo) = stage[i * 33 + lane];
+    } else {
+#pragma unroll 4
+      for (int i = 0; i < rows; ++i) {
+        const uint32_t w = stage[i * 33 + lane];
+        if (col < a.N) o[(int64_t)i * a.ldo] = (uint16_t)w;
+        if (col + 1 < a.N) o[(int64_t)i * a.ldo + 1] = (uint16_t)(w >> 16);
+      }
+    }
+  }
+}
 
 // Tile -> (token tile, weight tile): token tiles fastest within groups of 8,
 // so that the CTAs of a wave share few rows of both operands.
@@ -109,20 +243,46 @@ __device__ __forceinline__ void tile_of(const Args& a, int t, int& tm, int& tn) 
   tm = gr * 8 + in - tn * rows;
 }
 
-template <int BN>
-__global__ void __launch_bounds__(Wide<BN>::THREADS, 1)
-    k_fp8_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
-               const __grid_constant__ Args a) {
-  using C = Wide<BN>;
+// The scales of a row and of a 128-row weight block, clamped to what exists.
+__device__ __forceinline__ const float* sa_of(const Args& a, int row) {
+  return a.sa + (int64_t)min(row, a.M - 1) * a.nk;
+}
+__device__ __forceinline__ const float* sw_of(const Args& a, int block) {
+  return a.sw + (int64_t)min(block, (a.N - 1) / 128) * a.nk;
+}
+
+// One lane of a converged warp.  The warp that issues the MMAs runs its loop
+// whole, with the instructions under this predicate: the operands then stay
+// in uniform registers (a loop run by lane 0 alone took twice the time per
+// MMA, moving them there: 535 against 230 cycles per block of 4 MMAs and
+// their commits).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// ---------------------------------------------------------------------------
+// 128 x 128 tiles, one CTA each: four TMEM buffers of 128 columns.
+struct One {
+  static constexpr int STAGES = 6, STAGE = 2 * 128 * BK, BUFS = 4, THREADS = 384, COLS = 64;
+  static constexpr int SMEM = STAGES * STAGE + 8 * OUT_BYTES + 1024 + 256;
+};
+
+__global__ void __launch_bounds__(One::THREADS, 1)
+    k_fp8_one(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+              const __grid_constant__ Args a) {
+  using C = One;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~(uintptr_t)1023);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE);
+  uint32_t* out_stage = reinterpret_cast<uint32_t*>(smem + C::STAGES * C::STAGE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE + 8 * OUT_BYTES);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * C::STAGES;
   const uint32_t acc_full0 = empty0 + 8 * C::STAGES, acc_empty0 = acc_full0 + 8 * C::BUFS;
   const uint32_t drain = acc_empty0 + 8 * C::BUFS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::STAGES + 2 * C::BUFS + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) mbar_init(full0 + 8 * s, 1), mbar_init(empty0 + 8 * s, 1);
     for (int s = 0; s < C::BUFS; ++s) mbar_init(acc_full0 + 8 * s, 1), mbar_init(acc_empty0 + 8 * s, 8);
@@ -139,122 +299,232 @@ __global__ void __launch_bounds__(Wide<BN>::THREADS, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < a.tiles && ok; t += gridDim.x) {
-        int tm, tn;
-        tile_of(a, t, tm, tn);
-        for (int kt = 0; kt < a.nk; ++kt) {
-          if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, nullptr, ERR_EMPTY)) {
-            ok = false;
-            break;
-          }
-          const uint32_t dst = smem_u32(smem) + stage * C::STAGE;
-          mbar_expect_tx(full0 + 8 * stage, C::STAGE);
-          tma_load_2d(dst, &map_a, kt * BK, tm * 128, full0 + 8 * stage);
-          tma_load_2d(dst + C::A_BYTES, &map_w, kt * BK, tn * BN, full0 + 8 * stage);
-          if (++stage == C::STAGES) stage = 0, phase ^= 1;
-        }
-      }
-      drain_loads<C::STAGES>(full0, stage, phase);
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, bphase = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < a.tiles && ok; t += gridDim.x) {
-        for (int kt = 0; kt < a.nk; ++kt) {
-          if (!mbar_wait(acc_empty0 + 8 * buf, bphase ^ 1, nullptr, ERR_ACC) ||
-              !mbar_wait(full0 + 8 * stage, phase, nullptr, ERR_FULL)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t s0 = smem_u32(smem) + stage * C::STAGE;
-          mma_stage(tmem + buf * BN, sw128_desc(s0), sw128_desc(s0 + C::A_BYTES), idesc(128, BN));
-          tc_commit(empty0 + 8 * stage);
-          tc_commit(acc_full0 + 8 * buf);
-          if (++stage == C::STAGES) stage = 0, phase ^= 1;
-          if (++buf == C::BUFS) buf = 0, bphase ^= 1;
-        }
-      }
-      tc_commit(drain);
-      mbar_wait(drain, 0, nullptr, ERR_DRAIN);
-    }
-  } else {
-    // promotion: warps 2..9, two per TMEM lane quarter, COLS columns each
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    int buf = 0;
-    uint32_t bphase = 0;
+  if (warp == 0 && lane == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < a.tiles && ok; t += gridDim.x) {
       int tm, tn;
       tile_of(a, t, tm, tn);
-      const int row = tm * 128 + q * 32 + lane;
-      const int col0 = tn * BN + half * C::COLS;
-      const float* sa = a.sa + (int64_t)min(row, a.M - 1) * a.nk;
-      const float* sw = a.sw + (int64_t)min(col0 / 128, (a.N - 1) / 128) * a.nk;
-      float acc[C::COLS];
-#pragma unroll
-      for (int i = 0; i < C::COLS; ++i) acc[i] = 0.0f;
-      float na = __ldg(sa), nw = __ldg(sw);
       for (int kt = 0; kt < a.nk; ++kt) {
-        const float s = na * nw;
-        const int kn = min(kt + 1, a.nk - 1);
-        na = __ldg(sa + kn), nw = __ldg(sw + kn);
-        if (!mbar_wait_warp(acc_full0 + 8 * buf, bphase, nullptr, ERR_ACC)) {
+        if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, nullptr, ERR_EMPTY)) {
+          ok = false;
+          break;
+        }
+        const uint32_t dst = smem_u32(smem) + stage * C::STAGE;
+        mbar_expect_tx(full0 + 8 * stage, C::STAGE);
+        tma_load_2d(dst, &map_a, kt * BK, tm * 128, full0 + 8 * stage);
+        tma_load_2d(dst + 128 * BK, &map_w, kt * BK, tn * 128, full0 + 8 * stage);
+        if (++stage == C::STAGES) stage = 0, phase ^= 1;
+      }
+    }
+    drain_loads<C::STAGES>(full0, stage, phase);
+  } else if (warp == 1) {
+    const uint64_t da0 = sw128_desc(smem_u32(smem)), dw0 = sw128_desc(smem_u32(smem) + 128 * BK);
+    int stage = 0, buf = 0;
+    uint32_t phase = 0, bphase = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < a.tiles && ok; t += gridDim.x) {
+      for (int kt = 0; kt < a.nk; ++kt) {
+        if (!mbar_wait_warp(acc_empty0 + 8 * buf, bphase ^ 1, nullptr, ERR_ACC) ||
+            !mbar_wait_warp(full0 + 8 * stage, phase, nullptr, ERR_FULL)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + buf * BN + half * C::COLS;
-#pragma unroll
-        for (int c = 0; c < C::COLS / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld32(taddr + c * 32, r);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            acc[c * 32 + i] = fmaf(__uint_as_float(r[i]), s, acc[c * 32 + i]);
+        if (elect_one()) {
+          const uint32_t so = stage * (C::STAGE / 16);
+          mma_stage(tmem + buf * 128, desc_at(da0, so), desc_at(dw0, so), idesc(128, 128));
+          tc_commit(acc_full0 + 8 * buf);
+          tc_commit(empty0 + 8 * stage);
         }
-        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty0 + 8 * buf);
+        if (++stage == C::STAGES) stage = 0, phase ^= 1;
         if (++buf == C::BUFS) buf = 0, bphase ^= 1;
       }
-      if (row < a.M && ok) {
-        uint16_t* o = a.out + (int64_t)row * a.ldo + col0;
+    }
+    if (elect_one()) {
+      tc_commit(drain);
+      mbar_wait(drain, 0, nullptr, ERR_DRAIN);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // warps 4..11: two per TMEM lane quarter, 64 columns each
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    uint32_t* stage_out = out_stage + (warp - 4) * (OUT_BYTES / 4);
+    int buf = 0;
+    uint32_t bphase = 0;
+    for (int t = blockIdx.x; t < a.tiles; t += gridDim.x) {
+      int tm, tn;
+      tile_of(a, t, tm, tn);
+      const int r0 = tm * 128 + q * 32, col0 = tn * 128 + half * C::COLS;
+      fetch_bias<C::COLS>(a, stage_out, col0, lane);
+      uint64_t acc[C::COLS / 2];
 #pragma unroll
-        for (int c = 0; c < C::COLS; c += 8) {
-          if (a.vec && col0 + c + 8 <= a.N) {
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = acc[c + i];
-            if (a.bias) {
-              float bb[8];
-              BF16::load8(a.bias + col0 + c, bb);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] += bb[i];
-            }
-            BF16::store8(o + c, v);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (col0 + c + i < a.N)
-                BF16::store(o + c + i, acc[c + i] + (a.bias ? BF16::load(a.bias + col0 + c + i) : 0.0f));
-          }
-        }
-      }
+      for (int i = 0; i < C::COLS / 2; ++i) acc[i] = 0;
+      if (!promote<C::COLS, C::BUFS>(
+              acc, sa_of(a, r0 + lane), sw_of(a, tn), a.nk,
+              tmem + ((uint32_t)(q * 32) << 16) + half * C::COLS, 128, buf, bphase,
+              [&](int b, uint32_t ph) { return mbar_wait_warp(acc_full0 + 8 * b, ph, nullptr, ERR_ACC); },
+              [&](int b) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty0 + 8 * b);
+              }))
+        break;
+      store_rows<C::COLS>(a, acc, stage_out, r0, col0, lane);
     }
   }
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// 256 x 256 tiles on CTA pairs (cta_group::2): each CTA holds 128 token rows
+// in its TMEM and loads those and half of the weight rows, 32 KB per block
+// instead of the 48 KB that a CTA of its own needs for 128 x 256.  The even
+// CTA issues the MMAs.
+struct Pair {
+  static constexpr int BN = 256, COLS = BN / 2, A_BYTES = 128 * BK, STAGE = A_BYTES + BN / 2 * BK, STAGES = 6;
+  // 3 warpgroups per CTA: TMA and MMA issue, then two of promotion.  The
+  // launch gives every thread 168 registers; setmaxnreg moves them to the
+  // promotion (128 * 40 + 256 * 232 = 384 * 168), which needs about 215.
+  static constexpr int THREADS = 384, ISSUE_REGS = 40, PROMOTE_REGS = 232;
+  static constexpr int SMEM = STAGES * STAGE + 8 * OUT_BYTES + 1024 + 256;
+  static_assert(SMEM <= 227 * 1024 && STAGE % 1024 == 0, "shared memory");
+};
+
+__device__ __forceinline__ void mma_f8_pair(uint32_t d, uint64_t da, uint64_t db, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(da), "l"(db), "r"(id), "r"(acc));
+}
+
+__global__ void __launch_bounds__(Pair::THREADS, 1)
+    k_fp8_pair(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w,
+               const __grid_constant__ Args a) {
+  using C = Pair;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~(uintptr_t)1023);
+  uint32_t* out_stage = reinterpret_cast<uint32_t*>(smem + C::STAGES * C::STAGE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::STAGES * C::STAGE + 8 * OUT_BYTES);
+  const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * C::STAGES;
+  const uint32_t acc_full0 = empty0 + 8 * C::STAGES, acc_empty0 = acc_full0 + 8 * 2;
+  const uint32_t drain = acc_empty0 + 8 * 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::STAGES + 5);
+  const uint32_t rank = cluster_ctarank();  // 0: issues the pair's MMAs
+  const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int pair_id = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) mbar_init(full0 + 8 * s, 1), mbar_init(empty0 + 8 * s, 1);
+    for (int s = 0; s < 2; ++s) mbar_init(acc_full0 + 8 * s, 1), mbar_init(acc_empty0 + 8 * s, 16);
+    mbar_init(drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)), "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  tc_fence_before();
+  cluster_sync();  // both CTAs' barriers exist before any use across them
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::ISSUE_REGS));
+    if (warp == 0 && lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint32_t fb0 = mapa_shared(full0, 0);  // both CTAs' loads count on the even CTA
+      for (int t = pair_id; t < a.tiles && ok; t += npairs) {
+        int tm, tn;
+        tile_of(a, t, tm, tn);
+        const int ya = tm * 256 + (int)rank * 128, yw = tn * C::BN + (int)rank * (C::BN / 2);
+        for (int kt = 0; kt < a.nk; ++kt) {
+          if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, nullptr, ERR_EMPTY)) {
+            ok = false;
+            break;
+          }
+          const uint32_t dst = smem_u32(smem) + stage * C::STAGE, fb = fb0 + 8 * stage;
+          if (rank == 0) mbar_expect_tx(full0 + 8 * stage, 2 * C::STAGE);
+          tma_load_2d_pair(dst, &map_a, kt * BK, ya, fb);
+          tma_load_2d_pair(dst + C::A_BYTES, &map_w, kt * BK, yw, fb);
+          if (++stage == C::STAGES) stage = 0, phase ^= 1;
+        }
+      }
+      if (rank == 0) drain_loads<C::STAGES>(full0, stage, phase);
+    } else if (warp == 1 && rank == 0) {
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, bphase = 0;
+      bool ok = true;
+      const uint32_t s0 = smem_u32(smem);
+      const uint64_t da0 = sw128_desc(s0), dw0 = sw128_desc(s0 + C::A_BYTES);
+      for (int t = pair_id; t < a.tiles && ok; t += npairs) {
+        for (int kt = 0; kt < a.nk; ++kt) {
+          if (!mbar_wait_warp(acc_empty0 + 8 * buf, bphase ^ 1, nullptr, ERR_ACC) ||
+              !mbar_wait_warp(full0 + 8 * stage, phase, nullptr, ERR_FULL)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t so = stage * (C::STAGE / 16);
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+              mma_f8_pair(tmem + buf * C::BN, desc_at(da0, so + 2 * j), desc_at(dw0, so + 2 * j),
+                          idesc(256, C::BN), j > 0);
+            tc_commit_pair(acc_full0 + 8 * buf, 0x3);
+            tc_commit_pair(empty0 + 8 * stage, 0x3);
+          }
+          __syncwarp();
+          if (++stage == C::STAGES) stage = 0, phase ^= 1;
+          if (++buf == 2) buf = 0, bphase ^= 1;
+        }
+      }
+      if (elect_one()) {
+        tc_commit_pair(drain, 0x1);
+        mbar_wait(drain, 0, nullptr, ERR_DRAIN);
+      }
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::PROMOTE_REGS));
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    uint32_t* stage_out = out_stage + (warp - 4) * (OUT_BYTES / 4);
+    const uint32_t give0 = mapa_shared(acc_empty0, 0);
+    int buf = 0;
+    uint32_t bphase = 0;
+    for (int t = pair_id; t < a.tiles; t += npairs) {
+      int tm, tn;
+      tile_of(a, t, tm, tn);
+      const int r0 = tm * 256 + (int)rank * 128 + q * 32, col0 = tn * C::BN + half * C::COLS;
+      fetch_bias<C::COLS>(a, stage_out, col0, lane);
+      uint64_t acc[C::COLS / 2];
+#pragma unroll
+      for (int i = 0; i < C::COLS / 2; ++i) acc[i] = 0;
+      if (!promote<C::COLS, 2>(
+              acc, sa_of(a, r0 + lane), sw_of(a, col0 / 128), a.nk, tmem + ((uint32_t)(q * 32) << 16) + half * C::COLS, C::BN, buf, bphase,
+              [&](int b, uint32_t ph) { return mbar_wait_warp(acc_full0 + 8 * b, ph, nullptr, ERR_ACC); },
+              [&](int b) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(give0 + 8 * b);
+              }))
+        break;
+      store_rows<C::COLS>(a, acc, stage_out, r0, col0, lane);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();  // both CTAs are done with the pair's TMEM and barriers
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }
 }
 
@@ -287,7 +557,7 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
   const uint32_t acc_full0 = empty0 + 8 * C::STAGES, acc_empty0 = acc_full0 + 8 * C::BUFS;
   const uint32_t drain = acc_empty0 + 8 * C::BUFS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::STAGES + 2 * C::BUFS + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int rank = a.splits > 1 ? (int)cluster_ctarank() : 0;
   const int tile = blockIdx.x / a.splits, tm = tile / a.nt, tn = tile - tm * a.nt;
   const int kb0 = (int)((int64_t)a.nk * rank / a.splits);
@@ -323,24 +593,29 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
       drain_loads<C::STAGES>(full0, stage, phase);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0, buf = 0;
-      uint32_t phase = 0, bphase = 0;
-      for (int kt = kb0; kt < kb1; ++kt) {
-        if (!mbar_wait(acc_empty0 + 8 * buf, bphase ^ 1, nullptr, ERR_ACC) ||
-            !mbar_wait(full0 + 8 * stage, phase, nullptr, ERR_FULL))
-          break;
-        tc_fence_after();
-        const uint32_t s0 = smem_u32(smem) + stage * C::STAGE;
-        mma_stage(tmem + buf * BN, sw128_desc(s0), sw128_desc(s0 + C::W_BYTES), idesc(128, BN));
-        tc_commit(empty0 + 8 * stage);
+    int stage = 0, buf = 0;
+    uint32_t phase = 0, bphase = 0;
+    const uint64_t dw0 = sw128_desc(smem_u32(smem)), dx0 = sw128_desc(smem_u32(smem) + C::W_BYTES);
+    for (int kt = kb0; kt < kb1; ++kt) {
+      if (!mbar_wait_warp(acc_empty0 + 8 * buf, bphase ^ 1, nullptr, ERR_ACC) ||
+          !mbar_wait_warp(full0 + 8 * stage, phase, nullptr, ERR_FULL))
+        break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t so = stage * (C::STAGE / 16);
+        mma_stage(tmem + buf * BN, desc_at(dw0, so), desc_at(dx0, so), idesc(128, BN));
         tc_commit(acc_full0 + 8 * buf);
-        if (++stage == C::STAGES) stage = 0, phase ^= 1;
-        if (++buf == C::BUFS) buf = 0, bphase ^= 1;
+        tc_commit(empty0 + 8 * stage);
       }
+      __syncwarp();
+      if (++stage == C::STAGES) stage = 0, phase ^= 1;
+      if (++buf == C::BUFS) buf = 0, bphase ^= 1;
+    }
+    if (elect_one()) {
       tc_commit(drain);
       mbar_wait(drain, 0, nullptr, ERR_DRAIN);
     }
+    __syncwarp();
   }
   float acc[BN];
   const int q = warp & 3;  // TMEM lane quarter of warps 2..5
@@ -373,7 +648,7 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
         for (int c = 0; c < BN; c += 16) {
           uint32_t r[16];
           tmem_ld16(taddr + c, r);
-          tmem_ld_wait();
+          tmem_wait(r);
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
             const float4 s = *reinterpret_cast<const float4*>(s_scale + k * BN + c + i);
@@ -425,7 +700,7 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
       for (int k = 0; k < 4; ++k)
         if (n + k < a.N) v[k] += BF16::load(a.bias + n + k);
     }
-    if (a.vec && n + 4 <= a.N) {
+    if (a.vec4 && n + 4 <= a.N) {
       *reinterpret_cast<uint2*>(o) = make_uint2(bf_pack(v[0], v[1]), bf_pack(v[2], v[3]));
     } else {
 #pragma unroll
@@ -441,19 +716,39 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
 }
 
 // ---------------------------------------------------------------------------
-template <int BN>
-int launch_wide(const void* x, const void* w, int64_t K, Args a, cudaStream_t st) {
-  using C = Wide<BN>;
-  static_assert((2 * C::STAGES + 2 * C::BUFS + 2) * 8 <= 256, "barrier area");
+int launch_many(const void* x, const void* w, int64_t K, Args a, cudaStream_t st) {
+  static_assert((2 * One::STAGES + 2 * One::BUFS + 2) * 8 <= 256 && (2 * Pair::STAGES + 6) * 8 <= 256,
+                "barrier areas");
   CUtensorMap ma, mw;
-  if (!vq::mx::make_map(&ma, x, a.M, K, 128) || !vq::mx::make_map(&mw, w, a.N, K, BN)) return VQ_ERR_CUDA;
-  if (cudaFuncSetAttribute(k_fp8_wide<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) !=
-      cudaSuccess)
-    return VQ_ERR_CUDA;
+  const int sms = vq::mx::sm_count();
+  // pairs once their 256 x 256 tiles fill the SMs; below that, four times as
+  // many tiles of 128 x 128
+  const int64_t pair_tiles = (int64_t)((a.M + 255) / 256) * ((a.N + Pair::BN - 1) / Pair::BN);
+  if (pair_tiles * 2 >= sms) {
+    if (!vq::mx::make_map(&ma, x, a.M, K, 128) || !vq::mx::make_map(&mw, w, a.N, K, Pair::BN / 2))
+      return VQ_ERR_CUDA;
+    if (!allow_smem<k_fp8_pair>(Pair::SMEM)) return VQ_ERR_CUDA;
+    a.mt = (a.M + 255) / 256;
+    a.nt = (a.N + Pair::BN - 1) / Pair::BN;
+    a.tiles = a.mt * a.nt;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * std::min(a.tiles, sms / 2));
+    cfg.blockDim = dim3(Pair::THREADS);
+    cfg.dynamicSmemBytes = Pair::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_fp8_pair, ma, mw, a) == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
+  }
+  if (!vq::mx::make_map(&ma, x, a.M, K, 128) || !vq::mx::make_map(&mw, w, a.N, K, 128)) return VQ_ERR_CUDA;
+  if (!allow_smem<k_fp8_one>(One::SMEM)) return VQ_ERR_CUDA;
   a.mt = (a.M + 127) / 128;
-  a.nt = (a.N + BN - 1) / BN;
+  a.nt = (a.N + 127) / 128;
   a.tiles = a.mt * a.nt;
-  k_fp8_wide<BN><<<std::min(a.tiles, vq::mx::sm_count()), C::THREADS, C::SMEM, st>>>(ma, mw, a);
+  k_fp8_one<<<std::min(a.tiles, sms), One::THREADS, One::SMEM, st>>>(ma, mw, a);
   return cudaGetLastError() == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
 }
 
@@ -463,8 +758,7 @@ int launch_few(const void* x, const void* w, int64_t K, Args a, cudaStream_t st)
   static_assert((2 * C::STAGES + 2 * C::BUFS + 2) * 8 <= 256, "barrier area");
   CUtensorMap mx_, mw;
   if (!vq::mx::make_map(&mx_, x, a.M, K, BN) || !vq::mx::make_map(&mw, w, a.N, K, 128)) return VQ_ERR_CUDA;
-  if (cudaFuncSetAttribute(k_fp8_few<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) !=
-      cudaSuccess)
+  if (!allow_smem<k_fp8_few<BN>>(C::SMEM))
     return VQ_ERR_CUDA;
   a.mt = (a.M + BN - 1) / BN;
   a.nt = (a.N + 127) / 128;
@@ -519,12 +813,12 @@ extern "C" int vq_linear_fp8_block(const void* x, const float* x_scale, const vo
   a.out = (uint16_t*)out;
   a.ldo = ldo;
   a.M = (int)M, a.N = (int)N, a.nk = (int)((K + 127) / 128);
-  a.vec = ldo % 8 == 0 && !(reinterpret_cast<uintptr_t>(out) & 15) && !(reinterpret_cast<uintptr_t>(bias) & 15);
+  a.vec = ldo % 2 == 0 && !(reinterpret_cast<uintptr_t>(out) & 3);
+  a.vec4 = ldo % 4 == 0 && !(reinterpret_cast<uintptr_t>(out) & 7);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (M <= 16) return launch_few<16>(x, w, K, a, st);
   if (M <= 32) return launch_few<32>(x, w, K, a, st);
   if (M <= 64) return launch_few<64>(x, w, K, a, st);
   if (M <= 128) return launch_few<128>(x, w, K, a, st);
-  const int64_t big = ((M + 127) / 128) * ((N + 255) / 256);
-  return big >= vq::mx::sm_count() ? launch_wide<256>(x, w, K, a, st) : launch_wide<128>(x, w, K, a, st);
+  return launch_many(x, w, K, a, st);
 }

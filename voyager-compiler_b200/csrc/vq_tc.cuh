@@ -111,6 +111,20 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       : "memory");
 }
 
+// Host side: the dynamic shared memory limit of kernel K raised to `bytes`,
+// once per device.
+template <auto K>
+static inline bool allow_smem(int bytes) {
+  static bool done[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  if (dev < 64 && done[dev]) return true;
+  if (cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return false;
+  if (dev < 64) done[dev] = true;
+  return true;
+}
+
 // K-major SWIZZLE_128B shared-memory matrix descriptor (tcgen05 format,
 // version 1): start >> 4, LBO 1 (unused for swizzled K-major), SBO = 1024 B
 // between 8-row groups, layout type 2.  Rows are 128 bytes; the 16-byte

@@ -15,7 +15,7 @@ from typing import Optional, Tuple
 import torch
 
 from voyager_b200 import _lib
-from voyager_b200.ops import _stream
+from voyager_b200._launch import call
 
 BLOCK = 128
 E4M3 = torch.float8_e4m3fn
@@ -31,32 +31,37 @@ def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
 
 
 def _norm_quantize(x, residual, weight, eps, what):
-    code = _DTYPES.get(x.dtype)
+    dtype = x.dtype
+    code = _DTYPES.get(dtype)
     if code is None:
-        raise NotImplementedError(f"{what}: bfloat16 or float32, not {x.dtype}")
+        raise NotImplementedError(f"{what}: bfloat16 or float32, not {dtype}")
     if not x.is_cuda:
         raise NotImplementedError(f"{what}: the CUDA kernel needs CUDA tensors")
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f"{what}: x needs a last dimension to normalise, got {tuple(x.shape)}")
-    shape, cols, dev = x.shape, x.shape[-1], x.device
-    for n, t, s in (("residual", residual, shape), ("weight", weight, (cols,))):
-        if t is not None and (t.dtype != x.dtype or t.device != dev or t.shape != s):
-            raise ValueError(f"{what}: {n} must be {x.dtype} {tuple(s)} on {dev}")
+    shape, index = x.shape, x.get_device()
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"{what}: x needs a last dimension to normalise, got {tuple(shape)}")
+    cols = shape[-1]
     x2 = _rows(x, cols)
-    rows = x2.shape[0]
-    r2 = _rows(residual, cols) if residual is not None else None
-    codes = torch.empty(shape, dtype=E4M3, device=dev)
-    scale = torch.empty(shape[:-1] + ((cols + BLOCK - 1) // BLOCK,), dtype=torch.float32, device=dev)
-    hidden = torch.empty(shape, dtype=x.dtype, device=dev) if r2 is not None else None
-    w = weight.contiguous() if weight is not None else None
-    with torch.cuda.device(dev):
-        st = _lib.load().vq_norm_quantize_fp8(
-            x2.data_ptr(), max(x2.stride(0), cols), r2.data_ptr() if r2 is not None else None,
-            max(r2.stride(0), cols) if r2 is not None else 0,
-            w.data_ptr() if w is not None else None, code, rows, cols, eps, codes.data_ptr(),
-            scale.data_ptr(), hidden.data_ptr() if hidden is not None else None, _stream(dev))
-    if st:
-        _lib.check(st, what)
+    rows, ldx = x2.shape[0], max(x2.stride(0), cols)
+    w = r = h = hidden = None
+    ldr = 0
+    if weight is not None:
+        if weight.dtype != dtype or weight.get_device() != index or weight.shape != (cols,):
+            raise ValueError(f"{what}: weight must be {dtype} [{cols}] on {x.device}")
+        if weight.stride(0) != 1:
+            weight = weight.contiguous()
+        w = weight.data_ptr()
+    if residual is not None:
+        if residual.dtype != dtype or residual.get_device() != index or residual.shape != shape:
+            raise ValueError(f"{what}: residual must be {dtype} {tuple(shape)} on {x.device}")
+        residual = _rows(residual, cols)
+        r, ldr = residual.data_ptr(), max(residual.stride(0), cols)
+        hidden = x.new_empty(shape)
+        h = hidden.data_ptr()
+    codes = x.new_empty(shape, dtype=E4M3)
+    scale = x.new_empty(shape[:-1] + ((cols + BLOCK - 1) // BLOCK,), dtype=torch.float32)
+    call(_lib.load().vq_norm_quantize_fp8, index, what, x2.data_ptr(), ldx, r, ldr, w, code, rows, cols,
+         eps, codes.data_ptr(), scale.data_ptr(), h)
     return codes, scale, hidden
 
 
@@ -101,32 +106,29 @@ def linear(codes: torch.Tensor, scale: torch.Tensor, w_codes: torch.Tensor, w_sc
         raise NotImplementedError("fp8block.linear takes float8_e4m3fn codes")
     if scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
         raise NotImplementedError("fp8block.linear takes float32 scales")
-    dev = codes.device
     if not codes.is_cuda:
         raise NotImplementedError("fp8block.linear: the CUDA kernel needs CUDA tensors")
-    if w_codes.dim() != 2 or codes.dim() < 1 or codes.shape[-1] != w_codes.shape[1]:
-        raise ValueError(f"fp8block.linear: {tuple(codes.shape)} does not match a weight [N, K] "
-                         f"{tuple(w_codes.shape)}")
-    N, K = w_codes.shape
+    index, shape, ws = codes.get_device(), codes.shape, w_codes.shape
+    if len(ws) != 2 or not shape or shape[-1] != ws[1]:
+        raise ValueError(f"fp8block.linear: {tuple(shape)} does not match a weight [N, K] {tuple(ws)}")
+    N, K = ws
     if K == 0 or K % 16 or N == 0:
         raise ValueError(f"fp8block.linear: K = {K} must be a positive multiple of 16 and N = {N} positive")
     nk = (K + BLOCK - 1) // BLOCK
-    lead = codes.shape[:-1]
+    lead = shape[:-1]
     if scale.shape != lead + (nk,) or w_scale.shape != ((N + BLOCK - 1) // BLOCK, nk):
         raise ValueError(f"fp8block.linear: scales {tuple(scale.shape)} and {tuple(w_scale.shape)} are not "
                          f"one per 128 columns and one per 128 x 128 block")
-    if bias is not None and (bias.dtype != torch.bfloat16 or bias.shape != (N,) or bias.device != dev):
-        raise ValueError(f"fp8block.linear: bias must be bfloat16 [{N}] on {dev}")
-    for t in (scale, w_codes, w_scale):
-        if t.device != dev:
-            raise ValueError("fp8block.linear: operands on different devices")
-    c, s, w, ws = codes.contiguous(), scale.contiguous(), w_codes.contiguous(), w_scale.contiguous()
-    b = bias.contiguous() if bias is not None else None
-    out = torch.empty(lead + (N,), dtype=torch.bfloat16, device=dev)
-    with torch.cuda.device(dev):
-        st = _lib.load().vq_linear_fp8_block(
-            c.data_ptr(), s.data_ptr(), w.data_ptr(), ws.data_ptr(),
-            b.data_ptr() if b is not None else None, c.numel() // K, N, K, out.data_ptr(), N, _stream(dev))
-    if st:
-        _lib.check(st, "fp8block.linear")
+    if scale.get_device() != index or w_codes.get_device() != index or w_scale.get_device() != index:
+        raise ValueError("fp8block.linear: operands on different devices")
+    b = None
+    if bias is not None:
+        if bias.dtype != torch.bfloat16 or bias.shape != (N,) or bias.get_device() != index:
+            raise ValueError(f"fp8block.linear: bias must be bfloat16 [{N}] on {codes.device}")
+        bias = bias.contiguous()
+        b = bias.data_ptr()
+    codes, scale, w_codes, w_scale = codes.contiguous(), scale.contiguous(), w_codes.contiguous(), w_scale.contiguous()
+    out = codes.new_empty(lead + (N,), dtype=torch.bfloat16)
+    call(_lib.load().vq_linear_fp8_block, index, "fp8block.linear", codes.data_ptr(), scale.data_ptr(),
+         w_codes.data_ptr(), w_scale.data_ptr(), b, codes.numel() // K, N, K, out.data_ptr(), N)
     return out
