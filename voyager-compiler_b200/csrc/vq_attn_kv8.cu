@@ -21,12 +21,15 @@
 // the tensor cores with keys along the lanes; movmatrix turns the f16 pairs
 // into the operand of the second product.
 //
-// Work: one CTA of 4 warps per (sequence, kv head, row group, chunk of
-// keys); its warps take the chunk's tiles in turn, each with a ring of its
-// own that TMA fills (K and V, 32 x D bytes each, SWIZZLE_128B /
-// SWIZZLE_64B: the fragment loads then meet no bank conflict for D = 128).
-// Chunks of one row group are joined by the CTA that finishes last, in chunk
-// order, so the result does not depend on the order of arrival.
+// Work: the keys of every (sequence, row group, kv head) in units of 128,
+// laid end to end and cut into equal runs, one per CTA (two CTAs per SM), so
+// that unequal lengths leave no SM idle; a run may span several heads or
+// sequences.  Each of a CTA's 4 warps takes one 32-key tile of every unit and
+// has a ring of its own that TMA fills (K and V, 32 x D bytes each,
+// SWIZZLE_128B / SWIZZLE_64B: the fragment loads then meet no bank conflict
+// for D = 128).  The pieces of a head that was cut are joined by the CTA that
+// finishes last, in the CTAs' order, so the result does not depend on the
+// order of arrival.
 //
 // Bound by HBM: 2 D bytes per key and kv head.
 #include <cuda.h>
@@ -48,7 +51,7 @@ using namespace vq::tc;
 
 enum { ERR_WAIT = 311, ERR_PAGE = 312, ERR_CAPACITY = 313, ERR_COUNT = 314 };
 
-constexpr int WARPS = 4, THREADS = WARPS * 32, TILE = 32;
+constexpr int WARPS = 4, THREADS = WARPS * 32, TILE = 32, UNIT = WARPS * TILE;
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr float P_EXP = 15.0f;  // the largest weight is 2^15 in f16
 
@@ -58,10 +61,10 @@ struct Args {
   uint16_t* out;  // bf16 [B, T, H, D]
   const float *k_scale, *v_scale;
   const int32_t *block_table, *lengths, *counts;
-  float* part;        // [pairs * groups][chunks][ROWS * (D + 3)]
-  int32_t* done;      // [pairs * groups] zero before, zero after
+  float* part;        // [CTAs][2][ROWS * (D + 3)]: pieces of heads that were cut
+  int32_t* done;      // [B * groups * Hkv] zero before, zero after
   int B, T, H, Hkv, G, page_log2, width, pages;
-  int groups, chunks, chunk;  // row groups per (b, kv head); keys per chunk, a multiple of TILE
+  int groups;         // row groups per sequence
   float sm_log2;              // sm_scale * log2(e)
 };
 
@@ -72,10 +75,12 @@ struct Cfg {
   static constexpr int STAGES = D == 128 ? 3 : 5;
   static constexpr int RING = STAGES * 2 * TILE_BYTES;  // per warp
   static constexpr int SMEM_RING = WARPS * RING;
-  static constexpr int PAGES_MAX = 512;                 // pages of one chunk
-  static constexpr int MERGE = WARPS * ROWS * (D + 3) * 4;
-  static_assert(MERGE <= SMEM_RING, "the join reuses the ring");
-  static constexpr int SMEM = SMEM_RING + 1024 + PAGES_MAX * 12 + 256;
+  // the warps' O meet in SUMS buffers, rows LD floats apart
+  static constexpr int SUMS = NT == 1 ? 2 : 1, LD = D + 4;
+  static constexpr int JOIN = (SUMS * ROWS * LD + 3 * WARPS * ROWS + 4 * ROWS) * 4;
+  static constexpr int SMEM = SMEM_RING + JOIN + 1024 + 256;
+  static_assert(JOIN % 16 == 0 && WARPS * STAGES * 8 <= 256, "barriers after the join's area");
+  static_assert(2 * (SMEM + 1024 + 256) <= 227 * 1024, "two CTAs per SM");
 };
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -123,20 +128,38 @@ __device__ __forceinline__ uint32_t swz(int r, int c) {
                   : (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
 
-// A running softmax and one output value: m, l, w and O as above.
-struct State {
-  float m = NEG_INF, l = 0.0f, w = NEG_INF, x = 0.0f;
-  __device__ __forceinline__ void add(float m2, float l2, float w2, float x2) {
-    const float mn = fmaxf(m, m2), wn = fmaxf(w, w2);
-    const float mr = mn == NEG_INF ? 0.0f : mn, wr = wn == NEG_INF ? 0.0f : wn;
-    l = l * ex2(m - mr) + l2 * ex2(m2 - mr);
-    x = x * ex2(w - wr) + x2 * ex2(w2 - wr);
-    m = mn, w = wn;
-  }
-  __device__ __forceinline__ float value() const {
-    return l == 0.0f || w == NEG_INF ? 0.0f * x : __fdiv_rn(x * ex2(w - P_EXP - m), l);
-  }
+// The output's factor of O from a row's m, l and w (0 for a row without keys).
+__device__ __forceinline__ float out_scale(float m, float l, float w) {
+  return l == 0.0f || w == NEG_INF ? 0.0f : __fdiv_rn(ex2(w - P_EXP - m), l);
+}
+
+// Entry e = (sequence, row group): the rows of it that have a query, the
+// tokens held, and the keys that some of its rows sees.
+struct Entry {
+  int b, row0, nrows, held, end;
 };
+template <int ROWS>
+__device__ __forceinline__ Entry entry_of(const Args& a, int e, bool report) {
+  Entry x;
+  x.b = e / a.groups;
+  x.row0 = (e - x.b * a.groups) * ROWS;
+  x.held = a.lengths[x.b];
+  int cnt = a.counts ? a.counts[x.b] : a.T;
+  if (x.held < 0 || cnt < 0 || cnt > a.T) {
+    if (report) note_err(nullptr, ERR_COUNT);
+    cnt = x.held < 0 ? 0 : min(max(cnt, 0), a.T);
+    x.held = max(x.held, 0);
+  }
+  const int64_t cap = (int64_t)a.width << a.page_log2;
+  if (x.held + (int64_t)cnt > cap) {
+    if (report) note_err(nullptr, ERR_CAPACITY);
+    cnt = x.held >= cap ? 0 : (int)(cap - x.held);
+  }
+  x.nrows = min(ROWS, cnt * a.G - x.row0);
+  x.end = x.nrows > 0 ? x.held + (x.row0 + x.nrows - 1) / a.G + 1 : 0;
+  return x;
+}
+__device__ __forceinline__ int units_of(const Entry& x) { return (x.end + UNIT - 1) / UNIT; }
 
 template <int D, int NT>
 __global__ void __launch_bounds__(THREADS)
@@ -144,75 +167,155 @@ __global__ void __launch_bounds__(THREADS)
                const __grid_constant__ Args a) {
   using C = Cfg<D, NT>;
   constexpr int KS = D / 16;   // k steps of the scores, and m tiles of the output
+  constexpr int PART = C::ROWS * (D + 3);  // O, then m, l and w of each row
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~(uintptr_t)1023);
-  int32_t* s_row = reinterpret_cast<int32_t*>(smem + C::SMEM_RING);      // cache row of each page
-  float* s_ks = reinterpret_cast<float*>(s_row + C::PAGES_MAX);
-  float* s_lv = s_ks + C::PAGES_MAX;  // log2 of v_scale
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_lv + C::PAGES_MAX);     // [WARPS][STAGES]
-  __shared__ int s_last;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::SMEM_RING + C::JOIN);  // [WARPS][STAGES]
+  __shared__ int s_last, s_entry;
+  __shared__ long long s_sum[WARPS], s_before;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int chunk = blockIdx.x;
-  const int grp = blockIdx.y % a.groups, kvh = blockIdx.y / a.groups, b = blockIdx.z;
-  const int pair = ((b * a.Hkv) + kvh) * a.groups + grp;
-
-  // the plan of this sequence
-  int held = a.lengths[b], cnt = a.counts ? a.counts[b] : a.T;
-  if (held < 0 || cnt < 0 || cnt > a.T) {
-    note_err(nullptr, ERR_COUNT);
-    cnt = held < 0 ? 0 : min(max(cnt, 0), a.T);
-    held = max(held, 0);
-  }
-  const int64_t cap = (int64_t)a.width << a.page_log2;
-  if (held + (int64_t)cnt > cap) {
-    note_err(nullptr, ERR_CAPACITY);
-    cnt = held >= cap ? 0 : (int)(cap - held);
-  }
-  const int row0 = grp * C::ROWS;
-  const int nrows = min(C::ROWS, cnt * a.G - row0);  // rows of this group with a query
-  // keys that some row of this group sees
-  const int end = nrows > 0 ? held + (row0 + nrows - 1) / a.G + 1 : 0;
-  const int nchunks = max(1, (end + a.chunk - 1) / a.chunk);
-  if (chunk >= nchunks) return;
-  const int k0 = chunk * a.chunk, k1 = min(end, k0 + a.chunk);
-  const int ntiles = k1 > k0 ? (k1 - k0 + TILE - 1) / TILE : 0;
-
   if (lane == 0) {
     for (int s = 0; s < C::STAGES; ++s) mbar_init(smem_u32(bars + warp * C::STAGES + s), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  // the chunk's pages (a chunk starts on a page: it is a multiple of the page size or within one)
-  const int p0 = k0 >> a.page_log2;
-  const int np = ntiles ? ((k1 - 1) >> a.page_log2) - p0 + 1 : 0;
-  for (int i = threadIdx.x; i < np; i += THREADS) {
-    int pid = a.block_table[(int64_t)b * a.width + p0 + i];
-    if (pid < 0 || pid >= a.pages) {
-      note_err(nullptr, ERR_PAGE);
-      pid = 0;
+
+  // ---- this CTA's run of units: a scan of the entries' unit counts (and, in
+  // the bits from 40 on, of the entries that have any) ----
+  const int entries = a.B * a.groups, per = (entries + THREADS - 1) / THREADS;
+  const int e0 = min(entries, (int)threadIdx.x * per), e1 = min(entries, e0 + per);
+  long long own = 0;
+  for (int e = e0; e < e1; ++e) {
+    const int u = units_of(entry_of<C::ROWS>(a, e, blockIdx.x == 0));
+    own += u ? u + (1ll << 40) : 0;
+  }
+  long long sum = own;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long y = __shfl_up_sync(FULL, sum, d);
+    if (lane >= d) sum += y;
+  }
+  if (lane == 31) s_sum[warp] = sum;
+  __syncthreads();
+  long long total = 0, before = sum - own;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) before += s_sum[w];
+    total += s_sum[w];
+  }
+  const int active = (int)(total >> 40);
+  constexpr long long LOW = (1ll << 40) - 1;
+  total = (total & LOW) * a.Hkv;
+  before = (before & LOW) * a.Hkv;
+  own = (own & LOW) * a.Hkv;
+  // CTAs with work.  A piece more of a head costs its join about an eighth of
+  // a unit's time, so a run is at least sqrt(units / 8) of an average head.
+  const float avg = active ? (float)total / ((float)active * a.Hkv) : 1.0f;
+  const int runs = (int)min((long long)gridDim.x, (long long)ceilf((float)total / fmaxf(1.0f, sqrtf(avg * 0.125f))));
+  const long long lo = runs ? total * blockIdx.x / runs : 0, hi = runs ? total * (blockIdx.x + 1) / runs : 0;
+  if ((int)blockIdx.x < runs && before <= lo && lo < before + own) {
+    long long at = before;
+    for (int e = e0; e < e1; ++e) {
+      const long long u = (long long)units_of(entry_of<C::ROWS>(a, e, false)) * a.Hkv;
+      if (lo < at + u) {
+        s_entry = e;
+        s_before = at;
+        break;
+      }
+      at += u;
     }
-    const int blk = pid * a.Hkv + kvh;
-    s_row[i] = blk << a.page_log2;
-    s_ks[i] = a.k_scale[blk];
-    s_lv[i] = log2f(a.v_scale[blk]);
+  }
+  // row groups without a query are written here: no unit belongs to them
+  for (int e = blockIdx.x; e < entries; e += gridDim.x) {
+    const Entry x = entry_of<C::ROWS>(a, e, false);
+    if (x.nrows > 0) continue;
+    const int rows = min(C::ROWS, a.T * a.G - x.row0);
+    for (int i = threadIdx.x; i < rows * a.Hkv * (D / 8); i += THREADS) {
+      const int row = x.row0 + i / (D / 8) % rows, h = i / (D / 8) / rows;
+      reinterpret_cast<uint4*>(a.out + (((int64_t)x.b * a.T + row / a.G) * a.H + h * a.G + row % a.G) * D)
+          [i % (D / 8)] = make_uint4(0, 0, 0, 0);
+    }
   }
   __syncthreads();
+  if ((int)blockIdx.x >= runs) return;
 
   const uint32_t ring = smem_u32(smem) + warp * C::RING;
   const uint32_t bar0 = smem_u32(bars + warp * C::STAGES);
-  auto issue = [&](int tile, int stage) {  // lane 0
-    const int key = k0 + tile * TILE;
-    const int y = s_row[(key >> a.page_log2) - p0] + (key & ((1 << a.page_log2) - 1));
-    const uint32_t bar = bar0 + 8 * stage, dst = ring + stage * 2 * C::TILE_BYTES;
-    mbar_expect_tx(bar, 2 * C::TILE_BYTES);
-    tma_load_2d(dst, &map_k, 0, y, bar);
-    tma_load_2d(dst + C::TILE_BYTES, &map_v, 0, y, bar);
+  int stage = 0;      // of the next tile to read; the ring runs on from segment to segment
+  uint32_t phase = 0;
+  bool ok = true;
+  long long pos = lo, ebase = s_before;
+  int e = s_entry;
+  Entry x = entry_of<C::ROWS>(a, e, false);
+  int units = units_of(x);
+
+  // A segment: the part of one head (entry, kv head) in this run.
+  struct Seg {
+    int b, row0, nrows, held, end, kvh, k0, k1, units, slot, pair;
+    bool whole;
+    long long ps;  // the head's first unit
+  } sg = {};
+  // A lane knows the page of tile 32 m + lane of the warp's tiles: its row in
+  // the cache and its scales, n_ for the batch m that is being issued, c_ for
+  // the one being read; the block table is read a batch ahead.
+  int n_row = 0, pid_next = 0, mine = 0, issued = 0, wstage = 0;
+  float n_ks = 0.0f, n_lv = 0.0f, c_ks = 0.0f, c_lv = 0.0f;
+  auto key_of = [&](int tile) { return min(sg.k0 + (warp + tile * WARPS) * TILE, sg.k1 - 1); };
+  auto pid_of = [&](int tile) { return a.block_table[(int64_t)sg.b * a.width + (key_of(tile) >> a.page_log2)]; };
+  auto issue = [&]() {
+    if ((issued & 31) == 0) {
+      int pid = pid_next;
+      if (pid < 0 || pid >= a.pages) {
+        note_err(nullptr, ERR_PAGE);
+        pid = 0;
+      }
+      const int blk = pid * a.Hkv + sg.kvh;
+      n_row = (blk << a.page_log2) + (key_of(issued + lane) & ((1 << a.page_log2) - 1) & ~(TILE - 1));
+      n_ks = a.k_scale[blk];
+      n_lv = a.v_scale[blk];
+      pid_next = pid_of(issued + lane + 32);
+    }
+    const int y = __shfl_sync(FULL, n_row, issued & 31);
+    if (lane == 0) {
+      const uint32_t bar = bar0 + 8 * wstage, dst = ring + wstage * 2 * C::TILE_BYTES;
+      mbar_expect_tx(bar, 2 * C::TILE_BYTES);
+      tma_load_2d(dst, &map_k, 0, y, bar);
+      tma_load_2d(dst + C::TILE_BYTES, &map_v, 0, y, bar);
+    }
+    ++issued;
+    if (++wstage == C::STAGES) wstage = 0;
   };
-  const int mine = ntiles > warp ? (ntiles - warp + WARPS - 1) / WARPS : 0;  // tiles warp, warp + 4, ..
-  int issued = 0;
-  if (lane == 0)
-    for (; issued < min(mine, C::STAGES); ++issued) issue(warp + issued * WARPS, issued);
+  // The next segment, and its first loads on their way.
+  auto open = [&]() {
+    while (pos >= ebase + (long long)units * a.Hkv) {  // the next entry with keys
+      ebase += (long long)units * a.Hkv;
+      x = entry_of<C::ROWS>(a, ++e, false);
+      units = units_of(x);
+    }
+    sg.b = x.b, sg.row0 = x.row0, sg.nrows = x.nrows, sg.held = x.held, sg.end = x.end, sg.units = units;
+    sg.kvh = (int)((pos - ebase) / units);
+    sg.pair = e * a.Hkv + sg.kvh;
+    sg.ps = ebase + (long long)sg.kvh * units;
+    const int u0 = (int)(pos - sg.ps), u1 = (int)min((long long)units, hi - sg.ps);
+    sg.whole = u0 == 0 && u1 == units;
+    sg.slot = pos == lo ? 0 : 1;
+    sg.k0 = u0 * UNIT, sg.k1 = min(x.end, u1 * UNIT);
+    const int ntiles = (sg.k1 - sg.k0 + TILE - 1) / TILE;
+    // tiles warp, warp + 4, ..; none after a wait that gave up
+    mine = ok && ntiles > warp ? (ntiles - warp + WARPS - 1) / WARPS : 0;
+    issued = 0;
+    wstage = stage;
+    if (mine > 0) {
+      pid_next = pid_of(lane);
+      for (int i = 0; i < min(mine, C::STAGES); ++i) issue();
+    }
+    pos = sg.ps + u1;
+  };
+  open();
+
+  for (bool more = true; more;) {
+  const int b = sg.b, row0 = sg.row0, nrows = sg.nrows, held = sg.held, end = sg.end, kvh = sg.kvh, k0 = sg.k0;
 
   // Q as the second operand of S^T = K Q^T.  Lane (g, t) holds row g's
   // columns D/4 * t ..: k step w takes its 4 columns D/4 * t + 4 w ...
@@ -272,13 +375,13 @@ __global__ void __launch_bounds__(THREADS)
     sum[n][0] = sum[n][1] = 0.0f;
   }
 
-  int stage = 0;
-  uint32_t phase = 0;
-  for (int i = 0; i < mine; ++i) {
+  int i = 0;
+  for (; i < mine; ++i) {
     const int key0 = k0 + (warp + i * WARPS) * TILE;
-    const int pg = (key0 >> a.page_log2) - p0;
-    const float ks = s_ks[pg], lv = s_lv[pg];
-    if (!mbar_wait_warp(bar0 + 8 * stage, phase, nullptr, ERR_WAIT)) break;
+    if ((i & 31) == 0) c_ks = n_ks, c_lv = log2f(n_lv);
+    const float ks = __shfl_sync(FULL, c_ks, i & 31), lv = __shfl_sync(FULL, c_lv, i & 31);
+    ok = mbar_wait_warp(bar0 + 8 * stage, phase, nullptr, ERR_WAIT);
+    if (!ok) break;
     const uint32_t kb = ring + stage * 2 * C::TILE_BYTES, vb = kb + C::TILE_BYTES;
     const bool tail = key0 + TILE > free_end;
 
@@ -443,25 +546,26 @@ __global__ void __launch_bounds__(THREADS)
       }
     }
     __syncwarp();  // every lane has read the stage
-    if (lane == 0 && issued < mine) {
-      issue(warp + issued * WARPS, stage);
-      ++issued;
-    }
+    if (issued < mine) issue();
     if (++stage == C::STAGES) stage = 0, phase ^= 1;
   }
-  // after a wait that gave up: this warp's loads land before the ring is reused
-  {
-    const int n = __shfl_sync(FULL, issued, 0);
-    for (int i = max(0, n - C::STAGES); i < n; ++i)
-      mbar_wait(bar0 + 8 * (i % C::STAGES), (i / C::STAGES) & 1, nullptr, ERR_WAIT);
+  // after a wait that gave up: the loads in flight land before the ring is reused
+  for (; i < issued; ++i) {
+    mbar_wait(bar0 + 8 * stage, phase, nullptr, ERR_WAIT);
+    if (++stage == C::STAGES) stage = 0, phase ^= 1;
   }
 
-  // ---- join the warps: the ring becomes [WARPS][ROWS][D] O, then maxima and sums ----
-  __syncthreads();
-  float* so = reinterpret_cast<float*>(smem);
-  float* sm = so + WARPS * C::ROWS * D;
+  const Seg cur = sg;
+  more = pos < hi;
+  if (more) open();  // its loads run under the join
+
+  // ---- join the warps ----
+  float* sums = reinterpret_cast<float*>(smem + C::SMEM_RING);  // [SUMS][ROWS][LD]
+  float* sm = sums + C::SUMS * C::ROWS * C::LD;                 // [WARPS][ROWS] m, l, w
   float* sl = sm + WARPS * C::ROWS;
   float* sw = sl + WARPS * C::ROWS;
+  float* fin = sw + WARPS * C::ROWS;                            // [ROWS] m, l, w, the output's factor
+  __syncthreads();  // the last join's readers are done
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -470,93 +574,174 @@ __global__ void __launch_bounds__(THREADS)
       l += __shfl_xor_sync(FULL, l, 4);
       l += __shfl_xor_sync(FULL, l, 8);
       l += __shfl_xor_sync(FULL, l, 16);
-      const int r = n * 8 + 2 * t + c;
       if (g == 0) {
-        sm[warp * C::ROWS + r] = mx[n][c];
-        sl[warp * C::ROWS + r] = l;
-        sw[warp * C::ROWS + r] = wx[n][c];
+        const int r = warp * C::ROWS + n * 8 + 2 * t + c;
+        sm[r] = mx[n][c], sl[r] = l, sw[r] = wx[n][c];
       }
-      float* p = so + (warp * C::ROWS + r) * D + g * (D / 8);
-#pragma unroll
-      for (int j = 0; j < KS; ++j)
-        *reinterpret_cast<float2*>(p + 2 * j) = make_float2(o[n][j][c], o[n][j][c + 2]);
     }
   __syncthreads();
-  constexpr int PART = C::ROWS * (D + 3);  // O, then m, l and w of each row
-  float* mine_part = a.part + ((int64_t)pair * a.chunks + chunk) * PART;
-  for (int i = threadIdx.x; i < C::ROWS * D; i += THREADS) {
-    const int r = i / D, d = i % D;
-    State st;
+  if (threadIdx.x < C::ROWS) {
+    float m = NEG_INF, w = NEG_INF, l = 0.0f;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w)
-      st.add(sm[w * C::ROWS + r], sl[w * C::ROWS + r], sw[w * C::ROWS + r], so[(w * C::ROWS + r) * D + d]);
-    if (nchunks == 1) {
-      const int row = row0 + r;
-      if (row < a.T * a.G)
-        BF16::store(a.out + (((int64_t)b * a.T + row / a.G) * a.H + kvh * a.G + row % a.G) * D + d,
-                    r < nrows ? st.value() : 0.0f);
-    } else {
-      mine_part[r * D + d] = st.x;
-      if (d == 0) {
-        mine_part[C::ROWS * D + r] = st.m;
-        mine_part[C::ROWS * (D + 1) + r] = st.l;
-        mine_part[C::ROWS * (D + 2) + r] = st.w;
-      }
+    for (int k = 0; k < WARPS; ++k) {
+      m = fmaxf(m, sm[k * C::ROWS + threadIdx.x]);
+      w = fmaxf(w, sw[k * C::ROWS + threadIdx.x]);
     }
+    const float ref = m == NEG_INF ? 0.0f : m;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k)
+      l = fmaf(sl[k * C::ROWS + threadIdx.x], ex2(sm[k * C::ROWS + threadIdx.x] - ref), l);
+    fin[threadIdx.x] = m, fin[C::ROWS + threadIdx.x] = l, fin[2 * C::ROWS + threadIdx.x] = w;
+    fin[3 * C::ROWS + threadIdx.x] = (int)threadIdx.x < cur.nrows ? out_scale(m, l, w) : 0.0f;
   }
-  if (nchunks == 1) return;
+  // every warp's O relative to the CTA's w, added in the warps' order.  Column
+  // d = D/8 g + 2j + i of a row lies at place 16 j + 2 g + i of it: the lanes of
+  // a store then meet no bank twice.
+#pragma unroll
+  for (int k = 0; k < WARPS / C::SUMS; ++k) {
+    if (warp / C::SUMS == k) {
+      float* dst = sums + (warp % C::SUMS) * C::ROWS * C::LD;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int r = n * 8 + 2 * t + c;
+          float w = sw[r];
+#pragma unroll
+          for (int q = 1; q < WARPS; ++q) w = fmaxf(w, sw[q * C::ROWS + r]);
+          const float f = ex2(wx[n][c] - (w == NEG_INF ? 0.0f : w));
+#pragma unroll
+          for (int j = 0; j < KS; ++j) {
+            float2* p = reinterpret_cast<float2*>(dst + r * C::LD + 16 * j + 2 * g);
+            float2 v = k ? *p : make_float2(0.0f, 0.0f);
+            v.x = fmaf(o[n][j][c], f, v.x);
+            v.y = fmaf(o[n][j][c + 2], f, v.y);
+            *p = v;
+          }
+        }
+    }
+    __syncthreads();
+  }
+  auto out_row = [&](int r) {
+    const int row = cur.row0 + r;
+    return a.out + (((int64_t)cur.b * a.T + row / a.G) * a.H + cur.kvh * a.G + row % a.G) * D;
+  };
+  if (cur.whole) {
+    const int rows = min(C::ROWS, a.T * a.G - cur.row0);
+    for (int i = threadIdx.x; i < rows * (D / 2); i += THREADS) {
+      const int r = i / (D / 2), d = i % (D / 2) * 2;
+      const float2* p = reinterpret_cast<const float2*>(sums + r * C::LD + d % (D / 8) * 8 + d / (D / 8) * 2);
+      float2 v = *p;
+      if (C::SUMS == 2) {
+        const float2 u = p[C::ROWS * C::LD / 2];
+        v.x += u.x, v.y += u.y;
+      }
+      const float f = fin[3 * C::ROWS + r];
+      // a row without a query is 0 even where its sums are not finite
+      *reinterpret_cast<uint32_t*>(out_row(r) + d) = r < cur.nrows ? bf_pack(v.x * f, v.y * f) : 0u;
+    }
+    continue;
+  }
 
-  // ---- join the chunks: the last CTA of the pair reads them in order ----
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) s_last = atomicAdd(a.done + pair, 1) == nchunks - 1;
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  const float* all = a.part + (int64_t)pair * a.chunks * PART;
-  for (int i = threadIdx.x; i < C::ROWS * D; i += THREADS) {
-    const int r = i / D, d = i % D, row = row0 + r;
-    if (row >= a.T * a.G) continue;
-    State st;
-    for (int c = 0; c < nchunks; ++c) {
-      const float* p = all + (int64_t)c * PART;
-      st.add(__ldcg(p + C::ROWS * D + r), __ldcg(p + C::ROWS * (D + 1) + r),
-             __ldcg(p + C::ROWS * (D + 2) + r), __ldcg(p + r * D + d));
+  // ---- a piece of a head: [ROWS][D] of O in place order, then m, l and w ----
+  float* piece_out = a.part + ((int64_t)blockIdx.x * 2 + cur.slot) * PART;
+  for (int i = threadIdx.x; i < cur.nrows * (D / 4); i += THREADS) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    const float4* p = reinterpret_cast<const float4*>(sums + r * C::LD + d);
+    float4 v = *p;
+    if (C::SUMS == 2) {
+      const float4 u = p[C::ROWS * C::LD / 4];
+      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
     }
-    BF16::store(a.out + (((int64_t)b * a.T + row / a.G) * a.H + kvh * a.G + row % a.G) * D + d,
-                r < nrows ? st.value() : 0.0f);
+    reinterpret_cast<float4*>(piece_out)[i] = v;
   }
-  if (threadIdx.x == 0) a.done[pair] = 0;
+  if (threadIdx.x < 3 * C::ROWS) piece_out[C::ROWS * D + threadIdx.x] = fin[threadIdx.x];
+  // the CTA that finishes last reads the head's pieces in the CTAs' order
+  const int c0 = (int)(((cur.ps + 1) * runs - 1) / total);            // the CTA of its first unit
+  const int c1 = (int)(((cur.ps + cur.units) * runs - 1) / total);    // and of its last
+  const int pieces = c1 - c0 + 1;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) s_last = atomicAdd(a.done + cur.pair, 1) == pieces - 1;
+  __syncthreads();
+  if (!s_last) continue;
+  __threadfence();
+  const int slot0 = total * c0 / runs >= cur.ps ? 0 : 1;  // the first CTA's run may begin before the head
+  auto piece = [&](int c) { return a.part + ((int64_t)(c0 + c) * 2 + (c == 0 ? slot0 : 0)) * PART; };
+  // a group of D / 4 lanes takes a row, four places a lane
+  constexpr int LPR = D / 4, GROUPS = THREADS / LPR;
+  const int gl = lane % LPR, gbase = lane - gl;
+  const int rounds = (cur.nrows + GROUPS - 1) / GROUPS;
+  for (int k = 0; k < rounds; ++k) {
+    const int r = min(k * GROUPS + (int)threadIdx.x / LPR, cur.nrows - 1);  // beyond the last: that one again
+    float m = NEG_INF, w = NEG_INF, l = 0.0f;
+    for (int c = gl; c < pieces; c += LPR) {
+      const float* p = piece(c) + C::ROWS * D + r;
+      const float mc = __ldcg(p), lc = __ldcg(p + C::ROWS), wc = __ldcg(p + 2 * C::ROWS);
+      const float mn = fmaxf(m, mc), ref = mn == NEG_INF ? 0.0f : mn;
+      l = l * ex2(m - ref) + lc * ex2(mc - ref);
+      m = mn;
+      w = fmaxf(w, wc);
+    }
+#pragma unroll
+    for (int d = LPR / 2; d; d >>= 1) {
+      const float m2 = __shfl_xor_sync(FULL, m, d), l2 = __shfl_xor_sync(FULL, l, d);
+      const float mn = fmaxf(m, m2), ref = mn == NEG_INF ? 0.0f : mn;
+      l = l * ex2(m - ref) + l2 * ex2(m2 - ref);
+      m = mn;
+      w = fmaxf(w, __shfl_xor_sync(FULL, w, d));
+    }
+    const float wr = w == NEG_INF ? 0.0f : w;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int cb = 0; cb < pieces; cb += LPR) {
+      const int c = min(cb + gl, pieces - 1);
+      const float f = ex2(__ldcg(piece(c) + C::ROWS * (D + 2) + r) - wr);
+      const int cn = min(LPR, pieces - cb);
+#pragma unroll 8
+      for (int q = 0; q < cn; ++q) {
+        const float fq = __shfl_sync(FULL, f, gbase + q);
+        const float4 u = __ldcg(reinterpret_cast<const float4*>(piece(cb + q) + r * D) + gl);
+        v.x = fmaf(u.x, fq, v.x), v.y = fmaf(u.y, fq, v.y);
+        v.z = fmaf(u.z, fq, v.z), v.w = fmaf(u.w, fq, v.w);
+      }
+    }
+    const float f = out_scale(m, l, w);
+    // places 4 gl ..: columns D/8 g2 + 2j of g2 = 2 gl % 8 and the next
+    const int j = gl / 4, g2 = 2 * gl % 8;
+    uint16_t* p = out_row(r) + g2 * (D / 8) + 2 * j;
+    *reinterpret_cast<uint32_t*>(p) = bf_pack(v.x * f, v.y * f);
+    *reinterpret_cast<uint32_t*>(p + D / 8) = bf_pack(v.z * f, v.w * f);
+  }
+  // rows of the group that have no query
+  const int blank = min(C::ROWS, a.T * a.G - cur.row0) - cur.nrows;
+  for (int i = threadIdx.x; i < blank * (D / 2); i += THREADS)
+    reinterpret_cast<uint32_t*>(out_row(cur.nrows + i / (D / 2)))[i % (D / 2)] = 0u;
+  if (threadIdx.x == 0) a.done[cur.pair] = 0;
+  }
 }
 
-// How a call's work is cut: keys per chunk (a multiple of 128, at most
-// PAGES_MAX pages), chunks of the longest sequence, row tiles.
+// How a call's work is cut: row tiles of 8, row groups, and CTAs: two per SM,
+// or one per unit where the longest lengths give fewer.
 struct Cut {
-  int nt, groups, chunk, chunks;
+  int nt, groups, ctas;
 };
-Cut cut_of(int64_t batch, int64_t tokens, int heads, int kv_heads, int page, int64_t capacity) {
+Cut cut_of(int64_t batch, int64_t tokens, int heads, int kv_heads, int64_t capacity) {
   Cut c;
   const int64_t rows = tokens * (heads / kv_heads);
   c.nt = rows > 8 ? 2 : 1;
   c.groups = (int)((rows + 8 * c.nt - 1) / (8 * c.nt));
-  const int64_t pairs = batch * kv_heads * c.groups;
-  // about four waves of two CTAs per SM at the longest length, 512 keys or more
-  const int64_t want = std::max<int64_t>(1, (8 * vq::mx::sm_count() + pairs - 1) / pairs);
-  int64_t chunk = std::max<int64_t>(512, (capacity + want - 1) / want);
-  chunk = (chunk + 127) / 128 * 128;
-  chunk = std::min<int64_t>(chunk, 512ll * page);
-  c.chunk = (int)chunk;
-  c.chunks = (int)std::max<int64_t>(1, (capacity + chunk - 1) / chunk);
+  const int64_t units = std::max<int64_t>(1, (capacity + UNIT - 1) / UNIT);
+  c.ctas = (int)std::min<int64_t>(2 * vq::mx::sm_count(), batch * c.groups * kv_heads * units);
   return c;
 }
 
 template <int D, int NT>
-int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, cudaStream_t st) {
+int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int ctas, cudaStream_t st) {
   using C = Cfg<D, NT>;
   static_assert(WARPS * C::STAGES * 8 <= 256, "barrier area");
   if (!allow_smem<k_attn_kv8<D, NT>>(C::SMEM))
     return VQ_ERR_CUDA;
-  k_attn_kv8<D, NT><<<dim3(a.chunks, a.Hkv * a.groups, a.B), THREADS, C::SMEM, st>>>(mk, mv, a);
+  k_attn_kv8<D, NT><<<ctas, THREADS, C::SMEM, st>>>(mk, mv, a);
   return cudaGetLastError() == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
 }
 
@@ -576,10 +761,10 @@ int vq_attn_kv8_workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t 
   if (batch < 0 || tokens < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0 ||
       page <= 0 || table_width < 0)
     return VQ_ERR_INVALID;
-  const Cut c = cut_of(std::max<int64_t>(batch, 1), std::max<int64_t>(tokens, 1), heads, kv_heads, page,
+  const Cut c = cut_of(std::max<int64_t>(batch, 1), std::max<int64_t>(tokens, 1), heads, kv_heads,
                        table_width * page);
   *counters = batch * kv_heads * c.groups;
-  *floats = c.chunks == 1 ? 0 : *counters * c.chunks * 8 * c.nt * (head_dim + 3);
+  *floats = (int64_t)c.ctas * 2 * 8 * c.nt * (head_dim + 3);
   return VQ_OK;
 }
 
@@ -593,7 +778,7 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
   if (page != 32 && page != 64 && page != 128) return VQ_ERR_UNSUPPORTED;
   if (batch < 0 || tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || table_width < 0 ||
       pages < 0 || pages * kv_heads * page >= (1ll << 31) || table_width * page >= (1ll << 31) ||
-      tokens >= (1 << 20) || batch > 65535 || batch * tokens * heads >= (1ll << 31))
+      tokens >= (1 << 20) || batch > (1 << 24) || batch * tokens * heads >= (1ll << 31))
     return VQ_ERR_INVALID;
   if (batch == 0 || tokens == 0) return VQ_OK;
   if (!q || !q_strides || !k_codes || !v_codes || !k_scale || !v_scale || !block_table || !lengths ||
@@ -604,12 +789,10 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
     if (reinterpret_cast<uintptr_t>(p) & 15) return VQ_ERR_ALIGNMENT;
   for (int i = 0; i < 3; ++i)
     if (q_strides[i] % 8) return VQ_ERR_ALIGNMENT;
-  const Cut c = cut_of(batch, tokens, heads, kv_heads, page, table_width * page);
+  const Cut c = cut_of(batch, tokens, heads, kv_heads, table_width * page);
   const int64_t pairs = batch * kv_heads * c.groups;
-  if (c.groups * (int64_t)kv_heads > 65535) return VQ_ERR_INVALID;
-  if (counters_len < pairs) return VQ_ERR_INVALID;
-  if (c.chunks > 1 && (!workspace || workspace_floats < pairs * c.chunks * 8 * c.nt * (head_dim + 3)))
-    return VQ_ERR_INVALID;
+  if (pairs >= (1ll << 31) || counters_len < pairs) return VQ_ERR_INVALID;
+  if (!workspace || workspace_floats < (int64_t)c.ctas * 2 * 8 * c.nt * (head_dim + 3)) return VQ_ERR_INVALID;
   if (pages == 0 || table_width == 0) {  // an empty cache: no row sees a key
     if (table_width) return VQ_ERR_INVALID;
     return cudaMemsetAsync(out, 0, (size_t)(batch * tokens * heads * head_dim * 2),
@@ -633,11 +816,11 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
   a.B = (int)batch, a.T = (int)tokens, a.H = heads, a.Hkv = kv_heads, a.G = heads / kv_heads;
   a.page_log2 = page == 32 ? 5 : page == 64 ? 6 : 7;
   a.width = (int)table_width, a.pages = (int)pages;
-  a.groups = c.groups, a.chunks = c.chunks, a.chunk = c.chunk;
+  a.groups = c.groups;
   a.sm_log2 = sm_scale * 1.4426950408889634f;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (head_dim == 128) return c.nt == 1 ? launch<128, 1>(mk, mv, a, st) : launch<128, 2>(mk, mv, a, st);
-  return c.nt == 1 ? launch<64, 1>(mk, mv, a, st) : launch<64, 2>(mk, mv, a, st);
+  if (head_dim == 128) return c.nt == 1 ? launch<128, 1>(mk, mv, a, c.ctas, st) : launch<128, 2>(mk, mv, a, c.ctas, st);
+  return c.nt == 1 ? launch<64, 1>(mk, mv, a, c.ctas, st) : launch<64, 2>(mk, mv, a, c.ctas, st);
 }
 
 }  // extern "C"

@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(Pair::THREADS, 1)
 template <int BN>
 struct Few {
   static constexpr int W_BYTES = 128 * BK, X_BYTES = BN * BK, STAGE = W_BYTES + X_BYTES;
-  static constexpr int STAGES = BN == 16 ? 5 : BN == 32 ? 4 : BN == 64 ? 4 : 3;
+  static constexpr int STAGES = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : 3;
   static constexpr int BUFS = BN == 128 ? 2 : 4;
   static constexpr int TMEM = BUFS * BN < 32 ? 32 : BUFS * BN;
   static constexpr int THREADS = 192;
@@ -562,11 +562,19 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
   const int tile = blockIdx.x / a.splits, tm = tile / a.nt, tn = tile - tm * a.nt;
   const int kb0 = (int)((int64_t)a.nk * rank / a.splits);
   const int kb1 = (int)((int64_t)a.nk * (rank + 1) / a.splits);
+  auto load = [&](int kt, int stage) {
+    const uint32_t dst = smem_u32(smem) + stage * C::STAGE;
+    mbar_expect_tx(full0 + 8 * stage, C::STAGE);
+    tma_load_2d(dst, &map_w, kt * BK, tn * 128, full0 + 8 * stage);
+    tma_load_2d(dst + C::W_BYTES, &map_x, kt * BK, tm * BN, full0 + 8 * stage);
+  };
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) mbar_init(full0 + 8 * s, 1), mbar_init(empty0 + 8 * s, 1);
     for (int s = 0; s < C::BUFS; ++s) mbar_init(acc_full0 + 8 * s, 1), mbar_init(acc_empty0 + 8 * s, 4);
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    // the ring's first round needs no one's leave
+    for (int i = 0; i < min(C::STAGES, kb1 - kb0); ++i) load(kb0 + i, i);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -580,14 +588,12 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
 
   if (warp == 0) {
     if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int kt = kb0; kt < kb1; ++kt) {
+      const int first = min(C::STAGES, kb1 - kb0);
+      int stage = first == C::STAGES ? 0 : first;
+      uint32_t phase = first == C::STAGES ? 1 : 0;
+      for (int kt = kb0 + first; kt < kb1; ++kt) {
         if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, nullptr, ERR_EMPTY)) break;
-        const uint32_t dst = smem_u32(smem) + stage * C::STAGE;
-        mbar_expect_tx(full0 + 8 * stage, C::STAGE);
-        tma_load_2d(dst, &map_w, kt * BK, tn * 128, full0 + 8 * stage);
-        tma_load_2d(dst + C::W_BYTES, &map_x, kt * BK, tm * BN, full0 + 8 * stage);
+        load(kt, stage);
         if (++stage == C::STAGES) stage = 0, phase ^= 1;
       }
       drain_loads<C::STAGES>(full0, stage, phase);
@@ -628,13 +634,22 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
     for (int i = 0; i < BN; ++i) acc[i] = 0.0f;
     bool ok = true;
     for (int kc = kb0; kc < kb1; kc += C::KC) {
-      // the scales of the next KC blocks, sa * sw per block and token
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      // the scales of the next KC blocks, sa * sw per block and token, all
+      // loads in flight together (one at a time they cost 10 us at 128 tokens)
       const int n = min(C::KC, kb1 - kc);
-      for (int i = pt; i < C::KC * BN; i += 128) {
-        const int j = i / C::KC, k = i % C::KC;  // consecutive threads: consecutive blocks of a token
+      constexpr int PER = C::KC * BN / 128;
+      float sv[PER];
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        const int i = pt + u * 128, j = i / C::KC, k = min(i % C::KC, n - 1);
         const int m = min(tm * BN + j, a.M - 1);
-        if (k < n) s_scale[k * BN + j] = __ldg(a.sa + (int64_t)m * a.nk + kc + k) * __ldg(sw + kc + k);
+        sv[u] = __ldg(a.sa + (int64_t)m * a.nk + kc + k) * __ldg(sw + kc + k);
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+      for (int u = 0; u < PER; ++u) {
+        const int i = pt + u * 128;
+        s_scale[i % C::KC * BN + i / C::KC] = sv[u];
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");
       for (int k = 0; k < n && ok; ++k) {
@@ -685,15 +700,21 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
     const int j = (i >> 5) * a.splits + rank, f = (i & 31) * 4, n = tn * 128 + f;
     if (j >= ntok) break;
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int r = 0; r < a.splits; ++r) {
-      float x[4];
-      const uint32_t p = red_addr + (j * C::LD + f) * 4;
-      const uint32_t src = a.splits > 1 ? mapa_shared(p, r) : p;
-      asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-                   : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(src) : "memory");
+    const uint32_t p = red_addr + (j * C::LD + f) * 4;
+    float x[8][4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] += x[k];
-    }
+    for (int r = 0; r < 8; ++r)
+      if (r < a.splits) {
+        const uint32_t src = a.splits > 1 ? mapa_shared(p, r) : p;
+        asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                     : "=f"(x[r][0]), "=f"(x[r][1]), "=f"(x[r][2]), "=f"(x[r][3]) : "r"(src) : "memory");
+      }
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+      if (r < a.splits) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += x[r][k];
+      }
     uint16_t* o = a.out + (int64_t)(tm * BN + j) * a.ldo + n;
     if (a.bias) {
 #pragma unroll
@@ -752,6 +773,34 @@ int launch_many(const void* x, const void* w, int64_t K, Args a, cudaStream_t st
   return cudaGetLastError() == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
 }
 
+// Clusters of s CTAs of k_fp8_few<BN> that the device holds at once (asked
+// once per device and size).
+template <int BN>
+int resident_clusters(int s) {
+  static int known[64][9] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  dev = dev < 0 || dev > 63 ? 0 : dev;
+  if (known[dev][s] == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(s);
+    cfg.blockDim = dim3(Few<BN>::THREADS);
+    cfg.dynamicSmemBytes = Few<BN>::SMEM;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = s, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, k_fp8_few<BN>, &cfg) != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      n = std::max(1, 2 * vq::mx::sm_count() / s);
+    }
+    known[dev][s] = n;
+  }
+  return known[dev][s];
+}
+
 template <int BN>
 int launch_few(const void* x, const void* w, int64_t K, Args a, cudaStream_t st) {
   using C = Few<BN>;
@@ -763,13 +812,16 @@ int launch_few(const void* x, const void* w, int64_t K, Args a, cudaStream_t st)
   a.mt = (a.M + BN - 1) / BN;
   a.nt = (a.N + 127) / 128;
   a.tiles = a.mt * a.nt;
-  // K split so that the waves of two CTAs per SM take least: blocks per CTA,
-  // plus a constant 6 for a CTA's start and the join
-  const int slots = 2 * vq::mx::sm_count();
+  // K split so that the waves of resident clusters take least: blocks per
+  // CTA, plus a constant 6 for a CTA's start and the join.  How many clusters
+  // of a size are resident at once is asked of the runtime: clusters of 3, for
+  // one, do not fill the 2 * 148 places (288 CTAs in two waves took 18 us, 15
+  // in one).
   int best = 1;
   int64_t cost = 1ll << 60;
   for (int s = 1; s <= 8 && s <= a.nk; ++s) {
-    const int64_t c = ((int64_t)a.tiles * s + slots - 1) / slots * ((a.nk + s - 1) / s + 6);
+    const int64_t res = resident_clusters<BN>(s);
+    const int64_t c = (a.tiles + res - 1) / res * ((a.nk + s - 1) / s + 6);
     if (c < cost) cost = c, best = s;
   }
   a.splits = best;

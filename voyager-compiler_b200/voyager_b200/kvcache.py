@@ -251,10 +251,10 @@ def attend(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lengths: 
     out = q.new_empty(shape)
     floats, n = _workspace_sizes(index, B, T, H, Hkv, D, page, width)
     done = _join_counters(q, index, n)
-    part = q.new_empty(floats, dtype=torch.float32) if floats else None
+    part = q.new_empty(floats, dtype=torch.float32)
     call(_lib.load().vq_attn_kv8, index, what, q.data_ptr(), _I64x3(qb, qt, qh), B, T, H, Hkv, D,
          cache.k_codes.data_ptr(), cache.v_codes.data_ptr(), cache.k_scale.data_ptr(),
          cache.v_scale.data_ptr(), pages, page, bt, width, held, new,
-         1.0 / math.sqrt(D) if scale is None else scale, part.data_ptr() if floats else None, floats,
+         1.0 / math.sqrt(D) if scale is None else scale, part.data_ptr(), floats,
          done.data_ptr(), done.numel(), out.data_ptr())
     return out
