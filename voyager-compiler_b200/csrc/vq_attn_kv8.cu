@@ -52,6 +52,7 @@ using namespace vq::tc;
 enum { ERR_WAIT = 311, ERR_PAGE = 312, ERR_CAPACITY = 313, ERR_COUNT = 314 };
 
 constexpr int WARPS = 4, THREADS = WARPS * 32, TILE = 32, UNIT = WARPS * TILE;
+constexpr int PLANS = 256;
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr float P_EXP = 15.0f;  // the largest weight is 2^15 in f16
 
@@ -80,7 +81,7 @@ struct Cfg {
   static constexpr int JOIN = (SUMS * ROWS * LD + 3 * WARPS * ROWS + 4 * ROWS) * 4;
   static constexpr int SMEM = SMEM_RING + JOIN + 1024 + 256;
   static_assert(JOIN % 16 == 0 && WARPS * STAGES * 8 <= 256, "barriers after the join's area");
-  static_assert(2 * (SMEM + 1024 + 256) <= 227 * 1024, "two CTAs per SM");
+  static_assert(2 * (SMEM + 4096) <= 227 * 1024, "two CTAs per SM");
 };
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -133,29 +134,33 @@ __device__ __forceinline__ float out_scale(float m, float l, float w) {
   return l == 0.0f || w == NEG_INF ? 0.0f : __fdiv_rn(ex2(w - P_EXP - m), l);
 }
 
+// A sequence's tokens held and new tokens, brought to what fits.
+__device__ __forceinline__ int2 plan_of(const Args& a, int b, bool report) {
+  int held = a.lengths[b], cnt = a.counts ? a.counts[b] : a.T;
+  if (held < 0 || cnt < 0 || cnt > a.T) {
+    if (report) note_err(nullptr, ERR_COUNT);
+    cnt = held < 0 ? 0 : min(max(cnt, 0), a.T);
+    held = max(held, 0);
+  }
+  const int64_t cap = (int64_t)a.width << a.page_log2;
+  if (held + (int64_t)cnt > cap) {
+    if (report) note_err(nullptr, ERR_CAPACITY);
+    cnt = held >= cap ? 0 : (int)(cap - held);
+  }
+  return make_int2(held, cnt);
+}
 // Entry e = (sequence, row group): the rows of it that have a query, the
 // tokens held, and the keys that some of its rows sees.
 struct Entry {
   int b, row0, nrows, held, end;
 };
 template <int ROWS>
-__device__ __forceinline__ Entry entry_of(const Args& a, int e, bool report) {
+__device__ __forceinline__ Entry entry_of(const Args& a, int e, int2 plan) {
   Entry x;
   x.b = e / a.groups;
   x.row0 = (e - x.b * a.groups) * ROWS;
-  x.held = a.lengths[x.b];
-  int cnt = a.counts ? a.counts[x.b] : a.T;
-  if (x.held < 0 || cnt < 0 || cnt > a.T) {
-    if (report) note_err(nullptr, ERR_COUNT);
-    cnt = x.held < 0 ? 0 : min(max(cnt, 0), a.T);
-    x.held = max(x.held, 0);
-  }
-  const int64_t cap = (int64_t)a.width << a.page_log2;
-  if (x.held + (int64_t)cnt > cap) {
-    if (report) note_err(nullptr, ERR_CAPACITY);
-    cnt = x.held >= cap ? 0 : (int)(cap - x.held);
-  }
-  x.nrows = min(ROWS, cnt * a.G - x.row0);
+  x.held = plan.x;
+  x.nrows = min(ROWS, plan.y * a.G - x.row0);
   x.end = x.nrows > 0 ? x.held + (x.row0 + x.nrows - 1) / a.G + 1 : 0;
   return x;
 }
@@ -172,8 +177,9 @@ __global__ void __launch_bounds__(THREADS)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~(uintptr_t)1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::SMEM_RING + C::JOIN);  // [WARPS][STAGES]
-  __shared__ int s_last, s_entry;
-  __shared__ long long s_sum[WARPS], s_before;
+  __shared__ int s_last, s_entry, s_before;
+  __shared__ long long s_sum[WARPS];
+  __shared__ int2 s_plan[PLANS];  // the first sequences' plans
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (lane == 0) {
@@ -182,13 +188,19 @@ __global__ void __launch_bounds__(THREADS)
   }
 
   // ---- this CTA's run of units: a scan of the entries' unit counts (and, in
-  // the bits from 40 on, of the entries that have any) ----
+  // the upper 32 bits, of the entries that have any) ----
+  for (int b = threadIdx.x; b < min(a.B, PLANS); b += THREADS) s_plan[b] = plan_of(a, b, blockIdx.x == 0);
+  __syncthreads();
+  auto entry = [&](int e) {
+    const int b = e / a.groups;
+    return entry_of<C::ROWS>(a, e, b < PLANS ? s_plan[b] : plan_of(a, b, blockIdx.x == 0));
+  };
   const int entries = a.B * a.groups, per = (entries + THREADS - 1) / THREADS;
   const int e0 = min(entries, (int)threadIdx.x * per), e1 = min(entries, e0 + per);
   long long own = 0;
   for (int e = e0; e < e1; ++e) {
-    const int u = units_of(entry_of<C::ROWS>(a, e, blockIdx.x == 0));
-    own += u ? u + (1ll << 40) : 0;
+    const int u = units_of(entry(e));
+    own += u ? u + (1ll << 32) : 0;
   }
   long long sum = own;
 #pragma unroll
@@ -204,57 +216,56 @@ __global__ void __launch_bounds__(THREADS)
     if (w < warp) before += s_sum[w];
     total += s_sum[w];
   }
-  const int active = (int)(total >> 40);
-  constexpr long long LOW = (1ll << 40) - 1;
-  total = (total & LOW) * a.Hkv;
-  before = (before & LOW) * a.Hkv;
-  own = (own & LOW) * a.Hkv;
   // CTAs with work.  A piece more of a head costs its join about an eighth of
   // a unit's time, so a run is at least sqrt(units / 8) of an average head.
-  const float avg = active ? (float)total / ((float)active * a.Hkv) : 1.0f;
-  const int runs = (int)min((long long)gridDim.x, (long long)ceilf((float)total / fmaxf(1.0f, sqrtf(avg * 0.125f))));
-  const long long lo = runs ? total * blockIdx.x / runs : 0, hi = runs ? total * (blockIdx.x + 1) / runs : 0;
-  if ((int)blockIdx.x < runs && before <= lo && lo < before + own) {
-    long long at = before;
-    for (int e = e0; e < e1; ++e) {
-      const long long u = (long long)units_of(entry_of<C::ROWS>(a, e, false)) * a.Hkv;
-      if (lo < at + u) {
-        s_entry = e;
-        s_before = at;
-        break;
+  // A head counts HEAD units more than it has where runs span heads: opening,
+  // joining and closing one takes that long.
+  const int heads = (int)(total >> 32) * a.Hkv, real = (int)total * a.Hkv;
+  const float least = heads ? fmaxf(1.0f, sqrtf(0.125f * (float)real / (float)heads)) : 1.0f;
+  const int runs = min((int)gridDim.x, (int)ceilf((float)real / least));
+  const int HEAD = 2 * heads >= runs ? 4 : 0;
+  const int all = real + HEAD * heads;
+  const int base = runs ? all / runs : 0, rest = all - base * runs;  // the first `rest` runs have one more
+  auto run_of = [&](int at) {  // the run that holds this unit
+    return at < rest * (base + 1) ? at / (base + 1) : rest + (at - rest * (base + 1)) / base;
+  };
+  auto run_begin = [&](int c) { return c * base + min(c, rest); };
+  const int lo = run_begin(blockIdx.x), hi = run_begin(blockIdx.x + 1);
+  {
+    int at = ((int)before + HEAD * (int)(before >> 32)) * a.Hkv;
+    const int to = at + ((int)own + HEAD * (int)(own >> 32)) * a.Hkv;
+    if ((int)blockIdx.x < runs && at <= lo && lo < to)
+      for (int e = e0; e < e1; ++e) {
+        const int u = units_of(entry(e)), next = at + (u ? (u + HEAD) * a.Hkv : 0);
+        if (lo < next) {
+          s_entry = e;
+          s_before = at;
+          break;
+        }
+        at = next;
       }
-      at += u;
-    }
-  }
-  // row groups without a query are written here: no unit belongs to them
-  for (int e = blockIdx.x; e < entries; e += gridDim.x) {
-    const Entry x = entry_of<C::ROWS>(a, e, false);
-    if (x.nrows > 0) continue;
-    const int rows = min(C::ROWS, a.T * a.G - x.row0);
-    for (int i = threadIdx.x; i < rows * a.Hkv * (D / 8); i += THREADS) {
-      const int row = x.row0 + i / (D / 8) % rows, h = i / (D / 8) / rows;
-      reinterpret_cast<uint4*>(a.out + (((int64_t)x.b * a.T + row / a.G) * a.H + h * a.G + row % a.G) * D)
-          [i % (D / 8)] = make_uint4(0, 0, 0, 0);
-    }
   }
   __syncthreads();
-  if ((int)blockIdx.x >= runs) return;
 
   const uint32_t ring = smem_u32(smem) + warp * C::RING;
   const uint32_t bar0 = smem_u32(bars + warp * C::STAGES);
   int stage = 0;      // of the next tile to read; the ring runs on from segment to segment
   uint32_t phase = 0;
   bool ok = true;
-  long long pos = lo, ebase = s_before;
+  int pos = lo, ebase = s_before;
   int e = s_entry;
-  Entry x = entry_of<C::ROWS>(a, e, false);
-  int units = units_of(x);
+  Entry x = {};
+  int units = 0;
+  if ((int)blockIdx.x < runs) {
+    x = entry(e);
+    units = units_of(x);
+  }
 
   // A segment: the part of one head (entry, kv head) in this run.
   struct Seg {
     int b, row0, nrows, held, end, kvh, k0, k1, units, slot, pair;
+    int ps;  // where the head begins
     bool whole;
-    long long ps;  // the head's first unit
   } sg = {};
   // A lane knows the page of tile 32 m + lane of the warp's tiles: its row in
   // the cache and its scales, n_ for the batch m that is being issued, c_ for
@@ -286,60 +297,85 @@ __global__ void __launch_bounds__(THREADS)
     ++issued;
     if (++wstage == C::STAGES) wstage = 0;
   };
-  // The next segment, and its first loads on their way.
+  // The next segment; start() puts its first loads on their way.
   auto open = [&]() {
-    while (pos >= ebase + (long long)units * a.Hkv) {  // the next entry with keys
-      ebase += (long long)units * a.Hkv;
-      x = entry_of<C::ROWS>(a, ++e, false);
+    while (units == 0 || pos >= ebase + (units + HEAD) * a.Hkv) {  // the next entry with keys
+      if (units) ebase += (units + HEAD) * a.Hkv;
+      x = entry(++e);
       units = units_of(x);
     }
     sg.b = x.b, sg.row0 = x.row0, sg.nrows = x.nrows, sg.held = x.held, sg.end = x.end, sg.units = units;
-    sg.kvh = (int)((pos - ebase) / units);
+    sg.kvh = (pos - ebase) / (units + HEAD);
     sg.pair = e * a.Hkv + sg.kvh;
-    sg.ps = ebase + (long long)sg.kvh * units;
-    const int u0 = (int)(pos - sg.ps), u1 = (int)min((long long)units, hi - sg.ps);
+    sg.ps = ebase + sg.kvh * (units + HEAD);
+    const int u0 = max(0, pos - sg.ps - HEAD), u1 = min(units, hi - sg.ps - HEAD);
     sg.whole = u0 == 0 && u1 == units;
     sg.slot = pos == lo ? 0 : 1;
+    pos = min(hi, sg.ps + HEAD + units);
+    if (u1 <= 0) return false;  // the run ends within the head's extra units
     sg.k0 = u0 * UNIT, sg.k1 = min(x.end, u1 * UNIT);
     const int ntiles = (sg.k1 - sg.k0 + TILE - 1) / TILE;
     // tiles warp, warp + 4, ..; none after a wait that gave up
     mine = ok && ntiles > warp ? (ntiles - warp + WARPS - 1) / WARPS : 0;
     issued = 0;
     wstage = stage;
-    if (mine > 0) {
-      pid_next = pid_of(lane);
-      for (int i = 0; i < min(mine, C::STAGES); ++i) issue();
-    }
-    pos = sg.ps + u1;
+    if (mine > 0) pid_next = pid_of(lane);
+    return true;
   };
-  open();
+  auto start = [&]() {
+    for (int i = 0; i < min(mine, C::STAGES); ++i) issue();
+  };
+  // The queries of the segment as they lie in memory: lane (g, t) takes row
+  // g's columns D/4 * t ...
+  uint32_t qw[NT][D / 8];
+  auto load_q = [&]() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = sg.row0 + n * 8 + g;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) qw[n][i] = 0;
+      if (r < sg.row0 + sg.nrows) {
+        const uint16_t* p = a.q + (int64_t)sg.b * a.qb + (int64_t)(r / a.G) * a.qt +
+                            (int64_t)(sg.kvh * a.G + r % a.G) * a.qh + t * (D / 4);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+          qw[n][4 * i] = v.x, qw[n][4 * i + 1] = v.y, qw[n][4 * i + 2] = v.z, qw[n][4 * i + 3] = v.w;
+        }
+      }
+    }
+  };
+  bool more = (int)blockIdx.x < runs && open();
+  if (more) {
+    load_q();  // under the block table's latency
+    start();
+  }
+  // row groups without a query are written here: no unit belongs to them
+  for (int e = blockIdx.x; e < entries; e += gridDim.x) {
+    const Entry x = entry(e);
+    if (x.nrows > 0) continue;
+    const int rows = min(C::ROWS, a.T * a.G - x.row0);
+    for (int i = threadIdx.x; i < rows * a.Hkv * (D / 8); i += THREADS) {
+      const int row = x.row0 + i / (D / 8) % rows, h = i / (D / 8) / rows;
+      reinterpret_cast<uint4*>(a.out + (((int64_t)x.b * a.T + row / a.G) * a.H + h * a.G + row % a.G) * D)
+          [i % (D / 8)] = make_uint4(0, 0, 0, 0);
+    }
+  }
 
-  for (bool more = true; more;) {
-  const int b = sg.b, row0 = sg.row0, nrows = sg.nrows, held = sg.held, end = sg.end, kvh = sg.kvh, k0 = sg.k0;
+  for (bool first = true; more; first = false) {
+  if (!first) load_q();
+  const int row0 = sg.row0, held = sg.held, end = sg.end, k0 = sg.k0;
 
-  // Q as the second operand of S^T = K Q^T.  Lane (g, t) holds row g's
-  // columns D/4 * t ..: k step w takes its 4 columns D/4 * t + 4 w ...
+  // Q as the second operand of S^T = K Q^T: k step w takes the lane's 4
+  // columns D/4 * t + 4 w ...
   uint32_t qf[NT][KS][2];
   float qs[NT];  // the power of two taken out of row g's query
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    const int r = row0 + n * 8 + g;
-    uint32_t w[D / 8];
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) w[i] = 0;
-    if (r < row0 + nrows) {
-      const uint16_t* p = a.q + (int64_t)b * a.qb + (int64_t)(r / a.G) * a.qt +
-                          (int64_t)(kvh * a.G + r % a.G) * a.qh + t * (D / 4);
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
-        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-      }
-    }
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) {
-      const uint32_t v = w[i] & 0x7FFF7FFFu;
+      const uint32_t v = qw[n][i] & 0x7FFF7FFFu;
       m = max(m, max(v & 0xFFFFu, v >> 16));
     }
     m = max(m, __shfl_xor_sync(FULL, m, 1));
@@ -349,7 +385,7 @@ __global__ void __launch_bounds__(THREADS)
     qs[n] = __uint_as_float((uint32_t)(e - 14) << 23);
 #pragma unroll
     for (int i = 0; i < D / 8; ++i)
-      qf[n][i >> 1][i & 1] = f16x2(bf_lo(w[i]) * up, bf_hi(w[i]) * up);
+      qf[n][i >> 1][i & 1] = f16x2(bf_lo(qw[n][i]) * up, bf_hi(qw[n][i]) * up);
   }
   // for the scores' columns 2t, 2t + 1 of each row tile: the query's factor
   // and the last key the row sees (rows without a query are not written)
@@ -556,8 +592,8 @@ __global__ void __launch_bounds__(THREADS)
   }
 
   const Seg cur = sg;
-  more = pos < hi;
-  if (more) open();  // its loads run under the join
+  more = pos < hi && open();
+  if (more) start();  // its loads run under the join
 
   // ---- join the warps ----
   float* sums = reinterpret_cast<float*>(smem + C::SMEM_RING);  // [SUMS][ROWS][LD]
@@ -657,24 +693,33 @@ __global__ void __launch_bounds__(THREADS)
   }
   if (threadIdx.x < 3 * C::ROWS) piece_out[C::ROWS * D + threadIdx.x] = fin[threadIdx.x];
   // the CTA that finishes last reads the head's pieces in the CTAs' order
-  const int c0 = (int)(((cur.ps + 1) * runs - 1) / total);            // the CTA of its first unit
-  const int c1 = (int)(((cur.ps + cur.units) * runs - 1) / total);    // and of its last
+  const int c0 = run_of(cur.ps + HEAD), c1 = run_of(cur.ps + HEAD + cur.units - 1);  // of its first unit and its last
   const int pieces = c1 - c0 + 1;
-  __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) s_last = atomicAdd(a.done + cur.pair, 1) == pieces - 1;
+  if (threadIdx.x == 0) {
+    __threadfence();  // after the barrier: for every thread's stores
+    s_last = atomicAdd(a.done + cur.pair, 1) == pieces - 1;
+    __threadfence();
+  }
   __syncthreads();
   if (!s_last) continue;
-  __threadfence();
-  const int slot0 = total * c0 / runs >= cur.ps ? 0 : 1;  // the first CTA's run may begin before the head
+  const int slot0 = run_begin(c0) >= cur.ps ? 0 : 1;  // the first CTA's run may begin before the head
   auto piece = [&](int c) { return a.part + ((int64_t)(c0 + c) * 2 + (c == 0 ? slot0 : 0)) * PART; };
-  // a group of D / 4 lanes takes a row, four places a lane
-  constexpr int LPR = D / 4, GROUPS = THREADS / LPR;
+  // a group of D / 8 lanes takes a row, eight places a lane
+  constexpr int LPR = D / 8, GROUPS = THREADS / LPR, PRE = 8;
   const int gl = lane % LPR, gbase = lane - gl;
   const int rounds = (cur.nrows + GROUPS - 1) / GROUPS;
   for (int k = 0; k < rounds; ++k) {
     const int r = min(k * GROUPS + (int)threadIdx.x / LPR, cur.nrows - 1);  // beyond the last: that one again
-    float m = NEG_INF, w = NEG_INF, l = 0.0f;
+    // the first pieces' values travel with the maxima
+    float4 pre[PRE][2];
+    auto fetch = [&](int c, float4 (&u)[2]) {
+      const float4* p = reinterpret_cast<const float4*>(piece(c) + r * D) + gl;
+      u[0] = __ldcg(p), u[1] = __ldcg(p + LPR);
+    };
+#pragma unroll
+    for (int q = 0; q < PRE; ++q) fetch(min(q, pieces - 1), pre[q]);
+    float m = NEG_INF, w = NEG_INF, l = 0.0f, w0 = NEG_INF;
     for (int c = gl; c < pieces; c += LPR) {
       const float* p = piece(c) + C::ROWS * D + r;
       const float mc = __ldcg(p), lc = __ldcg(p + C::ROWS), wc = __ldcg(p + 2 * C::ROWS);
@@ -682,6 +727,7 @@ __global__ void __launch_bounds__(THREADS)
       l = l * ex2(m - ref) + lc * ex2(mc - ref);
       m = mn;
       w = fmaxf(w, wc);
+      if (c == gl) w0 = wc;
     }
 #pragma unroll
     for (int d = LPR / 2; d; d >>= 1) {
@@ -692,25 +738,35 @@ __global__ void __launch_bounds__(THREADS)
       w = fmaxf(w, __shfl_xor_sync(FULL, w, d));
     }
     const float wr = w == NEG_INF ? 0.0f : w;
-    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int cb = 0; cb < pieces; cb += LPR) {
-      const int c = min(cb + gl, pieces - 1);
-      const float f = ex2(__ldcg(piece(c) + C::ROWS * (D + 2) + r) - wr);
-      const int cn = min(LPR, pieces - cb);
-#pragma unroll 8
-      for (int q = 0; q < cn; ++q) {
-        const float fq = __shfl_sync(FULL, f, gbase + q);
-        const float4 u = __ldcg(reinterpret_cast<const float4*>(piece(cb + q) + r * D) + gl);
-        v.x = fmaf(u.x, fq, v.x), v.y = fmaf(u.y, fq, v.y);
-        v.z = fmaf(u.z, fq, v.z), v.w = fmaf(u.w, fq, v.w);
+    float v[8] = {};
+    auto add = [&](const float4 (&u)[2], float f) {
+      v[0] = fmaf(u[0].x, f, v[0]), v[1] = fmaf(u[0].y, f, v[1]), v[2] = fmaf(u[0].z, f, v[2]);
+      v[3] = fmaf(u[0].w, f, v[3]), v[4] = fmaf(u[1].x, f, v[4]), v[5] = fmaf(u[1].y, f, v[5]);
+      v[6] = fmaf(u[1].z, f, v[6]), v[7] = fmaf(u[1].w, f, v[7]);
+    };
+    float f = ex2(w0 - wr);  // of piece gl
+    for (int cb = 0; cb < pieces; cb += PRE) {
+      if (cb) {
+#pragma unroll
+        for (int q = 0; q < PRE; ++q) fetch(min(cb + q, pieces - 1), pre[q]);
+        if (cb % LPR == 0) f = ex2(__ldcg(piece(min(cb + gl, pieces - 1)) + C::ROWS * (D + 2) + r) - wr);
+      }
+#pragma unroll
+      for (int q = 0; q < PRE; ++q) {
+        const float fq = __shfl_sync(FULL, f, gbase + (cb + q) % LPR);
+        if (cb + q < pieces) add(pre[q], fq);
       }
     }
-    const float f = out_scale(m, l, w);
-    // places 4 gl ..: columns D/8 g2 + 2j of g2 = 2 gl % 8 and the next
-    const int j = gl / 4, g2 = 2 * gl % 8;
-    uint16_t* p = out_row(r) + g2 * (D / 8) + 2 * j;
-    *reinterpret_cast<uint32_t*>(p) = bf_pack(v.x * f, v.y * f);
-    *reinterpret_cast<uint32_t*>(p + D / 8) = bf_pack(v.z * f, v.w * f);
+    f = out_scale(m, l, w);
+    // places 4 gl .. and D/2 + 4 gl ..: columns D/8 g2 + 2j of g2 = 2 gl % 8
+    // and the next, j = gl / 4 and D/32 more
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int j = gl / 4 + h * (D / 32), g2 = 2 * gl % 8;
+      uint16_t* p = out_row(r) + g2 * (D / 8) + 2 * j;
+      *reinterpret_cast<uint32_t*>(p) = bf_pack(v[4 * h] * f, v[4 * h + 1] * f);
+      *reinterpret_cast<uint32_t*>(p + D / 8) = bf_pack(v[4 * h + 2] * f, v[4 * h + 3] * f);
+    }
   }
   // rows of the group that have no query
   const int blank = min(C::ROWS, a.T * a.G - cur.row0) - cur.nrows;
@@ -791,7 +847,9 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
     if (q_strides[i] % 8) return VQ_ERR_ALIGNMENT;
   const Cut c = cut_of(batch, tokens, heads, kv_heads, table_width * page);
   const int64_t pairs = batch * kv_heads * c.groups;
-  if (pairs >= (1ll << 31) || counters_len < pairs) return VQ_ERR_INVALID;
+  // the units of all heads, counted in 32 bits
+  if (pairs * ((table_width * page + UNIT - 1) / UNIT + 8) >= (1ll << 31) || counters_len < pairs)
+    return VQ_ERR_INVALID;
   if (!workspace || workspace_floats < (int64_t)c.ctas * 2 * 8 * c.nt * (head_dim + 3)) return VQ_ERR_INVALID;
   if (pages == 0 || table_width == 0) {  // an empty cache: no row sees a key
     if (table_width) return VQ_ERR_INVALID;
