@@ -61,6 +61,14 @@ __device__ __forceinline__ float block_scale(uint32_t m) {
   return m ? __fdiv_rn(__uint_as_float(m), QMAX) : 1.0f;
 }
 
+// y / s as y * (1 / s): within 1.5 float32 roundings of the quotient, which
+// moves a code only where the quotient lies that near a tie (16 divisions a
+// thread took a quarter of the kernel's time).  Where 1 / s could overflow
+// the division itself.
+__device__ __forceinline__ float quotient(float y, float s, float inv) {
+  return s < 0x1p-126f ? __fdiv_rn(y, s) : y * inv;
+}
+
 // One CTA per row, NV groups of 8 consecutive elements per thread; columns a
 // multiple of 8, rows 16-byte aligned.  A block of 128 columns is 16
 // neighbouring lanes.
@@ -111,9 +119,10 @@ __global__ void __launch_bounds__(1024) k_norm_vec(const Args a) {
     for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(FULL, m, d));
     if (c < a.cols) {
       const float s = block_scale(m);
+      const float inv_s = __fdiv_rn(1.0f, s);
       float q[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) q[k] = __fdiv_rn(h[i][k], s);
+      for (int k = 0; k < 8; ++k) q[k] = quotient(h[i][k], s, inv_s);
       *reinterpret_cast<uint2*>(a.codes + row * a.cols + c) =
           make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
       if ((threadIdx.x & 15) == 0) a.scale[row * a.nblk + (c >> 7)] = s;
@@ -121,8 +130,110 @@ __global__ void __launch_bounds__(1024) k_norm_vec(const Args a) {
   }
 }
 
-// Any number of columns and any alignment: one CTA per row, one warp per 128
-// columns, element loads; the row is read again for the quantization.
+// Columns that are no multiple of 8, or rows off 16 bytes: one CTA per row, a
+// warp takes NB blocks of 128 columns, VEC neighbouring elements a load (2
+// where rows keep the pairs aligned).  The values stay in registers, and with
+// NB = 4 a lane has 16 loads of x in flight (4 passes of one block each over
+// the row, read twice, took 60 us for 7158 x 1630 bf16 with a residual).
+template <typename T, int VEC>
+__device__ __forceinline__ void load_v(const typename T::type* p, float (&v)[VEC]) {
+  if (VEC == 1) {
+    v[0] = T::load(p);
+  } else if (sizeof(*p) == 2) {
+    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(p));
+    v[0] = bf_lo(w), v[VEC - 1] = bf_hi(w);
+  } else {
+    const float2 f = __ldg(reinterpret_cast<const float2*>(p));
+    v[0] = f.x, v[VEC - 1] = f.y;
+  }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_v(typename T::type* p, const float (&v)[VEC]) {
+  if (VEC == 1)
+    T::store(p, v[0]);
+  else if (sizeof(*p) == 2)
+    *reinterpret_cast<uint32_t*>(p) = bf_pack(v[0], v[VEC - 1]);
+  else
+    *reinterpret_cast<float2*>(p) = make_float2(v[0], v[VEC - 1]);
+}
+template <typename T, int NB, int VEC>
+__global__ void __launch_bounds__(1024) k_norm_blocks(const Args a) {
+  using E = typename T::type;
+  constexpr int PER = 4 / VEC;  // loads of a lane per block
+  __shared__ float part[32];
+  const int64_t row = blockIdx.x;
+  const E* x = reinterpret_cast<const E*>(a.x) + row * a.ldx;
+  const E* r = reinterpret_cast<const E*>(a.r) + row * a.ldr;
+  const E* w = reinterpret_cast<const E*>(a.w);
+  E* hid = reinterpret_cast<E*>(a.hidden) + row * a.cols;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c0 = warp * NB * 128 + lane * VEC;
+  float h[NB * PER][VEC];
+#pragma unroll
+  for (int i = 0; i < NB * PER; ++i) {
+    const int c = c0 + i * 32 * VEC;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) h[i][k] = 0.0f;
+    if (c < a.cols) load_v<T, VEC>(x + c, h[i]);
+  }
+  if (a.r) {
+    float q[NB * PER][VEC];
+#pragma unroll
+    for (int i = 0; i < NB * PER; ++i)
+      if (c0 + i * 32 * VEC < a.cols) load_v<T, VEC>(r + c0 + i * 32 * VEC, q[i]);
+#pragma unroll
+    for (int i = 0; i < NB * PER; ++i)
+      if (c0 + i * 32 * VEC < a.cols) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) h[i][k] += q[i][k];
+        store_v<T, VEC>(hid + c0 + i * 32 * VEC, h[i]);
+      }
+  }
+  if (a.w) {
+    float g[NB * PER][VEC];
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NB * PER; ++i) {
+      if (c0 + i * 32 * VEC < a.cols) load_v<T, VEC>(w + c0 + i * 32 * VEC, g[i]);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) ss = fmaf(h[i][k], h[i][k], ss);
+    }
+    const float inv = rsqrtf(__fdiv_rn(block_sum(ss, part), (float)a.cols) + a.eps);
+#pragma unroll
+    for (int i = 0; i < NB * PER; ++i)
+      if (c0 + i * 32 * VEC < a.cols) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) h[i][k] = h[i][k] * inv * g[i][k];
+      }
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) m = max(m, mag(h[b * PER + i][k]));
+    m = __reduce_max_sync(FULL, m);
+    const float s = block_scale(m);
+    const float inv_s = __fdiv_rn(1.0f, s);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int c = c0 + (b * PER + i) * 32 * VEC;
+      if (c < a.cols) {
+        const uint32_t q = pack2(quotient(h[b * PER + i][0], s, inv_s), quotient(h[b * PER + i][VEC - 1], s, inv_s));
+        if (VEC == 1)
+          a.codes[row * a.cols + c] = (uint8_t)q;
+        else
+          *reinterpret_cast<uint16_t*>(a.codes + row * a.cols + c) = (uint16_t)q;
+      }
+    }
+    const int blk = warp * NB + b;
+    if (lane == 0 && blk < a.nblk) a.scale[row * a.nblk + blk] = s;
+  }
+}
+
+// Rows too long for that: one warp per 128 columns at a time, element loads;
+// the row is read again for the quantization.
 template <typename T>
 __global__ void __launch_bounds__(1024) k_norm_any(const Args a) {
   using E = typename T::type;
@@ -160,31 +271,52 @@ __global__ void __launch_bounds__(1024) k_norm_any(const Args a) {
     }
     m = __reduce_max_sync(FULL, m);
     const float s = block_scale(m);
+    const float inv_s = __fdiv_rn(1.0f, s);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = b * 128 + j * 32 + lane;
-      if (c < a.cols) a.codes[row * a.cols + c] = (uint8_t)pack2(__fdiv_rn(y[j], s), 0.0f);
+      if (c < a.cols) a.codes[row * a.cols + c] = (uint8_t)pack2(quotient(y[j], s, inv_s), 0.0f);
     }
     if (lane == 0) a.scale[row * a.nblk + b] = s;
   }
 }
 
-template <typename T>
-void launch(const Args& a, bool vec, cudaStream_t st) {
-  const int groups = (a.cols + 7) / 8;
-  if (!vec || groups > 4096) {
-    k_norm_any<T><<<(unsigned)a.rows, std::min(1024, std::max(32, a.nblk * 32)), 0, st>>>(a);
-    return;
-  }
-  int nv = 1;
-  while (groups > nv * 256 && nv < 4) nv *= 2;
-  const int threads = std::min(1024, ((groups + nv - 1) / nv + 31) / 32 * 32);
-  if (nv == 1)
-    k_norm_vec<T, 1><<<(unsigned)a.rows, threads, 0, st>>>(a);
-  else if (nv == 2)
-    k_norm_vec<T, 2><<<(unsigned)a.rows, threads, 0, st>>>(a);
+template <typename T, int VEC>
+void launch_blocks(const Args& a, cudaStream_t st) {
+  // a block a warp while there are few rows (latency), four for many
+  const int nb = a.rows < 256 && a.nblk <= 32 ? 1 : a.nblk <= 2 ? 1 : a.nblk <= 6 ? 2 : 4;
+  const int threads = (a.nblk + nb - 1) / nb * 32;
+  const unsigned rows = (unsigned)a.rows;
+  if (nb == 1)
+    k_norm_blocks<T, 1, VEC><<<rows, threads, 0, st>>>(a);
+  else if (nb == 2)
+    k_norm_blocks<T, 2, VEC><<<rows, threads, 0, st>>>(a);
   else
-    k_norm_vec<T, 4><<<(unsigned)a.rows, threads, 0, st>>>(a);
+    k_norm_blocks<T, 4, VEC><<<rows, threads, 0, st>>>(a);
+}
+
+// vec: elements that every row start keeps together (8, 2 or 1).
+template <typename T>
+void launch(const Args& a, int vec, cudaStream_t st) {
+  const int groups = (a.cols + 7) / 8;
+  const unsigned rows = (unsigned)a.rows;
+  if (vec == 8 && groups <= 4096) {
+    // groups a thread: one while there are few rows (latency), else up to four
+    // in threads of at most 256, so that an SM holds several rows
+    int nv = 1;
+    while (groups > nv * (a.rows < 256 ? 1024 : 256) && nv < 4) nv *= 2;
+    const int threads = std::min(1024, ((groups + nv - 1) / nv + 31) / 32 * 32);
+    if (nv == 1)
+      k_norm_vec<T, 1><<<rows, threads, 0, st>>>(a);
+    else if (nv == 2)
+      k_norm_vec<T, 2><<<rows, threads, 0, st>>>(a);
+    else
+      k_norm_vec<T, 4><<<rows, threads, 0, st>>>(a);
+  } else if (a.nblk <= 128) {
+    vec >= 2 ? launch_blocks<T, 2>(a, st) : launch_blocks<T, 1>(a, st);
+  } else {
+    k_norm_any<T><<<rows, 1024, 0, st>>>(a);
+  }
 }
 
 }  // namespace fp8n
@@ -219,9 +351,13 @@ extern "C" int vq_norm_quantize_fp8(const void* x, int64_t ldx, const void* resi
   a.codes = reinterpret_cast<uint8_t*>(codes);
   a.scale = scale;
   a.hidden = residual ? hidden : nullptr;
-  const bool vec = cols % 8 == 0 && aligned(x, 16) && aligned(residual, 16) && aligned(weight, 16) &&
-                   aligned(a.hidden, 16) && aligned(codes, 8) && ldx * eb % 16 == 0 &&
-                   a.ldr * eb % 16 == 0;
+  auto keeps = [&](int n) {  // n elements together at the start of every row
+    const uintptr_t b = (uintptr_t)n * eb > 16 ? 16 : (uintptr_t)n * eb;
+    return cols % n == 0 && aligned(x, b) && aligned(residual, b) && aligned(weight, b) &&
+           aligned(a.hidden, b) && aligned(codes, n) && (uintptr_t)(ldx * eb) % b == 0 &&
+           (uintptr_t)(a.ldr * eb) % b == 0;
+  };
+  const int vec = keeps(8) ? 8 : keeps(2) ? 2 : 1;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == VQ_BF16)
     launch<BF16>(a, vec, st);

@@ -53,6 +53,7 @@ struct Args {
   const int32_t* counts;       // [B] new tokens, or null: T
   int B, T, H, Hkv, rot, page, width, pages, interleaved;
   int q_blocks, W;  // CTAs of the q part; pages that T tokens can touch
+  int hc;           // heads per CTA of the cache part
 };
 
 // One thread's 16 columns of a head as 8 pairs: unit u of D / 16 is pairs
@@ -69,38 +70,36 @@ __device__ __forceinline__ void unit_cols(int u, int rot, int& c0, int& c1) {
   }
 }
 
-// Load and rotate the unit: x0 / x1 hold columns c0.. / c1.. after it.
-template <typename T, bool IL>
-__device__ __forceinline__ void load_unit(const typename T::type* p, const float2* cs, int u, int rot,
-                                          float (&x0)[8], float (&x1)[8], int& c0, int& c1) {
-  unit_cols<IL>(u, rot, c0, c1);
-  T::load8(p + c0, x0);
-  T::load8(p + c1, x1);
-  if (cs && u * 16 < rot) {
+// The angles of unit u of one position (ones and zeros past rot).
+__device__ __forceinline__ void load_angles(const float2* cs, int u, int rot, float (&c)[8], float (&s)[8]) {
+  if (u * 16 < rot) {
     const float4* t = reinterpret_cast<const float4*>(cs + u * 8);
-    float c[8], s[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float4 f = __ldg(t + i);
       c[2 * i] = f.x, s[2 * i] = f.y, c[2 * i + 1] = f.z, s[2 * i + 1] = f.w;
     }
-    if (IL) {
+  }
+}
+// x0 / x1: columns c0.. / c1.. of the unit, turned.
+template <bool IL>
+__device__ __forceinline__ void turn(float (&x0)[8], float (&x1)[8], const float (&c)[8], const float (&s)[8]) {
+  if (IL) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = x0[2 * i], b = x0[2 * i + 1];
-        x0[2 * i] = a * c[i] - b * s[i];
-        x0[2 * i + 1] = a * s[i] + b * c[i];
-        const float d = x1[2 * i], e = x1[2 * i + 1];
-        x1[2 * i] = d * c[4 + i] - e * s[4 + i];
-        x1[2 * i + 1] = d * s[4 + i] + e * c[4 + i];
-      }
-    } else {
+    for (int i = 0; i < 4; ++i) {
+      const float a = x0[2 * i], b = x0[2 * i + 1];
+      x0[2 * i] = a * c[i] - b * s[i];
+      x0[2 * i + 1] = a * s[i] + b * c[i];
+      const float d = x1[2 * i], e = x1[2 * i + 1];
+      x1[2 * i] = d * c[4 + i] - e * s[4 + i];
+      x1[2 * i + 1] = d * s[4 + i] + e * c[4 + i];
+    }
+  } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float a = x0[i], b = x1[i];
-        x0[i] = a * c[i] - b * s[i];
-        x1[i] = a * s[i] + b * c[i];
-      }
+    for (int i = 0; i < 8; ++i) {
+      const float a = x0[i], b = x1[i];
+      x0[i] = a * c[i] - b * s[i];
+      x1[i] = a * s[i] + b * c[i];
     }
   }
 }
@@ -131,135 +130,269 @@ __device__ __forceinline__ float pow2_scale(float amax) {
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-constexpr int THREADS = 256;
+constexpr int QH = 2;  // heads of a token that a thread of the q part takes
 
-template <typename T, bool IL, int D, int IT>
-__global__ void __launch_bounds__(THREADS) k_rope_append(const Args a) {
+// The q part: thread `i` of it takes its unit of QH heads of a token, so that
+// the token's angles, twice the bytes of a bf16 unit, are read once for them.
+template <typename T, bool IL, int D>
+__device__ __forceinline__ void turn_q(const Args& a, int64_t i) {
   using E = typename T::type;
-  constexpr int U = D / 16;            // threads per head row
-  constexpr int ROWS = THREADS / U;    // rows per pass
-  if ((int)blockIdx.x < a.q_blocks) {
-    // ---- q: one unit per thread ----
-    const int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x;
-    const int u = (int)(i % U);
-    int64_t r = i / U;
-    const int64_t row = r;
-    if (row >= (int64_t)a.B * a.T * a.H) return;
-    const int h = (int)(r % a.H);
-    r /= a.H;
-    const int t = (int)(r % a.T), b = (int)(r / a.T);
-    int held;
-    const int n = plan(a, b, held);
-    E* out = reinterpret_cast<E*>(a.q_out) + row * D;
-    float x0[8], x1[8];
-    int c0, c1;
-    if (t < n) {
-      const E* p = reinterpret_cast<const E*>(a.q) + b * a.sq.b + t * a.sq.t + h * a.sq.h;
-      load_unit<T, IL>(p, a.table + (int64_t)(held + t) * (a.rot >> 1), u, a.rot, x0, x1, c0, c1);
-    } else {
-      unit_cols<IL>(u, a.rot, c0, c1);
+  constexpr int U = D / 16;
+  const int u = (int)(i % U);
+  int64_t r = i / U;
+  const int hg = (a.H + QH - 1) / QH, h0 = (int)(r % hg) * QH;
+  r /= hg;
+  if (r >= (int64_t)a.B * a.T) return;
+  const int t = (int)(r % a.T), b = (int)(r / a.T);
+  int c0, c1;
+  unit_cols<IL>(u, a.rot, c0, c1);
+  E* out = reinterpret_cast<E*>(a.q_out) + (r * a.H + h0) * D;
+  const E* p = reinterpret_cast<const E*>(a.q) + b * a.sq.b + t * a.sq.t + h0 * a.sq.h;
+  float x0[QH][8], x1[QH][8], c[8], s[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x0[j] = x1[j] = 0.0f;
+  for (int h = 0; h < QH; ++h)
+    if (h0 + h < a.H) {
+      T::load8(p + h * a.sq.h + c0, x0[h]);
+      T::load8(p + h * a.sq.h + c1, x1[h]);
     }
-    T::store8(out + c0, x0);
-    T::store8(out + c1, x1);
-    return;
-  }
-  // ---- one block (page, head) of the keys or the values per CTA ----
-  __shared__ float part[THREADS / 32];
-  int64_t i = (int64_t)blockIdx.x - a.q_blocks;
-  const int h = (int)(i % a.Hkv);
-  i /= a.Hkv;
-  const bool is_v = i & 1;
-  i >>= 1;
-  const int w = (int)(i % a.W), b = (int)(i / a.W);
+  int held;
+  const bool live = t < plan(a, b, held);
+  if (live) load_angles(a.table + (int64_t)(held + t) * (a.rot >> 1), u, a.rot, c, s);
+#pragma unroll
+  for (int h = 0; h < QH; ++h)
+    if (h0 + h < a.H) {
+      if (!live) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x0[h][j] = x1[h][j] = 0.0f;
+      } else if (u * 16 < a.rot) {
+        turn<IL>(x0[h], x1[h], c, s);
+      }
+      T::store8(out + h * D + c0, x0[h]);
+      T::store8(out + h * D + c1, x1[h]);
+    }
+}
+
+// The block that the w-th touched page of sequence b is for a head: which new
+// tokens go into it (t0 .. t0 + tokens - 1, from slot0 on) and where it lies.
+struct Block {
+  int t0, tokens, slot0, pid;
+  int64_t pos;  // of its first new token
+};
+__device__ __forceinline__ Block block_of(const Args& a, int b, int w) {
+  Block k;
   int held;
   const int n = plan(a, b, held);
   const int first = held / a.page + w;  // the sequence's page number
-  const int64_t lo = max((int64_t)held, (int64_t)first * a.page);
-  const int64_t hi = min((int64_t)held + n, (int64_t)(first + 1) * a.page);
-  if (lo >= hi) return;
-  const int pid = a.block_table[(int64_t)b * a.width + first];
-  if (pid < 0 || pid >= a.pages) {
-    if (threadIdx.x == 0) tc::note_err(nullptr, ERR_PAGE);
+  const int64_t begin = (int64_t)first * a.page;
+  k.pos = max((int64_t)held, begin);
+  k.tokens = (int)max(min((int64_t)held + n, begin + a.page) - k.pos, (int64_t)0);
+  k.t0 = (int)(k.pos - held);
+  k.slot0 = (int)(k.pos - begin);
+  k.pid = 0;
+  if (k.tokens > 0) {
+    k.pid = a.block_table[(int64_t)b * a.width + first];
+    if (k.pid < 0 || k.pid >= a.pages) {
+      tc::note_err(nullptr, ERR_PAGE);
+      k.tokens = 0;
+    }
+  }
+  return k;
+}
+
+__device__ __forceinline__ float amax16(const float (&x0)[8], const float (&x1)[8], float m) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = fmaxf(m, fmaxf(fabsf(x0[j]), fabsf(x1[j])));
+  return m;
+}
+// 16 columns as codes, 8 bytes at o + c0 and at o + c1.
+__device__ __forceinline__ void store_codes(uint8_t* o, int c0, int c1, const float (&x0)[8],
+                                            const float (&x1)[8], float inv) {
+  uint2 k0, k1;
+  k0.x = pack4(x0[0] * inv, x0[1] * inv, x0[2] * inv, x0[3] * inv);
+  k0.y = pack4(x0[4] * inv, x0[5] * inv, x0[6] * inv, x0[7] * inv);
+  k1.x = pack4(x1[0] * inv, x1[1] * inv, x1[2] * inv, x1[3] * inv);
+  k1.y = pack4(x1[4] * inv, x1[5] * inv, x1[6] * inv, x1[7] * inv);
+  *reinterpret_cast<uint2*>(o + c0) = k0;
+  *reinterpret_cast<uint2*>(o + c1) = k1;
+}
+// 16 codes brought to the scale was / f.
+__device__ __forceinline__ void rescale16(uint4* p, float f) {
+  uint4 v = *p;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 l = half2f(unpack2(w[j])), g = half2f(unpack2_hi(w[j]));
+    w[j] = pack4(l.x * f, l.y * f, g.x * f, g.y * f);
+  }
+  *p = v;
+}
+
+// Many new tokens: a CTA takes a.hc blocks (page, head) of the keys or the
+// values one after the other, so that the angles of a page's tokens come from
+// L1 after the first.  TH = page * D / 32 threads: two units of every thread
+// are a whole block, held in registers between its maximum and its codes.
+// 64 registers a thread at most: the loads of 1024 threads per SM (64 bytes
+// each) are what the HBM's latency needs.
+template <typename T, bool IL, int D, int TH>
+__global__ void __launch_bounds__(TH, 1024 / TH) k_rope_append(const __grid_constant__ Args a) {
+  using E = typename T::type;
+  constexpr int U = D / 16, ROWS = TH / U, IT = 2;  // threads per token, tokens per pass, passes
+  if ((int)blockIdx.x < a.q_blocks) {
+    turn_q<T, IL, D>(a, (int64_t)blockIdx.x * TH + threadIdx.x);
     return;
   }
-  const int t0 = (int)(lo - held), tokens = (int)(hi - lo), slot0 = (int)(lo - (int64_t)first * a.page);
+  __shared__ uint32_t part[2][TH / 32];
+  int i = (int)blockIdx.x - a.q_blocks;
+  const int hg = (a.Hkv + a.hc - 1) / a.hc, h0 = i % hg * a.hc, h1 = min(a.Hkv, h0 + a.hc);
+  i /= hg;
+  const bool is_v = i & 1;
+  i >>= 1;
+  const int b = i / a.W;
+  const Block k = block_of(a, b, i % a.W);
+  if (k.tokens <= 0) return;
   const int u = threadIdx.x % U, r0 = threadIdx.x / U;
-  const E* src = is_v ? reinterpret_cast<const E*>(a.v) + b * a.sv.b + h * a.sv.h
-                      : reinterpret_cast<const E*>(a.k) + b * a.sk.b + h * a.sk.h;
-  const int64_t st = is_v ? a.sv.t : a.sk.t;
-  const int64_t blk = (int64_t)pid * a.Hkv + h;
-  uint8_t* codes = (is_v ? a.v_codes : a.k_codes) + blk * a.page * D;
-  float* scale = (is_v ? a.v_scale : a.k_scale) + blk;
-  float x0[IT][8], x1[IT][8];
+  const Strides st = is_v ? a.sv : a.sk;
+  const E* src = reinterpret_cast<const E*>(is_v ? a.v : a.k) + b * st.b + k.t0 * st.t + r0 * st.t;
   int c0, c1;
   unit_cols<IL>(u, a.rot, c0, c1);
-  float m = 0.0f;
+  const bool turns = !is_v && u * 16 < a.rot;
+  for (int h = h0; h < h1; ++h) {
+    const int64_t blk = (int64_t)k.pid * a.Hkv + h;
+    uint8_t* codes = (is_v ? a.v_codes : a.k_codes) + blk * a.page * D;
+    float* scale = (is_v ? a.v_scale : a.k_scale) + blk;
+    float x0[IT][8], x1[IT][8];
 #pragma unroll
-  for (int it = 0; it < IT; ++it) {
-    const int r = it * ROWS + r0;
-    if (r < tokens) {
-      const float2* cs = is_v ? nullptr : a.table + (lo + r) * (a.rot >> 1);
-      load_unit<T, IL>(src + (t0 + r) * st, cs, u, a.rot, x0[it], x1[it], c0, c1);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) m = fmaxf(m, fmaxf(fabsf(x0[it][j]), fabsf(x1[it][j])));
-    }
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, d));
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
-  const float was = slot0 ? *scale : 0.0f;  // slot 0 written now: a fresh block
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < THREADS / 32; ++j) m = fmaxf(m, part[j]);
-  const float s = fmaxf(pow2_scale(m), was), inv = __fdiv_rn(1.0f, s);  // exact: s is a power of two
-#pragma unroll
-  for (int it = 0; it < IT; ++it) {
-    const int r = it * ROWS + r0;
-    if (r < tokens) {
-      uint8_t* o = codes + (slot0 + r) * D;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x0[it][j] *= inv, x1[it][j] *= inv;
-      *reinterpret_cast<uint2*>(o + c0) = make_uint2(pack4(x0[it][0], x0[it][1], x0[it][2], x0[it][3]),
-                                                     pack4(x0[it][4], x0[it][5], x0[it][6], x0[it][7]));
-      *reinterpret_cast<uint2*>(o + c1) = make_uint2(pack4(x1[it][0], x1[it][1], x1[it][2], x1[it][3]),
-                                                     pack4(x1[it][4], x1[it][5], x1[it][6], x1[it][7]));
-    }
-  }
-  if (slot0 && s != was) {  // the tokens that the block holds, at the new scale
-    const float f = was * inv;
-    for (int c = threadIdx.x; c < slot0 * U; c += THREADS) {
-      uint4* p = reinterpret_cast<uint4*>(codes) + c;
-      uint4 v = *p;
-      uint32_t* wv = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 l = half2f(unpack2(wv[j])), g = half2f(unpack2_hi(wv[j]));
-        wv[j] = pack4(l.x * f, l.y * f, g.x * f, g.y * f);
+    for (int it = 0; it < IT; ++it)
+      if (it * ROWS + r0 < k.tokens) {
+        const E* p = src + h * st.h + it * ROWS * st.t;
+        T::load8(p + c0, x0[it]);
+        T::load8(p + c1, x1[it]);
       }
-      *p = v;
-    }
+    const float was = k.slot0 ? *scale : 0.0f;  // slot 0 written now: a fresh block
+    float m = 0.0f;
+#pragma unroll
+    for (int it = 0; it < IT; ++it)
+      if (it * ROWS + r0 < k.tokens) {
+        if (turns) {
+          float c[8], s[8];
+          load_angles(a.table + (k.pos + it * ROWS + r0) * (a.rot >> 1), u, a.rot, c, s);
+          turn<IL>(x0[it], x1[it], c, s);
+        }
+        m = amax16(x0[it], x1[it], m);
+      }
+    // magnitudes order as their bit patterns do
+    uint32_t mb = __reduce_max_sync(FULL, __float_as_uint(m));
+    if ((threadIdx.x & 31) == 0) part[h & 1][threadIdx.x >> 5] = mb;
+    __syncthreads();  // two buffers: the next head's maxima do not meet this one's readers
+#pragma unroll
+    for (int j = 0; j < TH / 32; ++j) mb = max(mb, part[h & 1][j]);
+    const float s = fmaxf(pow2_scale(__uint_as_float(mb)), was);
+    const float inv = __fdiv_rn(1.0f, s);  // exact: s is a power of two
+#pragma unroll
+    for (int it = 0; it < IT; ++it)
+      if (it * ROWS + r0 < k.tokens)
+        store_codes(codes + (k.slot0 + it * ROWS + r0) * D, c0, c1, x0[it], x1[it], inv);
+    if (k.slot0 && s != was)  // the tokens that the block holds, at the new scale
+      for (int c = threadIdx.x; c < k.slot0 * U; c += TH)
+        rescale16(reinterpret_cast<uint4*>(codes) + c, was * inv);
+    if (threadIdx.x == 0) *scale = s;  // every thread read the old one before the barrier
   }
-  if (threadIdx.x == 0) *scale = s;
+}
+
+// Few new tokens (T <= G of 1, 2 or 4, or 8 at D = 64): G * D / 16 lanes take
+// a block, so that a warp holds several and no lane waits at a barrier.
+constexpr int FEW_THREADS = 128;
+template <typename T, bool IL, int D, int G>
+__global__ void __launch_bounds__(FEW_THREADS) k_rope_append_few(const __grid_constant__ Args a) {
+  using E = typename T::type;
+  constexpr int U = D / 16, L = G * U;  // lanes per block
+  if ((int)blockIdx.x < a.q_blocks) {
+    turn_q<T, IL, D>(a, (int64_t)blockIdx.x * FEW_THREADS + threadIdx.x);
+    return;
+  }
+  int i = (((int)blockIdx.x - a.q_blocks) * FEW_THREADS + (int)threadIdx.x) / L;
+  const bool live = i < a.B * a.W * 2 * a.Hkv;
+  i = live ? i : 0;
+  const int h = i % a.Hkv;
+  i /= a.Hkv;
+  const bool is_v = i & 1;
+  i >>= 1;
+  const int b = i / a.W, l = threadIdx.x % L, u = l % U, r = l / U;
+  const Block k = block_of(a, b, i % a.W);
+  const bool mine = live && r < k.tokens;
+  const Strides st = is_v ? a.sv : a.sk;
+  int c0, c1;
+  unit_cols<IL>(u, a.rot, c0, c1);
+  const int64_t blk = (int64_t)k.pid * a.Hkv + h;
+  uint8_t* codes = (is_v ? a.v_codes : a.k_codes) + blk * a.page * D;
+  float* scale = (is_v ? a.v_scale : a.k_scale) + blk;
+  float x0[8], x1[8], was = 0.0f, m = 0.0f;
+  if (mine) {
+    const E* p = reinterpret_cast<const E*>(is_v ? a.v : a.k) + b * st.b + (k.t0 + r) * st.t + h * st.h;
+    T::load8(p + c0, x0);
+    T::load8(p + c1, x1);
+    if (!is_v && u * 16 < a.rot) {
+      float c[8], s[8];
+      load_angles(a.table + (k.pos + r) * (a.rot >> 1), u, a.rot, c, s);
+      turn<IL>(x0, x1, c, s);
+    }
+    m = amax16(x0, x1, 0.0f);
+  }
+  if (live && k.tokens > 0 && k.slot0) was = *scale;
+#pragma unroll
+  for (int d = L / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, d));
+  const float s = fmaxf(pow2_scale(m), was), inv = __fdiv_rn(1.0f, s);
+  if (mine) store_codes(codes + (k.slot0 + r) * D, c0, c1, x0, x1, inv);
+  if (live && k.tokens > 0) {
+    if (k.slot0 && s != was)
+      for (int c = l; c < k.slot0 * U; c += L) rescale16(reinterpret_cast<uint4*>(codes) + c, was * inv);
+    if (l == 0) *scale = s;  // the shuffles stand between it and the lanes that read the old one
+  }
 }
 
 template <typename T, bool IL, int D>
-void launch_it(const Args& a, unsigned grid, cudaStream_t st) {
-  const int it = std::max(1, a.page * (D / 16) / THREADS);
-  if (it == 1)
-    k_rope_append<T, IL, D, 1><<<grid, THREADS, 0, st>>>(a);
-  else if (it == 2)
-    k_rope_append<T, IL, D, 2><<<grid, THREADS, 0, st>>>(a);
+void launch_d(Args& a, int64_t& blocks, cudaStream_t st) {
+  const int64_t q = (int64_t)a.B * a.T * ((a.H + QH - 1) / QH) * (D / 16);  // threads of the q part
+  const int64_t items = (int64_t)a.B * a.W * 2 * a.Hkv;
+  auto grid = [&](int th, int64_t cache_ctas) {
+    a.q_blocks = (int)std::min<int64_t>((q + th - 1) / th, 1ll << 30);
+    blocks = (q + th - 1) / th + cache_ctas;
+    return (unsigned)blocks;
+  };
+  const int per_warp = 512 / D;  // tokens a warp holds
+  if (a.T <= per_warp) {
+    const int g = a.T == 1 ? 1 : a.T == 2 ? 2 : a.T <= 4 ? 4 : 8;
+    const unsigned n = grid(FEW_THREADS, (items * g * (D / 16) + FEW_THREADS - 1) / FEW_THREADS);
+    if (blocks >= (1ll << 31)) return;
+    if (g == 1)
+      k_rope_append_few<T, IL, D, 1><<<n, FEW_THREADS, 0, st>>>(a);
+    else if (g == 2)
+      k_rope_append_few<T, IL, D, 2><<<n, FEW_THREADS, 0, st>>>(a);
+    else if (g == 4)
+      k_rope_append_few<T, IL, D, 4><<<n, FEW_THREADS, 0, st>>>(a);
+    else
+      k_rope_append_few<T, IL, D, 512 / D><<<n, FEW_THREADS, 0, st>>>(a);
+    return;
+  }
+  // several heads per CTA once there are CTAs for a few waves all the same
+  a.hc = 1;
+  while (a.hc < 8 && a.hc < a.Hkv && items / (2 * a.hc) >= 16 * vq::mx::sm_count()) a.hc *= 2;
+  const int th = a.page * D / 32;
+  const unsigned n = grid(th, (int64_t)a.B * a.W * 2 * ((a.Hkv + a.hc - 1) / a.hc));
+  if (blocks >= (1ll << 31)) return;
+  if (a.page == 32)
+    k_rope_append<T, IL, D, D><<<n, D, 0, st>>>(a);
+  else if (a.page == 64)
+    k_rope_append<T, IL, D, 2 * D><<<n, 2 * D, 0, st>>>(a);
   else
-    k_rope_append<T, IL, D, 4><<<grid, THREADS, 0, st>>>(a);
+    k_rope_append<T, IL, D, 4 * D><<<n, 4 * D, 0, st>>>(a);
 }
 template <typename T>
-void launch(const Args& a, int D, unsigned grid, cudaStream_t st) {
+void launch(Args& a, int D, int64_t& blocks, cudaStream_t st) {
   if (D == 128)
-    a.interleaved ? launch_it<T, true, 128>(a, grid, st) : launch_it<T, false, 128>(a, grid, st);
+    a.interleaved ? launch_d<T, true, 128>(a, blocks, st) : launch_d<T, false, 128>(a, blocks, st);
   else
-    a.interleaved ? launch_it<T, true, 64>(a, grid, st) : launch_it<T, false, 64>(a, grid, st);
+    a.interleaved ? launch_d<T, true, 64>(a, blocks, st) : launch_d<T, false, 64>(a, blocks, st);
 }
 
 // This file's sticky word (vq_device_errors).
@@ -312,14 +445,13 @@ extern "C" int vq_rope_append_kv8(const void* q, const void* k, const void* v, c
   a.rot = rot, a.page = page, a.width = (int)table_width, a.pages = (int)pages;
   a.interleaved = interleaved;
   a.W = (int)((tokens - 1 + page - 1) / page) + 1;
-  const int64_t qb = (batch * tokens * heads * (head_dim / 16) + THREADS - 1) / THREADS;
-  const int64_t kb = batch * a.W * 2 * kv_heads;
-  if (qb + kb >= (1ll << 31)) return VQ_ERR_INVALID;
-  a.q_blocks = (int)qb;
+  if (batch * a.W * 2 * kv_heads >= (1ll << 27)) return VQ_ERR_INVALID;  // items in 32 bits, with their lanes
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  int64_t blocks = 0;
   if (dtype == VQ_BF16)
-    launch<BF16>(a, head_dim, (unsigned)(qb + kb), st);
+    launch<BF16>(a, head_dim, blocks, st);
   else
-    launch<F32>(a, head_dim, (unsigned)(qb + kb), st);
+    launch<F32>(a, head_dim, blocks, st);
+  if (blocks >= (1ll << 31)) return VQ_ERR_INVALID;
   return cudaGetLastError() == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
 }
