@@ -718,7 +718,8 @@ int vq_linear_fp8_block(const void* x, const float* x_scale, const void* w, cons
  *   b gets position lengths[b] + t.
  *   k_codes, v_codes E4M3 [pages, kv_heads, page, head_dim]; k_scale, v_scale
  *   float32 [pages, kv_heads].  page 32, 64 or 128; head_dim 64 or 128.
- *   q_out [batch, tokens, heads, head_dim] in q's type; 0 for tokens past counts.
+ *   q_out [batch, tokens, heads, head_dim] in q's type, 32-byte aligned; 0 for
+ *   tokens past counts.
  * Scales are powers of two, the least with max|value| / scale <= 448 over a
  * block's tokens, within [2^-100, 2^120]; a block that holds tokens keeps its
  * scale unless the new ones need a larger one, and its codes are then brought

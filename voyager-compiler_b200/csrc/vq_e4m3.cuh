@@ -58,11 +58,20 @@ struct BF16 {
     __nv_bfloat16 b = __float2bfloat16_rn(v);
     *p = *reinterpret_cast<uint16_t*>(&b);
   }
-  static __device__ __forceinline__ void load8(const uint16_t* p, float (&v)[8]) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+  // 8 elements as they lie in memory (to be held while the loads of others
+  // are used) and as floats
+  struct Raw {
+    uint4 a;
+  };
+  static __device__ __forceinline__ Raw fetch8(const uint16_t* p) {
+    return {__ldg(reinterpret_cast<const uint4*>(p))};
+  }
+  static __device__ __forceinline__ void widen8(const Raw& r, float (&v)[8]) {
+    const uint4 u = r.a;
     v[0] = bf_lo(u.x), v[1] = bf_hi(u.x), v[2] = bf_lo(u.y), v[3] = bf_hi(u.y);
     v[4] = bf_lo(u.z), v[5] = bf_hi(u.z), v[6] = bf_lo(u.w), v[7] = bf_hi(u.w);
   }
+  static __device__ __forceinline__ void load8(const uint16_t* p, float (&v)[8]) { widen8(fetch8(p), v); }
   static __device__ __forceinline__ void store8(uint16_t* p, const float (&v)[8]) {
     *reinterpret_cast<uint4*>(p) = make_uint4(bf_pack(v[0], v[1]), bf_pack(v[2], v[3]),
                                               bf_pack(v[4], v[5]), bf_pack(v[6], v[7]));
@@ -72,12 +81,17 @@ struct F32 {
   using type = float;
   static __device__ __forceinline__ float load(const float* p) { return *p; }
   static __device__ __forceinline__ void store(float* p, float v) { *p = v; }
-  static __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-    v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  struct Raw {
+    float4 a, b;
+  };
+  static __device__ __forceinline__ Raw fetch8(const float* p) {
+    return {__ldg(reinterpret_cast<const float4*>(p)), __ldg(reinterpret_cast<const float4*>(p) + 1)};
   }
+  static __device__ __forceinline__ void widen8(const Raw& r, float (&v)[8]) {
+    v[0] = r.a.x, v[1] = r.a.y, v[2] = r.a.z, v[3] = r.a.w;
+    v[4] = r.b.x, v[5] = r.b.y, v[6] = r.b.z, v[7] = r.b.w;
+  }
+  static __device__ __forceinline__ void load8(const float* p, float (&v)[8]) { widen8(fetch8(p), v); }
   static __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
     reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
     reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);

@@ -21,6 +21,7 @@
 
 #include "voyager_b200.h"
 #include "vq_e4m3.cuh"
+#include "vq_tc.cuh"
 
 namespace vq {
 namespace fp8n {
@@ -69,63 +70,86 @@ __device__ __forceinline__ float quotient(float y, float s, float inv) {
   return s < 0x1p-126f ? __fdiv_rn(y, s) : y * inv;
 }
 
-// One CTA per row, NV groups of 8 consecutive elements per thread; columns a
-// multiple of 8, rows 16-byte aligned.  A block of 128 columns is 16
-// neighbouring lanes.
-template <typename T, int NV>
-__global__ void __launch_bounds__(1024) k_norm_vec(const Args a) {
+// A CTA takes rows blockIdx.x, + gridDim.x, ..; NV groups of 8 consecutive
+// elements per thread; columns a multiple of 8, rows 16-byte aligned.  A block
+// of 128 columns is 16 neighbouring lanes.  The next row's loads are in
+// flight while this one is summed and quantized (without that the SMs waited
+// for them half the time: 16384 x 4096 bf16 with a residual took 111 us), and
+// the weight stays in registers.
+template <typename T, int NV, int MAXT>
+__global__ void __launch_bounds__(MAXT) k_norm_vec(const Args a) {
   using E = typename T::type;
-  __shared__ float part[32];
-  const int64_t row = blockIdx.x;
-  const E* x = reinterpret_cast<const E*>(a.x) + row * a.ldx;
-  const E* r = reinterpret_cast<const E*>(a.r) + row * a.ldr;
+  using Raw = typename T::Raw;
+  __shared__ float part[2][32];
+  const E* x = reinterpret_cast<const E*>(a.x);
+  const E* r = reinterpret_cast<const E*>(a.r);
   const E* w = reinterpret_cast<const E*>(a.w);
-  E* hid = reinterpret_cast<E*>(a.hidden) + row * a.cols;
-  float h[NV][8];
-  float ss = 0.0f;
+  auto col = [&](int i) { return (i * (int)blockDim.x + (int)threadIdx.x) * 8; };
+  Raw rx[NV] = {}, rr[NV] = {}, rw[NV] = {};
+  auto fetch = [&](int64_t row) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * 8;
+    for (int i = 0; i < NV; ++i)
+      if (col(i) < a.cols) {
+        rx[i] = T::fetch8(x + row * a.ldx + col(i));
+        if (a.r) rr[i] = T::fetch8(r + row * a.ldr + col(i));
+      }
+  };
+  fetch(blockIdx.x);
+  if (a.w) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) h[i][k] = 0.0f;
-    if (c < a.cols) {
-      T::load8(x + c, h[i]);
+    for (int i = 0; i < NV; ++i)
+      if (col(i) < a.cols) rw[i] = T::fetch8(w + col(i));
+  }
+  int flip = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, flip ^= 1) {
+    E* hid = reinterpret_cast<E*>(a.hidden) + row * a.cols;
+    float h[NV][8];
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      T::widen8(rx[i], h[i]);
       if (a.r) {
         float q[8];
-        T::load8(r + c, q);
+        T::widen8(rr[i], q);
 #pragma unroll
         for (int k = 0; k < 8; ++k) h[i][k] += q[k];
-        T::store8(hid + c, h[i]);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) ss = fmaf(h[i][k], h[i][k], ss);
     }
-  }
-  float inv = 1.0f;
-  if (a.w) inv = rsqrtf(__fdiv_rn(block_sum(ss, part), (float)a.cols) + a.eps);
+    if (row + gridDim.x < a.rows) fetch(row + gridDim.x);
+    if (a.r) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * blockDim.x + threadIdx.x) * 8;
-    if (a.w && c < a.cols) {
-      float g[8];
-      T::load8(w + c, g);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) h[i][k] = h[i][k] * inv * g[k];
+      for (int i = 0; i < NV; ++i)
+        if (col(i) < a.cols) T::store8(hid + col(i), h[i]);
     }
-    uint32_t m = 0;
+    float inv = 1.0f;
+    // two buffers of partial sums: the next row's do not meet this one's readers
+    if (a.w) inv = rsqrtf(__fdiv_rn(block_sum(ss, part[flip]), (float)a.cols) + a.eps);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m = max(m, mag(h[i][k]));
+    for (int i = 0; i < NV; ++i) {
+      const int c = col(i);
+      if (a.w) {
+        float g[8];
+        T::widen8(rw[i], g);
 #pragma unroll
-    for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(FULL, m, d));
-    if (c < a.cols) {
-      const float s = block_scale(m);
-      const float inv_s = __fdiv_rn(1.0f, s);
-      float q[8];
+        for (int k = 0; k < 8; ++k) h[i][k] = h[i][k] * inv * g[k];
+      }
+      uint32_t m = 0;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) q[k] = quotient(h[i][k], s, inv_s);
-      *reinterpret_cast<uint2*>(a.codes + row * a.cols + c) =
-          make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
-      if ((threadIdx.x & 15) == 0) a.scale[row * a.nblk + (c >> 7)] = s;
+      for (int k = 0; k < 8; ++k) m = max(m, mag(h[i][k]));
+#pragma unroll
+      for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(FULL, m, d));
+      if (c < a.cols) {
+        const float s = block_scale(m);
+        const float inv_s = __fdiv_rn(1.0f, s);
+        float q[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) q[k] = quotient(h[i][k], s, inv_s);
+        *reinterpret_cast<uint2*>(a.codes + row * a.cols + c) =
+            make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+        if ((threadIdx.x & 15) == 0) a.scale[row * a.nblk + (c >> 7)] = s;
+      }
     }
   }
 }
@@ -281,6 +305,26 @@ __global__ void __launch_bounds__(1024) k_norm_any(const Args a) {
   }
 }
 
+// As many CTAs as fit at once (asked once per device and CTA size), or one per row.
+template <typename T, int NV, int MAXT>
+void launch_vec(const Args& a, int threads, cudaStream_t st) {
+  static int known[64][33] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  dev = dev < 0 || dev > 63 ? 0 : dev;
+  int& per_sm = known[dev][threads / 32];
+  if (per_sm == 0) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_norm_vec<T, NV, MAXT>, threads, 0) != cudaSuccess || n < 1) {
+      (void)cudaGetLastError();
+      n = 1;
+    }
+    per_sm = n;
+  }
+  const int64_t grid = std::min<int64_t>(a.rows, (int64_t)per_sm * vq::mx::sm_count());
+  k_norm_vec<T, NV, MAXT><<<(unsigned)grid, threads, 0, st>>>(a);
+}
+
 template <typename T, int VEC>
 void launch_blocks(const Args& a, cudaStream_t st) {
   // a block a warp while there are few rows (latency), four for many
@@ -307,11 +351,11 @@ void launch(const Args& a, int vec, cudaStream_t st) {
     while (groups > nv * (a.rows < 256 ? 1024 : 256) && nv < 4) nv *= 2;
     const int threads = std::min(1024, ((groups + nv - 1) / nv + 31) / 32 * 32);
     if (nv == 1)
-      k_norm_vec<T, 1><<<rows, threads, 0, st>>>(a);
+      threads <= 256 ? launch_vec<T, 1, 256>(a, threads, st) : launch_vec<T, 1, 1024>(a, threads, st);
     else if (nv == 2)
-      k_norm_vec<T, 2><<<rows, threads, 0, st>>>(a);
+      threads <= 256 ? launch_vec<T, 2, 256>(a, threads, st) : launch_vec<T, 2, 1024>(a, threads, st);
     else
-      k_norm_vec<T, 4><<<rows, threads, 0, st>>>(a);
+      threads <= 256 ? launch_vec<T, 4, 256>(a, threads, st) : launch_vec<T, 4, 1024>(a, threads, st);
   } else if (a.nblk <= 128) {
     vec >= 2 ? launch_blocks<T, 2>(a, st) : launch_blocks<T, 1>(a, st);
   } else {

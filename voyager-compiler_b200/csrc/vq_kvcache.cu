@@ -53,7 +53,7 @@ struct Args {
   const int32_t* counts;       // [B] new tokens, or null: T
   int B, T, H, Hkv, rot, page, width, pages, interleaved;
   int q_blocks, W;  // CTAs of the q part; pages that T tokens can touch
-  int hc;           // heads per CTA of the cache part
+  int hq, hc;       // heads per thread of the q part, per CTA of the cache part
 };
 
 // One thread's 16 columns of a head as 8 pairs: unit u of D / 16 is pairs
@@ -130,46 +130,162 @@ __device__ __forceinline__ float pow2_scale(float amax) {
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
-constexpr int QH = 2;  // heads of a token that a thread of the q part takes
+// A unit of a row to memory: in one 32-byte store where its columns lie side
+// by side (two of 16 bytes would each fill half of every sector that a warp
+// touches: 178 us against 172 for the 8 prompts below, turned by 16 columns).
+template <typename T>
+__device__ __forceinline__ void store_unit(typename T::type* row, int c0, int c1, const float (&x0)[8],
+                                           const float (&x1)[8]) {
+  if (sizeof(*row) == 2 && c1 == c0 + 8) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(row + c0), "r"(bf_pack(x0[0], x0[1])),
+                 "r"(bf_pack(x0[2], x0[3])), "r"(bf_pack(x0[4], x0[5])), "r"(bf_pack(x0[6], x0[7])),
+                 "r"(bf_pack(x1[0], x1[1])), "r"(bf_pack(x1[2], x1[3])), "r"(bf_pack(x1[4], x1[5])),
+                 "r"(bf_pack(x1[6], x1[7])) : "memory");
+  } else {
+    T::store8(row + c0, x0);
+    T::store8(row + c1, x1);
+  }
+}
 
-// The q part: thread `i` of it takes its unit of QH heads of a token, so that
-// the token's angles, twice the bytes of a bf16 unit, are read once for them.
+constexpr int QH = 2;  // heads of a token that a thread of the q part takes at a time
+
+// The q part: thread `i` of it takes its unit of a.hq heads of a token (a
+// multiple of QH), so that the token's angles, twice the bytes of a bf16 unit,
+// are read once for them.
+struct QUnit {
+  int u, h0, h1, b, t, c0, c1;
+  int64_t row;
+  bool any;
+};
+template <bool IL, int D>
+__device__ __forceinline__ QUnit q_unit(const Args& a, int64_t i) {
+  constexpr int U = D / 16;
+  QUnit x;
+  x.u = (int)(i % U);
+  int64_t r = i / U;
+  const int hg = (a.H + a.hq - 1) / a.hq;
+  x.h0 = (int)(r % hg) * a.hq, x.h1 = min(a.H, x.h0 + a.hq);
+  r /= hg;
+  x.any = r < (int64_t)a.B * a.T;
+  x.row = r;
+  x.b = (int)(r / a.T), x.t = (int)(r - (int64_t)x.b * a.T);
+  unit_cols<IL>(x.u, a.rot, x.c0, x.c1);
+  return x;
+}
 template <typename T, bool IL, int D>
 __device__ __forceinline__ void turn_q(const Args& a, int64_t i) {
   using E = typename T::type;
-  constexpr int U = D / 16;
-  const int u = (int)(i % U);
-  int64_t r = i / U;
-  const int hg = (a.H + QH - 1) / QH, h0 = (int)(r % hg) * QH;
-  r /= hg;
-  if (r >= (int64_t)a.B * a.T) return;
-  const int t = (int)(r % a.T), b = (int)(r / a.T);
-  int c0, c1;
-  unit_cols<IL>(u, a.rot, c0, c1);
-  E* out = reinterpret_cast<E*>(a.q_out) + (r * a.H + h0) * D;
-  const E* p = reinterpret_cast<const E*>(a.q) + b * a.sq.b + t * a.sq.t + h0 * a.sq.h;
+  const QUnit x = q_unit<IL, D>(a, i);
+  if (!x.any) return;
+  E* out = reinterpret_cast<E*>(a.q_out) + x.row * a.H * D;
+  const E* p = reinterpret_cast<const E*>(a.q) + x.b * a.sq.b + x.t * a.sq.t;
   float x0[QH][8], x1[QH][8], c[8], s[8];
 #pragma unroll
-  for (int h = 0; h < QH; ++h)
-    if (h0 + h < a.H) {
-      T::load8(p + h * a.sq.h + c0, x0[h]);
-      T::load8(p + h * a.sq.h + c1, x1[h]);
+  for (int q = 0; q < QH; ++q)
+    if (x.h0 + q < x.h1) {
+      T::load8(p + (x.h0 + q) * a.sq.h + x.c0, x0[q]);
+      T::load8(p + (x.h0 + q) * a.sq.h + x.c1, x1[q]);
     }
   int held;
-  const bool live = t < plan(a, b, held);
-  if (live) load_angles(a.table + (int64_t)(held + t) * (a.rot >> 1), u, a.rot, c, s);
+  const bool live = x.t < plan(a, x.b, held), turns = live && x.u * 16 < a.rot;
+  if (turns) load_angles(a.table + (int64_t)(held + x.t) * (a.rot >> 1), x.u, a.rot, c, s);
 #pragma unroll
-  for (int h = 0; h < QH; ++h)
-    if (h0 + h < a.H) {
+  for (int q = 0; q < QH; ++q)
+    if (x.h0 + q < x.h1) {
+      if (turns) turn<IL>(x0[q], x1[q], c, s);
       if (!live) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x0[h][j] = x1[h][j] = 0.0f;
-      } else if (u * 16 < a.rot) {
-        turn<IL>(x0[h], x1[h], c, s);
+        for (int j = 0; j < 8; ++j) x0[q][j] = x1[q][j] = 0.0f;
       }
-      T::store8(out + h * D + c0, x0[h]);
-      T::store8(out + h * D + c1, x1[h]);
+      store_unit<T>(out + (x.h0 + q) * D, x.c0, x.c1, x0[q], x1[q]);
     }
+}
+
+// A thread's own ring in shared memory, filled by cp.async: DEPTH steps of four
+// groups of 8 elements.  Only the thread itself reads it, so waiting for its
+// own copies is enough; registers for that many loads in flight would halve
+// the threads that fit (one step ahead in registers: 159 us for 8 prompts of
+// 2048 tokens and 32 heads, against 105 at the HBM copy rate).
+template <typename T, int TH>
+struct Ring {
+  using E = typename T::type;
+  static constexpr int DEPTH = 3, CH = sizeof(E) / 2;  // 16-byte chunks per group
+  static constexpr int BYTES = DEPTH * 4 * CH * 16 * TH;
+  uint32_t base;
+  __device__ __forceinline__ explicit Ring(void* smem) : base(tc::smem_u32(smem) + threadIdx.x * 16) {}
+  __device__ __forceinline__ uint32_t at(int step, int group) const {
+    return base + ((step % DEPTH) * 4 + group) * CH * 16 * TH;
+  }
+  __device__ __forceinline__ void fetch(int step, int group, const E* p) const {
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(step, group) + c * 16 * TH),
+                   "l"(reinterpret_cast<const char*>(p) + 16 * c) : "memory");
+  }
+  __device__ __forceinline__ void commit() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  // every step but the newest DEPTH - 1 has landed
+  __device__ __forceinline__ void wait() const {
+    asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+  }
+  __device__ __forceinline__ void read(int step, int group, float (&v)[8]) const {
+    typename T::Raw r;
+    uint4* u = reinterpret_cast<uint4*>(&r);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+      asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(u[c].x), "=r"(u[c].y), "=r"(u[c].z), "=r"(u[c].w)
+                   : "r"(at(step, group) + c * 16 * TH) : "memory");
+    T::widen8(r, v);
+  }
+};
+
+// The q part alone, beside k_rope_append.
+constexpr int Q_THREADS = 256;
+template <typename T, bool IL, int D>
+__global__ void __launch_bounds__(Q_THREADS) k_turn_q(const __grid_constant__ Args a) {
+  using E = typename T::type;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const Ring<T, Q_THREADS> ring(smem);
+  const QUnit x = q_unit<IL, D>(a, (int64_t)blockIdx.x * Q_THREADS + threadIdx.x);
+  if (!x.any) return;
+  E* out = reinterpret_cast<E*>(a.q_out) + x.row * a.H * D;
+  const E* p = reinterpret_cast<const E*>(a.q) + x.b * a.sq.b + x.t * a.sq.t;
+  const int steps = (x.h1 - x.h0 + QH - 1) / QH;
+  auto fetch = [&](int k) {
+    if (k < steps) {
+#pragma unroll
+      for (int q = 0; q < QH; ++q) {
+        const E* r = p + min(x.h0 + k * QH + q, x.h1 - 1) * a.sq.h;
+        ring.fetch(k, 2 * q, r + x.c0);
+        ring.fetch(k, 2 * q + 1, r + x.c1);
+      }
+    }
+    ring.commit();
+  };
+#pragma unroll
+  for (int k = 0; k < Ring<T, Q_THREADS>::DEPTH - 1; ++k) fetch(k);
+  int held;
+  const bool live = x.t < plan(a, x.b, held), turns = live && x.u * 16 < a.rot;
+  float c[8], s[8];
+  if (turns) load_angles(a.table + (int64_t)(held + x.t) * (a.rot >> 1), x.u, a.rot, c, s);
+  for (int k = 0; k < steps; ++k) {
+    fetch(k + Ring<T, Q_THREADS>::DEPTH - 1);
+    ring.wait();
+#pragma unroll
+    for (int q = 0; q < QH; ++q) {
+      const int h = x.h0 + k * QH + q;
+      float x0[8], x1[8];
+      ring.read(k, 2 * q, x0);
+      ring.read(k, 2 * q + 1, x1);
+      if (turns) turn<IL>(x0, x1, c, s);
+      if (!live) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x0[j] = x1[j] = 0.0f;
+      }
+      if (h < x.h1) store_unit<T>(out + h * D, x.c0, x.c1, x0, x1);
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // The block that the w-th touched page of sequence b is for a head: which new
@@ -212,8 +328,12 @@ __device__ __forceinline__ void store_codes(uint8_t* o, int c0, int c1, const fl
   k0.y = pack4(x0[4] * inv, x0[5] * inv, x0[6] * inv, x0[7] * inv);
   k1.x = pack4(x1[0] * inv, x1[1] * inv, x1[2] * inv, x1[3] * inv);
   k1.y = pack4(x1[4] * inv, x1[5] * inv, x1[6] * inv, x1[7] * inv);
-  *reinterpret_cast<uint2*>(o + c0) = k0;
-  *reinterpret_cast<uint2*>(o + c1) = k1;
+  if (c1 == c0 + 8) {
+    *reinterpret_cast<uint4*>(o + c0) = make_uint4(k0.x, k0.y, k1.x, k1.y);
+  } else {
+    *reinterpret_cast<uint2*>(o + c0) = k0;
+    *reinterpret_cast<uint2*>(o + c1) = k1;
+  }
 }
 // 16 codes brought to the scale was / f.
 __device__ __forceinline__ void rescale16(uint4* p, float f) {
@@ -230,19 +350,14 @@ __device__ __forceinline__ void rescale16(uint4* p, float f) {
 // Many new tokens: a CTA takes a.hc blocks (page, head) of the keys or the
 // values one after the other, so that the angles of a page's tokens come from
 // L1 after the first.  TH = page * D / 32 threads: two units of every thread
-// are a whole block, held in registers between its maximum and its codes.
-// 64 registers a thread at most: the loads of 1024 threads per SM (64 bytes
-// each) are what the HBM's latency needs.
+// are a whole block, held in registers between its maximum and its codes,
+// while the next two blocks' loads are in flight.
 template <typename T, bool IL, int D, int TH>
-__global__ void __launch_bounds__(TH, 1024 / TH) k_rope_append(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(TH) k_rope_append(const __grid_constant__ Args a) {
   using E = typename T::type;
   constexpr int U = D / 16, ROWS = TH / U, IT = 2;  // threads per token, tokens per pass, passes
-  if ((int)blockIdx.x < a.q_blocks) {
-    turn_q<T, IL, D>(a, (int64_t)blockIdx.x * TH + threadIdx.x);
-    return;
-  }
   __shared__ uint32_t part[2][TH / 32];
-  int i = (int)blockIdx.x - a.q_blocks;
+  int i = blockIdx.x;
   const int hg = (a.Hkv + a.hc - 1) / a.hc, h0 = i % hg * a.hc, h1 = min(a.Hkv, h0 + a.hc);
   i /= hg;
   const bool is_v = i & 1;
@@ -256,19 +371,36 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_rope_append(const __grid_cons
   int c0, c1;
   unit_cols<IL>(u, a.rot, c0, c1);
   const bool turns = !is_v && u * 16 < a.rot;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const Ring<T, TH> ring(smem);
+  auto fetch = [&](int h) {
+    if (h < h1) {
+#pragma unroll
+      for (int it = 0; it < IT; ++it)
+        if (it * ROWS + r0 < k.tokens) {
+          const E* p = src + h * st.h + it * ROWS * st.t;
+          ring.fetch(h - h0, 2 * it, p + c0);
+          ring.fetch(h - h0, 2 * it + 1, p + c1);
+        }
+    }
+    ring.commit();
+  };
+#pragma unroll
+  for (int d = 0; d < Ring<T, TH>::DEPTH - 1; ++d) fetch(h0 + d);
   for (int h = h0; h < h1; ++h) {
     const int64_t blk = (int64_t)k.pid * a.Hkv + h;
     uint8_t* codes = (is_v ? a.v_codes : a.k_codes) + blk * a.page * D;
     float* scale = (is_v ? a.v_scale : a.k_scale) + blk;
+    const float was = k.slot0 ? *scale : 0.0f;  // slot 0 written now: a fresh block
+    fetch(h + Ring<T, TH>::DEPTH - 1);
+    ring.wait();
     float x0[IT][8], x1[IT][8];
 #pragma unroll
     for (int it = 0; it < IT; ++it)
       if (it * ROWS + r0 < k.tokens) {
-        const E* p = src + h * st.h + it * ROWS * st.t;
-        T::load8(p + c0, x0[it]);
-        T::load8(p + c1, x1[it]);
+        ring.read(h - h0, 2 * it, x0[it]);
+        ring.read(h - h0, 2 * it + 1, x1[it]);
       }
-    const float was = k.slot0 ? *scale : 0.0f;  // slot 0 written now: a fresh block
     float m = 0.0f;
 #pragma unroll
     for (int it = 0; it < IT; ++it)
@@ -297,6 +429,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_rope_append(const __grid_cons
         rescale16(reinterpret_cast<uint4*>(codes) + c, was * inv);
     if (threadIdx.x == 0) *scale = s;  // every thread read the old one before the barrier
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // Few new tokens (T <= G of 1, 2 or 4, or 8 at D = 64): G * D / 16 lanes take
@@ -350,20 +483,28 @@ __global__ void __launch_bounds__(FEW_THREADS) k_rope_append_few(const __grid_co
   }
 }
 
+template <typename T, bool IL, int D, int TH>
+void launch_cache(const Args& a, unsigned n, int64_t& blocks, cudaStream_t st) {
+  if (!tc::allow_smem<k_rope_append<T, IL, D, TH>>(Ring<T, TH>::BYTES))
+    blocks = -1;
+  else
+    k_rope_append<T, IL, D, TH><<<n, TH, Ring<T, TH>::BYTES, st>>>(a);
+}
+// blocks: of the largest launch (2^31 or more: nothing launched), -1: a CUDA call failed.
 template <typename T, bool IL, int D>
 void launch_d(Args& a, int64_t& blocks, cudaStream_t st) {
-  const int64_t q = (int64_t)a.B * a.T * ((a.H + QH - 1) / QH) * (D / 16);  // threads of the q part
   const int64_t items = (int64_t)a.B * a.W * 2 * a.Hkv;
-  auto grid = [&](int th, int64_t cache_ctas) {
-    a.q_blocks = (int)std::min<int64_t>((q + th - 1) / th, 1ll << 30);
-    blocks = (q + th - 1) / th + cache_ctas;
-    return (unsigned)blocks;
+  auto q_ctas = [&](int th) {
+    return ((int64_t)a.B * a.T * ((a.H + a.hq - 1) / a.hq) * (D / 16) + th - 1) / th;
   };
+  a.hq = QH;
   const int per_warp = 512 / D;  // tokens a warp holds
   if (a.T <= per_warp) {
     const int g = a.T == 1 ? 1 : a.T == 2 ? 2 : a.T <= 4 ? 4 : 8;
-    const unsigned n = grid(FEW_THREADS, (items * g * (D / 16) + FEW_THREADS - 1) / FEW_THREADS);
+    blocks = q_ctas(FEW_THREADS) + (items * g * (D / 16) + FEW_THREADS - 1) / FEW_THREADS;
     if (blocks >= (1ll << 31)) return;
+    a.q_blocks = (int)q_ctas(FEW_THREADS);
+    const unsigned n = (unsigned)blocks;
     if (g == 1)
       k_rope_append_few<T, IL, D, 1><<<n, FEW_THREADS, 0, st>>>(a);
     else if (g == 2)
@@ -374,18 +515,26 @@ void launch_d(Args& a, int64_t& blocks, cudaStream_t st) {
       k_rope_append_few<T, IL, D, 512 / D><<<n, FEW_THREADS, 0, st>>>(a);
     return;
   }
-  // several heads per CTA once there are CTAs for a few waves all the same
+  // more heads per thread and per CTA while the SMs are filled all the same:
+  // twice over by the q part, in 8 CTAs each by the cache part
+  const int sms = vq::mx::sm_count();
+  while (a.hq < a.H && q_ctas(Q_THREADS) >= 12 * sms) a.hq *= 2;
   a.hc = 1;
-  while (a.hc < 8 && a.hc < a.Hkv && items / (2 * a.hc) >= 16 * vq::mx::sm_count()) a.hc *= 2;
-  const int th = a.page * D / 32;
-  const unsigned n = grid(th, (int64_t)a.B * a.W * 2 * ((a.Hkv + a.hc - 1) / a.hc));
+  while (a.hc < 8 && a.hc < a.Hkv && items / (2 * a.hc) >= 8 * sms) a.hc *= 2;
+  blocks = std::max(q_ctas(Q_THREADS), (int64_t)a.B * a.W * 2 * ((a.Hkv + a.hc - 1) / a.hc));
   if (blocks >= (1ll << 31)) return;
+  if (!tc::allow_smem<k_turn_q<T, IL, D>>(Ring<T, Q_THREADS>::BYTES)) {
+    blocks = -1;
+    return;
+  }
+  k_turn_q<T, IL, D><<<(unsigned)q_ctas(Q_THREADS), Q_THREADS, Ring<T, Q_THREADS>::BYTES, st>>>(a);
+  const unsigned n = (unsigned)(a.B * a.W * 2 * ((a.Hkv + a.hc - 1) / a.hc));
   if (a.page == 32)
-    k_rope_append<T, IL, D, D><<<n, D, 0, st>>>(a);
+    launch_cache<T, IL, D, D>(a, n, blocks, st);
   else if (a.page == 64)
-    k_rope_append<T, IL, D, 2 * D><<<n, 2 * D, 0, st>>>(a);
+    launch_cache<T, IL, D, 2 * D>(a, n, blocks, st);
   else
-    k_rope_append<T, IL, D, 4 * D><<<n, 4 * D, 0, st>>>(a);
+    launch_cache<T, IL, D, 4 * D>(a, n, blocks, st);
 }
 template <typename T>
 void launch(Args& a, int D, int64_t& blocks, cudaStream_t st) {
@@ -426,7 +575,8 @@ extern "C" int vq_rope_append_kv8(const void* q, const void* k, const void* v, c
   const void* p16[6] = {q, k, v, q_out, k_codes, v_codes};
   for (const void* p : p16)
     if (reinterpret_cast<uintptr_t>(p) & 15) return VQ_ERR_ALIGNMENT;
-  if (reinterpret_cast<uintptr_t>(table) & 15) return VQ_ERR_ALIGNMENT;
+  if ((reinterpret_cast<uintptr_t>(table) & 15) || (reinterpret_cast<uintptr_t>(q_out) & 31))
+    return VQ_ERR_ALIGNMENT;
   for (int i = 0; i < 9; ++i)
     if (strides[i] * eb % 16) return VQ_ERR_ALIGNMENT;
   Args a;
@@ -452,6 +602,7 @@ extern "C" int vq_rope_append_kv8(const void* q, const void* k, const void* v, c
     launch<BF16>(a, head_dim, blocks, st);
   else
     launch<F32>(a, head_dim, blocks, st);
+  if (blocks < 0) return VQ_ERR_CUDA;
   if (blocks >= (1ll << 31)) return VQ_ERR_INVALID;
   return cudaGetLastError() == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
 }
