@@ -1,23 +1,19 @@
-"""Calling a kernel entry point with little host time: a decoding step's calls
-take a few microseconds on the device, so the wrapper's own time is the call's."""
+"""The native binding of the cached-decoding operators (``_decode.so``).
 
-import torch
+Its functions check their arguments, allocate the outputs and launch on the
+current stream of the tensors' device, all natively: a decoding step's calls
+take a few microseconds on the device, so a wrapper's own time is the call's.
+"""
+
+import torch  # noqa: F401  (its libraries are the binding's)
 
 from voyager_b200 import _lib
 
-# the current stream's handle as an integer, without a Stream object (0.1 us
-# against 2 us)
-raw_stream = torch._C._cuda_getCurrentRawStream
-_device = torch._C._cuda_getDevice
+_lib.load()
+try:
+    from voyager_b200 import _decode as native
+except ImportError as e:
+    raise ImportError("voyager_b200/_decode.so is missing or does not fit this torch: build it with "
+                      "`python -c 'import __graft_entry__ as g; g.build()'`") from e
 
-
-def call(fn, index: int, what: str, *args) -> None:
-    """``fn(*args, stream)`` on device ``index`` and its current stream; raises
-    the status it returns."""
-    if _device() == index:
-        st = fn(*args, raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            st = fn(*args, raw_stream(index))
-    if st:
-        _lib.check(st, what)
+native.bind(_lib.check)

@@ -5,13 +5,18 @@ Every ``csrc/*.cu`` and ``csrc/*.cpp`` file is compiled to an object under
 ``voyager_b200/libvoyager_b200.so``.  The CUDA runtime is linked statically,
 so the library needs only the driver at run time.  No fast-math: the
 numerics rely on IEEE division and round-to-nearest-even.
+
+``csrc/py/vq_decode_py.cpp`` becomes ``voyager_b200/_decode.so``, the CPython
+binding of the cached-decoding operators (g++, torch's headers and libraries).
 """
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 PROJ = os.path.dirname(PKG)
@@ -20,6 +25,8 @@ CSRC = os.path.join(PROJ, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(ROOT, "_build")
 OUT = os.path.join(PKG, "libvoyager_b200.so")
+PY_SRC = os.path.join(CSRC, "py", "vq_decode_py.cpp")
+PY_OUT = os.path.join(PKG, "_decode.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-ffp-contract=off",
@@ -66,6 +73,27 @@ def _compile(src: str, verbose: bool, extra) -> str:
     return obj
 
 
+def _build_binding(verbose: bool) -> None:
+    """``_decode.so``, linked with the library beside it and with torch's."""
+    if (os.path.exists(PY_OUT) and os.path.getmtime(PY_OUT) >= os.path.getmtime(PY_SRC)
+            and os.path.getmtime(PY_OUT) >= os.path.getmtime(os.path.join(INCLUDE, "voyager_b200.h"))):
+        return
+    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
+    inc = [INCLUDE, os.path.join(torch, "include"), os.path.join(torch, "include/torch/csrc/api/include"),
+           os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *[f"-I{inc[0]}"],
+           *[a for i in inc[1:] for a in ("-isystem", i)], "-D_GLIBCXX_USE_CXX11_ABI=1", PY_SRC, "-o", PY_OUT + ".tmp",
+           f"-L{PKG}", "-l:" + os.path.basename(OUT), f"-L{os.path.join(torch, 'lib')}", "-lc10", "-lc10_cuda",
+           "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {PY_SRC}:\n{r.stdout}\n{r.stderr}")
+    os.replace(PY_OUT + ".tmp", PY_OUT)
+
+
 def build(verbose: bool = False, extra=()) -> str:
     """Compile and link; returns the path of the shared object."""
     os.makedirs(BUILD, exist_ok=True)
@@ -74,6 +102,7 @@ def build(verbose: bool = False, extra=()) -> str:
         objs = list(ex.map(lambda s: _compile(s, verbose, list(extra)), srcs))
     newest = max(os.path.getmtime(o) for o in objs)
     if os.path.exists(OUT) and os.path.getmtime(OUT) >= newest:
+        _build_binding(verbose)
         return OUT
     cmd = [nvcc(), *ARCH, "-shared", "-o", OUT + ".tmp", *objs]
     if verbose:
@@ -82,6 +111,7 @@ def build(verbose: bool = False, extra=()) -> str:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(OUT + ".tmp", OUT)
+    _build_binding(verbose)
     return OUT
 
 
