@@ -50,7 +50,7 @@ struct Args {
   int64_t ldo;
   int M, N, nk;        // nk = ceil(K / 128)
   int mt, nt, tiles;   // tiles of this kernel's shape
-  int splits;          // k_fp8_few: CTAs of a cluster
+  int splits;          // CTAs of a cluster that share a tile's K (k_fp8_few, k_fp8_one)
   int vec, vec4;       // out rows take 4-byte, 8-byte stores
 };
 
@@ -262,10 +262,51 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+// Four neighbouring float32 sums at `p` (this CTA's shared address) of the
+// cluster's CTAs, added in rank order; all loads in flight together.
+__device__ __forceinline__ void cluster_sum4(uint32_t p, int splits, float (&v)[4]) {
+  float x[8][4];
+#pragma unroll
+  for (int r = 0; r < 8; ++r)
+    if (r < splits) {
+      const uint32_t src = splits > 1 ? mapa_shared(p, r) : p;
+      asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                   : "=f"(x[r][0]), "=f"(x[r][1]), "=f"(x[r][2]), "=f"(x[r][3]) : "r"(src) : "memory");
+    }
+  v[0] = v[1] = v[2] = v[3] = 0.0f;
+#pragma unroll
+  for (int r = 0; r < 8; ++r)
+    if (r < splits) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] += x[r][k];
+    }
+}
+// Four neighbouring outputs (+ bias) of a row, from column n on.
+__device__ __forceinline__ void store4(const Args& a, int row, int n, float (&v)[4]) {
+  uint16_t* o = a.out + (int64_t)row * a.ldo + n;
+  if (a.bias) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n + k < a.N) v[k] += BF16::load(a.bias + n + k);
+  }
+  if (a.vec4 && n + 4 <= a.N) {
+    *reinterpret_cast<uint2*>(o) = make_uint2(bf_pack(v[0], v[1]), bf_pack(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n + k < a.N) BF16::store(o + k, v[k]);
+  }
+}
+
 // ---------------------------------------------------------------------------
-// 128 x 128 tiles, one CTA each: four TMEM buffers of 128 columns.
+// 128 x 128 tiles: four TMEM buffers of 128 columns.  Persistent, one CTA per
+// tile; where there are tiles for half of the SMs or less, a cluster of
+// a.splits CTAs per tile, each with a part of K, whose float32 sums meet in
+// shared memory (the grid then has every tile's CTAs).
 struct One {
   static constexpr int STAGES = 6, STAGE = 2 * 128 * BK, BUFS = 4, THREADS = 384, COLS = 64;
+  static constexpr int LD = 132;  // floats per row of the sums in shared memory
+  static_assert(128 * LD * 4 <= STAGES * STAGE, "the sums fit the ring");
   static constexpr int SMEM = STAGES * STAGE + 8 * OUT_BYTES + 1024 + 256;
 };
 
@@ -283,6 +324,9 @@ __global__ void __launch_bounds__(One::THREADS, 1)
   const uint32_t drain = acc_empty0 + 8 * C::BUFS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::STAGES + 2 * C::BUFS + 1);
   const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = a.splits > 1 ? (int)cluster_ctarank() : 0;
+  const int first = blockIdx.x / a.splits, step = gridDim.x / a.splits;
+  const int kb0 = (int)((int64_t)a.nk * rank / a.splits), kb1 = (int)((int64_t)a.nk * (rank + 1) / a.splits);
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) mbar_init(full0 + 8 * s, 1), mbar_init(empty0 + 8 * s, 1);
     for (int s = 0; s < C::BUFS; ++s) mbar_init(acc_full0 + 8 * s, 1), mbar_init(acc_empty0 + 8 * s, 8);
@@ -303,10 +347,10 @@ __global__ void __launch_bounds__(One::THREADS, 1)
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < a.tiles && ok; t += gridDim.x) {
+    for (int t = first; t < a.tiles && ok; t += step) {
       int tm, tn;
       tile_of(a, t, tm, tn);
-      for (int kt = 0; kt < a.nk; ++kt) {
+      for (int kt = kb0; kt < kb1; ++kt) {
         if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, nullptr, ERR_EMPTY)) {
           ok = false;
           break;
@@ -324,8 +368,8 @@ __global__ void __launch_bounds__(One::THREADS, 1)
     int stage = 0, buf = 0;
     uint32_t phase = 0, bphase = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < a.tiles && ok; t += gridDim.x) {
-      for (int kt = 0; kt < a.nk; ++kt) {
+    for (int t = first; t < a.tiles && ok; t += step) {
+      for (int kt = kb0; kt < kb1; ++kt) {
         if (!mbar_wait_warp(acc_empty0 + 8 * buf, bphase ^ 1, nullptr, ERR_ACC) ||
             !mbar_wait_warp(full0 + 8 * stage, phase, nullptr, ERR_FULL)) {
           ok = false;
@@ -354,7 +398,7 @@ __global__ void __launch_bounds__(One::THREADS, 1)
     uint32_t* stage_out = out_stage + (warp - 4) * (OUT_BYTES / 4);
     int buf = 0;
     uint32_t bphase = 0;
-    for (int t = blockIdx.x; t < a.tiles; t += gridDim.x) {
+    for (int t = first; t < a.tiles; t += step) {
       int tm, tn;
       tile_of(a, t, tm, tn);
       const int r0 = tm * 128 + q * 32, col0 = tn * 128 + half * C::COLS;
@@ -363,7 +407,7 @@ __global__ void __launch_bounds__(One::THREADS, 1)
 #pragma unroll
       for (int i = 0; i < C::COLS / 2; ++i) acc[i] = 0;
       if (!promote<C::COLS, C::BUFS>(
-              acc, sa_of(a, r0 + lane), sw_of(a, tn), a.nk,
+              acc, sa_of(a, r0 + lane) + kb0, sw_of(a, tn) + kb0, kb1 - kb0,
               tmem + ((uint32_t)(q * 32) << 16) + half * C::COLS, 128, buf, bphase,
               [&](int b, uint32_t ph) { return mbar_wait_warp(acc_full0 + 8 * b, ph, nullptr, ERR_ACC); },
               [&](int b) {
@@ -371,14 +415,36 @@ __global__ void __launch_bounds__(One::THREADS, 1)
                 if (lane == 0) mbar_arrive(acc_empty0 + 8 * b);
               }))
         break;
-      store_rows<C::COLS>(a, acc, stage_out, r0, col0, lane);
+      if (a.splits == 1) {
+        store_rows<C::COLS>(a, acc, stage_out, r0, col0, lane);
+      } else {
+        // every MMA is done, so the ring is free: [128 rows][128 sums]
+        float* red = reinterpret_cast<float*>(smem) + (q * 32 + lane) * C::LD + half * C::COLS;
+#pragma unroll
+        for (int i = 0; i < C::COLS / 4; ++i) {
+          const float2 x = unpair(acc[2 * i]), y = unpair(acc[2 * i + 1]);
+          reinterpret_cast<float4*>(red)[i] = make_float4(x.x, x.y, y.x, y.y);
+        }
+      }
     }
   }
   __syncthreads();
+  if (a.splits > 1) {
+    cluster_sync();
+    int tm, tn;
+    tile_of(a, first, tm, tn);
+    // rows rank, rank + splits, ..; a warp takes a row
+    for (int r = rank + warp * a.splits; r < min(128, a.M - tm * 128); r += C::THREADS / 32 * a.splits) {
+      float v[4];
+      cluster_sum4(smem_u32(smem) + (r * C::LD + lane * 4) * 4, a.splits, v);
+      store4(a, tm * 128 + r, tn * 128 + lane * 4, v);
+    }
+  }
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }
+  if (a.splits > 1) cluster_sync();  // the peers have read this CTA's sums
 }
 
 // ---------------------------------------------------------------------------
@@ -532,8 +598,8 @@ __global__ void __launch_bounds__(Pair::THREADS, 1)
 template <int BN>
 struct Few {
   static constexpr int W_BYTES = 128 * BK, X_BYTES = BN * BK, STAGE = W_BYTES + X_BYTES;
-  static constexpr int STAGES = BN == 16 ? 6 : BN == 32 ? 5 : BN == 64 ? 4 : 3;
-  static constexpr int BUFS = BN == 128 ? 2 : 4;
+  static constexpr int STAGES = BN == 16 ? 6 : BN == 32 ? 5 : 4;
+  static constexpr int BUFS = 4;
   static constexpr int TMEM = BUFS * BN < 32 ? 32 : BUFS * BN;
   static constexpr int THREADS = 192;
   static constexpr int KC = 16;  // K blocks per refill of the scales
@@ -699,35 +765,9 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
   for (int i = threadIdx.x; i < BN * 32; i += C::THREADS) {
     const int j = (i >> 5) * a.splits + rank, f = (i & 31) * 4, n = tn * 128 + f;
     if (j >= ntok) break;
-    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const uint32_t p = red_addr + (j * C::LD + f) * 4;
-    float x[8][4];
-#pragma unroll
-    for (int r = 0; r < 8; ++r)
-      if (r < a.splits) {
-        const uint32_t src = a.splits > 1 ? mapa_shared(p, r) : p;
-        asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-                     : "=f"(x[r][0]), "=f"(x[r][1]), "=f"(x[r][2]), "=f"(x[r][3]) : "r"(src) : "memory");
-      }
-#pragma unroll
-    for (int r = 0; r < 8; ++r)
-      if (r < a.splits) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] += x[r][k];
-      }
-    uint16_t* o = a.out + (int64_t)(tm * BN + j) * a.ldo + n;
-    if (a.bias) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (n + k < a.N) v[k] += BF16::load(a.bias + n + k);
-    }
-    if (a.vec4 && n + 4 <= a.N) {
-      *reinterpret_cast<uint2*>(o) = make_uint2(bf_pack(v[0], v[1]), bf_pack(v[2], v[3]));
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (n + k < a.N) BF16::store(o + k, v[k]);
-    }
+    float v[4];
+    cluster_sum4(red_addr + (j * C::LD + f) * 4, a.splits, v);
+    store4(a, tm * BN + j, n, v);
   }
   if (warp == 1) {
     tc_fence_after();
@@ -737,6 +777,65 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
 }
 
 // ---------------------------------------------------------------------------
+// Clusters of s CTAs of kernel F that the device holds at once (asked once per
+// device and size): clusters of 3, for one, do not fill two CTAs per SM (288
+// CTAs in two waves took 18 us, 12 in one).
+template <auto F>
+int resident_clusters(int s, int threads, int smem) {
+  static int known[64][9] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  dev = dev < 0 || dev > 63 ? 0 : dev;
+  if (known[dev][s] == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(s);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = s, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, F, &cfg) != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      n = 1;
+    }
+    known[dev][s] = n;
+  }
+  return known[dev][s];
+}
+
+// K split so that the waves of resident clusters take least: blocks per CTA,
+// plus 6 for a CTA's start and, split, the join.
+template <auto F>
+int best_split(int tiles, int nk, int threads, int smem) {
+  int best = 1;
+  int64_t cost = 1ll << 60;
+  for (int s = 1; s <= 8 && s <= nk; ++s) {
+    const int64_t res = resident_clusters<F>(s, threads, smem);
+    const int64_t c = (tiles + res - 1) / res * ((nk + s - 1) / s + 6);
+    if (c < cost) cost = c, best = s;
+  }
+  return best;
+}
+
+template <auto F>
+int launch_clusters(int size, int grid, int threads, int smem, cudaStream_t st, const CUtensorMap& ma,
+                    const CUtensorMap& mw, const Args& a) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = size, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, F, ma, mw, a) == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
+}
+
 int launch_many(const void* x, const void* w, int64_t K, Args a, cudaStream_t st) {
   static_assert((2 * One::STAGES + 2 * One::BUFS + 2) * 8 <= 256 && (2 * Pair::STAGES + 6) * 8 <= 256,
                 "barrier areas");
@@ -752,53 +851,18 @@ int launch_many(const void* x, const void* w, int64_t K, Args a, cudaStream_t st
     a.mt = (a.M + 255) / 256;
     a.nt = (a.N + Pair::BN - 1) / Pair::BN;
     a.tiles = a.mt * a.nt;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * std::min(a.tiles, sms / 2));
-    cfg.blockDim = dim3(Pair::THREADS);
-    cfg.dynamicSmemBytes = Pair::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = 2, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k_fp8_pair, ma, mw, a) == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
+    return launch_clusters<k_fp8_pair>(2, 2 * std::min(a.tiles, sms / 2), Pair::THREADS, Pair::SMEM, st, ma, mw, a);
   }
   if (!vq::mx::make_map(&ma, x, a.M, K, 128) || !vq::mx::make_map(&mw, w, a.N, K, 128)) return VQ_ERR_CUDA;
   if (!allow_smem<k_fp8_one>(One::SMEM)) return VQ_ERR_CUDA;
   a.mt = (a.M + 127) / 128;
   a.nt = (a.N + 127) / 128;
   a.tiles = a.mt * a.nt;
+  a.splits = 2 * a.tiles <= sms ? best_split<k_fp8_one>(a.tiles, a.nk, One::THREADS, One::SMEM) : 1;
+  if (a.splits > 1)
+    return launch_clusters<k_fp8_one>(a.splits, a.tiles * a.splits, One::THREADS, One::SMEM, st, ma, mw, a);
   k_fp8_one<<<std::min(a.tiles, sms), One::THREADS, One::SMEM, st>>>(ma, mw, a);
   return cudaGetLastError() == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
-}
-
-// Clusters of s CTAs of k_fp8_few<BN> that the device holds at once (asked
-// once per device and size).
-template <int BN>
-int resident_clusters(int s) {
-  static int known[64][9] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  dev = dev < 0 || dev > 63 ? 0 : dev;
-  if (known[dev][s] == 0) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(s);
-    cfg.blockDim = dim3(Few<BN>::THREADS);
-    cfg.dynamicSmemBytes = Few<BN>::SMEM;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = s, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, k_fp8_few<BN>, &cfg) != cudaSuccess || n <= 0) {
-      (void)cudaGetLastError();
-      n = std::max(1, 2 * vq::mx::sm_count() / s);
-    }
-    known[dev][s] = n;
-  }
-  return known[dev][s];
 }
 
 template <int BN>
@@ -812,30 +876,8 @@ int launch_few(const void* x, const void* w, int64_t K, Args a, cudaStream_t st)
   a.mt = (a.M + BN - 1) / BN;
   a.nt = (a.N + 127) / 128;
   a.tiles = a.mt * a.nt;
-  // K split so that the waves of resident clusters take least: blocks per
-  // CTA, plus a constant 6 for a CTA's start and the join.  How many clusters
-  // of a size are resident at once is asked of the runtime: clusters of 3, for
-  // one, do not fill the 2 * 148 places (288 CTAs in two waves took 18 us, 15
-  // in one).
-  int best = 1;
-  int64_t cost = 1ll << 60;
-  for (int s = 1; s <= 8 && s <= a.nk; ++s) {
-    const int64_t res = resident_clusters<BN>(s);
-    const int64_t c = (a.tiles + res - 1) / res * ((a.nk + s - 1) / s + 6);
-    if (c < cost) cost = c, best = s;
-  }
-  a.splits = best;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.tiles * best));
-  cfg.blockDim = dim3(C::THREADS);
-  cfg.dynamicSmemBytes = C::SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = best, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k_fp8_few<BN>, mx_, mw, a) == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
+  a.splits = best_split<k_fp8_few<BN>>(a.tiles, a.nk, C::THREADS, C::SMEM);
+  return launch_clusters<k_fp8_few<BN>>(a.splits, a.tiles * a.splits, C::THREADS, C::SMEM, st, mx_, mw, a);
 }
 
 int sticky_f8(int* out, int clear, cudaStream_t st) { return vq::tc::sticky_read(out, clear, st); }
@@ -871,6 +913,5 @@ extern "C" int vq_linear_fp8_block(const void* x, const float* x_scale, const vo
   if (M <= 16) return launch_few<16>(x, w, K, a, st);
   if (M <= 32) return launch_few<32>(x, w, K, a, st);
   if (M <= 64) return launch_few<64>(x, w, K, a, st);
-  if (M <= 128) return launch_few<128>(x, w, K, a, st);
   return launch_many(x, w, K, a, st);
 }
