@@ -41,6 +41,7 @@
 
 #include "voyager_b200.h"
 #include "vq_e4m3.cuh"
+#include "vq_pdl.cuh"
 #include "vq_tc.cuh"
 
 namespace vq {
@@ -182,10 +183,17 @@ __global__ void __launch_bounds__(THREADS)
   __shared__ int2 s_plan[PLANS];  // the first sequences' plans
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  pdl::trigger();
   if (lane == 0) {
     for (int s = 0; s < C::STAGES; ++s) mbar_init(smem_u32(bars + warp * C::STAGES + s), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+
+  if (threadIdx.x == 0) {
+    prefetch_map(&map_k);
+    prefetch_map(&map_v);
+  }
+  pdl::wait();
 
   // ---- this CTA's run of units: a scan of the entries' unit counts (and, in
   // the upper 32 bits, of the entries that have any) ----
@@ -797,8 +805,7 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int ctas
   static_assert(WARPS * C::STAGES * 8 <= 256, "barrier area");
   if (!allow_smem<k_attn_kv8<D, NT>>(C::SMEM))
     return VQ_ERR_CUDA;
-  k_attn_kv8<D, NT><<<ctas, THREADS, C::SMEM, st>>>(mk, mv, a);
-  return cudaGetLastError() == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
+  return pdl::launch<k_attn_kv8<D, NT>>(ctas, THREADS, C::SMEM, st, 1, mk, mv, a) ? VQ_OK : VQ_ERR_CUDA;
 }
 
 int sticky_kva(int* out, int clear, cudaStream_t st) { return vq::tc::sticky_read(out, clear, st); }

@@ -21,6 +21,7 @@
 
 #include "voyager_b200.h"
 #include "vq_e4m3.cuh"
+#include "vq_pdl.cuh"
 #include "vq_tc.cuh"
 
 namespace vq {
@@ -84,6 +85,8 @@ __global__ void __launch_bounds__(MAXT) k_norm_vec(const Args a) {
   const E* x = reinterpret_cast<const E*>(a.x);
   const E* r = reinterpret_cast<const E*>(a.r);
   const E* w = reinterpret_cast<const E*>(a.w);
+  pdl::trigger();
+  pdl::wait();
   auto col = [&](int i) { return (i * (int)blockDim.x + (int)threadIdx.x) * 8; };
   Raw rx[NV] = {}, rr[NV] = {}, rw[NV] = {};
   auto fetch = [&](int64_t row) {
@@ -185,6 +188,8 @@ __global__ void __launch_bounds__(1024) k_norm_blocks(const Args a) {
   using E = typename T::type;
   constexpr int PER = 4 / VEC;  // loads of a lane per block
   __shared__ float part[32];
+  pdl::trigger();
+  pdl::wait();
   const int64_t row = blockIdx.x;
   const E* x = reinterpret_cast<const E*>(a.x) + row * a.ldx;
   const E* r = reinterpret_cast<const E*>(a.r) + row * a.ldr;
@@ -262,6 +267,8 @@ template <typename T>
 __global__ void __launch_bounds__(1024) k_norm_any(const Args a) {
   using E = typename T::type;
   __shared__ float part[32];
+  pdl::trigger();
+  pdl::wait();
   const int64_t row = blockIdx.x;
   const E* x = reinterpret_cast<const E*>(a.x) + row * a.ldx;
   const E* r = a.r ? reinterpret_cast<const E*>(a.r) + row * a.ldr : nullptr;
@@ -307,7 +314,7 @@ __global__ void __launch_bounds__(1024) k_norm_any(const Args a) {
 
 // As many CTAs as fit at once (asked once per device and CTA size), or one per row.
 template <typename T, int NV, int MAXT>
-void launch_vec(const Args& a, int threads, cudaStream_t st) {
+bool launch_vec(const Args& a, int threads, cudaStream_t st) {
   static int known[64][33] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -322,26 +329,28 @@ void launch_vec(const Args& a, int threads, cudaStream_t st) {
     per_sm = n;
   }
   const int64_t grid = std::min<int64_t>(a.rows, (int64_t)per_sm * vq::mx::sm_count());
-  k_norm_vec<T, NV, MAXT><<<(unsigned)grid, threads, 0, st>>>(a);
+  if (a.rows > grid)  // long enough
+    return pdl::launch<k_norm_vec<T, NV, MAXT>, false>((unsigned)grid, threads, 0, st, 1, a);
+  return pdl::launch<k_norm_vec<T, NV, MAXT>>((unsigned)grid, threads, 0, st, 1, a);
 }
 
 template <typename T, int VEC>
-void launch_blocks(const Args& a, cudaStream_t st) {
+bool launch_blocks(const Args& a, cudaStream_t st) {
   // a block a warp while there are few rows (latency), four for many
   const int nb = a.rows < 256 && a.nblk <= 32 ? 1 : a.nblk <= 2 ? 1 : a.nblk <= 6 ? 2 : 4;
   const int threads = (a.nblk + nb - 1) / nb * 32;
   const unsigned rows = (unsigned)a.rows;
   if (nb == 1)
-    k_norm_blocks<T, 1, VEC><<<rows, threads, 0, st>>>(a);
+    return pdl::launch<k_norm_blocks<T, 1, VEC>>(rows, threads, 0, st, 1, a);
   else if (nb == 2)
-    k_norm_blocks<T, 2, VEC><<<rows, threads, 0, st>>>(a);
+    return pdl::launch<k_norm_blocks<T, 2, VEC>>(rows, threads, 0, st, 1, a);
   else
-    k_norm_blocks<T, 4, VEC><<<rows, threads, 0, st>>>(a);
+    return pdl::launch<k_norm_blocks<T, 4, VEC>>(rows, threads, 0, st, 1, a);
 }
 
 // vec: elements that every row start keeps together (8, 2 or 1).
 template <typename T>
-void launch(const Args& a, int vec, cudaStream_t st) {
+bool launch(const Args& a, int vec, cudaStream_t st) {
   const int groups = (a.cols + 7) / 8;
   const unsigned rows = (unsigned)a.rows;
   if (vec == 8 && groups <= 4096) {
@@ -351,15 +360,15 @@ void launch(const Args& a, int vec, cudaStream_t st) {
     while (groups > nv * (a.rows < 256 ? 1024 : 256) && nv < 4) nv *= 2;
     const int threads = std::min(1024, ((groups + nv - 1) / nv + 31) / 32 * 32);
     if (nv == 1)
-      threads <= 256 ? launch_vec<T, 1, 256>(a, threads, st) : launch_vec<T, 1, 1024>(a, threads, st);
+      return threads <= 256 ? launch_vec<T, 1, 256>(a, threads, st) : launch_vec<T, 1, 1024>(a, threads, st);
     else if (nv == 2)
-      threads <= 256 ? launch_vec<T, 2, 256>(a, threads, st) : launch_vec<T, 2, 1024>(a, threads, st);
+      return threads <= 256 ? launch_vec<T, 2, 256>(a, threads, st) : launch_vec<T, 2, 1024>(a, threads, st);
     else
-      threads <= 256 ? launch_vec<T, 4, 256>(a, threads, st) : launch_vec<T, 4, 1024>(a, threads, st);
+      return threads <= 256 ? launch_vec<T, 4, 256>(a, threads, st) : launch_vec<T, 4, 1024>(a, threads, st);
   } else if (a.nblk <= 128) {
-    vec >= 2 ? launch_blocks<T, 2>(a, st) : launch_blocks<T, 1>(a, st);
+    return vec >= 2 ? launch_blocks<T, 2>(a, st) : launch_blocks<T, 1>(a, st);
   } else {
-    k_norm_any<T><<<rows, 1024, 0, st>>>(a);
+    return pdl::launch<k_norm_any<T>>(rows, 1024, 0, st, 1, a);
   }
 }
 
@@ -403,9 +412,6 @@ extern "C" int vq_norm_quantize_fp8(const void* x, int64_t ldx, const void* resi
   };
   const int vec = keeps(8) ? 8 : keeps(2) ? 2 : 1;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == VQ_BF16)
-    launch<BF16>(a, vec, st);
-  else
-    launch<F32>(a, vec, st);
-  return cudaGetLastError() == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
+  const bool ok = dtype == VQ_BF16 ? launch<BF16>(a, vec, st) : launch<F32>(a, vec, st);
+  return ok ? VQ_OK : VQ_ERR_CUDA;
 }

@@ -31,6 +31,7 @@
 
 #include "voyager_b200.h"
 #include "vq_e4m3.cuh"
+#include "vq_pdl.cuh"
 #include "vq_tc.cuh"
 
 namespace vq {
@@ -327,11 +328,25 @@ __global__ void __launch_bounds__(One::THREADS, 1)
   const int rank = a.splits > 1 ? (int)cluster_ctarank() : 0;
   const int first = blockIdx.x / a.splits, step = gridDim.x / a.splits;
   const int kb0 = (int)((int64_t)a.nk * rank / a.splits), kb1 = (int)((int64_t)a.nk * (rank + 1) / a.splits);
+  pdl::trigger();
+  auto load = [&](int tm, int tn, int kt, int stage) {
+    const uint32_t dst = smem_u32(smem) + stage * C::STAGE;
+    mbar_expect_tx(full0 + 8 * stage, C::STAGE);
+    tma_load_2d(dst, &map_a, kt * BK, tm * 128, full0 + 8 * stage);
+    tma_load_2d(dst + 128 * BK, &map_w, kt * BK, tn * 128, full0 + 8 * stage);
+  };
+  const int pre = min(C::STAGES, kb1 - kb0);  // loads that need no one's leave
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) mbar_init(full0 + 8 * s, 1), mbar_init(empty0 + 8 * s, 1);
     for (int s = 0; s < C::BUFS; ++s) mbar_init(acc_full0 + 8 * s, 1), mbar_init(acc_empty0 + 8 * s, 8);
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&map_a);
+    prefetch_map(&map_w);
+    pdl::wait();
+    int tm, tn;
+    tile_of(a, first, tm, tn);
+    for (int i = 0; i < pre; ++i) load(tm, tn, kb0 + i, i);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -342,23 +357,21 @@ __global__ void __launch_bounds__(One::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl::wait();
 
   if (warp == 0 && lane == 0) {
-    int stage = 0;
-    uint32_t phase = 0;
+    int stage = pre == C::STAGES ? 0 : pre;
+    uint32_t phase = pre == C::STAGES ? 1 : 0;
     bool ok = true;
     for (int t = first; t < a.tiles && ok; t += step) {
       int tm, tn;
       tile_of(a, t, tm, tn);
-      for (int kt = kb0; kt < kb1; ++kt) {
+      for (int kt = t == first ? kb0 + pre : kb0; kt < kb1; ++kt) {
         if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, nullptr, ERR_EMPTY)) {
           ok = false;
           break;
         }
-        const uint32_t dst = smem_u32(smem) + stage * C::STAGE;
-        mbar_expect_tx(full0 + 8 * stage, C::STAGE);
-        tma_load_2d(dst, &map_a, kt * BK, tm * 128, full0 + 8 * stage);
-        tma_load_2d(dst + 128 * BK, &map_w, kt * BK, tn * 128, full0 + 8 * stage);
+        load(tm, tn, kt, stage);
         if (++stage == C::STAGES) stage = 0, phase ^= 1;
       }
     }
@@ -485,6 +498,7 @@ __global__ void __launch_bounds__(Pair::THREADS, 1)
   const uint32_t rank = cluster_ctarank();  // 0: issues the pair's MMAs
   const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int pair_id = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  pdl::trigger();
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) mbar_init(full0 + 8 * s, 1), mbar_init(empty0 + 8 * s, 1);
     for (int s = 0; s < 2; ++s) mbar_init(acc_full0 + 8 * s, 1), mbar_init(acc_empty0 + 8 * s, 16);
@@ -500,6 +514,7 @@ __global__ void __launch_bounds__(Pair::THREADS, 1)
   cluster_sync();  // both CTAs' barriers exist before any use across them
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl::wait();
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::ISSUE_REGS));
@@ -624,6 +639,7 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
   const uint32_t drain = acc_empty0 + 8 * C::BUFS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::STAGES + 2 * C::BUFS + 1);
   const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  pdl::trigger();
   const int rank = a.splits > 1 ? (int)cluster_ctarank() : 0;
   const int tile = blockIdx.x / a.splits, tm = tile / a.nt, tn = tile - tm * a.nt;
   const int kb0 = (int)((int64_t)a.nk * rank / a.splits);
@@ -639,6 +655,9 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
     for (int s = 0; s < C::BUFS; ++s) mbar_init(acc_full0 + 8 * s, 1), mbar_init(acc_empty0 + 8 * s, 4);
     mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_map(&map_x);
+    prefetch_map(&map_w);
+    pdl::wait();
     // the ring's first round needs no one's leave
     for (int i = 0; i < min(C::STAGES, kb1 - kb0); ++i) load(kb0 + i, i);
   }
@@ -651,6 +670,7 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl::wait();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -820,22 +840,6 @@ int best_split(int tiles, int nk, int threads, int smem) {
   return best;
 }
 
-template <auto F>
-int launch_clusters(int size, int grid, int threads, int smem, cudaStream_t st, const CUtensorMap& ma,
-                    const CUtensorMap& mw, const Args& a) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = size, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, F, ma, mw, a) == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
-}
-
 int launch_many(const void* x, const void* w, int64_t K, Args a, cudaStream_t st) {
   static_assert((2 * One::STAGES + 2 * One::BUFS + 2) * 8 <= 256 && (2 * Pair::STAGES + 6) * 8 <= 256,
                 "barrier areas");
@@ -851,7 +855,8 @@ int launch_many(const void* x, const void* w, int64_t K, Args a, cudaStream_t st
     a.mt = (a.M + 255) / 256;
     a.nt = (a.N + Pair::BN - 1) / Pair::BN;
     a.tiles = a.mt * a.nt;
-    return launch_clusters<k_fp8_pair>(2, 2 * std::min(a.tiles, sms / 2), Pair::THREADS, Pair::SMEM, st, ma, mw, a);
+    return pdl::launch<k_fp8_pair>(2 * std::min(a.tiles, sms / 2), Pair::THREADS, Pair::SMEM, st, 2, ma, mw, a)
+               ? VQ_OK : VQ_ERR_CUDA;
   }
   if (!vq::mx::make_map(&ma, x, a.M, K, 128) || !vq::mx::make_map(&mw, w, a.N, K, 128)) return VQ_ERR_CUDA;
   if (!allow_smem<k_fp8_one>(One::SMEM)) return VQ_ERR_CUDA;
@@ -859,10 +864,8 @@ int launch_many(const void* x, const void* w, int64_t K, Args a, cudaStream_t st
   a.nt = (a.N + 127) / 128;
   a.tiles = a.mt * a.nt;
   a.splits = 2 * a.tiles <= sms ? best_split<k_fp8_one>(a.tiles, a.nk, One::THREADS, One::SMEM) : 1;
-  if (a.splits > 1)
-    return launch_clusters<k_fp8_one>(a.splits, a.tiles * a.splits, One::THREADS, One::SMEM, st, ma, mw, a);
-  k_fp8_one<<<std::min(a.tiles, sms), One::THREADS, One::SMEM, st>>>(ma, mw, a);
-  return cudaGetLastError() == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
+  const int grid = a.splits > 1 ? a.tiles * a.splits : std::min(a.tiles, sms);
+  return pdl::launch<k_fp8_one>(grid, One::THREADS, One::SMEM, st, a.splits, ma, mw, a) ? VQ_OK : VQ_ERR_CUDA;
 }
 
 template <int BN>
@@ -877,7 +880,8 @@ int launch_few(const void* x, const void* w, int64_t K, Args a, cudaStream_t st)
   a.nt = (a.N + 127) / 128;
   a.tiles = a.mt * a.nt;
   a.splits = best_split<k_fp8_few<BN>>(a.tiles, a.nk, C::THREADS, C::SMEM);
-  return launch_clusters<k_fp8_few<BN>>(a.splits, a.tiles * a.splits, C::THREADS, C::SMEM, st, mx_, mw, a);
+  return pdl::launch<k_fp8_few<BN>>(a.tiles * a.splits, C::THREADS, C::SMEM, st, a.splits, mx_, mw, a)
+             ? VQ_OK : VQ_ERR_CUDA;
 }
 
 int sticky_f8(int* out, int clear, cudaStream_t st) { return vq::tc::sticky_read(out, clear, st); }

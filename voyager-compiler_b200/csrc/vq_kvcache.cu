@@ -26,6 +26,7 @@
 
 #include "voyager_b200.h"
 #include "vq_e4m3.cuh"
+#include "vq_pdl.cuh"
 #include "vq_tc.cuh"
 
 namespace vq {
@@ -246,6 +247,8 @@ __global__ void __launch_bounds__(Q_THREADS) k_turn_q(const __grid_constant__ Ar
   using E = typename T::type;
   extern __shared__ __align__(16) uint8_t smem[];
   const Ring<T, Q_THREADS> ring(smem);
+  pdl::trigger();
+  pdl::wait();
   const QUnit x = q_unit<IL, D>(a, (int64_t)blockIdx.x * Q_THREADS + threadIdx.x);
   if (!x.any) return;
   E* out = reinterpret_cast<E*>(a.q_out) + x.row * a.H * D;
@@ -357,6 +360,8 @@ __global__ void __launch_bounds__(TH) k_rope_append(const __grid_constant__ Args
   using E = typename T::type;
   constexpr int U = D / 16, ROWS = TH / U, IT = 2;  // threads per token, tokens per pass, passes
   __shared__ uint32_t part[2][TH / 32];
+  pdl::trigger();
+  pdl::wait();
   int i = blockIdx.x;
   const int hg = (a.Hkv + a.hc - 1) / a.hc, h0 = i % hg * a.hc, h1 = min(a.Hkv, h0 + a.hc);
   i /= hg;
@@ -439,6 +444,8 @@ template <typename T, bool IL, int D, int G>
 __global__ void __launch_bounds__(FEW_THREADS) k_rope_append_few(const __grid_constant__ Args a) {
   using E = typename T::type;
   constexpr int U = D / 16, L = G * U;  // lanes per block
+  pdl::trigger();
+  pdl::wait();
   if ((int)blockIdx.x < a.q_blocks) {
     turn_q<T, IL, D>(a, (int64_t)blockIdx.x * FEW_THREADS + threadIdx.x);
     return;
@@ -485,10 +492,9 @@ __global__ void __launch_bounds__(FEW_THREADS) k_rope_append_few(const __grid_co
 
 template <typename T, bool IL, int D, int TH>
 void launch_cache(const Args& a, unsigned n, int64_t& blocks, cudaStream_t st) {
-  if (!tc::allow_smem<k_rope_append<T, IL, D, TH>>(Ring<T, TH>::BYTES))
+  if (!tc::allow_smem<k_rope_append<T, IL, D, TH>>(Ring<T, TH>::BYTES) ||
+      !pdl::launch<k_rope_append<T, IL, D, TH>, false>(n, TH, Ring<T, TH>::BYTES, st, 1, a))
     blocks = -1;
-  else
-    k_rope_append<T, IL, D, TH><<<n, TH, Ring<T, TH>::BYTES, st>>>(a);
 }
 // blocks: of the largest launch (2^31 or more: nothing launched), -1: a CUDA call failed.
 template <typename T, bool IL, int D>
@@ -505,14 +511,11 @@ void launch_d(Args& a, int64_t& blocks, cudaStream_t st) {
     if (blocks >= (1ll << 31)) return;
     a.q_blocks = (int)q_ctas(FEW_THREADS);
     const unsigned n = (unsigned)blocks;
-    if (g == 1)
-      k_rope_append_few<T, IL, D, 1><<<n, FEW_THREADS, 0, st>>>(a);
-    else if (g == 2)
-      k_rope_append_few<T, IL, D, 2><<<n, FEW_THREADS, 0, st>>>(a);
-    else if (g == 4)
-      k_rope_append_few<T, IL, D, 4><<<n, FEW_THREADS, 0, st>>>(a);
-    else
-      k_rope_append_few<T, IL, D, 512 / D><<<n, FEW_THREADS, 0, st>>>(a);
+    const bool ok = g == 1   ? pdl::launch<k_rope_append_few<T, IL, D, 1>>(n, FEW_THREADS, 0, st, 1, a)
+                    : g == 2 ? pdl::launch<k_rope_append_few<T, IL, D, 2>>(n, FEW_THREADS, 0, st, 1, a)
+                    : g == 4 ? pdl::launch<k_rope_append_few<T, IL, D, 4>>(n, FEW_THREADS, 0, st, 1, a)
+                             : pdl::launch<k_rope_append_few<T, IL, D, 512 / D>>(n, FEW_THREADS, 0, st, 1, a);
+    if (!ok) blocks = -1;
     return;
   }
   // more heads per thread and per CTA while the SMs are filled all the same:
@@ -523,11 +526,11 @@ void launch_d(Args& a, int64_t& blocks, cudaStream_t st) {
   while (a.hc < 8 && a.hc < a.Hkv && items / (2 * a.hc) >= 8 * sms) a.hc *= 2;
   blocks = std::max(q_ctas(Q_THREADS), (int64_t)a.B * a.W * 2 * ((a.Hkv + a.hc - 1) / a.hc));
   if (blocks >= (1ll << 31)) return;
-  if (!tc::allow_smem<k_turn_q<T, IL, D>>(Ring<T, Q_THREADS>::BYTES)) {
+  if (!tc::allow_smem<k_turn_q<T, IL, D>>(Ring<T, Q_THREADS>::BYTES) ||
+      !pdl::launch<k_turn_q<T, IL, D>, false>((unsigned)q_ctas(Q_THREADS), Q_THREADS, Ring<T, Q_THREADS>::BYTES, st, 1, a)) {
     blocks = -1;
     return;
   }
-  k_turn_q<T, IL, D><<<(unsigned)q_ctas(Q_THREADS), Q_THREADS, Ring<T, Q_THREADS>::BYTES, st>>>(a);
   const unsigned n = (unsigned)(a.B * a.W * 2 * ((a.Hkv + a.hc - 1) / a.hc));
   if (a.page == 32)
     launch_cache<T, IL, D, D>(a, n, blocks, st);
@@ -604,5 +607,5 @@ extern "C" int vq_rope_append_kv8(const void* q, const void* k, const void* v, c
     launch<F32>(a, head_dim, blocks, st);
   if (blocks < 0) return VQ_ERR_CUDA;
   if (blocks >= (1ll << 31)) return VQ_ERR_INVALID;
-  return cudaGetLastError() == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
+  return VQ_OK;
 }
