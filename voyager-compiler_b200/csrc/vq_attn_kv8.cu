@@ -70,11 +70,17 @@ struct Args {
   float sm_log2;              // sm_scale * log2(e)
 };
 
+// CTAs per SM.  Three with heads of 64 and one row tile (24 sequences of 28631
+// keys: 130 us against 149 with two); otherwise the third CTA costs more in
+// joins and shallower rings than its warps give (heads of 128, 32 sequences:
+// 66 us against 55).
+constexpr int ctas_per_sm(int head_dim, int nt) { return head_dim == 64 && nt == 1 ? 3 : 2; }
+
 template <int D, int NT>
 struct Cfg {
   static constexpr int ROWS = 8 * NT;
   static constexpr int TILE_BYTES = TILE * D;
-  static constexpr int STAGES = D == 128 ? 3 : 5;
+  static constexpr int PER_SM = ctas_per_sm(D, NT), STAGES = D == 128 ? 3 : PER_SM == 3 ? 4 : 5;
   static constexpr int RING = STAGES * 2 * TILE_BYTES;  // per warp
   static constexpr int SMEM_RING = WARPS * RING;
   // the warps' O meet in SUMS buffers, rows LD floats apart
@@ -82,7 +88,8 @@ struct Cfg {
   static constexpr int JOIN = (SUMS * ROWS * LD + 3 * WARPS * ROWS + 4 * ROWS) * 4;
   static constexpr int SMEM = SMEM_RING + JOIN + 1024 + 256;
   static_assert(JOIN % 16 == 0 && WARPS * STAGES * 8 <= 256, "barriers after the join's area");
-  static_assert(2 * (SMEM + 4096) <= 227 * 1024, "two CTAs per SM");
+  static_assert(3 * ROWS <= THREADS, "a thread for each of a row's m, l and w");
+  static_assert(PER_SM * (SMEM + 3200 + 1024) <= 227 * 1024, "CTAs per SM");
 };
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -168,7 +175,7 @@ __device__ __forceinline__ Entry entry_of(const Args& a, int e, int2 plan) {
 __device__ __forceinline__ int units_of(const Entry& x) { return (x.end + UNIT - 1) / UNIT; }
 
 template <int D, int NT>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
     k_attn_kv8(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                const __grid_constant__ Args a) {
   using C = Cfg<D, NT>;
@@ -563,22 +570,21 @@ __global__ void __launch_bounds__(THREADS)
     } else {
       // 0 * NaN is NaN, also for a row that may not see the value: each row
       // gets a product of its own with the values it does not see taken as 0
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
 #pragma unroll 1
-      for (int n8 = 0; n8 < C::ROWS; ++n8) {
-        const int last = held + (row0 + n8) / a.G;
-        uint32_t x[2][4][VW];
+        for (int r = 0; r < 8; ++r) {
+          const int last = held + (row0 + n * 8 + r) / a.G;
+          uint32_t x[2][4][VW];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int w = 0; w < VW; ++w)
-              x[mt][k][w] =
-                  key0 + mt * 16 + 2 * t + (k & 1) + (k >> 1) * 8 > last ? 0u : v[mt][k][w];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          if (n != n8 >> 3) continue;
-          const bool c0 = (n8 & 7) == 2 * t, c1 = (n8 & 7) == 2 * t + 1;
+              for (int w = 0; w < VW; ++w)
+                x[mt][k][w] =
+                    key0 + mt * 16 + 2 * t + (k & 1) + (k >> 1) * 8 > last ? 0u : v[mt][k][w];
+          const bool c0 = r == 2 * t, c1 = r == 2 * t + 1;
 #pragma unroll
           for (int j = 0; j < KS; ++j) {
             float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -587,7 +593,6 @@ __global__ void __launch_bounds__(THREADS)
             if (c1) o[n][j][1] += acc[1], o[n][j][3] += acc[3];
           }
         }
-      }
     }
     __syncwarp();  // every lane has read the stage
     if (issued < mine) issue();
@@ -714,7 +719,7 @@ __global__ void __launch_bounds__(THREADS)
   const int slot0 = run_begin(c0) >= cur.ps ? 0 : 1;  // the first CTA's run may begin before the head
   auto piece = [&](int c) { return a.part + ((int64_t)(c0 + c) * 2 + (c == 0 ? slot0 : 0)) * PART; };
   // a group of D / 8 lanes takes a row, eight places a lane
-  constexpr int LPR = D / 8, GROUPS = THREADS / LPR, PRE = 8;
+  constexpr int LPR = D / 8, GROUPS = THREADS / LPR, PRE = C::PER_SM == 3 ? 4 : 8;
   const int gl = lane % LPR, gbase = lane - gl;
   const int rounds = (cur.nrows + GROUPS - 1) / GROUPS;
   for (int k = 0; k < rounds; ++k) {
@@ -784,18 +789,22 @@ __global__ void __launch_bounds__(THREADS)
   }
 }
 
-// How a call's work is cut: row tiles of 8, row groups, and CTAs: two per SM,
-// or one per unit where the longest lengths give fewer.
+// How a call's work is cut: row tiles of 8, row groups, and CTAs: as many as
+// fit at once, or one per unit where the longest lengths give fewer.
 struct Cut {
   int nt, groups, ctas;
 };
-Cut cut_of(int64_t batch, int64_t tokens, int heads, int kv_heads, int64_t capacity) {
+Cut cut_of(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim, int64_t capacity) {
   Cut c;
-  const int64_t rows = tokens * (heads / kv_heads);
-  c.nt = rows > 8 ? 2 : 1;
-  c.groups = (int)((rows + 8 * c.nt - 1) / (8 * c.nt));
+  // Row tiles per group: two.  Three, which fit the registers at heads of 64,
+  // where the tiles come out even (96 rows: 120 us against 129, 24 rows 48
+  // against 55; 35 rows would take 32 against 26).
+  const int64_t tiles = (tokens * (heads / kv_heads) + 7) / 8;
+  const int64_t most = head_dim == 64 && tiles % 3 == 0 ? 3 : 2;
+  c.groups = (int)((tiles + most - 1) / most);
+  c.nt = (int)((tiles + c.groups - 1) / c.groups);
   const int64_t units = std::max<int64_t>(1, (capacity + UNIT - 1) / UNIT);
-  c.ctas = (int)std::min<int64_t>(2 * vq::mx::sm_count(), batch * c.groups * kv_heads * units);
+  c.ctas = (int)std::min<int64_t>(ctas_per_sm(head_dim, c.nt) * vq::mx::sm_count(), batch * c.groups * kv_heads * units);
   return c;
 }
 
@@ -825,7 +834,7 @@ int vq_attn_kv8_workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t 
       page <= 0 || table_width < 0)
     return VQ_ERR_INVALID;
   const Cut c = cut_of(std::max<int64_t>(batch, 1), std::max<int64_t>(tokens, 1), heads, kv_heads,
-                       table_width * page);
+                       head_dim, table_width * page);
   *counters = batch * kv_heads * c.groups;
   *floats = (int64_t)c.ctas * 2 * 8 * c.nt * (head_dim + 3);
   return VQ_OK;
@@ -852,7 +861,7 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
     if (reinterpret_cast<uintptr_t>(p) & 15) return VQ_ERR_ALIGNMENT;
   for (int i = 0; i < 3; ++i)
     if (q_strides[i] % 8) return VQ_ERR_ALIGNMENT;
-  const Cut c = cut_of(batch, tokens, heads, kv_heads, table_width * page);
+  const Cut c = cut_of(batch, tokens, heads, kv_heads, head_dim, table_width * page);
   const int64_t pairs = batch * kv_heads * c.groups;
   // the units of all heads, counted in 32 bits
   if (pairs * ((table_width * page + UNIT - 1) / UNIT + 8) >= (1ll << 31) || counters_len < pairs)
@@ -884,8 +893,11 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
   a.groups = c.groups;
   a.sm_log2 = sm_scale * 1.4426950408889634f;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (head_dim == 128) return c.nt == 1 ? launch<128, 1>(mk, mv, a, c.ctas, st) : launch<128, 2>(mk, mv, a, c.ctas, st);
-  return c.nt == 1 ? launch<64, 1>(mk, mv, a, c.ctas, st) : launch<64, 2>(mk, mv, a, c.ctas, st);
+  if (head_dim == 128)
+    return c.nt == 1 ? launch<128, 1>(mk, mv, a, c.ctas, st) : launch<128, 2>(mk, mv, a, c.ctas, st);
+  return c.nt == 1   ? launch<64, 1>(mk, mv, a, c.ctas, st)
+         : c.nt == 2 ? launch<64, 2>(mk, mv, a, c.ctas, st)
+                     : launch<64, 3>(mk, mv, a, c.ctas, st);
 }
 
 }  // extern "C"
