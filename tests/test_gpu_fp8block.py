@@ -114,6 +114,34 @@ def test_norm_special_values():
         assert not bool(codes[2, :256].float().isnan().any()) and not bool(scale[2, :2].isnan().any())
 
 
+@pytest.mark.parametrize("C", [1024, 1022, 1021, 40001])
+def test_quantize_extremes(C):
+    """Blocks whose largest magnitude lies at the ends of float32's range: the
+    codes follow the quotient in the reals, the scale is rounded once more
+    where it is denormal, a scale that underflows counts as 0 (scale 1), and an
+    infinity leaves 0 in the rest of its block."""
+    from voyager_b200 import fp8block
+
+    g = _gen(2)
+    x = torch.rand(2, C, generator=g, device="cuda") * 2 - 1
+    tops = [3.4e38, 1e38, 2.0**-118, 2.0**-119, 2.0**-126, 2.0**-135]
+    for b, top in enumerate(tops):
+        x[:, b * 128] = 1
+        x[:, b * 128:(b + 1) * 128] *= top
+    x[0, 6 * 128:7 * 128] *= 2.0**-147
+    x[1, 6 * 128 + 5] = -float("inf")
+    x[1, 7 * 128 + 5] = float("nan")
+    codes, scale = fp8block.quantize(x)
+    q, s = _exact_norm(x, None, 0.0, None)
+    n = len(tops)
+    check_close(scale[:, :n], s[:, :n], s[:, :n] * 1e-5 + 2.0**-149)
+    check_codes(codes[:, :n * 128], q[:, :n * 128], 1e-5)
+    assert scale[0, 6] == 1 and bool((codes[0, 6 * 128:7 * 128].float() == 0).all())
+    c = codes[1, 6 * 128:7 * 128].float()
+    assert scale[1, 6] == float("inf") and bool(c[5].isnan()) and bool((torch.cat([c[:5], c[6:]]) == 0).all())
+    assert bool(scale[1, 7].isnan()) and bool(codes[1, 7 * 128:8 * 128].float().isnan().all())
+
+
 def test_quantize_weight():
     from voyager_b200 import fp8block
 

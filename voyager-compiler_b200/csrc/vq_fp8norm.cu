@@ -3,11 +3,16 @@
 //
 //   h = x + r                          (float32; hidden = h in x's type)
 //   y = h * rsqrt(mean(h^2) + eps) * w (float32; without w: y = h)
-//   s = max|y| / 448 per 128 columns   (1 where the maximum is 0)
+//   s = max|y| / 448 per 128 columns   (1 where that is 0)
 //   code = E4M3(y / s)
 //
 // Everything between the loads and the stores is float32: the norm is that
-// of the unrounded sum, and each output is rounded once.  A NaN in a block
+// of the unrounded sum, and each output is rounded once.  The row's factor
+// f cancels in y / s = 448 z / max|z|, z = h w; computed so, a quotient that
+// is a tie in the reals (with bf16 inputs many are, both products having few
+// bits) comes out as one, where roundings of y and s would move it.  So that
+// z has y's range, f = p m with p a power of two and 1 <= m < 2: z = (h p) w,
+// the first product exact, and s = max|z| m / 448.  A NaN in a block
 // makes its scale and codes NaN (maxima are taken on magnitude bits, where
 // NaN sorts above infinity).
 //
@@ -59,24 +64,50 @@ __device__ __forceinline__ float block_sum(float v, float* part) {
   return warp_sum(lane < n ? part[lane] : 0.0f);
 }
 
-__device__ __forceinline__ float block_scale(uint32_t m) {
-  return m ? __fdiv_rn(__uint_as_float(m), QMAX) : 1.0f;
-}
+// f = p m.  Zero, infinity and NaN (a row whose squares overflow, or of zeros
+// with eps = 0) stay whole.
+struct Factor {
+  float p = 1.0f, m = 1.0f;
+  __device__ __forceinline__ void set(float f) {
+    const uint32_t b = __float_as_uint(f), e = b & 0x7F800000u;
+    const bool whole = e == 0 || e == 0x7F800000u;
+    p = whole ? f : __uint_as_float(e);
+    m = whole ? 1.0f : __uint_as_float((b & 0x7FFFFFu) | 0x3F800000u);
+  }
+};
 
-// y / s as y * (1 / s): within 1.5 float32 roundings of the quotient, which
-// moves a code only where the quotient lies that near a tie (16 divisions a
-// thread took a quarter of the kernel's time).  Where 1 / s could overflow
-// the division itself.
-__device__ __forceinline__ float quotient(float y, float s, float inv) {
-  return s < 0x1p-126f ? __fdiv_rn(y, s) : y * inv;
-}
+// A block's scale and its values over that scale, from max|z| as bits.  With
+// max|z| = 2^e n and 1 <= n < 2 (less than 1 below 2^-118), 448 z / max|z| =
+// t / n, t = (448 2^-e) z: nothing but a z too small for a code leaves
+// float32's range, so the product with 1 / n and one correction by its
+// remainder (Markstein, IBM J. Res. Dev. 34, 1990) serve every block.
+struct Block {
+  float c, n, r, s;
+  __device__ __forceinline__ Block(uint32_t bits, const Factor& f) {
+    const int e = min(max((int)(bits >> 23), 9), 254);  // biased
+    c = __uint_as_float((uint32_t)(254 + 8 - e) << 23) * 1.75f;
+    n = __uint_as_float(bits) * __uint_as_float(e == 254 ? 0x00400000u : (uint32_t)(254 - e) << 23);
+    s = __fdiv_rn(n * f.m, QMAX) * __uint_as_float((uint32_t)e << 23);
+    if (s == 0.0f) s = n = 1.0f, c = 0.0f;
+    if (bits >= 0x7F800000u) {  // infinity over infinity is NaN, the rest of its block 0
+      s = __uint_as_float(bits);
+      c = bits == 0x7F800000u ? 0.0f : s;
+      n = 1.0f;
+    }
+    r = __fdiv_rn(1.0f, n);
+  }
+  __device__ __forceinline__ float operator()(float z) const {
+    const float t = z * c, q = t * r;
+    return fmaf(fmaf(-q, n, t), r, q);
+  }
+};
 
 // A CTA takes rows blockIdx.x, + gridDim.x, ..; NV groups of 8 consecutive
 // elements per thread; columns a multiple of 8, rows 16-byte aligned.  A block
 // of 128 columns is 16 neighbouring lanes.  The next row's loads are in
 // flight while this one is summed and quantized (without that the SMs waited
-// for them half the time: 16384 x 4096 bf16 with a residual took 111 us), and
-// the weight stays in registers.
+// for them half the time: 16384 x 4096 bf16 with a residual took 111 us, now
+// 78, 0.93 of the copy rate), and the weight stays in registers.
 template <typename T, int NV, int MAXT>
 __global__ void __launch_bounds__(MAXT) k_norm_vec(const Args a) {
   using E = typename T::type;
@@ -126,9 +157,9 @@ __global__ void __launch_bounds__(MAXT) k_norm_vec(const Args a) {
       for (int i = 0; i < NV; ++i)
         if (col(i) < a.cols) T::store8(hid + col(i), h[i]);
     }
-    float inv = 1.0f;
+    Factor f;
     // two buffers of partial sums: the next row's do not meet this one's readers
-    if (a.w) inv = rsqrtf(__fdiv_rn(block_sum(ss, part[flip]), (float)a.cols) + a.eps);
+    if (a.w) f.set(rsqrtf(__fdiv_rn(block_sum(ss, part[flip]), (float)a.cols) + a.eps));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = col(i);
@@ -136,7 +167,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_vec(const Args a) {
         float g[8];
         T::widen8(rw[i], g);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) h[i][k] = h[i][k] * inv * g[k];
+        for (int k = 0; k < 8; ++k) h[i][k] = h[i][k] * f.p * g[k];
       }
       uint32_t m = 0;
 #pragma unroll
@@ -144,14 +175,13 @@ __global__ void __launch_bounds__(MAXT) k_norm_vec(const Args a) {
 #pragma unroll
       for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(FULL, m, d));
       if (c < a.cols) {
-        const float s = block_scale(m);
-        const float inv_s = __fdiv_rn(1.0f, s);
+        const Block blk(m, f);
         float q[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) q[k] = quotient(h[i][k], s, inv_s);
+        for (int k = 0; k < 8; ++k) q[k] = blk(h[i][k]);
         *reinterpret_cast<uint2*>(a.codes + row * a.cols + c) =
             make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
-        if ((threadIdx.x & 15) == 0) a.scale[row * a.nblk + (c >> 7)] = s;
+        if ((threadIdx.x & 15) == 0) a.scale[row * a.nblk + (c >> 7)] = blk.s;
       }
     }
   }
@@ -218,6 +248,7 @@ __global__ void __launch_bounds__(1024) k_norm_blocks(const Args a) {
         store_v<T, VEC>(hid + c0 + i * 32 * VEC, h[i]);
       }
   }
+  Factor f;
   if (a.w) {
     float g[NB * PER][VEC];
     float ss = 0.0f;
@@ -227,12 +258,12 @@ __global__ void __launch_bounds__(1024) k_norm_blocks(const Args a) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) ss = fmaf(h[i][k], h[i][k], ss);
     }
-    const float inv = rsqrtf(__fdiv_rn(block_sum(ss, part), (float)a.cols) + a.eps);
+    f.set(rsqrtf(__fdiv_rn(block_sum(ss, part), (float)a.cols) + a.eps));
 #pragma unroll
     for (int i = 0; i < NB * PER; ++i)
       if (c0 + i * 32 * VEC < a.cols) {
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) h[i][k] = h[i][k] * inv * g[i][k];
+        for (int k = 0; k < VEC; ++k) h[i][k] = h[i][k] * f.p * g[i][k];
       }
   }
 #pragma unroll
@@ -243,13 +274,12 @@ __global__ void __launch_bounds__(1024) k_norm_blocks(const Args a) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) m = max(m, mag(h[b * PER + i][k]));
     m = __reduce_max_sync(FULL, m);
-    const float s = block_scale(m);
-    const float inv_s = __fdiv_rn(1.0f, s);
+    const Block over(m, f);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = c0 + (b * PER + i) * 32 * VEC;
       if (c < a.cols) {
-        const uint32_t q = pack2(quotient(h[b * PER + i][0], s, inv_s), quotient(h[b * PER + i][VEC - 1], s, inv_s));
+        const uint32_t q = pack2(over(h[b * PER + i][0]), over(h[b * PER + i][VEC - 1]));
         if (VEC == 1)
           a.codes[row * a.cols + c] = (uint8_t)q;
         else
@@ -257,7 +287,7 @@ __global__ void __launch_bounds__(1024) k_norm_blocks(const Args a) {
       }
     }
     const int blk = warp * NB + b;
-    if (lane == 0 && blk < a.nblk) a.scale[row * a.nblk + blk] = s;
+    if (lane == 0 && blk < a.nblk) a.scale[row * a.nblk + blk] = over.s;
   }
 }
 
@@ -273,42 +303,41 @@ __global__ void __launch_bounds__(1024) k_norm_any(const Args a) {
   const E* x = reinterpret_cast<const E*>(a.x) + row * a.ldx;
   const E* r = a.r ? reinterpret_cast<const E*>(a.r) + row * a.ldr : nullptr;
   const E* w = reinterpret_cast<const E*>(a.w);
-  float inv = 1.0f;
+  Factor f;
   if (a.w) {
     float ss = 0.0f;
     for (int c = threadIdx.x; c < a.cols; c += blockDim.x) {
       const float h = T::load(x + c) + (r ? T::load(r + c) : 0.0f);
       ss = fmaf(h, h, ss);
     }
-    inv = rsqrtf(__fdiv_rn(block_sum(ss, part), (float)a.cols) + a.eps);
+    f.set(rsqrtf(__fdiv_rn(block_sum(ss, part), (float)a.cols) + a.eps));
   }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
   for (int b = warp; b < a.nblk; b += nw) {
-    float y[4];
+    float z[4];
     uint32_t m = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = b * 128 + j * 32 + lane;
-      y[j] = 0.0f;
+      z[j] = 0.0f;
       if (c < a.cols) {
         float h = T::load(x + c);
         if (r) {
           h += T::load(r + c);
           T::store(reinterpret_cast<E*>(a.hidden) + row * a.cols + c, h);
         }
-        y[j] = a.w ? h * inv * T::load(w + c) : h;
+        z[j] = a.w ? h * f.p * T::load(w + c) : h;
       }
-      m = max(m, mag(y[j]));
+      m = max(m, mag(z[j]));
     }
     m = __reduce_max_sync(FULL, m);
-    const float s = block_scale(m);
-    const float inv_s = __fdiv_rn(1.0f, s);
+    const Block over(m, f);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = b * 128 + j * 32 + lane;
-      if (c < a.cols) a.codes[row * a.cols + c] = (uint8_t)pack2(quotient(y[j], s, inv_s), 0.0f);
+      if (c < a.cols) a.codes[row * a.cols + c] = (uint8_t)pack2(over(z[j]), 0.0f);
     }
-    if (lane == 0) a.scale[row * a.nblk + b] = s;
+    if (lane == 0) a.scale[row * a.nblk + b] = over.s;
   }
 }
 
