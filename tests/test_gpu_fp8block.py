@@ -88,6 +88,20 @@ def test_norm_strides_and_shapes(C):
     assert codes.shape == (0, 5, C) and scale.shape == (0, 5, (C + 127) // 128) and hidden.shape == codes.shape
 
 
+@pytest.mark.parametrize("C", [1, 128, 300])
+def test_norm_overlapping_rows(C):
+    """Rows shared by expansion, and windows of one row that overlap."""
+    g = _gen(C)
+    x = torch.randn(4, 3, C, generator=g, device="cuda").bfloat16()
+    w = torch.randn(C, generator=g, device="cuda").bfloat16()
+    one = torch.randn(2 * C + 40, generator=g, device="cuda").bfloat16()
+    for t in (one[:C].expand(4, 3, C), one.as_strided((4, 3, C), (3, 1, 1)), one[:C].expand(12, C)):
+        v = x.reshape(t.shape)
+        _check_norm(t, w)
+        _check_norm(t, w, residual=v)
+        _check_norm(v, w, residual=t)
+
+
 def test_norm_special_values():
     """All-zero blocks get scale 1; a NaN makes its row's codes NaN (and only
     its row's), without a norm its block's; large and tiny rows stay exact."""

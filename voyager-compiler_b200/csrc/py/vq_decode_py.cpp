@@ -55,10 +55,12 @@ struct On {
   }
 };
 
-// t as [rows, cols] with dense rows: itself, a view, or a copy.
+// t as [rows, cols] with dense rows that do not overlap (an expanded tensor's
+// do): itself, a view, or a copy.
 Tensor rows_of(const Tensor& t, int64_t cols) {
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, cols});
-  return r.stride(1) == 1 || cols == 1 ? r : r.contiguous();
+  const bool dense = r.stride(1) == 1 || cols == 1;
+  return dense && (r.size(0) <= 1 || r.stride(0) >= cols) ? r : r.contiguous();
 }
 
 // x, residual or None, weight or None, eps, what -> (codes, scale, hidden or None)
