@@ -139,6 +139,7 @@ def test_rope_abi():
         assert _rope(lib, **kw) == 1, kw
     for n in ("q", "k", "v", "table", "bt", "lengths", "q_out", "kc", "vc", "ks", "vs"):
         assert _rope(lib, tokens=1, **{n: None}) == 6, n
+    assert _rope(lib, tokens=1, batch=1 << 20, heads=32, kv=32) == 1  # 2^26 blocks, up to 32 threads each
     assert _rope(lib, tokens=1, positions=63) == 5
     assert _rope(lib, tokens=1, q=P + 8) == 3
     assert _rope(lib, tokens=1, strides=(ctypes.c_int64 * 9)(*[129] * 9)) == 3

@@ -385,6 +385,11 @@ def test_refusals():
             kvcache.rope_append(q, k, k, tab, cache, *plan)
         with pytest.raises(ValueError):
             kvcache.attend(q, cache, *plan)
+    none = kvcache.KVCache(*(t[:, :0] for t in (cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale)))
+    with pytest.raises(ValueError):
+        kvcache.rope_append(q, k[:, :, :0], k[:, :, :0], tab, none, bt, held)
+    with pytest.raises(ValueError):
+        kvcache.attend(q, none, bt, held)
     with pytest.raises(NotImplementedError):
         kvcache.attend(q.float(), cache, bt, held)
     with pytest.raises(ValueError):

@@ -231,7 +231,7 @@ PyObject* rope_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
                     what, ": q ", q.sizes(), ", k ", k.sizes(), ", v ", v.sizes(), " do not match a cache of ",
                     c.heads, " heads of ", c.dim);
   const int64_t B = q.size(0), T = q.size(1), H = q.size(2);
-  TORCH_CHECK_VALUE(H > 0 && H % c.heads == 0, what, ": ", H, " query heads do not group over ", c.heads, " kv heads");
+  TORCH_CHECK_VALUE(H > 0 && c.heads > 0 && H % c.heads == 0, what, ": ", H, " query heads do not group over ", c.heads, " kv heads");
   TORCH_CHECK_VALUE(table.scalar_type() == at::kFloat && table.dim() == 3 && table.size(2) == 2 && table.is_contiguous(),
                     what, ": table must be contiguous float32 [positions, rotary_dim / 2, 2]");
   const int64_t rot = 2 * table.size(1);

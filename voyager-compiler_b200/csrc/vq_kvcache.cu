@@ -598,7 +598,7 @@ extern "C" int vq_rope_append_kv8(const void* q, const void* k, const void* v, c
   a.rot = rot, a.page = page, a.width = (int)table_width, a.pages = (int)pages;
   a.interleaved = interleaved;
   a.W = (int)((tokens - 1 + page - 1) / page) + 1;
-  if (batch * a.W * 2 * kv_heads >= (1ll << 27)) return VQ_ERR_INVALID;  // items in 32 bits, with their lanes
+  if (batch * a.W * 2 * kv_heads >= (1ll << 26)) return VQ_ERR_INVALID;  // items times 32 lanes in 31 bits
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   int64_t blocks = 0;
   if (dtype == VQ_BF16)
