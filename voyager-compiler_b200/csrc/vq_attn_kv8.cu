@@ -67,6 +67,7 @@ struct Args {
   int32_t* done;      // [B * groups * Hkv] zero before, zero after
   int B, T, H, Hkv, G, page_log2, width, pages;
   int groups;         // row groups per sequence
+  uint32_t by_g;      // ceil(2^31 / G)
   float sm_log2;              // sm_scale * log2(e)
 };
 
@@ -88,6 +89,7 @@ struct Cfg {
   static constexpr int JOIN = (SUMS * ROWS * LD + 3 * WARPS * ROWS + 4 * ROWS) * 4;
   static constexpr int SMEM = SMEM_RING + JOIN + 1024 + 256;
   static_assert(JOIN % 16 == 0 && WARPS * STAGES * 8 <= 256, "barriers after the join's area");
+  static_assert(SUMS * ROWS * LD >= 8 * THREADS, "a join's groups meet there");
   static_assert(3 * ROWS <= THREADS, "a thread for each of a row's m, l and w");
   static_assert(PER_SM * (SMEM + 3200 + 1024) <= 227 * 1024, "CTAs per SM");
 };
@@ -125,10 +127,8 @@ __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
   __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&h);
 }
-// A word has an E4M3 NaN byte (0x7F or 0xFF).
-__device__ __forceinline__ uint32_t has_nan(uint32_t w) {
-  return __vcmpeq4(w & 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-}
+// Bits 0x80 of it: the word's bytes that are an E4M3 NaN (0x7F or 0xFF).
+__device__ __forceinline__ uint32_t nan_bits(uint32_t w) { return (w & 0x7F7F7F7Fu) + 0x01010101u; }
 
 // Byte offset of 16-byte chunk c of row r in a TMA-swizzled tile of D-byte rows.
 template <int D>
@@ -143,16 +143,16 @@ __device__ __forceinline__ float out_scale(float m, float l, float w) {
 }
 
 // A sequence's tokens held and new tokens, brought to what fits.
-__device__ __forceinline__ int2 plan_of(const Args& a, int b, bool report) {
+__device__ __forceinline__ int2 plan_of(const Args& a, int b, int& err) {
   int held = a.lengths[b], cnt = a.counts ? a.counts[b] : a.T;
   if (held < 0 || cnt < 0 || cnt > a.T) {
-    if (report) note_err(nullptr, ERR_COUNT);
+    err = ERR_COUNT;
     cnt = held < 0 ? 0 : min(max(cnt, 0), a.T);
     held = max(held, 0);
   }
   const int64_t cap = (int64_t)a.width << a.page_log2;
   if (held + (int64_t)cnt > cap) {
-    if (report) note_err(nullptr, ERR_CAPACITY);
+    err = ERR_CAPACITY;
     cnt = held >= cap ? 0 : (int)(cap - held);
   }
   return make_int2(held, cnt);
@@ -163,13 +163,16 @@ struct Entry {
   int b, row0, nrows, held, end;
 };
 template <int ROWS>
-__device__ __forceinline__ Entry entry_of(const Args& a, int e, int2 plan) {
+__device__ __forceinline__ Entry entry_of(const Args& a, int e, const int2* plans) {
   Entry x;
-  x.b = e / a.groups;
+  x.b = a.groups == 1 ? e : e / a.groups;
   x.row0 = (e - x.b * a.groups) * ROWS;
+  int err;
+  const int2 plan = x.b < PLANS ? plans[x.b] : plan_of(a, x.b, err);
   x.held = plan.x;
   x.nrows = min(ROWS, plan.y * a.G - x.row0);
-  x.end = x.nrows > 0 ? x.held + (x.row0 + x.nrows - 1) / a.G + 1 : 0;
+  x.end = 0;
+  if (x.nrows > 0) x.end = x.held + (a.groups == 1 ? plan.y : (x.row0 + x.nrows - 1) / a.G + 1);
   return x;
 }
 __device__ __forceinline__ int units_of(const Entry& x) { return (x.end + UNIT - 1) / UNIT; }
@@ -185,7 +188,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~(uintptr_t)1023);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::SMEM_RING + C::JOIN);  // [WARPS][STAGES]
-  __shared__ int s_last, s_entry, s_before;
+  __shared__ int s_last, s_entry, s_before, s_run[2];
   __shared__ long long s_sum[WARPS];
   __shared__ int2 s_plan[PLANS];  // the first sequences' plans
 
@@ -204,28 +207,31 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
 
   // ---- this CTA's run of units: a scan of the entries' unit counts (and, in
   // the upper 32 bits, of the entries that have any) ----
-  for (int b = threadIdx.x; b < min(a.B, PLANS); b += THREADS) s_plan[b] = plan_of(a, b, blockIdx.x == 0);
+  for (int b = threadIdx.x; b < (blockIdx.x == 0 ? a.B : min(a.B, PLANS)); b += THREADS) {
+    int err = 0;
+    const int2 plan = plan_of(a, b, err);
+    if (b < PLANS) s_plan[b] = plan;
+    if (err && blockIdx.x == 0) note_err(nullptr, err);
+  }
   __syncthreads();
-  auto entry = [&](int e) {
-    const int b = e / a.groups;
-    return entry_of<C::ROWS>(a, e, b < PLANS ? s_plan[b] : plan_of(a, b, blockIdx.x == 0));
-  };
+  auto entry = [&](int e) { return entry_of<C::ROWS>(a, e, s_plan); };
   const int entries = a.B * a.groups, per = (entries + THREADS - 1) / THREADS;
   const int e0 = min(entries, (int)threadIdx.x * per), e1 = min(entries, e0 + per);
   long long own = 0;
+#pragma unroll 1
   for (int e = e0; e < e1; ++e) {
     const int u = units_of(entry(e));
     own += u ? u + (1ll << 32) : 0;
   }
-  long long sum = own;
+  long long scan = own;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const long long y = __shfl_up_sync(FULL, sum, d);
-    if (lane >= d) sum += y;
+    const long long y = __shfl_up_sync(FULL, scan, d);
+    if (lane >= d) scan += y;
   }
-  if (lane == 31) s_sum[warp] = sum;
+  if (lane == 31) s_sum[warp] = scan;
   __syncthreads();
-  long long total = 0, before = sum - own;
+  long long total = 0, before = scan - own;
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) {
     if (w < warp) before += s_sum[w];
@@ -233,52 +239,64 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
   }
   // CTAs with work.  A piece more of a head costs its join about an eighth of
   // a unit's time, so a run is at least sqrt(units / 8) of an average head.
-  // A head counts HEAD units more than it has where runs span heads: opening,
-  // joining and closing one takes that long.
+  // Where heads are not few a head counts HEAD units more than it has: opening,
+  // joining and closing one takes that long.  A cut in those moves to the
+  // head's begin, and with about a head per run or more one within HEAD of its
+  // end moves there (256 heads of 609 keys on 296 CTAs: 15.2 us against 19.8;
+  // 112 heads, up to 2229 keys: 19.4 against 15.1).
   const int heads = (int)(total >> 32) * a.Hkv, real = (int)total * a.Hkv;
   const float least = heads ? fmaxf(1.0f, sqrtf(0.125f * (float)real / (float)heads)) : 1.0f;
   const int runs = min((int)gridDim.x, (int)ceilf((float)real / least));
-  const int HEAD = 2 * heads >= runs ? 4 : 0;
+  const int HEAD = 6 * heads >= runs ? 5 : 0, near_end = 4 * heads >= 3 * runs ? HEAD : 0;
   const int all = real + HEAD * heads;
   const int base = runs ? all / runs : 0, rest = all - base * runs;  // the first `rest` runs have one more
-  auto run_of = [&](int at) {  // the run that holds this unit
-    return at < rest * (base + 1) ? at / (base + 1) : rest + (at - rest * (base + 1)) / base;
+  auto run_of = [&](int at) {  // the run that holds this unit, by the cuts as they were before they moved
+    const int far = at - rest * (base + 1);
+    return (far < 0 ? 0 : rest) + (far < 0 ? at : far) / (far < 0 ? base + 1 : base);
   };
   auto run_begin = [&](int c) { return c * base + min(c, rest); };
-  const int lo = run_begin(blockIdx.x), hi = run_begin(blockIdx.x + 1);
-  {
+  if ((int)blockIdx.x < runs) {
+    const int cut0 = run_begin(blockIdx.x), cut1 = run_begin(blockIdx.x + 1);
     int at = ((int)before + HEAD * (int)(before >> 32)) * a.Hkv;
     const int to = at + ((int)own + HEAD * (int)(own >> 32)) * a.Hkv;
-    if ((int)blockIdx.x < runs && at <= lo && lo < to)
+    if ((at <= cut0 && cut0 < to) || (at <= cut1 && cut1 < to)) {
+#pragma unroll 1
       for (int e = e0; e < e1; ++e) {
-        const int u = units_of(entry(e)), next = at + (u ? (u + HEAD) * a.Hkv : 0);
-        if (lo < next) {
+        const int w = units_of(entry(e)) + HEAD;
+        if (w == HEAD) continue;
+        auto moved = [&](int cut) {
+          const int ps = at + (cut - at) / w * w;
+          return ps + w - cut <= near_end ? ps + w : cut - ps <= HEAD ? ps : cut;
+        };
+        const int next = at + w * a.Hkv;
+        if (at <= cut0 && cut0 < next) {
           s_entry = e;
           s_before = at;
-          break;
+          s_run[0] = moved(cut0);
         }
+        if (at <= cut1 && cut1 < next) s_run[1] = moved(cut1);
         at = next;
       }
+    }
+    if (threadIdx.x == 0 && cut1 == all) s_run[1] = all;
+  } else if (threadIdx.x == 0) {
+    s_run[0] = s_run[1] = 0;
   }
   __syncthreads();
+  const int lo = s_run[0], hi = s_run[1];
 
   const uint32_t ring = smem_u32(smem) + warp * C::RING;
   const uint32_t bar0 = smem_u32(bars + warp * C::STAGES);
   int stage = 0;      // of the next tile to read; the ring runs on from segment to segment
   uint32_t phase = 0;
   bool ok = true;
-  int pos = lo, ebase = s_before;
-  int e = s_entry;
+  int pos = lo, ebase = s_before, e = s_entry - 1, units = 0;
   Entry x = {};
-  int units = 0;
-  if ((int)blockIdx.x < runs) {
-    x = entry(e);
-    units = units_of(x);
-  }
 
   // A segment: the part of one head (entry, kv head) in this run.
   struct Seg {
     int b, row0, nrows, held, end, kvh, k0, k1, units, slot, pair;
+    int tok0, head0;  // of row 0
     int ps;  // where the head begins
     bool whole;
   } sg = {};
@@ -314,12 +332,15 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
   };
   // The next segment; start() puts its first loads on their way.
   auto open = [&]() {
+#pragma unroll 1
     while (units == 0 || pos >= ebase + (units + HEAD) * a.Hkv) {  // the next entry with keys
       if (units) ebase += (units + HEAD) * a.Hkv;
       x = entry(++e);
       units = units_of(x);
     }
     sg.b = x.b, sg.row0 = x.row0, sg.nrows = x.nrows, sg.held = x.held, sg.end = x.end, sg.units = units;
+    sg.tok0 = a.groups == 1 ? 0 : x.row0 / a.G;
+    sg.head0 = x.row0 - sg.tok0 * a.G;
     sg.kvh = (pos - ebase) / (units + HEAD);
     sg.pair = e * a.Hkv + sg.kvh;
     sg.ps = ebase + sg.kvh * (units + HEAD);
@@ -327,7 +348,6 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
     sg.whole = u0 == 0 && u1 == units;
     sg.slot = pos == lo ? 0 : 1;
     pos = min(hi, sg.ps + HEAD + units);
-    if (u1 <= 0) return false;  // the run ends within the head's extra units
     sg.k0 = u0 * UNIT, sg.k1 = min(x.end, u1 * UNIT);
     const int ntiles = (sg.k1 - sg.k0 + TILE - 1) / TILE;
     // tiles warp, warp + 4, ..; none after a wait that gave up
@@ -335,10 +355,15 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
     issued = 0;
     wstage = stage;
     if (mine > 0) pid_next = pid_of(lane);
-    return true;
   };
   auto start = [&]() {
+#pragma unroll 1
     for (int i = 0; i < min(mine, C::STAGES); ++i) issue();
+  };
+  // Row r of a segment: its token and its head in the group.
+  auto row_of = [&](const Seg& sg, int r) {
+    const int at = sg.head0 + r, n = (int)__umulhi(2u * at, a.by_g);
+    return make_int2(sg.tok0 + n, at - n * a.G);
   };
   // The queries of the segment as they lie in memory: lane (g, t) takes row
   // g's columns D/4 * t ...
@@ -346,12 +371,12 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
   auto load_q = [&]() {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = sg.row0 + n * 8 + g;
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) qw[n][i] = 0;
-      if (r < sg.row0 + sg.nrows) {
-        const uint16_t* p = a.q + (int64_t)sg.b * a.qb + (int64_t)(r / a.G) * a.qt +
-                            (int64_t)(sg.kvh * a.G + r % a.G) * a.qh + t * (D / 4);
+      if (n * 8 + g < sg.nrows) {
+        const int2 row = row_of(sg, n * 8 + g);
+        const uint16_t* p = a.q + (int64_t)sg.b * a.qb + (int64_t)row.x * a.qt +
+                            (int64_t)(sg.kvh * a.G + row.y) * a.qh + t * (D / 4);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
           const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
@@ -360,26 +385,245 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
       }
     }
   };
-  bool more = (int)blockIdx.x < runs && open();
-  if (more) {
-    load_q();  // under the block table's latency
-    start();
-  }
-  // row groups without a query are written here: no unit belongs to them
-  for (int e = blockIdx.x; e < entries; e += gridDim.x) {
-    const Entry x = entry(e);
-    if (x.nrows > 0) continue;
-    const int rows = min(C::ROWS, a.T * a.G - x.row0);
-    for (int i = threadIdx.x; i < rows * a.Hkv * (D / 8); i += THREADS) {
-      const int row = x.row0 + i / (D / 8) % rows, h = i / (D / 8) / rows;
-      reinterpret_cast<uint4*>(a.out + (((int64_t)x.b * a.T + row / a.G) * a.H + h * a.G + row % a.G) * D)
-          [i % (D / 8)] = make_uint4(0, 0, 0, 0);
+  float o[NT][KS][4] = {};
+  float mx[NT][2] = {}, sum[NT][2] = {}, wx[NT][2] = {};  // m, l, w of columns 2t, 2t + 1
+  auto join = [&](const Seg& cur) {
+  // ---- join the warps ----
+  float* sums = reinterpret_cast<float*>(smem + C::SMEM_RING);  // [SUMS][ROWS][LD]
+  float* sm = sums + C::SUMS * C::ROWS * C::LD;                 // [WARPS][ROWS] m, l, w
+  float* sl = sm + WARPS * C::ROWS;
+  float* sw = sl + WARPS * C::ROWS;
+  float* fin = sw + WARPS * C::ROWS;                            // [ROWS] m, l, w, the output's factor
+  __syncthreads();  // the last join's readers are done
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float l = sum[n][c];
+      l += __shfl_xor_sync(FULL, l, 4);
+      l += __shfl_xor_sync(FULL, l, 8);
+      l += __shfl_xor_sync(FULL, l, 16);
+      if (g == 0) {
+        const int r = warp * C::ROWS + n * 8 + 2 * t + c;
+        sm[r] = mx[n][c], sl[r] = l, sw[r] = wx[n][c];
+      }
     }
+  __syncthreads();
+  if (threadIdx.x < C::ROWS) {
+    float m = NEG_INF, w = NEG_INF, l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) {
+      m = fmaxf(m, sm[k * C::ROWS + threadIdx.x]);
+      w = fmaxf(w, sw[k * C::ROWS + threadIdx.x]);
+    }
+    const float ref = m == NEG_INF ? 0.0f : m;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k)
+      l = fmaf(sl[k * C::ROWS + threadIdx.x], ex2(sm[k * C::ROWS + threadIdx.x] - ref), l);
+    fin[threadIdx.x] = m, fin[C::ROWS + threadIdx.x] = l, fin[2 * C::ROWS + threadIdx.x] = w;
+    fin[3 * C::ROWS + threadIdx.x] = (int)threadIdx.x < cur.nrows ? out_scale(m, l, w) : 0.0f;
+  }
+  // every warp's O relative to the CTA's w, added in the warps' order.  Column
+  // d = D/8 g + 2j + i of a row lies at place 16 j + 2 g + i of it: the lanes of
+  // a store then meet no bank twice.
+#pragma unroll
+  for (int k = 0; k < WARPS / C::SUMS; ++k) {
+    if (warp / C::SUMS == k) {
+      float* dst = sums + (warp % C::SUMS) * C::ROWS * C::LD;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int r = n * 8 + 2 * t + c;
+          float w = sw[r];
+#pragma unroll
+          for (int q = 1; q < WARPS; ++q) w = fmaxf(w, sw[q * C::ROWS + r]);
+          const float f = ex2(wx[n][c] - (w == NEG_INF ? 0.0f : w));
+#pragma unroll
+          for (int j = 0; j < KS; ++j) {
+            float2* p = reinterpret_cast<float2*>(dst + r * C::LD + 16 * j + 2 * g);
+            float2 v = k ? *p : make_float2(0.0f, 0.0f);
+            v.x = fmaf(o[n][j][c], f, v.x);
+            v.y = fmaf(o[n][j][c + 2], f, v.y);
+            *p = v;
+          }
+        }
+    }
+    __syncthreads();
+  }
+  auto out_row = [&](int r) {
+    const int2 row = row_of(cur, r);
+    return a.out + (((int64_t)cur.b * a.T + row.x) * a.H + cur.kvh * a.G + row.y) * D;
+  };
+  if (cur.whole) {
+    const int rows = min(C::ROWS, a.T * a.G - cur.row0);
+    for (int i = threadIdx.x; i < rows * (D / 2); i += THREADS) {
+      const int r = i / (D / 2), d = i % (D / 2) * 2;
+      const float2* p = reinterpret_cast<const float2*>(sums + r * C::LD + d % (D / 8) * 8 + d / (D / 8) * 2);
+      float2 v = *p;
+      if (C::SUMS == 2) {
+        const float2 u = p[C::ROWS * C::LD / 2];
+        v.x += u.x, v.y += u.y;
+      }
+      const float f = fin[3 * C::ROWS + r];
+      // a row without a query is 0 even where its sums are not finite
+      *reinterpret_cast<uint32_t*>(out_row(r) + d) = r < cur.nrows ? bf_pack(v.x * f, v.y * f) : 0u;
+    }
+    return;
   }
 
-  for (bool first = true; more; first = false) {
-  if (!first) load_q();
-  const int row0 = sg.row0, held = sg.held, end = sg.end, k0 = sg.k0;
+  // ---- a piece of a head: [ROWS][D] of O in place order, then m, l and w ----
+  float* piece_out = a.part + ((int64_t)blockIdx.x * 2 + cur.slot) * PART;
+  for (int i = threadIdx.x; i < cur.nrows * (D / 4); i += THREADS) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    const float4* p = reinterpret_cast<const float4*>(sums + r * C::LD + d);
+    float4 v = *p;
+    if (C::SUMS == 2) {
+      const float4 u = p[C::ROWS * C::LD / 4];
+      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+    }
+    reinterpret_cast<float4*>(piece_out)[i] = v;
+  }
+  if (threadIdx.x < 3 * C::ROWS) piece_out[C::ROWS * D + threadIdx.x] = fin[threadIdx.x];
+  // the CTA that finishes last reads the head's pieces in the CTAs' order
+  const int still = cur.units + HEAD - near_end - 1;  // the last place where a cut stays in the head
+  const int c0 = run_of(cur.ps + min(HEAD, still)), c1 = run_of(cur.ps + still);
+  const int pieces = c1 - c0 + 1;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int n;  // releases every thread's stores, which the barrier has ordered before it
+    asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(n) : "l"(a.done + cur.pair) : "memory");
+    s_last = n == pieces - 1;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  const int slot0 = run_begin(c0) + near_end >= cur.ps ? 0 : 1;  // the first CTA's run may begin before the head
+  auto piece = [&](int c) { return a.part + ((int64_t)(c0 + c) * 2 + (c == 0 ? slot0 : 0)) * PART; };
+  // A group of D / 8 lanes takes a row, eight places a lane; where there are
+  // groups enough, `split` of them share a row and take every split-th piece.
+  // All loads of PRE pieces a group travel together.
+  constexpr int LPR = D / 8, GROUPS = THREADS / LPR, PRE = C::PER_SM == 3 ? 4 : 8;
+  const int gl = lane % LPR, grp = threadIdx.x / LPR;
+  int log_split = 0;
+  while ((cur.nrows << (log_split + 1)) <= GROUPS) ++log_split;
+  const int split = 1 << log_split, sub = grp & (split - 1);
+#pragma unroll 1
+  for (int k = grp >> log_split; k - (grp >> log_split) < cur.nrows; k += GROUPS >> log_split) {
+    const int r = min(k, cur.nrows - 1);  // beyond the last: that one again
+    float4 pre[PRE][2];
+    float pw[PRE];
+    auto fetch = [&](int cb) {
+#pragma unroll
+      for (int q = 0; q < PRE; ++q) {
+        const float* p = piece(min(cb + q * split, pieces - 1));
+        const float4* o4 = reinterpret_cast<const float4*>(p + r * D) + gl;
+        pre[q][0] = __ldcg(o4), pre[q][1] = __ldcg(o4 + LPR);
+        pw[q] = __ldcg(p + C::ROWS * (D + 2) + r);
+      }
+    };
+    fetch(sub);
+    float m = NEG_INF, w = NEG_INF, l = 0.0f;
+#pragma unroll 1
+    for (int cb = gl; cb < pieces; cb += 4 * LPR) {
+      float mc[4], lc[4];
+      float mn = m;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {  // beyond the last: that one's maxima again, no sum
+        const int c = cb + q * LPR;
+        const float* p = piece(min(c, pieces - 1)) + C::ROWS * D + r;
+        mc[q] = __ldcg(p), lc[q] = c < pieces ? __ldcg(p + C::ROWS) : 0.0f;
+        w = fmaxf(w, __ldcg(p + 2 * C::ROWS));
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) mn = fmaxf(mn, mc[q]);
+      const float ref = mn == NEG_INF ? 0.0f : mn;
+      l *= ex2(m - ref);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) l = fmaf(lc[q], ex2(mc[q] - ref), l);
+      m = mn;
+    }
+#pragma unroll
+    for (int d = LPR / 2; d; d >>= 1) {
+      const float m2 = __shfl_xor_sync(FULL, m, d), l2 = __shfl_xor_sync(FULL, l, d);
+      const float mn = fmaxf(m, m2), ref = mn == NEG_INF ? 0.0f : mn;
+      l = l * ex2(m - ref) + l2 * ex2(m2 - ref);
+      m = mn;
+      w = fmaxf(w, __shfl_xor_sync(FULL, w, d));
+    }
+    const float wr = w == NEG_INF ? 0.0f : w;
+    float v[8] = {};
+#pragma unroll 1
+    for (int cb = sub; cb < pieces; cb += PRE * split) {
+      if (cb != sub) fetch(cb);
+#pragma unroll
+      for (int q = 0; q < PRE; ++q)
+        if (cb + q * split < pieces) {
+          const float f = ex2(pw[q] - wr);
+          const float4 x = pre[q][0], y = pre[q][1];
+          v[0] = fmaf(x.x, f, v[0]), v[1] = fmaf(x.y, f, v[1]), v[2] = fmaf(x.z, f, v[2]);
+          v[3] = fmaf(x.w, f, v[3]), v[4] = fmaf(y.x, f, v[4]), v[5] = fmaf(y.y, f, v[5]);
+          v[6] = fmaf(y.z, f, v[6]), v[7] = fmaf(y.w, f, v[7]);
+        }
+    }
+    if (split > 1) {  // one round; the sums' readers are past the barriers above
+      float4* mine = reinterpret_cast<float4*>(sums) + threadIdx.x;
+      mine[0] = make_float4(v[0], v[1], v[2], v[3]);
+      mine[THREADS] = make_float4(v[4], v[5], v[6], v[7]);
+      __syncthreads();
+      if (sub == 0) {
+#pragma unroll 1
+        for (int q = 1; q < split; ++q) {
+          const float4 x = mine[q * LPR], y = mine[THREADS + q * LPR];
+          v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+          v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+        }
+      }
+    }
+    if (sub == 0) {
+      const float f = out_scale(m, l, w);
+      // places 4 gl .. and D/2 + 4 gl ..: columns D/8 g2 + 2j of g2 = 2 gl % 8
+      // and the next, j = gl / 4 and D/32 more
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = gl / 4 + h * (D / 32), g2 = 2 * gl % 8;
+        uint16_t* p = out_row(r) + g2 * (D / 8) + 2 * j;
+        *reinterpret_cast<uint32_t*>(p) = bf_pack(v[4 * h] * f, v[4 * h + 1] * f);
+        *reinterpret_cast<uint32_t*>(p + D / 8) = bf_pack(v[4 * h + 2] * f, v[4 * h + 3] * f);
+      }
+    }
+  }
+  // rows of the group that have no query
+  const int blank = min(C::ROWS, a.T * a.G - cur.row0) - cur.nrows;
+  for (int i = threadIdx.x; i < blank * (D / 2); i += THREADS)
+    reinterpret_cast<uint32_t*>(out_row(cur.nrows + i / (D / 2)))[i % (D / 2)] = 0u;
+  if (threadIdx.x == 0) a.done[cur.pair] = 0;
+  };
+  for (bool done = false;; done = true) {
+  const Seg cur = sg;
+  const bool more = pos < hi;
+  if (more) {  // its loads run under the join
+    open();
+    start();
+    load_q();
+  }
+  if (done) {
+    join(cur);
+  } else {
+    // row groups without a query are written here: no unit belongs to them
+#pragma unroll 1
+    for (int e = blockIdx.x; e < entries; e += gridDim.x) {
+      const Entry x = entry(e);
+      if (x.nrows > 0) continue;
+      const int rows = min(C::ROWS, a.T * a.G - x.row0);
+      for (int i = threadIdx.x; i < rows * a.Hkv * (D / 8); i += THREADS) {
+        const int row = x.row0 + i / (D / 8) % rows, h = i / (D / 8) / rows;
+        reinterpret_cast<uint4*>(a.out + (((int64_t)x.b * a.T + row / a.G) * a.H + h * a.G + row % a.G) * D)
+            [i % (D / 8)] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+  if (!more) break;
+  const int held = sg.held, end = sg.end, k0 = sg.k0;
 
   // Q as the second operand of S^T = K Q^T: k step w takes the lane's 4
   // columns D/4 * t + 4 w ...
@@ -411,13 +655,10 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       cs[n][c] = __shfl_sync(FULL, qs[n], (2 * t + c) * 4) * a.sm_log2;
-      const int r = n * 8 + 2 * t + c;
-      lim[n][c] = held + (row0 + r) / a.G;
+      lim[n][c] = held + row_of(sg, n * 8 + 2 * t + c).x;
     }
-  const int free_end = held + row0 / a.G + 1;  // keys below: every row sees them
+  const int free_end = held + sg.tok0 + 1;  // keys below: every row sees them
 
-  float o[NT][KS][4];
-  float mx[NT][2], sum[NT][2], wx[NT][2];  // m, l, w of columns 2t, 2t + 1
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -557,10 +798,10 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
 #pragma unroll
           for (int w = 0; w < VW; ++w) {
             if (key >= end) v[mt][k][w] = 0;  // slots that hold no token of this sequence
-            odd |= has_nan(v[mt][k][w]);
+            odd |= nan_bits(v[mt][k][w]);
           }
         }
-      odd = __any_sync(FULL, odd != 0);
+      odd = __any_sync(FULL, (odd & 0x80808080u) != 0);
     }
     if (!odd) {
 #pragma unroll
@@ -574,7 +815,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
       for (int n = 0; n < NT; ++n)
 #pragma unroll 1
         for (int r = 0; r < 8; ++r) {
-          const int last = held + (row0 + n * 8 + r) / a.G;
+          const int last = held + row_of(sg, n * 8 + r).x;
           uint32_t x[2][4][VW];
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt)
@@ -604,188 +845,6 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
     if (++stage == C::STAGES) stage = 0, phase ^= 1;
   }
 
-  const Seg cur = sg;
-  more = pos < hi && open();
-  if (more) start();  // its loads run under the join
-
-  // ---- join the warps ----
-  float* sums = reinterpret_cast<float*>(smem + C::SMEM_RING);  // [SUMS][ROWS][LD]
-  float* sm = sums + C::SUMS * C::ROWS * C::LD;                 // [WARPS][ROWS] m, l, w
-  float* sl = sm + WARPS * C::ROWS;
-  float* sw = sl + WARPS * C::ROWS;
-  float* fin = sw + WARPS * C::ROWS;                            // [ROWS] m, l, w, the output's factor
-  __syncthreads();  // the last join's readers are done
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float l = sum[n][c];
-      l += __shfl_xor_sync(FULL, l, 4);
-      l += __shfl_xor_sync(FULL, l, 8);
-      l += __shfl_xor_sync(FULL, l, 16);
-      if (g == 0) {
-        const int r = warp * C::ROWS + n * 8 + 2 * t + c;
-        sm[r] = mx[n][c], sl[r] = l, sw[r] = wx[n][c];
-      }
-    }
-  __syncthreads();
-  if (threadIdx.x < C::ROWS) {
-    float m = NEG_INF, w = NEG_INF, l = 0.0f;
-#pragma unroll
-    for (int k = 0; k < WARPS; ++k) {
-      m = fmaxf(m, sm[k * C::ROWS + threadIdx.x]);
-      w = fmaxf(w, sw[k * C::ROWS + threadIdx.x]);
-    }
-    const float ref = m == NEG_INF ? 0.0f : m;
-#pragma unroll
-    for (int k = 0; k < WARPS; ++k)
-      l = fmaf(sl[k * C::ROWS + threadIdx.x], ex2(sm[k * C::ROWS + threadIdx.x] - ref), l);
-    fin[threadIdx.x] = m, fin[C::ROWS + threadIdx.x] = l, fin[2 * C::ROWS + threadIdx.x] = w;
-    fin[3 * C::ROWS + threadIdx.x] = (int)threadIdx.x < cur.nrows ? out_scale(m, l, w) : 0.0f;
-  }
-  // every warp's O relative to the CTA's w, added in the warps' order.  Column
-  // d = D/8 g + 2j + i of a row lies at place 16 j + 2 g + i of it: the lanes of
-  // a store then meet no bank twice.
-#pragma unroll
-  for (int k = 0; k < WARPS / C::SUMS; ++k) {
-    if (warp / C::SUMS == k) {
-      float* dst = sums + (warp % C::SUMS) * C::ROWS * C::LD;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int r = n * 8 + 2 * t + c;
-          float w = sw[r];
-#pragma unroll
-          for (int q = 1; q < WARPS; ++q) w = fmaxf(w, sw[q * C::ROWS + r]);
-          const float f = ex2(wx[n][c] - (w == NEG_INF ? 0.0f : w));
-#pragma unroll
-          for (int j = 0; j < KS; ++j) {
-            float2* p = reinterpret_cast<float2*>(dst + r * C::LD + 16 * j + 2 * g);
-            float2 v = k ? *p : make_float2(0.0f, 0.0f);
-            v.x = fmaf(o[n][j][c], f, v.x);
-            v.y = fmaf(o[n][j][c + 2], f, v.y);
-            *p = v;
-          }
-        }
-    }
-    __syncthreads();
-  }
-  auto out_row = [&](int r) {
-    const int row = cur.row0 + r;
-    return a.out + (((int64_t)cur.b * a.T + row / a.G) * a.H + cur.kvh * a.G + row % a.G) * D;
-  };
-  if (cur.whole) {
-    const int rows = min(C::ROWS, a.T * a.G - cur.row0);
-    for (int i = threadIdx.x; i < rows * (D / 2); i += THREADS) {
-      const int r = i / (D / 2), d = i % (D / 2) * 2;
-      const float2* p = reinterpret_cast<const float2*>(sums + r * C::LD + d % (D / 8) * 8 + d / (D / 8) * 2);
-      float2 v = *p;
-      if (C::SUMS == 2) {
-        const float2 u = p[C::ROWS * C::LD / 2];
-        v.x += u.x, v.y += u.y;
-      }
-      const float f = fin[3 * C::ROWS + r];
-      // a row without a query is 0 even where its sums are not finite
-      *reinterpret_cast<uint32_t*>(out_row(r) + d) = r < cur.nrows ? bf_pack(v.x * f, v.y * f) : 0u;
-    }
-    continue;
-  }
-
-  // ---- a piece of a head: [ROWS][D] of O in place order, then m, l and w ----
-  float* piece_out = a.part + ((int64_t)blockIdx.x * 2 + cur.slot) * PART;
-  for (int i = threadIdx.x; i < cur.nrows * (D / 4); i += THREADS) {
-    const int r = i / (D / 4), d = i % (D / 4) * 4;
-    const float4* p = reinterpret_cast<const float4*>(sums + r * C::LD + d);
-    float4 v = *p;
-    if (C::SUMS == 2) {
-      const float4 u = p[C::ROWS * C::LD / 4];
-      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-    }
-    reinterpret_cast<float4*>(piece_out)[i] = v;
-  }
-  if (threadIdx.x < 3 * C::ROWS) piece_out[C::ROWS * D + threadIdx.x] = fin[threadIdx.x];
-  // the CTA that finishes last reads the head's pieces in the CTAs' order
-  const int c0 = run_of(cur.ps + HEAD), c1 = run_of(cur.ps + HEAD + cur.units - 1);  // of its first unit and its last
-  const int pieces = c1 - c0 + 1;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();  // after the barrier: for every thread's stores
-    s_last = atomicAdd(a.done + cur.pair, 1) == pieces - 1;
-    __threadfence();
-  }
-  __syncthreads();
-  if (!s_last) continue;
-  const int slot0 = run_begin(c0) >= cur.ps ? 0 : 1;  // the first CTA's run may begin before the head
-  auto piece = [&](int c) { return a.part + ((int64_t)(c0 + c) * 2 + (c == 0 ? slot0 : 0)) * PART; };
-  // a group of D / 8 lanes takes a row, eight places a lane
-  constexpr int LPR = D / 8, GROUPS = THREADS / LPR, PRE = C::PER_SM == 3 ? 4 : 8;
-  const int gl = lane % LPR, gbase = lane - gl;
-  const int rounds = (cur.nrows + GROUPS - 1) / GROUPS;
-  for (int k = 0; k < rounds; ++k) {
-    const int r = min(k * GROUPS + (int)threadIdx.x / LPR, cur.nrows - 1);  // beyond the last: that one again
-    // the first pieces' values travel with the maxima
-    float4 pre[PRE][2];
-    auto fetch = [&](int c, float4 (&u)[2]) {
-      const float4* p = reinterpret_cast<const float4*>(piece(c) + r * D) + gl;
-      u[0] = __ldcg(p), u[1] = __ldcg(p + LPR);
-    };
-#pragma unroll
-    for (int q = 0; q < PRE; ++q) fetch(min(q, pieces - 1), pre[q]);
-    float m = NEG_INF, w = NEG_INF, l = 0.0f, w0 = NEG_INF;
-    for (int c = gl; c < pieces; c += LPR) {
-      const float* p = piece(c) + C::ROWS * D + r;
-      const float mc = __ldcg(p), lc = __ldcg(p + C::ROWS), wc = __ldcg(p + 2 * C::ROWS);
-      const float mn = fmaxf(m, mc), ref = mn == NEG_INF ? 0.0f : mn;
-      l = l * ex2(m - ref) + lc * ex2(mc - ref);
-      m = mn;
-      w = fmaxf(w, wc);
-      if (c == gl) w0 = wc;
-    }
-#pragma unroll
-    for (int d = LPR / 2; d; d >>= 1) {
-      const float m2 = __shfl_xor_sync(FULL, m, d), l2 = __shfl_xor_sync(FULL, l, d);
-      const float mn = fmaxf(m, m2), ref = mn == NEG_INF ? 0.0f : mn;
-      l = l * ex2(m - ref) + l2 * ex2(m2 - ref);
-      m = mn;
-      w = fmaxf(w, __shfl_xor_sync(FULL, w, d));
-    }
-    const float wr = w == NEG_INF ? 0.0f : w;
-    float v[8] = {};
-    auto add = [&](const float4 (&u)[2], float f) {
-      v[0] = fmaf(u[0].x, f, v[0]), v[1] = fmaf(u[0].y, f, v[1]), v[2] = fmaf(u[0].z, f, v[2]);
-      v[3] = fmaf(u[0].w, f, v[3]), v[4] = fmaf(u[1].x, f, v[4]), v[5] = fmaf(u[1].y, f, v[5]);
-      v[6] = fmaf(u[1].z, f, v[6]), v[7] = fmaf(u[1].w, f, v[7]);
-    };
-    float f = ex2(w0 - wr);  // of piece gl
-    for (int cb = 0; cb < pieces; cb += PRE) {
-      if (cb) {
-#pragma unroll
-        for (int q = 0; q < PRE; ++q) fetch(min(cb + q, pieces - 1), pre[q]);
-        if (cb % LPR == 0) f = ex2(__ldcg(piece(min(cb + gl, pieces - 1)) + C::ROWS * (D + 2) + r) - wr);
-      }
-#pragma unroll
-      for (int q = 0; q < PRE; ++q) {
-        const float fq = __shfl_sync(FULL, f, gbase + (cb + q) % LPR);
-        if (cb + q < pieces) add(pre[q], fq);
-      }
-    }
-    f = out_scale(m, l, w);
-    // places 4 gl .. and D/2 + 4 gl ..: columns D/8 g2 + 2j of g2 = 2 gl % 8
-    // and the next, j = gl / 4 and D/32 more
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int j = gl / 4 + h * (D / 32), g2 = 2 * gl % 8;
-      uint16_t* p = out_row(r) + g2 * (D / 8) + 2 * j;
-      *reinterpret_cast<uint32_t*>(p) = bf_pack(v[4 * h] * f, v[4 * h + 1] * f);
-      *reinterpret_cast<uint32_t*>(p + D / 8) = bf_pack(v[4 * h + 2] * f, v[4 * h + 3] * f);
-    }
-  }
-  // rows of the group that have no query
-  const int blank = min(C::ROWS, a.T * a.G - cur.row0) - cur.nrows;
-  for (int i = threadIdx.x; i < blank * (D / 2); i += THREADS)
-    reinterpret_cast<uint32_t*>(out_row(cur.nrows + i / (D / 2)))[i % (D / 2)] = 0u;
-  if (threadIdx.x == 0) a.done[cur.pair] = 0;
   }
 }
 
@@ -850,7 +909,7 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
   if (page != 32 && page != 64 && page != 128) return VQ_ERR_UNSUPPORTED;
   if (batch < 0 || tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || table_width < 0 ||
       pages < 0 || pages * kv_heads * page >= (1ll << 31) || table_width * page >= (1ll << 31) ||
-      tokens >= (1 << 20) || batch > (1 << 24) || batch * tokens * heads >= (1ll << 31))
+      tokens >= (1 << 20) || batch > (1 << 24) || batch * tokens * heads >= (1ll << 31) || heads / kv_heads > (1 << 15))
     return VQ_ERR_INVALID;
   if (batch == 0 || tokens == 0) return VQ_OK;
   if (!q || !q_strides || !k_codes || !v_codes || !k_scale || !v_scale || !block_table || !lengths ||
@@ -891,6 +950,7 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
   a.page_log2 = page == 32 ? 5 : page == 64 ? 6 : 7;
   a.width = (int)table_width, a.pages = (int)pages;
   a.groups = c.groups;
+  a.by_g = (uint32_t)(((1ll << 31) + a.G - 1) / a.G);
   a.sm_log2 = sm_scale * 1.4426950408889634f;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (head_dim == 128)
