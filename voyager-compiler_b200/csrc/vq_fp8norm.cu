@@ -54,6 +54,42 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 __device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
+// Two neighbouring float32 in one register pair, each lane rounded as the
+// scalar operation rounds it.
+using Two = uint64_t;
+__device__ __forceinline__ Two two(float lo, float hi) {
+  Two v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 each(Two v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+// max(|m|, |v.lo|, |v.hi|), NaN if one is.
+__device__ __forceinline__ float max_abs(float m, Two v) {
+  const float2 f = each(v);
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(f.x), "f"(f.y));
+  return d;
+}
+
 // The sum of v over the CTA's threads, in every thread; `part` holds one
 // float per warp.
 __device__ __forceinline__ float block_sum(float v, float* part) {
@@ -128,6 +164,12 @@ __global__ void __launch_bounds__(MAXT) k_norm_vec(const Args a) {
         if (a.r) rr[i] = T::fetch8(r + row * a.ldr + col(i));
       }
   };
+  auto widen = [](const Raw& r, Two (&v)[4]) {
+    float f[8];
+    T::widen8(r, f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = two(f[2 * k], f[2 * k + 1]);
+  };
   fetch(blockIdx.x);
   if (a.w) {
 #pragma unroll
@@ -137,50 +179,61 @@ __global__ void __launch_bounds__(MAXT) k_norm_vec(const Args a) {
   int flip = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, flip ^= 1) {
     E* hid = reinterpret_cast<E*>(a.hidden) + row * a.cols;
-    float h[NV][8];
-    float ss = 0.0f;
+    Two h[NV][4], sq = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      T::widen8(rx[i], h[i]);
+      widen(rx[i], h[i]);
       if (a.r) {
-        float q[8];
-        T::widen8(rr[i], q);
+        Two q[4];
+        widen(rr[i], q);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) h[i][k] += q[k];
+        for (int k = 0; k < 4; ++k) h[i][k] = add2(h[i][k], q[k]);
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) ss = fmaf(h[i][k], h[i][k], ss);
+      for (int k = 0; k < 4; ++k) sq = fma2(h[i][k], h[i][k], sq);
     }
     if (row + gridDim.x < a.rows) fetch(row + gridDim.x);
     if (a.r) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (col(i) < a.cols) T::store8(hid + col(i), h[i]);
+        if (col(i) < a.cols) {
+          float v[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[2 * k] = each(h[i][k]).x, v[2 * k + 1] = each(h[i][k]).y;
+          T::store8(hid + col(i), v);
+        }
     }
     Factor f;
+    const float ss = each(sq).x + each(sq).y;
     // two buffers of partial sums: the next row's do not meet this one's readers
     if (a.w) f.set(rsqrtf(__fdiv_rn(block_sum(ss, part[flip]), (float)a.cols) + a.eps));
+    const Two p = two(f.p, f.p);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = col(i);
       if (a.w) {
-        float g[8];
-        T::widen8(rw[i], g);
+        Two g[4];
+        widen(rw[i], g);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) h[i][k] = h[i][k] * f.p * g[k];
+        for (int k = 0; k < 4; ++k) h[i][k] = mul2(mul2(h[i][k], p), g[k]);
       }
-      uint32_t m = 0;
+      float top = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) m = max(m, mag(h[i][k]));
+      for (int k = 0; k < 4; ++k) top = max_abs(top, h[i][k]);
+      uint32_t m = mag(top);
 #pragma unroll
       for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(FULL, m, d));
       if (c < a.cols) {
         const Block blk(m, f);
-        float q[8];
+        const Two bc = two(blk.c, blk.c), br = two(blk.r, blk.r), bn = two(-blk.n, -blk.n);
+        uint32_t q[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) q[k] = blk(h[i][k]);
-        *reinterpret_cast<uint2*>(a.codes + row * a.cols + c) =
-            make_uint2(pack4(q[0], q[1], q[2], q[3]), pack4(q[4], q[5], q[6], q[7]));
+        for (int k = 0; k < 4; ++k) {  // Block's operator(), two at a time
+          const Two t = mul2(h[i][k], bc), u = mul2(t, br);
+          const float2 v = each(fma2(fma2(u, bn, t), br, u));
+          q[k] = pack2(v.x, v.y);
+        }
+        *reinterpret_cast<uint2*>(a.codes + row * a.cols + c) = make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
         if ((threadIdx.x & 15) == 0) a.scale[row * a.nblk + (c >> 7)] = blk.s;
       }
     }
