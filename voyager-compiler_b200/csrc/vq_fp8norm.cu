@@ -41,6 +41,7 @@ struct Args {
   int64_t ldx, ldr;
   int64_t rows;
   int cols, nblk;  // nblk = ceil(cols / 128)
+  int eb;          // bytes of an element
   float eps;
   uint8_t* codes;  // [rows, cols]
   float* scale;    // [rows, nblk]
@@ -123,19 +124,21 @@ struct Block {
     const int e = min(max((int)(bits >> 23), 9), 254);  // biased
     c = __uint_as_float((uint32_t)(254 + 8 - e) << 23) * 1.75f;
     n = __uint_as_float(bits) * __uint_as_float(e == 254 ? 0x00400000u : (uint32_t)(254 - e) << 23);
-    s = __fdiv_rn(n * f.m, QMAX) * __uint_as_float((uint32_t)e << 23);
+    s = over(n * f.m, QMAX, 1.0f / QMAX) * __uint_as_float((uint32_t)e << 23);
     if (s == 0.0f) s = n = 1.0f, c = 0.0f;
     if (bits >= 0x7F800000u) {  // infinity over infinity is NaN, the rest of its block 0
       s = __uint_as_float(bits);
       c = bits == 0x7F800000u ? 0.0f : s;
       n = 1.0f;
     }
-    r = __fdiv_rn(1.0f, n);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(n));
   }
-  __device__ __forceinline__ float operator()(float z) const {
-    const float t = z * c, q = t * r;
+  // t / n with r near 1 / n
+  static __device__ __forceinline__ float over(float t, float n, float r) {
+    const float q = t * r;
     return fmaf(fmaf(-q, n, t), r, q);
   }
+  __device__ __forceinline__ float operator()(float z) const { return over(z * c, n, r); }
 };
 
 // A CTA takes rows blockIdx.x, + gridDim.x, ..; NV groups of 8 consecutive
@@ -143,7 +146,8 @@ struct Block {
 // of 128 columns is 16 neighbouring lanes.  The next row's loads are in
 // flight while this one is summed and quantized (without that the SMs waited
 // for them half the time: 16384 x 4096 bf16 with a residual took 111 us, now
-// 78, 0.93 of the copy rate), and the weight stays in registers.
+// 72, the copy rate), and the weight stays in registers.  Two neighbouring
+// elements go through each float32 instruction (one by one: 78 us).
 template <typename T, int NV, int MAXT>
 __global__ void __launch_bounds__(MAXT) k_norm_vec(const Args a) {
   using E = typename T::type;
@@ -240,23 +244,25 @@ __global__ void __launch_bounds__(MAXT) k_norm_vec(const Args a) {
   }
 }
 
-// Columns that are no multiple of 8, or rows off 16 bytes: one CTA per row, a
-// warp takes NB blocks of 128 columns, VEC neighbouring elements a load (2
-// where rows keep the pairs aligned).  The values stay in registers, and with
-// NB = 4 a lane has 16 loads of x in flight (4 passes of one block each over
-// the row, read twice, took 60 us for 7158 x 1630 bf16 with a residual).
+// Columns that are no multiple of 8, or rows off 16 bytes: a warp takes NB
+// blocks of 128 columns, VEC neighbouring elements a load (2 where rows keep
+// the pairs aligned), so that its loads and stores stay dense.  Rows as in
+// k_norm_vec; with NB = 4 the registers hold no second row.
+// (One CTA per row took 34.6 us for 7158 x 1630 bf16 with a residual, 22.3
+// now; instructions bound it: 20 us without the residual.)
 template <typename T, int VEC>
-__device__ __forceinline__ void load_v(const typename T::type* p, float (&v)[VEC]) {
-  if (VEC == 1) {
-    v[0] = T::load(p);
-  } else if (sizeof(*p) == 2) {
-    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(p));
-    v[0] = bf_lo(w), v[VEC - 1] = bf_hi(w);
-  } else {
-    const float2 f = __ldg(reinterpret_cast<const float2*>(p));
-    v[0] = f.x, v[VEC - 1] = f.y;
+struct Few {  // VEC elements as they lie in memory
+  using E = typename T::type;
+  E v[VEC];
+  __device__ __forceinline__ void load(const E* p) {
+    if (VEC == 1)
+      v[0] = __ldg(p);
+    else if (sizeof(E) == 2)
+      *reinterpret_cast<uint32_t*>(v) = __ldg(reinterpret_cast<const uint32_t*>(p));
+    else
+      *reinterpret_cast<float2*>(v) = __ldg(reinterpret_cast<const float2*>(p));
   }
-}
+};
 template <typename T, int VEC>
 __device__ __forceinline__ void store_v(typename T::type* p, const float (&v)[VEC]) {
   if (VEC == 1)
@@ -266,81 +272,92 @@ __device__ __forceinline__ void store_v(typename T::type* p, const float (&v)[VE
   else
     *reinterpret_cast<float2*>(p) = make_float2(v[0], v[VEC - 1]);
 }
-template <typename T, int NB, int VEC>
-__global__ void __launch_bounds__(1024) k_norm_blocks(const Args a) {
+template <typename T, int NB, int VEC, int MAXT>
+__global__ void __launch_bounds__(MAXT) k_norm_blocks(const Args a) {
   using E = typename T::type;
   constexpr int PER = 4 / VEC;  // loads of a lane per block
-  __shared__ float part[32];
+  constexpr int N = NB * PER;
+  constexpr bool AHEAD = NB < 4;
+  __shared__ float part[2][32];
+  const E* x = reinterpret_cast<const E*>(a.x);
+  const E* r = reinterpret_cast<const E*>(a.r);
+  const E* w = reinterpret_cast<const E*>(a.w);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto col = [&](int i) { return warp * NB * 128 + lane * VEC + i * 32 * VEC; };
   pdl::trigger();
   pdl::wait();
-  const int64_t row = blockIdx.x;
-  const E* x = reinterpret_cast<const E*>(a.x) + row * a.ldx;
-  const E* r = reinterpret_cast<const E*>(a.r) + row * a.ldr;
-  const E* w = reinterpret_cast<const E*>(a.w);
-  E* hid = reinterpret_cast<E*>(a.hidden) + row * a.cols;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c0 = warp * NB * 128 + lane * VEC;
-  float h[NB * PER][VEC];
+  alignas(8) Few<T, VEC> rx[N] = {}, rr[N] = {}, rw[N] = {};
+  auto fetch = [&](int64_t row) {
 #pragma unroll
-  for (int i = 0; i < NB * PER; ++i) {
-    const int c = c0 + i * 32 * VEC;
+    for (int i = 0; i < N; ++i)
+      if (col(i) < a.cols) rx[i].load(x + row * a.ldx + col(i));
+    if (a.r) {
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) h[i][k] = 0.0f;
-    if (c < a.cols) load_v<T, VEC>(x + c, h[i]);
-  }
-  if (a.r) {
-    float q[NB * PER][VEC];
-#pragma unroll
-    for (int i = 0; i < NB * PER; ++i)
-      if (c0 + i * 32 * VEC < a.cols) load_v<T, VEC>(r + c0 + i * 32 * VEC, q[i]);
-#pragma unroll
-    for (int i = 0; i < NB * PER; ++i)
-      if (c0 + i * 32 * VEC < a.cols) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) h[i][k] += q[i][k];
-        store_v<T, VEC>(hid + c0 + i * 32 * VEC, h[i]);
-      }
-  }
-  Factor f;
-  if (a.w) {
-    float g[NB * PER][VEC];
-    float ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NB * PER; ++i) {
-      if (c0 + i * 32 * VEC < a.cols) load_v<T, VEC>(w + c0 + i * 32 * VEC, g[i]);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) ss = fmaf(h[i][k], h[i][k], ss);
+      for (int i = 0; i < N; ++i)
+        if (col(i) < a.cols) rr[i].load(r + row * a.ldr + col(i));
     }
-    f.set(rsqrtf(__fdiv_rn(block_sum(ss, part), (float)a.cols) + a.eps));
+  };
+  auto fetch_w = [&]() {
 #pragma unroll
-    for (int i = 0; i < NB * PER; ++i)
-      if (c0 + i * 32 * VEC < a.cols) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) h[i][k] = h[i][k] * f.p * g[i][k];
-      }
+    for (int i = 0; i < N; ++i)
+      if (col(i) < a.cols) rw[i].load(w + col(i));
+  };
+  if (AHEAD) {
+    fetch(blockIdx.x);
+    if (a.w) fetch_w();
   }
+  int flip = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, flip ^= 1) {
+    E* hid = reinterpret_cast<E*>(a.hidden) + row * a.cols;
+    if (!AHEAD) fetch(row);
+    float h[N][VEC], ss = 0.0f;
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    uint32_t m = 0;
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int i = 0; i < PER; ++i)
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) m = max(m, mag(h[b * PER + i][k]));
-    m = __reduce_max_sync(FULL, m);
-    const Block over(m, f);
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int c = c0 + (b * PER + i) * 32 * VEC;
-      if (c < a.cols) {
-        const uint32_t q = pack2(over(h[b * PER + i][0]), over(h[b * PER + i][VEC - 1]));
-        if (VEC == 1)
-          a.codes[row * a.cols + c] = (uint8_t)q;
-        else
-          *reinterpret_cast<uint16_t*>(a.codes + row * a.cols + c) = (uint16_t)q;
+      for (int k = 0; k < VEC; ++k) {
+        h[i][k] = T::load(rx[i].v + k);
+        if (a.r) h[i][k] += T::load(rr[i].v + k);
+        ss = fmaf(h[i][k], h[i][k], ss);
       }
+    if (AHEAD && row + gridDim.x < a.rows) fetch(row + gridDim.x);
+    if (a.r) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (col(i) < a.cols) store_v<T, VEC>(hid + col(i), h[i]);
     }
-    const int blk = warp * NB + b;
-    if (lane == 0 && blk < a.nblk) a.scale[row * a.nblk + blk] = over.s;
+    Factor f;
+    if (a.w) {
+      if (!AHEAD) fetch_w();
+      f.set(rsqrtf(__fdiv_rn(block_sum(ss, part[flip]), (float)a.cols) + a.eps));
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)  // past the row 0, whatever f is
+          h[i][k] = col(i) < a.cols ? h[i][k] * f.p * T::load(rw[i].v + k) : 0.0f;
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) m = max(m, mag(h[b * PER + i][k]));
+      m = __reduce_max_sync(FULL, m);
+      const Block over(m, f);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int c = col(b * PER + i);
+        if (c < a.cols) {
+          const uint32_t q = pack2(over(h[b * PER + i][0]), over(h[b * PER + i][VEC - 1]));
+          if (VEC == 1)
+            a.codes[row * a.cols + c] = (uint8_t)q;
+          else
+            *reinterpret_cast<uint16_t*>(a.codes + row * a.cols + c) = (uint16_t)q;
+        }
+      }
+      const int blk = warp * NB + b;
+      if (lane == 0 && blk < a.nblk) a.scale[row * a.nblk + blk] = over.s;
+    }
   }
 }
 
@@ -394,9 +411,13 @@ __global__ void __launch_bounds__(1024) k_norm_any(const Args a) {
   }
 }
 
-// As many CTAs as fit at once (asked once per device and CTA size), or one per row.
-template <typename T, int NV, int MAXT>
-bool launch_vec(const Args& a, int threads, cudaStream_t st) {
+// As many CTAs as fit at once (asked once per device and CTA size), or one per
+// row; but no more per SM than have 56 KB of next rows in flight, beyond which
+// HBM slows down (16384 x 4096 bf16 with a residual: 72 us with three CTAs of
+// 16 KB, 81 with four; 16384 x 3328: 60 with four of 13 KB, 65 with three), and
+// three at least (9000 x 5120: 55 us, with two 70).
+template <auto F>
+bool launch_rows(const Args& a, int threads, cudaStream_t st) {
   static int known[64][33] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -404,30 +425,34 @@ bool launch_vec(const Args& a, int threads, cudaStream_t st) {
   int& per_sm = known[dev][threads / 32];
   if (per_sm == 0) {
     int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_norm_vec<T, NV, MAXT>, threads, 0) != cudaSuccess || n < 1) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, F, threads, 0) != cudaSuccess || n < 1) {
       (void)cudaGetLastError();
       n = 1;
     }
     per_sm = n;
   }
-  const int64_t grid = std::min<int64_t>(a.rows, (int64_t)per_sm * vq::mx::sm_count());
+  const int64_t ahead = (int64_t)a.cols * a.eb * (a.r ? 2 : 1);
+  const int64_t most = std::max<int64_t>(3, (56 << 10) / ahead);
+  const int64_t grid = std::min(a.rows, std::min<int64_t>(per_sm, most) * vq::mx::sm_count());
   if (a.rows > grid)  // long enough
-    return pdl::launch<k_norm_vec<T, NV, MAXT>, false>((unsigned)grid, threads, 0, st, 1, a);
-  return pdl::launch<k_norm_vec<T, NV, MAXT>>((unsigned)grid, threads, 0, st, 1, a);
+    return pdl::launch<F, false>((unsigned)grid, threads, 0, st, 1, a);
+  return pdl::launch<F>((unsigned)grid, threads, 0, st, 1, a);
 }
 
 template <typename T, int VEC>
 bool launch_blocks(const Args& a, cudaStream_t st) {
-  // a block a warp while there are few rows (latency), four for many
-  const int nb = a.rows < 256 && a.nblk <= 32 ? 1 : a.nblk <= 2 ? 1 : a.nblk <= 6 ? 2 : 4;
+  // blocks a warp: one while there are few rows (latency), else two (four:
+  // 34.6 against 26.9 us for 7158 x 1630) where a CTA holds the row so
+  const int nb = (a.rows < 256 && a.nblk <= 32) || a.nblk <= 2 ? 1 : a.nblk <= 64 ? 2 : 4;
   const int threads = (a.nblk + nb - 1) / nb * 32;
-  const unsigned rows = (unsigned)a.rows;
   if (nb == 1)
-    return pdl::launch<k_norm_blocks<T, 1, VEC>>(rows, threads, 0, st, 1, a);
+    return threads <= 256 ? launch_rows<k_norm_blocks<T, 1, VEC, 256>>(a, threads, st)
+                          : launch_rows<k_norm_blocks<T, 1, VEC, 1024>>(a, threads, st);
   else if (nb == 2)
-    return pdl::launch<k_norm_blocks<T, 2, VEC>>(rows, threads, 0, st, 1, a);
+    return threads <= 256 ? launch_rows<k_norm_blocks<T, 2, VEC, 256>>(a, threads, st)
+                          : launch_rows<k_norm_blocks<T, 2, VEC, 1024>>(a, threads, st);
   else
-    return pdl::launch<k_norm_blocks<T, 4, VEC>>(rows, threads, 0, st, 1, a);
+    return launch_rows<k_norm_blocks<T, 4, VEC, 1024>>(a, threads, st);
 }
 
 // vec: elements that every row start keeps together (8, 2 or 1).
@@ -442,11 +467,11 @@ bool launch(const Args& a, int vec, cudaStream_t st) {
     while (groups > nv * (a.rows < 256 ? 1024 : 256) && nv < 4) nv *= 2;
     const int threads = std::min(1024, ((groups + nv - 1) / nv + 31) / 32 * 32);
     if (nv == 1)
-      return threads <= 256 ? launch_vec<T, 1, 256>(a, threads, st) : launch_vec<T, 1, 1024>(a, threads, st);
+      return threads <= 256 ? launch_rows<k_norm_vec<T, 1, 256>>(a, threads, st) : launch_rows<k_norm_vec<T, 1, 1024>>(a, threads, st);
     else if (nv == 2)
-      return threads <= 256 ? launch_vec<T, 2, 256>(a, threads, st) : launch_vec<T, 2, 1024>(a, threads, st);
+      return threads <= 256 ? launch_rows<k_norm_vec<T, 2, 256>>(a, threads, st) : launch_rows<k_norm_vec<T, 2, 1024>>(a, threads, st);
     else
-      return threads <= 256 ? launch_vec<T, 4, 256>(a, threads, st) : launch_vec<T, 4, 1024>(a, threads, st);
+      return threads <= 256 ? launch_rows<k_norm_vec<T, 4, 256>>(a, threads, st) : launch_rows<k_norm_vec<T, 4, 1024>>(a, threads, st);
   } else if (a.nblk <= 128) {
     return vec >= 2 ? launch_blocks<T, 2>(a, st) : launch_blocks<T, 1>(a, st);
   } else {
@@ -481,6 +506,7 @@ extern "C" int vq_norm_quantize_fp8(const void* x, int64_t ldx, const void* resi
   a.ldr = residual ? ldr : 0;
   a.rows = rows;
   a.cols = (int)cols;
+  a.eb = eb;
   a.nblk = (int)((cols + 127) / 128);
   a.eps = eps;
   a.codes = reinterpret_cast<uint8_t*>(codes);
