@@ -303,7 +303,9 @@ __device__ __forceinline__ void store4(const Args& a, int row, int n, float (&v)
 // 128 x 128 tiles: four TMEM buffers of 128 columns.  Persistent, one CTA per
 // tile; where there are tiles for half of the SMs or less, a cluster of
 // a.splits CTAs per tile, each with a part of K, whose float32 sums meet in
-// shared memory (the grid then has every tile's CTAs).
+// shared memory (the grid then has every tile's CTAs).  Bound by the hand-over
+// of the buffers, about 0.4 us a block of K, and by start and end: 333 tokens,
+// 5003 x 2000, 120 tiles of 16 blocks: 11.1 us.
 struct One {
   static constexpr int STAGES = 6, STAGE = 2 * 128 * BK, BUFS = 4, THREADS = 384, COLS = 64;
   static constexpr int LD = 132;  // floats per row of the sums in shared memory
@@ -464,7 +466,9 @@ __global__ void __launch_bounds__(One::THREADS, 1)
 // 256 x 256 tiles on CTA pairs (cta_group::2): each CTA holds 128 token rows
 // in its TMEM and loads those and half of the weight rows, 32 KB per block
 // instead of the 48 KB that a CTA of its own needs for 128 x 256.  The even
-// CTA issues the MMAs.
+// CTA issues the MMAs.  4096 tokens, 22016 x 4096: 362 us, 2.04 PFLOP/s (429
+// where the power cap sets the clock); the tensor pipe is 51 % active, the
+// promotion's readback and multiply-adds of 256 columns a block set the pace.
 struct Pair {
   static constexpr int BN = 256, COLS = BN / 2, A_BYTES = 128 * BK, STAGE = A_BYTES + BN / 2 * BK, STAGES = 6;
   // 3 warpgroups per CTA: TMA and MMA issue, then two of promotion.  The
@@ -610,30 +614,37 @@ __global__ void __launch_bounds__(Pair::THREADS, 1)
 }
 
 // ---------------------------------------------------------------------------
-template <int BN>
+// Bound by HBM, one token 12288 x 4096: 11.9 us, 4.2 TB/s, of which start, first
+// loads and the end take 4.  PER_SM: CTAs on an SM.  One with a deep ring and
+// registers for a whole buffer's readback while the tiles are no more than the
+// SMs (64 tokens, 12288 x 4096: 16.5 us, with two 23.2; one CTA a SM also
+// spreads the clusters), two where they are more (one token, 22016 x 4096, 172
+// tiles: 19.1 us, with one 26.6).
+template <int BN, int PER_SM>
 struct Few {
   static constexpr int W_BYTES = 128 * BK, X_BYTES = BN * BK, STAGE = W_BYTES + X_BYTES;
-  static constexpr int STAGES = BN == 16 ? 6 : BN == 32 ? 5 : 4;
+  static constexpr int STAGES = PER_SM == 1 ? (BN == 16 ? 10 : BN == 32 ? 9 : 7) : BN == 16 ? 6 : BN == 32 ? 5 : 4;
   static constexpr int BUFS = 4;
   static constexpr int TMEM = BUFS * BN < 32 ? 32 : BUFS * BN;
   static constexpr int THREADS = 192;
-  static constexpr int KC = 16;  // K blocks per refill of the scales
+  static constexpr int KC = 32;  // K blocks per refill of the scales
+  static constexpr int LS = BN + 4;  // floats per block of them in shared memory
   static constexpr int LD = 132; // floats per token of the sums in shared memory
   static constexpr int RING = STAGES * STAGE > BN * LD * 4 ? STAGES * STAGE : BN * LD * 4;
-  static constexpr int SMEM = RING + KC * BN * 4 + 1024 + 256;
-  static_assert(2 * SMEM + 2048 <= 227 * 1024, "two CTAs per SM");
+  static constexpr int SMEM = RING + KC * LS * 4 + 1024 + 256;
+  static_assert(PER_SM * (SMEM + 1024) <= 228 * 1024, "CTAs per SM");
 };
 
-template <int BN>
-__global__ void __launch_bounds__(Few<BN>::THREADS, 2)
+template <int BN, int PER_SM>
+__global__ void __launch_bounds__(Few<BN, PER_SM>::THREADS, PER_SM)
     k_fp8_few(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
               const __grid_constant__ Args a) {
-  using C = Few<BN>;
+  using C = Few<BN, PER_SM>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~(uintptr_t)1023);
-  float* s_scale = reinterpret_cast<float*>(smem + C::RING);  // [KC][BN]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_scale + C::KC * BN);
+  float* s_scale = reinterpret_cast<float*>(smem + C::RING);  // [KC][LS]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_scale + C::KC * C::LS);
   const uint32_t full0 = smem_u32(bars), empty0 = full0 + 8 * C::STAGES;
   const uint32_t acc_full0 = empty0 + 8 * C::STAGES, acc_empty0 = acc_full0 + 8 * C::BUFS;
   const uint32_t drain = acc_empty0 + 8 * C::BUFS;
@@ -709,7 +720,7 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
     }
     __syncwarp();
   }
-  float acc[BN];
+  uint64_t acc[BN / 2];  // two tokens each
   const int q = warp & 3;  // TMEM lane quarter of warps 2..5
   if (warp >= 2) {
     int buf = 0;
@@ -717,7 +728,7 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
     const int pt = threadIdx.x - 64;
     const float* sw = a.sw + (int64_t)tn * a.nk;
 #pragma unroll
-    for (int i = 0; i < BN; ++i) acc[i] = 0.0f;
+    for (int i = 0; i < BN / 2; ++i) acc[i] = 0;
     bool ok = true;
     for (int kc = kb0; kc < kb1; kc += C::KC) {
       // the scales of the next KC blocks, sa * sw per block and token, all
@@ -735,7 +746,7 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
 #pragma unroll
       for (int u = 0; u < PER; ++u) {
         const int i = pt + u * 128;
-        s_scale[i % C::KC * BN + i / C::KC] = sv[u];
+        s_scale[i % C::KC * C::LS + i / C::KC] = sv[u];
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");
       for (int k = 0; k < n && ok; ++k) {
@@ -745,18 +756,17 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
         }
         tc_fence_after();
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + buf * BN;
+        uint32_t r[BN / 16][16];
 #pragma unroll
-        for (int c = 0; c < BN; c += 16) {
-          uint32_t r[16];
-          tmem_ld16(taddr + c, r);
-          tmem_wait(r);
+        for (int c = 0; c < BN / 16; ++c) tmem_ld16(taddr + 16 * c, r[c]);
+#pragma unroll
+        for (int c = 0; c < BN / 16; ++c) {
+          tmem_wait(r[c]);
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
-            const float4 s = *reinterpret_cast<const float4*>(s_scale + k * BN + c + i);
-            acc[c + i] = fmaf(__uint_as_float(r[i]), s.x, acc[c + i]);
-            acc[c + i + 1] = fmaf(__uint_as_float(r[i + 1]), s.y, acc[c + i + 1]);
-            acc[c + i + 2] = fmaf(__uint_as_float(r[i + 2]), s.z, acc[c + i + 2]);
-            acc[c + i + 3] = fmaf(__uint_as_float(r[i + 3]), s.w, acc[c + i + 3]);
+            const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(s_scale + k * C::LS + 16 * c + i);
+            fma2(acc[8 * c + i / 2], r[c][i], r[c][i + 1], s.x);
+            fma2(acc[8 * c + i / 2 + 1], r[c][i + 2], r[c][i + 3], s.y);
           }
         }
         tc_fence_before();
@@ -773,7 +783,8 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
   float* red = reinterpret_cast<float*>(smem);
   if (warp >= 2) {
 #pragma unroll
-    for (int i = 0; i < BN; ++i) red[i * C::LD + q * 32 + lane] = acc[i];
+    for (int i = 0; i < BN; ++i)
+      red[i * C::LD + q * 32 + lane] = i % 2 ? unpair(acc[i / 2]).y : unpair(acc[i / 2]).x;
   }
   if (a.splits > 1)
     cluster_sync();
@@ -798,8 +809,7 @@ __global__ void __launch_bounds__(Few<BN>::THREADS, 2)
 
 // ---------------------------------------------------------------------------
 // Clusters of s CTAs of kernel F that the device holds at once (asked once per
-// device and size): clusters of 3, for one, do not fill two CTAs per SM (288
-// CTAs in two waves took 18 us, 12 in one).
+// device and size; one CTA an SM): clusters of 3, for one, reach 135 SMs.
 template <auto F>
 int resident_clusters(int s, int threads, int smem) {
   static int known[64][9] = {};
@@ -868,20 +878,23 @@ int launch_many(const void* x, const void* w, int64_t K, Args a, cudaStream_t st
   return pdl::launch<k_fp8_one>(grid, One::THREADS, One::SMEM, st, a.splits, ma, mw, a) ? VQ_OK : VQ_ERR_CUDA;
 }
 
-template <int BN>
+template <int BN, int PER_SM>
 int launch_few(const void* x, const void* w, int64_t K, Args a, cudaStream_t st) {
-  using C = Few<BN>;
+  using C = Few<BN, PER_SM>;
   static_assert((2 * C::STAGES + 2 * C::BUFS + 2) * 8 <= 256, "barrier area");
   CUtensorMap mx_, mw;
   if (!vq::mx::make_map(&mx_, x, a.M, K, BN) || !vq::mx::make_map(&mw, w, a.N, K, 128)) return VQ_ERR_CUDA;
-  if (!allow_smem<k_fp8_few<BN>>(C::SMEM))
-    return VQ_ERR_CUDA;
+  if (!allow_smem<k_fp8_few<BN, PER_SM>>(C::SMEM)) return VQ_ERR_CUDA;
+  a.splits = PER_SM == 1 ? best_split<k_fp8_few<BN, PER_SM>>(a.tiles, a.nk, C::THREADS, C::SMEM) : 1;
+  return pdl::launch<k_fp8_few<BN, PER_SM>>(a.tiles * a.splits, C::THREADS, C::SMEM, st, a.splits, mx_, mw, a)
+             ? VQ_OK : VQ_ERR_CUDA;
+}
+template <int BN>
+int launch_few(const void* x, const void* w, int64_t K, Args a, cudaStream_t st) {
   a.mt = (a.M + BN - 1) / BN;
   a.nt = (a.N + 127) / 128;
   a.tiles = a.mt * a.nt;
-  a.splits = best_split<k_fp8_few<BN>>(a.tiles, a.nk, C::THREADS, C::SMEM);
-  return pdl::launch<k_fp8_few<BN>>(a.tiles * a.splits, C::THREADS, C::SMEM, st, a.splits, mx_, mw, a)
-             ? VQ_OK : VQ_ERR_CUDA;
+  return a.tiles <= vq::mx::sm_count() ? launch_few<BN, 1>(x, w, K, a, st) : launch_few<BN, 2>(x, w, K, a, st);
 }
 
 int sticky_f8(int* out, int clear, cudaStream_t st) { return vq::tc::sticky_read(out, clear, st); }
