@@ -247,8 +247,8 @@ __global__ void __launch_bounds__(Q_THREADS) k_turn_q(const __grid_constant__ Ar
   using E = typename T::type;
   extern __shared__ __align__(16) uint8_t smem[];
   const Ring<T, Q_THREADS> ring(smem);
-  pdl::trigger();
   pdl::wait();
+  pdl::trigger();  // k_rope_append waits for nothing else that this one waited for
   const QUnit x = q_unit<IL, D>(a, (int64_t)blockIdx.x * Q_THREADS + threadIdx.x);
   if (!x.any) return;
   E* out = reinterpret_cast<E*>(a.q_out) + x.row * a.H * D;
@@ -354,14 +354,15 @@ __device__ __forceinline__ void rescale16(uint4* p, float f) {
 // values one after the other, so that the angles of a page's tokens come from
 // L1 after the first.  TH = page * D / 32 threads: two units of every thread
 // are a whole block, held in registers between its maximum and its codes,
-// while the next two blocks' loads are in flight.
+// while the next two blocks' loads are in flight.  768 threads an SM: 8 prompts
+// of 2048 tokens, 32 heads of 128, q included: 132 us (5.1 TB/s); with 512, 140,
+// with 1024 and spilled registers 162.
 template <typename T, bool IL, int D, int TH>
-__global__ void __launch_bounds__(TH) k_rope_append(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(TH, TH > 512 ? 1 : 768 / TH) k_rope_append(const __grid_constant__ Args a) {
   using E = typename T::type;
   constexpr int U = D / 16, ROWS = TH / U, IT = 2;  // threads per token, tokens per pass, passes
   __shared__ uint32_t part[2][TH / 32];
   pdl::trigger();
-  pdl::wait();
   int i = blockIdx.x;
   const int hg = (a.Hkv + a.hc - 1) / a.hc, h0 = i % hg * a.hc, h1 = min(a.Hkv, h0 + a.hc);
   i /= hg;
@@ -369,7 +370,12 @@ __global__ void __launch_bounds__(TH) k_rope_append(const __grid_constant__ Args
   i >>= 1;
   const int b = i / a.W;
   const Block k = block_of(a, b, i % a.W);
-  if (k.tokens <= 0) return;
+  // k_turn_q, launched before this kernel, shares nothing with it, so only the
+  // end waits: kernels behind this one then come after both
+  if (k.tokens <= 0) {
+    pdl::wait();
+    return;
+  }
   const int u = threadIdx.x % U, r0 = threadIdx.x / U;
   const Strides st = is_v ? a.sv : a.sk;
   const E* src = reinterpret_cast<const E*>(is_v ? a.v : a.k) + b * st.b + k.t0 * st.t + r0 * st.t;
@@ -435,6 +441,7 @@ __global__ void __launch_bounds__(TH) k_rope_append(const __grid_constant__ Args
     if (threadIdx.x == 0) *scale = s;  // every thread read the old one before the barrier
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
+  pdl::wait();
 }
 
 // Few new tokens (T <= G of 1, 2 or 4, or 8 at D = 64): G * D / 16 lanes take
@@ -493,7 +500,7 @@ __global__ void __launch_bounds__(FEW_THREADS) k_rope_append_few(const __grid_co
 template <typename T, bool IL, int D, int TH>
 void launch_cache(const Args& a, unsigned n, int64_t& blocks, cudaStream_t st) {
   if (!tc::allow_smem<k_rope_append<T, IL, D, TH>>(Ring<T, TH>::BYTES) ||
-      !pdl::launch<k_rope_append<T, IL, D, TH>, false>(n, TH, Ring<T, TH>::BYTES, st, 1, a))
+      !pdl::launch<k_rope_append<T, IL, D, TH>>(n, TH, Ring<T, TH>::BYTES, st, 1, a))
     blocks = -1;
 }
 // blocks: of the largest launch (2^31 or more: nothing launched), -1: a CUDA call failed.
@@ -523,7 +530,7 @@ void launch_d(Args& a, int64_t& blocks, cudaStream_t st) {
   const int sms = vq::mx::sm_count();
   while (a.hq < a.H && q_ctas(Q_THREADS) >= 12 * sms) a.hq *= 2;
   a.hc = 1;
-  while (a.hc < 8 && a.hc < a.Hkv && items / (2 * a.hc) >= 8 * sms) a.hc *= 2;
+  while (a.hc < 4 && a.hc < a.Hkv && items / (2 * a.hc) >= 8 * sms) a.hc *= 2;
   blocks = std::max(q_ctas(Q_THREADS), (int64_t)a.B * a.W * 2 * ((a.Hkv + a.hc - 1) / a.hc));
   if (blocks >= (1ll << 31)) return;
   if (!tc::allow_smem<k_turn_q<T, IL, D>>(Ring<T, Q_THREADS>::BYTES) ||
