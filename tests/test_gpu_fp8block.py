@@ -69,6 +69,18 @@ def test_norm(R, C, dtype):
     _check_norm(x, None)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("R,C", [(7000, 264), (9001, 250), (6000, 633), (3000, 1630), (1500, 4104), (700, 11007)])
+def test_norm_many_rows(R, C, dtype):
+    """More rows than CTAs: each takes several, with the next one in flight."""
+    g = _gen(R + C)
+    x, r = (torch.randn(R, C, generator=g, device="cuda").to(dtype) for _ in range(2))
+    w = (1 + 0.2 * torch.randn(C, generator=g, device="cuda")).to(dtype)
+    _check_norm(x, w)
+    _check_norm(x, w, residual=r)
+    _check_norm(x, None)
+
+
 @pytest.mark.parametrize("C", [384, 401])
 def test_norm_strides_and_shapes(C):
     """Leading dims, row strides beyond the row, starts off 16 bytes, a
@@ -198,6 +210,13 @@ def test_linear(M, N, K):
                                    (64, 22016, 128), (2, 70000, 64), (1, 128, 65536)])
 def test_linear_large(M, N, K):
     _linear_case(M, N, K, N)
+
+
+@pytest.mark.parametrize("M", [3, 16, 30, 64])
+@pytest.mark.parametrize("N,K", [(20000, 720), (19001, 5008), (4096, 12304)])
+def test_linear_few_tokens_many_tiles(M, N, K):
+    """More tiles than SMs and fewer; K beyond one filling of the scales."""
+    _linear_case(M, N, K, M + N)
 
 
 def test_linear_views_and_empty():

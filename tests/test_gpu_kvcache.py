@@ -273,6 +273,23 @@ def test_attend_long(B, held):
     _check_attend(B, 6, 1, 8, 64, 32, [held - 77 * b for b in range(B)], seed=3)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,G", [(1, 1), (1, 2), (1, 3), (1, 5), (1, 8), (3, 4), (5, 4)])
+def test_attend_many_pieces(D, T, G):
+    """One head over all SMs: joins of more pieces than travel at once, for
+    every number of groups that share a row, and for several row tiles."""
+    _check_attend(1, T, 1, G, D, 128, [70001], seed=T * G)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,Hkv,top", [(8, 32, 700), (40, 7, 900), (24, 16, 200), (60, 5, 1500), (300, 1, 600)])
+def test_attend_cuts(D, B, Hkv, top):
+    """About a head per CTA, and more of them: cuts at heads' ends, within
+    heads, and within none, for equal and unequal lengths."""
+    _check_attend(B, 1, Hkv, 1, D, 64, [top] * B, seed=B)
+    _check_attend(B, 1, Hkv, 2, D, 64, [(i * 7919) % top if i % 5 else 0 for i in range(B)], seed=B + 1)
+
+
 def test_attend_empty_sequences():
     """No key at all, no new token, and both beside ordinary sequences."""
     _check_attend(4, 1, 2, 4, 128, 64, [0, 300, 0, 64], [0, 1, 1, 0], seed=1, stale=0xFF)
