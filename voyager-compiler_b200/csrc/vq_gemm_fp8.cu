@@ -20,6 +20,10 @@
 //             K is split over a cluster of CTAs, whose float32 sums are added
 //             in rank order through distributed shared memory.
 //
+// A kernel lets the next one start (programmatic dependent launch) only when
+// all its CTAs hold their TMEM: the next one's CTAs could otherwise take it
+// first and wait for a kernel that waits for them.
+//
 // TMA zero-fills rows and columns past the operands' ends.  Waits are
 // bounded.  No TMA multicast is used.
 #include <cuda.h>
@@ -330,7 +334,6 @@ __global__ void __launch_bounds__(One::THREADS, 1)
   const int rank = a.splits > 1 ? (int)cluster_ctarank() : 0;
   const int first = blockIdx.x / a.splits, step = gridDim.x / a.splits;
   const int kb0 = (int)((int64_t)a.nk * rank / a.splits), kb1 = (int)((int64_t)a.nk * (rank + 1) / a.splits);
-  pdl::trigger();
   auto load = [&](int tm, int tn, int kt, int stage) {
     const uint32_t dst = smem_u32(smem) + stage * C::STAGE;
     mbar_expect_tx(full0 + 8 * stage, C::STAGE);
@@ -359,6 +362,7 @@ __global__ void __launch_bounds__(One::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl::trigger();  // after the allocation
   pdl::wait();
 
   if (warp == 0 && lane == 0) {
@@ -502,7 +506,6 @@ __global__ void __launch_bounds__(Pair::THREADS, 1)
   const uint32_t rank = cluster_ctarank();  // 0: issues the pair's MMAs
   const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int pair_id = blockIdx.x >> 1, npairs = gridDim.x >> 1;
-  pdl::trigger();
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) mbar_init(full0 + 8 * s, 1), mbar_init(empty0 + 8 * s, 1);
     for (int s = 0; s < 2; ++s) mbar_init(acc_full0 + 8 * s, 1), mbar_init(acc_empty0 + 8 * s, 16);
@@ -518,6 +521,7 @@ __global__ void __launch_bounds__(Pair::THREADS, 1)
   cluster_sync();  // both CTAs' barriers exist before any use across them
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl::trigger();  // after the allocation
   pdl::wait();
 
   if (warp < 4) {
@@ -650,7 +654,6 @@ __global__ void __launch_bounds__(Few<BN, PER_SM>::THREADS, PER_SM)
   const uint32_t drain = acc_empty0 + 8 * C::BUFS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * C::STAGES + 2 * C::BUFS + 1);
   const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  pdl::trigger();
   const int rank = a.splits > 1 ? (int)cluster_ctarank() : 0;
   const int tile = blockIdx.x / a.splits, tm = tile / a.nt, tn = tile - tm * a.nt;
   const int kb0 = (int)((int64_t)a.nk * rank / a.splits);
@@ -681,6 +684,7 @@ __global__ void __launch_bounds__(Few<BN, PER_SM>::THREADS, PER_SM)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl::trigger();  // after the allocation
   pdl::wait();
 
   if (warp == 0) {
