@@ -85,7 +85,7 @@ def _build_binding(verbose: bool) -> None:
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *[f"-I{inc[0]}"],
            *[a for i in inc[1:] for a in ("-isystem", i)], "-D_GLIBCXX_USE_CXX11_ABI=1", PY_SRC, "-o", PY_OUT + ".tmp",
            f"-L{PKG}", "-l:" + os.path.basename(OUT), f"-L{os.path.join(torch, 'lib')}", "-lc10", "-lc10_cuda",
-           "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+           "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
