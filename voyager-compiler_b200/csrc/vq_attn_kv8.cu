@@ -81,7 +81,11 @@ template <int D, int NT>
 struct Cfg {
   static constexpr int ROWS = 8 * NT;
   static constexpr int TILE_BYTES = TILE * D;
-  static constexpr int PER_SM = ctas_per_sm(D, NT), STAGES = D == 128 ? 3 : PER_SM == 3 ? 4 : 5;
+  // Two stages a warp: 128 KB in flight an SM (96 KB at heads of 64) fill HBM, and
+  // more only lengthens the queue that every other access waits in (4 sequences
+  // of 131000 keys: 168 us, with three 178; heads of 64, 24 sequences of 28631:
+  // 118, with four 126).
+  static constexpr int PER_SM = ctas_per_sm(D, NT), STAGES = D == 128 || PER_SM == 3 ? 2 : 3;
   static constexpr int RING = STAGES * 2 * TILE_BYTES;  // per warp
   static constexpr int SMEM_RING = WARPS * RING;
   // the warps' O meet in SUMS buffers, rows LD floats apart
