@@ -194,6 +194,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::SMEM_RING + C::JOIN);  // [WARPS][STAGES]
   __shared__ int s_last, s_entry, s_before, s_run[2];
   __shared__ long long s_sum[WARPS];
+  __shared__ int s_top[WARPS];
   __shared__ int2 s_plan[PLANS];  // the first sequences' plans
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -222,10 +223,12 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
   const int entries = a.B * a.groups, per = (entries + THREADS - 1) / THREADS;
   const int e0 = min(entries, (int)threadIdx.x * per), e1 = min(entries, e0 + per);
   long long own = 0;
+  int top = 0;  // units of the longest head
 #pragma unroll 1
   for (int e = e0; e < e1; ++e) {
     const int u = units_of(entry(e));
     own += u ? u + (1ll << 32) : 0;
+    top = max(top, u);
   }
   long long scan = own;
 #pragma unroll
@@ -233,27 +236,30 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
     const long long y = __shfl_up_sync(FULL, scan, d);
     if (lane >= d) scan += y;
   }
-  if (lane == 31) s_sum[warp] = scan;
+  top = __reduce_max_sync(FULL, top);
+  if (lane == 31) s_sum[warp] = scan, s_top[warp] = top;
   __syncthreads();
   long long total = 0, before = scan - own;
 #pragma unroll
   for (int w = 0; w < WARPS; ++w) {
     if (w < warp) before += s_sum[w];
     total += s_sum[w];
+    top = max(top, s_top[w]);
   }
   // CTAs with work.  A piece more of a head costs its join about an eighth of
   // a unit's time, so a run is at least sqrt(units / 8) of an average head.
   // Where heads are not few a head counts HEAD units more than it has: opening,
   // joining and closing one takes that long.  A cut in those moves to the
-  // head's begin, and with about a head per run or more one within HEAD of its
-  // end moves there (256 heads of 609 keys on 296 CTAs: 15.2 us against 19.8;
-  // 112 heads, up to 2229 keys: 19.4 against 15.1).
+  // head's begin, and where a run about holds the longest head one within HEAD
+  // of a head's end moves there (256 heads of 609 keys on 296 CTAs: 15 us
+  // against 20; longer heads only give unequal runs).
   const int heads = (int)(total >> 32) * a.Hkv, real = (int)total * a.Hkv;
   const float least = heads ? fmaxf(1.0f, sqrtf(0.125f * (float)real / (float)heads)) : 1.0f;
   const int runs = min((int)gridDim.x, (int)ceilf((float)real / least));
-  const int HEAD = 6 * heads >= runs ? 5 : 0, near_end = 4 * heads >= 3 * runs ? HEAD : 0;
+  const int HEAD = 6 * heads >= runs ? 5 : 0;
   const int all = real + HEAD * heads;
-  const int base = runs ? all / runs : 0, rest = all - base * runs;  // the first `rest` runs have one more
+  const int base = runs ? all / runs : 0, near_end = 4 * (top + HEAD) <= 5 * base ? HEAD : 0;
+  const int rest = all - base * runs;  // the first `rest` runs have one more
   auto run_of = [&](int at) {  // the run that holds this unit, by the cuts as they were before they moved
     const int far = at - rest * (base + 1);
     return (far < 0 ? 0 : rest) + (far < 0 ? at : far) / (far < 0 ? base + 1 : base);
