@@ -445,7 +445,9 @@ __global__ void __launch_bounds__(TH, TH > 512 ? 1 : 768 / TH) k_rope_append(con
 }
 
 // Few new tokens (T <= G of 1, 2 or 4, or 8 at D = 64): G * D / 16 lanes take
-// a block, so that a warp holds several and no lane waits at a barrier.
+// a block, so that a warp holds several and no lane waits at a barrier.  Bound
+// by latency (plan, block table, the block's scale): one token 2.3 us, 64
+// sequences 2.6, of which the bytes take 0.2.
 constexpr int FEW_THREADS = 128;
 template <typename T, bool IL, int D, int G>
 __global__ void __launch_bounds__(FEW_THREADS) k_rope_append_few(const __grid_constant__ Args a) {
