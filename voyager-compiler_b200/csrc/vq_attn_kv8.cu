@@ -315,22 +315,22 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
   } sg = {};
   // A lane knows the page of tile 32 m + lane of the warp's tiles: its row in
   // the cache and its scales, n_ for the batch m that is being issued, c_ for
-  // the one being read; the block table is read a batch ahead.
+  // the one being read; the block table is read a batch ahead.  A page outside
+  // the cache has n_v = -1, so that its logarithm is NaN: its tiles load page 0
+  // and are passed over.
   int n_row = 0, pid_next = 0, mine = 0, issued = 0, wstage = 0;
-  float n_ks = 0.0f, n_lv = 0.0f, c_ks = 0.0f, c_lv = 0.0f;
+  float n_ks = 0.0f, n_v = 0.0f, c_ks = 0.0f, c_lv = 0.0f;
   auto key_of = [&](int tile) { return min(sg.k0 + (warp + tile * WARPS) * TILE, sg.k1 - 1); };
   auto pid_of = [&](int tile) { return a.block_table[(int64_t)sg.b * a.width + (key_of(tile) >> a.page_log2)]; };
   auto issue = [&]() {
     if ((issued & 31) == 0) {
-      int pid = pid_next;
-      if (pid < 0 || pid >= a.pages) {
-        note_err(nullptr, ERR_PAGE);
-        pid = 0;
-      }
-      const int blk = pid * a.Hkv + sg.kvh;
+      const bool outside = pid_next < 0 || pid_next >= a.pages;
+      if (outside) note_err(nullptr, ERR_PAGE);
+      const int blk = (outside ? 0 : pid_next) * a.Hkv + sg.kvh;
       n_row = (blk << a.page_log2) + (key_of(issued + lane) & ((1 << a.page_log2) - 1) & ~(TILE - 1));
       n_ks = a.k_scale[blk];
-      n_lv = a.v_scale[blk];
+      n_v = a.v_scale[blk];
+      n_v = outside ? -1.0f : n_v >= 0.0f ? n_v : -NEG_INF;  // no logarithm: the output is NaN
       pid_next = pid_of(issued + lane + 32);
     }
     const int y = __shfl_sync(FULL, n_row, issued & 31);
@@ -681,12 +681,18 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
   }
 
   int i = 0;
-  for (; i < mine; ++i) {
+  auto advance = [&]() {
+    __syncwarp();  // every lane has read the stage
+    if (issued < mine) issue();
+    if (++stage == C::STAGES) stage = 0, phase ^= 1;
+  };
+  for (; i < mine; ++i, advance()) {
     const int key0 = k0 + (warp + i * WARPS) * TILE;
-    if ((i & 31) == 0) c_ks = n_ks, c_lv = log2f(n_lv);
+    if ((i & 31) == 0) c_ks = n_ks, c_lv = log2f(n_v);
     const float ks = __shfl_sync(FULL, c_ks, i & 31), lv = __shfl_sync(FULL, c_lv, i & 31);
     ok = mbar_wait_warp(bar0 + 8 * stage, phase, nullptr, ERR_WAIT);
     if (!ok) break;
+    if (lv != lv) continue;  // a page outside the cache
     const uint32_t kb = ring + stage * 2 * C::TILE_BYTES, vb = kb + C::TILE_BYTES;
     const bool tail = key0 + TILE > free_end;
 
@@ -848,9 +854,6 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
           }
         }
     }
-    __syncwarp();  // every lane has read the stage
-    if (issued < mine) issue();
-    if (++stage == C::STAGES) stage = 0, phase ^= 1;
   }
   // after a wait that gave up: the loads in flight land before the ring is reused
   for (; i < issued; ++i) {
