@@ -121,3 +121,36 @@ def test_attend_leaves_out_pages_in_long_heads():
         voyager_b200.check_errors()
     want, mag = _attention_without(q[0].double(), cache, bt, 0, 0, held, 1)
     check_close(out[0], want, mag * 2.0 ** -10 + want.abs() * 2.0 ** -8)
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("D,T", [(64, 1), (64, 2), (64, 3), (64, 8), (128, 1), (128, 2), (128, 4)])
+def test_every_held_code_follows_a_grown_scale(D, T):
+    """Few new tokens whose values need larger scales in every block: all the
+    codes that a block holds are brought to its new scale, for any number of
+    lanes a block, and the scale is the one that the new values need."""
+    from voyager_b200 import kvcache
+
+    B, Hkv, page = 150, 3, 64
+    cache = _cache(2 * B, Hkv, page, D, D + T)
+    old = [t.clone() for t in (cache.k_codes.view(torch.uint8), cache.v_codes.view(torch.uint8), cache.k_scale,
+                               cache.v_scale)]
+    bt = torch.randperm(2 * B, generator=_gen(6), device="cuda").view(B, 2).int()
+    held = torch.randint(1, page - T + 1, (B,), generator=_gen(7), device="cuda").int()  # the new tokens end in page 0
+    k, v = (torch.randn(B, T, Hkv, D, generator=_gen(s), device="cuda") for s in (8, 9))
+    # keys of +-2^10, values of +-2^4: scales 2^2 and 2^-4, larger than the 2^-9 .. 2^-4 held
+    k, v = (k.sign() * 2.0 ** 10).bfloat16(), (v.sign() * 2.0 ** 4).bfloat16()
+    one = torch.tensor([1.0, 0.0], device="cuda").expand(2 * page, D // 2, 2).contiguous()  # no rotation
+    kvcache.rope_append(k, k, v, one, cache, bt, held)
+    pid = bt[:, 0].long()
+    for codes, scale, was, s0, new, s1 in ((cache.k_codes, cache.k_scale, old[0], old[2], k, 2.0 ** 2),
+                                           (cache.v_codes, cache.v_scale, old[1], old[3], v, 2.0 ** -4)):
+        assert bool((scale[pid] == s1).all())
+        assert torch.equal(scale[bt[:, 1].long()], s0[bt[:, 1].long()])
+        want = (was.view(E4M3)[pid].float() * (s0[pid] / s1)[..., None, None]).to(E4M3)  # a power of two: exact
+        for b in range(B):
+            h = int(held[b])
+            got = codes[pid[b]].float()
+            assert torch.equal(got[:, :h], want[b, :, :h].float())
+            assert torch.equal(got[:, h:h + T], new[b].transpose(0, 1).float() / s1)
+            assert torch.equal(codes.view(torch.uint8)[pid[b], :, h + T:], was[pid[b], :, h + T:])

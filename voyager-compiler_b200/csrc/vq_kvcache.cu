@@ -492,10 +492,11 @@ __global__ void __launch_bounds__(FEW_THREADS) k_rope_append_few(const __grid_co
   for (int d = L / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, d));
   const float s = fmaxf(pow2_scale(m), was), inv = __fdiv_rn(1.0f, s);
   if (mine) store_codes(codes + (k.slot0 + r) * D, c0, c1, x0, x1, inv);
+  __syncwarp();  // every lane has read the old scale before one writes the new
   if (live && k.tokens > 0) {
     if (k.slot0 && s != was)
       for (int c = l; c < k.slot0 * U; c += L) rescale16(reinterpret_cast<uint4*>(codes) + c, was * inv);
-    if (l == 0) *scale = s;  // the shuffles stand between it and the lanes that read the old one
+    if (l == 0) *scale = s;
   }
 }
 
