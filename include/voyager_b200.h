@@ -727,7 +727,8 @@ int vq_linear_fp8_block(const void* x, const float* x_scale, const void* w, cons
  * of a call may append to the same page.  A plan that does not fit (a count
  * outside 0..tokens, a negative length, tokens past table_width * page, a page
  * outside the cache) leaves the tokens concerned out and sets the device's
- * sticky word (301-303). */
+ * sticky word (301-303).  With table_width 0 (or pages 0) no token fits, and
+ * table and block_table (the cache's pointers) may be NULL. */
 int vq_rope_append_kv8(const void* q, const void* k, const void* v, const int64_t* strides,
                        int32_t dtype, const float* table, int64_t positions, int32_t rot,
                        int32_t interleaved, int64_t batch, int64_t tokens, int32_t heads,
@@ -747,7 +748,9 @@ int vq_rope_append_kv8(const void* q, const void* k, const void* v, const int64_
  *   vq_attn_kv8_workspace gives; the counters are 0 before the first call and
  *   left 0 by each; calls that can overlap on the GPU need their own.
  * Slots past a sequence's last token may hold anything.  Plans that do not fit
- * and waits that give up set the device's sticky word (311-314). */
+ * and waits that give up set the device's sticky word (311-314); the keys of a
+ * page outside the cache are left out.  With pages or table_width 0 no row sees
+ * a key; the inputs but lengths and counts may then be NULL. */
 int vq_attn_kv8_workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_heads,
                           int32_t head_dim, int32_t page, int64_t table_width, int64_t* floats,
                           int64_t* counters);

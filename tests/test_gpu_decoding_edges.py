@@ -154,3 +154,35 @@ def test_every_held_code_follows_a_grown_scale(D, T):
             assert torch.equal(got[:, :h], want[b, :, :h].float())
             assert torch.equal(got[:, h:h + T], new[b].transpose(0, 1).float() / s1)
             assert torch.equal(codes.view(torch.uint8)[pid[b], :, h + T:], was[pid[b], :, h + T:])
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("pages,width", [(3, 0), (0, 0), (0, 2)])
+def test_empty_tables_and_caches(pages, width):
+    """A block table of no columns and a cache of no pages hold no token: rows
+    see no key, nothing is written, and only a plan that names tokens is
+    reported."""
+    import voyager_b200
+    from voyager_b200 import _lib, kvcache
+
+    B, T, H, Hkv, D, page = 3, 2, 4, 2, 64, 32
+    cache = _cache(pages, Hkv, page, D, 1)
+    before = cache.k_codes.view(torch.uint8).clone()
+    bt = torch.zeros(B, width, dtype=torch.int32, device="cuda")
+    table = kvcache.rotary_table(width * page, D)
+    q = torch.ones(B, T, H, D, device="cuda").bfloat16()
+    k = torch.ones(B, T, Hkv, D, device="cuda").bfloat16()
+    zero = _i32([0] * B)
+    turned = kvcache.rope_append(q, k, k, table, cache, bt, zero, zero)
+    out = kvcache.attend(q, cache, bt, zero, zero)
+    assert turned.shape == out.shape == q.shape and not bool(turned.any()) and not bool(out.any())
+    voyager_b200.check_errors()
+    kvcache.rope_append(q, k, k, table, cache, bt, zero)
+    with pytest.raises(_lib.VqError, match="plan"):
+        voyager_b200.check_errors()
+    for counts in (None, _i32([0, T, 0]), _i32([0, -1, 0])):
+        out = kvcache.attend(q, cache, bt, zero, counts)
+        assert not bool(out.any())
+        with pytest.raises(_lib.VqError, match="plan"):
+            voyager_b200.check_errors()
+    assert torch.equal(cache.k_codes.view(torch.uint8), before)

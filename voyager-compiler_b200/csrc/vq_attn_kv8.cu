@@ -864,6 +864,21 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
   }
 }
 
+// A cache of no pages or a block table of no columns: no row sees a key.  The
+// output is 0 and the plan is checked as ever.
+__global__ void __launch_bounds__(THREADS) k_attn_none(const __grid_constant__ Args a, int64_t chunks) {
+  pdl::trigger();
+  pdl::wait();
+  const int64_t first = (int64_t)blockIdx.x * THREADS + threadIdx.x, step = (int64_t)gridDim.x * THREADS;
+  for (int64_t i = first; i < chunks; i += step) reinterpret_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0);
+  for (int64_t b = first; b < a.B; b += step) {
+    int err = 0;
+    const int2 plan = plan_of(a, (int)b, err);
+    if (!err && plan.y > 0) err = ERR_PAGE;  // tokens, but no page to hold them
+    if (err) note_err(nullptr, err);
+  }
+}
+
 // How a call's work is cut: row tiles of 8, row groups, and CTAs: as many as
 // fit at once, or one per unit where the longest lengths give fewer.
 struct Cut {
@@ -928,6 +943,21 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
       tokens >= (1 << 20) || batch > (1 << 24) || batch * tokens * heads >= (1ll << 31) || heads / kv_heads > (1 << 15))
     return VQ_ERR_INVALID;
   if (batch == 0 || tokens == 0) return VQ_OK;
+  Args a;
+  a.out = (uint16_t*)out;
+  a.lengths = (const int32_t*)lengths;
+  a.counts = (const int32_t*)counts;
+  a.B = (int)batch, a.T = (int)tokens, a.H = heads, a.Hkv = kv_heads, a.G = heads / kv_heads;
+  a.page_log2 = page == 32 ? 5 : page == 64 ? 6 : 7;
+  a.width = (int)table_width, a.pages = (int)pages;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (pages == 0 || table_width == 0) {  // nothing to read: their pointers may be null
+    if (!lengths || !out) return VQ_ERR_NULL;
+    if (reinterpret_cast<uintptr_t>(out) & 15) return VQ_ERR_ALIGNMENT;
+    const int64_t chunks = batch * tokens * heads * (head_dim / 8);
+    const int64_t ctas = std::min<int64_t>((chunks + THREADS - 1) / THREADS, 8 * vq::mx::sm_count());
+    return vq::pdl::launch<k_attn_none>((unsigned)ctas, THREADS, 0, st, 1, a, chunks) ? VQ_OK : VQ_ERR_CUDA;
+  }
   if (!q || !q_strides || !k_codes || !v_codes || !k_scale || !v_scale || !block_table || !lengths ||
       !counters || !out)
     return VQ_ERR_NULL;
@@ -942,33 +972,20 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
   if (pairs * ((table_width * page + UNIT - 1) / UNIT + 8) >= (1ll << 31) || counters_len < pairs)
     return VQ_ERR_INVALID;
   if (!workspace || workspace_floats < (int64_t)c.ctas * 2 * 8 * c.nt * (head_dim + 3)) return VQ_ERR_INVALID;
-  if (pages == 0 || table_width == 0) {  // an empty cache: no row sees a key
-    if (table_width) return VQ_ERR_INVALID;
-    return cudaMemsetAsync(out, 0, (size_t)(batch * tokens * heads * head_dim * 2),
-                           reinterpret_cast<cudaStream_t>(stream)) == cudaSuccess ? VQ_OK : VQ_ERR_CUDA;
-  }
   CUtensorMap mk, mv;
   const uint64_t rows = (uint64_t)pages * kv_heads * page;
   if (!vq::mx::make_map_box(&mk, k_codes, rows, head_dim, head_dim, TILE, head_dim) ||
       !vq::mx::make_map_box(&mv, v_codes, rows, head_dim, head_dim, TILE, head_dim))
     return VQ_ERR_CUDA;
-  Args a;
   a.q = (const uint16_t*)q;
   a.qb = q_strides[0], a.qt = q_strides[1], a.qh = q_strides[2];
-  a.out = (uint16_t*)out;
   a.k_scale = k_scale, a.v_scale = v_scale;
   a.block_table = (const int32_t*)block_table;
-  a.lengths = (const int32_t*)lengths;
-  a.counts = (const int32_t*)counts;
   a.part = workspace;
   a.done = counters;
-  a.B = (int)batch, a.T = (int)tokens, a.H = heads, a.Hkv = kv_heads, a.G = heads / kv_heads;
-  a.page_log2 = page == 32 ? 5 : page == 64 ? 6 : 7;
-  a.width = (int)table_width, a.pages = (int)pages;
   a.groups = c.groups;
   a.by_g = (uint32_t)(((1ll << 31) + a.G - 1) / a.G);
   a.sm_log2 = sm_scale * 1.4426950408889634f;
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (head_dim == 128)
     return c.nt == 1 ? launch<128, 1>(mk, mv, a, c.ctas, st) : launch<128, 2>(mk, mv, a, c.ctas, st);
   return c.nt == 1   ? launch<64, 1>(mk, mv, a, c.ctas, st)

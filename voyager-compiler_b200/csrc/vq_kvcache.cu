@@ -580,9 +580,10 @@ extern "C" int vq_rope_append_kv8(const void* q, const void* k, const void* v, c
       tokens > (1 << 24) || table_width > (1 << 24) || pages * kv_heads * page >= (1ll << 31))
     return VQ_ERR_INVALID;
   if (batch == 0 || tokens == 0) return VQ_OK;
-  if (!q || !k || !v || !strides || !table || !block_table || !lengths || !q_out || !k_codes ||
-      !v_codes || !k_scale || !v_scale)
-    return VQ_ERR_NULL;
+  if (!q || !k || !v || !strides || !lengths || !q_out) return VQ_ERR_NULL;
+  // a table of no columns and a cache of no pages are not read: may be null
+  if (table_width && (!table || !block_table)) return VQ_ERR_NULL;
+  if (pages && (!k_codes || !v_codes || !k_scale || !v_scale)) return VQ_ERR_NULL;
   if (positions < table_width * page) return VQ_ERR_SHAPE;  // every position the plan can name
   const int eb = dtype == VQ_BF16 ? 2 : 4;
   const void* p16[6] = {q, k, v, q_out, k_codes, v_codes};
