@@ -186,3 +186,17 @@ def test_empty_tables_and_caches(pages, width):
         with pytest.raises(_lib.VqError, match="plan"):
             voyager_b200.check_errors()
     assert torch.equal(cache.k_codes.view(torch.uint8), before)
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("C", [120, 136, 392, 1032, 129, 131, 250])
+def test_norm_of_a_row_whose_squares_vanish(C):
+    """With eps = 0 and squares below float32's range the row's factor is
+    infinite: y and the scales are infinities in every block, the last and
+    shorter one too, and the codes NaN."""
+    from voyager_b200 import fp8block
+
+    x = torch.full((2, C), 1e-30, device="cuda")
+    codes, scale, _ = fp8block.rmsnorm_quantize(x, torch.ones(C, device="cuda"), 0.0)
+    assert bool((scale == math.inf).all()), scale
+    assert bool(codes.float().isnan().all())

@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_vec(const Args a) {
       float top = 0.0f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) top = max_abs(top, h[i][k]);
-      uint32_t m = mag(top);
+      uint32_t m = c < a.cols ? mag(top) : 0;  // past the row 0, whatever f is
 #pragma unroll
       for (int d = 8; d; d >>= 1) m = max(m, __shfl_xor_sync(FULL, m, d));
       if (c < a.cols) {
