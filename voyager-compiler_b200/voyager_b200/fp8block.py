@@ -34,7 +34,7 @@ def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
 
 def quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """x [.., K] -> (codes, scale): ``scale = max|x| / 448`` per 128 columns (1
-    where that is 0), ``codes = E4M3(x / scale)``."""
+    where that is 0 in float32), ``codes = E4M3(x / scale)``."""
     return native.norm_quantize(x, None, None, 0.0, "quantize")[:2]
 
 
@@ -47,8 +47,8 @@ def quantize_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     N, K = w.shape
     f = torch.nn.functional.pad(w.float(), (0, -K % BLOCK, 0, -N % BLOCK))
     f = f.view(f.shape[0] // BLOCK, BLOCK, f.shape[1] // BLOCK, BLOCK)
-    amax = f.abs().amax((1, 3))
-    scale = torch.where(amax == 0, torch.ones_like(amax), amax / QMAX)
+    scale = f.abs().amax((1, 3)) / QMAX
+    scale = torch.where(scale == 0, 1.0, scale)
     codes = (f / scale[:, None, :, None]).clamp(-QMAX, QMAX).to(E4M3)
     return codes.view(codes.shape[0] * BLOCK, -1)[:N, :K].contiguous(), scale
 
