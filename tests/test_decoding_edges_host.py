@@ -21,3 +21,11 @@ def test_quantize_weight_of_a_block_whose_scale_underflows():
     assert scale[0, 1] == 2.0 ** -149 and f[3, 130] == 448  # 2^9 saturates
     assert scale[1, 2] == 1 / 448 and f[129, 259] == -448
     assert scale[0, 2] == 1 and scale[1, 0] == 1 and scale[1, 1] == 1
+
+
+def test_a_norm_needs_its_weight():
+    """Without a weight there is no norm to compute: None is refused, not taken
+    as `quantize`."""
+    for residual in (None, torch.ones(2, 128)):
+        with pytest.raises(TypeError, match="weight"):
+            fp8block.rmsnorm_quantize(torch.ones(2, 128), None, 1e-5, residual)

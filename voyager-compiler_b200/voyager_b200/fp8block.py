@@ -29,6 +29,8 @@ def rmsnorm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5,
     float32 [.., ceil(K / 128)], hidden = h in x's type (None without a
     residual).  x bfloat16 or float32 [.., K], any K; the norm is that of the
     unrounded sum."""
+    if weight is None:  # to the binding: no norm
+        raise TypeError("rmsnorm_quantize: weight must be a tensor")
     return native.norm_quantize(x, residual, weight, eps, "rmsnorm_quantize")
 
 
