@@ -200,3 +200,50 @@ def test_norm_of_a_row_whose_squares_vanish(C):
     codes, scale, _ = fp8block.rmsnorm_quantize(x, torch.ones(C, device="cuda"), 0.0)
     assert bool((scale == math.inf).all()), scale
     assert bool(codes.float().isnan().all())
+
+
+# ---------------------------------------------------------------------------
+def test_a_gradient_is_not_lost_in_silence():
+    """The operators have no derivative: asked for one, the backward pass says
+    so.  The values are those without gradients."""
+    from voyager_b200 import fp8block, kvcache
+
+    def raises(y):
+        assert y.requires_grad
+        with pytest.raises(RuntimeError, match="not implemented"):
+            y.float().sum().backward()
+
+    x = torch.randn(4, 256, generator=_gen(1), device="cuda")
+    w = torch.ones(256, device="cuda")
+    plain = fp8block.rmsnorm_quantize(x, w, residual=x)
+    assert not any(t.requires_grad for t in plain)
+    for args in ((x.clone().requires_grad_(), w, x), (x, w.clone().requires_grad_(), x),
+                 (x, w, x.clone().requires_grad_())):
+        got = fp8block.rmsnorm_quantize(args[0], args[1], residual=args[2])
+        for a, b in zip(got, plain):
+            assert torch.equal(a.detach().float(), b.float())
+            raises(a)
+        with torch.no_grad():
+            assert not any(t.requires_grad for t in fp8block.rmsnorm_quantize(args[0], args[1], residual=args[2]))
+    raises(fp8block.quantize(x.clone().requires_grad_())[1])
+    c, s = fp8block.quantize(x)
+    wc, ws = fp8block.quantize_weight(torch.randn(96, 256, generator=_gen(2), device="cuda"))
+    bias = torch.zeros(96, device="cuda").bfloat16()
+    want = fp8block.linear(c, s, wc, ws, bias)
+    for i in (1, 3, 4):
+        args = [c, s, wc, ws, bias]
+        args[i] = args[i].clone().requires_grad_()
+        got = fp8block.linear(*args)
+        assert torch.equal(got.detach(), want)
+        raises(got)
+    qkv = [torch.randn(1, 3, h, 64, generator=_gen(3), device="cuda").bfloat16() for h in (4, 2, 2)]
+    table, bt, held = kvcache.rotary_table(64, 64), _i32([[0, 1]]), _i32([0])
+    for i in range(3):
+        cache = kvcache.KVCache.empty(2, 2, 64, 32)
+        args = list(qkv)
+        args[i] = args[i].clone().requires_grad_()
+        q = kvcache.rope_append(*args, table, cache, bt, held)
+        raises(q)
+        raises(kvcache.attend(kvcache.rope_append(*args, table, cache, bt, held), cache, bt, held))
+    with torch.inference_mode():
+        assert not kvcache.attend(qkv[0], cache, bt, held).requires_grad

@@ -14,6 +14,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -51,6 +53,20 @@ void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_
 // An output on t's device, past the dispatcher (which takes 0.4 us a tensor).
 Tensor output(at::IntArrayRef sizes, at::ScalarType type, const Tensor& t) {
   return Tensor(at::detail::empty_cuda(sizes, type, t.device(), std::nullopt));
+}
+
+// The operators have no derivative.  Where one of `in` wants a gradient, a
+// backward pass that reaches one of `out` raises instead of ending there.
+void no_derivative(const char* what, std::initializer_list<const Tensor*> in, std::initializer_list<Tensor*> out) {
+  if (!at::GradMode::is_enabled()) return;
+  torch::autograd::edge_list edges;
+  for (const Tensor* t : in)
+    if (t->defined() && t->requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(*t));
+  if (edges.empty()) return;
+  const std::shared_ptr<torch::autograd::Node> fn(new torch::autograd::NotImplemented(what, std::move(edges)),
+                                                  torch::autograd::deleteNode);
+  for (Tensor* t : out)
+    if (t->defined()) torch::autograd::set_history(*t, fn);
 }
 
 // Makes the tensor's device current where it is not.
@@ -110,6 +126,7 @@ PyObject* norm_quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
                                       (float)eps, codes.data_ptr(), scale.data_ptr<float>(), ptr(hidden),
                                       stream_of(x));
   if (failed(st, what)) return nullptr;
+  no_derivative(what, {&x, &residual, &weight}, {&codes, &scale, &hidden});
   PyObject* out = PyTuple_New(3);
   if (!out) return nullptr;
   PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(codes)));
@@ -163,6 +180,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int st = vq_linear_fp8_block(c.data_ptr(), s.data_ptr<float>(), w.data_ptr(), ws.data_ptr<float>(),
                                      ptr(bias), c.numel() / K, N, K, out.data_ptr(), N, stream_of(c));
   if (failed(st, what)) return nullptr;
+  no_derivative(what, {&c, &s, &w, &ws, &bias}, {&out});
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
@@ -261,6 +279,7 @@ PyObject* rope_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
       ptr(plan.counts), c.pages, (int)c.page, out.data_ptr(), c.kc.data_ptr(), c.vc.data_ptr(),
       c.ks.data_ptr<float>(), c.vs.data_ptr<float>(), stream_of(q));
   if (failed(st, what)) return nullptr;
+  no_derivative(what, {&q, &k, &v, &table}, {&out});
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
@@ -314,6 +333,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
                              part.data_ptr<float>(), floats, done.data_ptr<int>(), done.numel(), out.data_ptr(),
                              stream_of(q));
   if (failed(st, what)) return nullptr;
+  no_derivative(what, {&q, &c.kc, &c.vc, &c.ks, &c.vs}, {&out});
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }

@@ -2,7 +2,8 @@
 
 Activations [.., K] carry one scale per 128 columns of a row, weights [N, K]
 one per 128 x 128 block.  These are the operands of a decoding step beside the
-MXFP8 ones of ``quantize_mx``; codes are ``torch.float8_e4m3fn`` tensors.
+MXFP8 ones of ``quantize_mx``; codes are ``torch.float8_e4m3fn`` tensors.  They
+serve inference: a backward pass that reaches their outputs raises.
 
   rmsnorm_quantize  (x + residual) -> RMSNorm -> codes, scales (and x + residual)
   quantize          x -> codes, scales

@@ -13,7 +13,8 @@ t) and writes the new keys and values; ``attend`` then takes the same plan.
 The plan stays on the device and is not read by the host: one that does not
 fit (a count outside 0..T, tokens past the block table, a page outside the
 cache) leaves the tokens concerned out and is reported by
-``voyager_b200.check_errors()``.
+``voyager_b200.check_errors()``.  There is no derivative: a backward pass that
+reaches an output raises.
 
   rotary_table  cos / sin of every position, with the scalings for long contexts
   rope_append   rotary positions + append
