@@ -247,3 +247,42 @@ def test_a_gradient_is_not_lost_in_silence():
         raises(kvcache.attend(kvcache.rope_append(*args, table, cache, bt, held), cache, bt, held))
     with torch.inference_mode():
         assert not kvcache.attend(qkv[0], cache, bt, held).requires_grad
+
+
+# ---------------------------------------------------------------------------
+def test_calls_on_the_per_thread_default_stream():
+    """One handle names a stream of its own in each thread: calls that overlap
+    there do not share their joins.  Each thread allocates from a pool of its
+    own, as the allocator too knows streams by their handles."""
+    import threading
+
+    from voyager_b200 import kvcache
+
+    cache = _cache(500, 1, 64, 128, 2)
+    bt = torch.randperm(500, generator=_gen(1), device="cuda").view(1, 500).int()
+    qs = [torch.randn(1, 1, 8, 128, generator=_gen(i), device="cuda").bfloat16() for i in range(3)]
+    held = _i32([31000])
+    want = [kvcache.attend(q, cache, bt, held) for q in qs]
+    torch.cuda.synchronize()
+    pools, got, errors = [torch.cuda.MemPool() for _ in qs], [[] for _ in qs], []
+
+    def work(i):
+        try:
+            side = torch.cuda.ExternalStream(2)  # cudaStreamPerThread
+            with torch.cuda.use_mem_pool(pools[i]), torch.cuda.stream(side):
+                torch.cuda._sleep(10_000_000)
+                for _ in range(30):
+                    got[i].append(kvcache.attend(qs[i], cache, bt, held))
+                side.synchronize()
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(qs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    for w, outs in zip(want, got):
+        assert len(outs) == 30 and all(torch.equal(o, w) for o in outs)

@@ -286,11 +286,15 @@ PyObject* rope_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // Zeroed counters for a call on the current stream; each call leaves them
 // zero, and calls on one stream do not overlap, so they share them.  A
-// captured call gets its own, which live and die with its graph.  The map is
-// never destroyed: the tensors outlive the CUDA context's end at exit.
+// captured call gets its own, which live and die with its graph; so does a call
+// on the per-thread default stream, whose one handle names a stream of its own
+// in every thread.  The map is never destroyed: the tensors outlive the CUDA
+// context's end at exit.
 Tensor join_counters(const Tensor& q, int64_t n) {
   const auto opt = q.options().dtype(at::kInt);
-  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return at::zeros({n}, opt);
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None ||
+      stream_of(q) == cudaStreamPerThread)
+    return at::zeros({n}, opt);
   static std::mutex m;
   static auto* kept = new std::map<std::pair<int, void*>, Tensor>();
   std::lock_guard<std::mutex> lock(m);
