@@ -29,3 +29,52 @@ def test_a_norm_needs_its_weight():
     for residual in (None, torch.ones(2, 128)):
         with pytest.raises(TypeError, match="weight"):
             fp8block.rmsnorm_quantize(torch.ones(2, 128), None, 1e-5, residual)
+
+
+def test_the_binding_is_built_again_for_another_torch_or_python(tmp_path, monkeypatch):
+    """_decode.so is up to date only for the torch, the Python and the command
+    that it was built with; a build that fails leaves no record."""
+    import os
+    import subprocess
+
+    import torch as real
+    from voyager_b200 import build
+
+    runs = []
+
+    def run(cmd, **kw):
+        runs.append(cmd)
+        if fails:
+            return subprocess.CompletedProcess(cmd, 1, "", "no")
+        open(cmd[cmd.index("-o") + 1], "w").close()
+        return subprocess.CompletedProcess(cmd, 0, "", "")
+
+    fails = False
+    monkeypatch.setattr(build, "PY_OUT", str(tmp_path / "_decode.so"))
+    monkeypatch.setattr(build, "BUILD", str(tmp_path))
+    monkeypatch.setattr(build.subprocess, "run", run)
+
+    def builds():
+        n = len(runs)
+        build._build_binding(False)
+        return len(runs) - n
+
+    assert builds() == 1 and builds() == 0
+    monkeypatch.setattr(real, "__version__", "9.9.9")
+    assert builds() == 1 and builds() == 0
+    monkeypatch.setattr(build.sysconfig, "get_config_var", lambda name: "cpython-399-" + name)
+    assert builds() == 1 and builds() == 0
+    monkeypatch.setattr(real, "compiled_with_cxx11_abi", lambda: False)
+    assert builds() == 1 and builds() == 0
+    assert "-D_GLIBCXX_USE_CXX11_ABI=0" in runs[-1]
+    os.utime(build.PY_OUT, (1, 1))  # older than its source
+    assert builds() == 1 and builds() == 0
+    fails = True
+    monkeypatch.setattr(real, "__version__", "9.9.10")
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="g\\+\\+ failed"):
+            build._build_binding(False)
+    fails = False
+    assert builds() == 1 and builds() == 0
+    os.remove(build.PY_OUT)
+    assert builds() == 1

@@ -11,7 +11,6 @@ binding of the cached-decoding operators (g++, torch's headers and libraries).
 """
 
 import concurrent.futures as cf
-import importlib.util
 import os
 import shutil
 import subprocess
@@ -74,24 +73,34 @@ def _compile(src: str, verbose: bool, extra) -> str:
 
 
 def _build_binding(verbose: bool) -> None:
-    """``_decode.so``, linked with the library beside it and with torch's."""
-    if (os.path.exists(PY_OUT) and os.path.getmtime(PY_OUT) >= os.path.getmtime(PY_SRC)
-            and os.path.getmtime(PY_OUT) >= os.path.getmtime(os.path.join(INCLUDE, "voyager_b200.h"))):
-        return
-    torch = os.path.dirname(importlib.util.find_spec("torch").origin)
+    """``_decode.so``, linked with the library beside it and with torch's.  It
+    holds torch's inline code and Python's ABI, so it is built again when the
+    record of what it was built with (``_build/_decode.stamp``) differs."""
+    import torch
+
+    root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
-    inc = [INCLUDE, os.path.join(torch, "include"), os.path.join(torch, "include/torch/csrc/api/include"),
+    inc = [os.path.join(root, "include"), os.path.join(root, "include/torch/csrc/api/include"),
            os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *[f"-I{inc[0]}"],
-           *[a for i in inc[1:] for a in ("-isystem", i)], "-D_GLIBCXX_USE_CXX11_ABI=1", PY_SRC, "-o", PY_OUT + ".tmp",
-           f"-L{PKG}", "-l:" + os.path.basename(OUT), f"-L{os.path.join(torch, 'lib')}", "-lc10", "-lc10_cuda",
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-I{INCLUDE}", *[a for i in inc for a in ("-isystem", i)],
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", PY_SRC, "-o", PY_OUT + ".tmp",
+           f"-L{PKG}", "-l:" + os.path.basename(OUT), f"-L{os.path.join(root, 'lib')}", "-lc10", "-lc10_cuda",
            "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    stamp = os.path.join(BUILD, "_decode.stamp")
+    made_with = "\n".join([torch.__version__, str(sysconfig.get_config_var("SOABI")), " ".join(cmd)])
+    newest = max(os.path.getmtime(f) for f in (PY_SRC, os.path.join(INCLUDE, "voyager_b200.h")))
+    if os.path.exists(PY_OUT) and os.path.getmtime(PY_OUT) >= newest and os.path.exists(stamp):
+        with open(stamp) as f:
+            if f.read() == made_with:
+                return
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {PY_SRC}:\n{r.stdout}\n{r.stderr}")
     os.replace(PY_OUT + ".tmp", PY_OUT)
+    with open(stamp, "w") as f:
+        f.write(made_with)
 
 
 def build(verbose: bool = False, extra=()) -> str:
