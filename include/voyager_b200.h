@@ -750,7 +750,8 @@ int vq_rope_append_kv8(const void* q, const void* k, const void* v, const int64_
  * Slots past a sequence's last token may hold anything.  Plans that do not fit
  * and waits that give up set the device's sticky word (311-314); the keys of a
  * page outside the cache are left out.  With pages or table_width 0 no row sees
- * a key; the inputs but lengths and counts may then be NULL. */
+ * a key; the inputs but lengths and counts may then be NULL.  table_width * page
+ * at most 2^31 - 2^14. */
 int vq_attn_kv8_workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_heads,
                           int32_t head_dim, int32_t page, int64_t table_width, int64_t* floats,
                           int64_t* counters);

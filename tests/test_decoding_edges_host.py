@@ -78,3 +78,29 @@ def test_the_binding_is_built_again_for_another_torch_or_python(tmp_path, monkey
     assert builds() == 1 and builds() == 0
     os.remove(build.PY_OUT)
     assert builds() == 1
+
+
+@pytest.mark.parametrize("page", [32, 64, 128])
+def test_attention_refuses_tables_whose_keys_leave_31_bits(page):
+    """Keys are counted in 31 bits, up to 2^14 past a table's end (the block
+    table is read two batches of tiles ahead): a longer table is refused before
+    any launch."""
+    import ctypes
+
+    from voyager_b200 import _lib
+
+    lib = _lib.load()
+    P = 0x1000  # never dereferenced
+
+    def go(width):
+        floats, counters = ctypes.c_int64(), ctypes.c_int64()
+        st = lib.vq_attn_kv8_workspace(1, 1, 1, 1, 128, page, width, ctypes.byref(floats), ctypes.byref(counters))
+        assert st in (0, 1)
+        floats.value, counters.value = 1 << 40, 1 << 40
+        strides = (ctypes.c_int64 * 3)(128, 128, 128)
+        return lib.vq_attn_kv8(P, strides, 1, 1, 1, 1, 128, P, P, P, P, 1, page, P, width, P, None, 1.0, P, floats.value,
+                               P, counters.value, P, None)
+
+    top = (1 << 31) // page
+    for width in (top, top - 1, top - (1 << 14) // page + 1, 1 << 62):
+        assert go(width) == 1, width

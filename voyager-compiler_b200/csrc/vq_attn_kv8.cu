@@ -879,6 +879,10 @@ __global__ void __launch_bounds__(THREADS) k_attn_none(const __grid_constant__ A
   }
 }
 
+// The longest block table: its keys, and the 2^14 beyond them that the batches
+// read ahead may name before they are brought back to the last, fit 31 bits.
+constexpr int64_t max_width(int32_t page) { return ((1ll << 31) - (1 << 14)) / page; }
+
 // How a call's work is cut: row tiles of 8, row groups, and CTAs: as many as
 // fit at once, or one per unit where the longest lengths give fewer.
 struct Cut {
@@ -921,7 +925,7 @@ int vq_attn_kv8_workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t 
                           int64_t* counters) {
   if (!floats || !counters) return VQ_ERR_NULL;
   if (batch < 0 || tokens < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0 ||
-      page <= 0 || table_width < 0)
+      page <= 0 || table_width < 0 || table_width > max_width(page))
     return VQ_ERR_INVALID;
   const Cut c = cut_of(std::max<int64_t>(batch, 1), std::max<int64_t>(tokens, 1), heads, kv_heads,
                        head_dim, table_width * page);
@@ -939,7 +943,7 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
   if (head_dim != 64 && head_dim != 128) return VQ_ERR_UNSUPPORTED;
   if (page != 32 && page != 64 && page != 128) return VQ_ERR_UNSUPPORTED;
   if (batch < 0 || tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || table_width < 0 ||
-      pages < 0 || pages * kv_heads * page >= (1ll << 31) || table_width * page >= (1ll << 31) ||
+      pages < 0 || pages * kv_heads * page >= (1ll << 31) || table_width > max_width(page) ||
       tokens >= (1 << 20) || batch > (1 << 24) || batch * tokens * heads >= (1ll << 31) || heads / kv_heads > (1 << 15))
     return VQ_ERR_INVALID;
   if (batch == 0 || tokens == 0) return VQ_OK;
