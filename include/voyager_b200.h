@@ -680,7 +680,7 @@ int vq_codebook_lookup(const vq_tensor* input, const int64_t* counts, int32_t nc
 
 /* y = rms_norm(x + residual) * weight in float32 (mean of squares over the
  * row, + eps), quantized per 128 columns: scale = max|y| / 448 (1 where the
- * maximum is 0), code = E4M3(y / scale), nearest even, saturating.
+ * quotient is 0), code = E4M3(y / scale), nearest even, saturating.
  *   x         VQ_BF16 or VQ_F32 [rows, cols], rows ldx elements apart
  *   residual  the same type, rows ldr apart, or NULL
  *   weight    the same type [cols], or NULL: no norm, y = x (+ residual)
@@ -695,7 +695,8 @@ int vq_norm_quantize_fp8(const void* x, int64_t ldx, const void* residual, int64
 /* out[m, n] = bf16(bias[n] + sum_kb x_scale[m, kb] * w_scale[n / 128, kb] *
  *             sum_{k in kb} x[m, k] w[n, k]), kb the blocks of 128 along K.
  *   x [M, K], w [N, K] E4M3 bytes, 16-byte aligned, K a multiple of 16
- *   x_scale float32 [M, nkb], w_scale float32 [ceil(N / 128), nkb], nkb = ceil(K / 128)
+ *   x_scale float32 [M, nkb], w_scale float32 [ceil(N / 128), nkb], nkb = ceil(K / 128);
+ *   their product is formed in float32 first, so it has to lie in its normal range
  *   bias bf16 [N] or NULL; out bf16, rows ldo >= N elements apart
  * Any M and N.  Waits are bounded; one that gives up sets the device's sticky
  * word (vq_device_errors, 321-324). */

@@ -4,8 +4,9 @@
 //   out[m, n] = bf16( bias[n] + sum_kb sa[m, kb] * sw[n / 128, kb]
 //                     * sum_{k in block kb} a[m, k] * w[n, k] )
 //
-// The scales are any float32 values, so they cannot ride in the MMA: each
-// 128-column block of K is one tensor-core product (exact products, float32
+// The scales are float32 values of any mantissa, so they cannot ride in the MMA
+// (their product sa * sw is formed first, in float32: below 2^-126 it loses
+// bits, beyond the range it is an infinity): each 128-column block of K is one tensor-core product (exact products, float32
 // sums) into its own TMEM buffer, and the promotion warps read it back
 // (tcgen05.ld) and add it, times its scale, to float32 sums in registers.
 // The MMAs of the next blocks run meanwhile: one multiply-add per output and

@@ -60,5 +60,7 @@ def linear(codes: torch.Tensor, scale: torch.Tensor, w_codes: torch.Tensor, w_sc
            bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``[.., K] x [N, K]^T (+ bias) -> [.., N]`` bfloat16 of the values that the
     codes and their block scales stand for: exact products, float32 sums, one
-    rounding.  K a multiple of 16; any N and number of rows."""
+    rounding.  The product of an activation's and a weight's scale is formed in
+    float32 (normal from 2^-126 to 2^128).  K a multiple of 16; any N and number
+    of rows."""
     return native.linear(codes, scale, w_codes, w_scale, bias)
