@@ -286,3 +286,26 @@ def test_calls_on_the_per_thread_default_stream():
     assert not errors, errors
     for w, outs in zip(want, got):
         assert len(outs) == 30 and all(torch.equal(o, w) for o in outs)
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("C", [12288, 16384])
+def test_norm_many_wide_rows(C, dtype):
+    """More rows than CTAs where a row takes a CTA's whole width."""
+    from test_gpu_fp8block import _check_norm
+
+    g = _gen(C)
+    x, r = (torch.randn(700, C, generator=g, device="cuda").to(dtype) for _ in range(2))
+    w = (1 + 0.2 * torch.randn(C, generator=g, device="cuda")).to(dtype)
+    _check_norm(x, w)
+    _check_norm(x, w, residual=r)
+    _check_norm(x, None)
+
+
+@pytest.mark.parametrize("D,Hkv,G", [(128, 2, 4), (64, 1, 5)])
+def test_attend_prompts(D, Hkv, G):
+    """Prompts of hundreds of tokens, on an empty and on a held cache."""
+    from test_gpu_kvcache import _check_attend
+
+    _check_attend(2, 515, Hkv, G, D, 64, [0, 700], [515, 300], seed=D, stale=0x7F)
