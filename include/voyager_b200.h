@@ -738,6 +738,41 @@ int vq_rope_append_kv8(const void* q, const void* k, const void* v, const int64_
                        int32_t page, void* q_out, void* k_codes, void* v_codes, float* k_scale,
                        float* v_scale, void* stream);
 
+/* vq_rope_append_kv8 with an RMSNorm of the query and key heads before they
+ * turn: y = x * rsqrt(mean(x^2) + eps) * weight over head_dim, in float32.
+ * q_norm, k_norm [head_dim] in q's type, 16-byte aligned; NULL: no norm. */
+int vq_rope_append_kv8_norm(const void* q, const void* k, const void* v, const int64_t* strides,
+                            int32_t dtype, const float* table, int64_t positions, int32_t rot,
+                            int32_t interleaved, int64_t batch, int64_t tokens, int32_t heads,
+                            int32_t kv_heads, int32_t head_dim, const void* block_table,
+                            int64_t table_width, const void* lengths, const void* counts,
+                            int64_t pages, int32_t page, const void* q_norm, const void* k_norm,
+                            float eps, void* q_out, void* k_codes, void* v_codes, float* k_scale,
+                            float* v_scale, void* stream);
+
+/* The same into a cache held in 4 bits: k_codes, v_codes [pages, kv_heads,
+ * page, head_dim / 2], two E2M1 codes a byte, the even column in the low half;
+ * k_scale, v_scale E4M3 [pages, kv_heads, page, head_dim / 16]; k_factor,
+ * v_factor float32 [kv_heads], positive.  A value is code * scale * factor:
+ *   scale = E4M3(max|x| / (6 factor)) over 16 columns of a token, at least 2^-9,
+ *   code = E2M1(x / (scale * factor))
+ * both rounded to nearest even and saturating; a NaN makes its block's scale
+ * NaN.  A token's blocks are its own: what the cache holds is neither read nor
+ * changed, and sequences may append to the same page at different slots. */
+int vq_rope_append_kv4(const void* q, const void* k, const void* v, const int64_t* strides,
+                       int32_t dtype, const float* table, int64_t positions, int32_t rot,
+                       int32_t interleaved, int64_t batch, int64_t tokens, int32_t heads,
+                       int32_t kv_heads, int32_t head_dim, const void* block_table,
+                       int64_t table_width, const void* lengths, const void* counts, int64_t pages,
+                       int32_t page, const void* q_norm, const void* k_norm, float eps, void* q_out,
+                       void* k_codes, void* v_codes, void* k_scale, void* v_scale,
+                       const float* k_factor, const float* v_factor, void* stream);
+
+/* The codes of a 4-bit cache, `bytes` of each (a multiple of 16), as E4M3 codes
+ * of the same values, one a byte: k_out and v_out [2 * bytes]. */
+int vq_kv4_unpack(const void* k_codes, const void* v_codes, int64_t bytes, void* k_out, void* v_out,
+                  void* stream);
+
 /* Causal attention of the newest tokens over that cache, which already holds
  * their keys and values (lengths and counts as vq_rope_append_kv8 got them):
  *   out[b, t, h] = sum_j softmax_j(sm_scale q . k_j) v_j, j <= lengths[b] + t;
@@ -762,6 +797,18 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
                 int32_t page, const void* block_table, int64_t table_width, const void* lengths,
                 const void* counts, float sm_scale, float* workspace, int64_t workspace_floats,
                 int32_t* counters, int64_t counters_len, void* out, void* stream);
+
+/* vq_attn_kv8 over the 4-bit cache of vq_rope_append_kv4. */
+int vq_attn_kv4_workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_heads,
+                          int32_t head_dim, int32_t page, int64_t table_width, int64_t* floats,
+                          int64_t* counters);
+int vq_attn_kv4(const void* q, const int64_t* q_strides, int64_t batch, int64_t tokens,
+                int32_t heads, int32_t kv_heads, int32_t head_dim, const void* k_codes,
+                const void* v_codes, const void* k_scale, const void* v_scale, const float* k_factor,
+                const float* v_factor, int64_t pages, int32_t page, const void* block_table,
+                int64_t table_width, const void* lengths, const void* counts, float sm_scale,
+                float* workspace, int64_t workspace_floats, int32_t* counters, int64_t counters_len,
+                void* out, void* stream);
 
 /* dst [..., C, R] = src [..., R, C] transposed (2- or 4-byte elements). */
 int vq_transpose(const vq_tensor* src, vq_tensor* dst, void* stream);

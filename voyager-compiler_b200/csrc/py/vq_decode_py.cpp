@@ -185,27 +185,39 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// A cache in E4M3, or in 4 bits (codes uint8, two a byte; E4M3 scales; factors).
 struct Cache {
-  Tensor kc, vc, ks, vs;
+  Tensor kc, vc, ks, vs, kf, vf;
   int64_t pages, heads, page, dim;
-  // args: k_codes, v_codes, k_scale, v_scale
-  Cache(PyObject* const* a, const char* what)
+  bool four;
+  // a: k_codes, v_codes, k_scale, v_scale; f: k_factor, v_factor, or None of an E4M3 cache
+  Cache(PyObject* const* a, PyObject* const* f, const char* what)
       : kc(tensor(a[0], "k_codes")), vc(tensor(a[1], "v_codes")), ks(tensor(a[2], "k_scale")),
-        vs(tensor(a[3], "v_scale")) {
-    TORCH_CHECK_NOT_IMPLEMENTED(kc.scalar_type() == at::kFloat8_e4m3fn && vc.scalar_type() == at::kFloat8_e4m3fn &&
-                                    ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat,
-                                what, ": a cache is float8_e4m3fn codes and float32 scales");
-    TORCH_CHECK_VALUE(kc.dim() == 4 && vc.sizes() == kc.sizes() && ks.sizes() == kc.sizes().slice(0, 2) &&
-                          vs.sizes() == ks.sizes(),
+        vs(tensor(a[3], "v_scale")), kf(optional(f[0], "k_factor")), vf(optional(f[1], "v_factor")) {
+    four = kf.defined();
+    TORCH_CHECK_TYPE(vf.defined() == four, what, ": k_factor and v_factor go together");
+    const auto type = four ? at::kByte : at::kFloat8_e4m3fn, scales = four ? at::kFloat8_e4m3fn : at::kFloat;
+    TORCH_CHECK_NOT_IMPLEMENTED(kc.scalar_type() == type && vc.scalar_type() == type && ks.scalar_type() == scales &&
+                                    vs.scalar_type() == scales,
+                                what, four ? ": a 4-bit cache is uint8 codes and float8_e4m3fn scales"
+                                           : ": a cache is float8_e4m3fn codes and float32 scales");
+    TORCH_CHECK_VALUE(kc.dim() == 4 && vc.sizes() == kc.sizes() && vs.sizes() == ks.sizes() &&
+                          ks.dim() == (four ? 4 : 2) && ks.sizes().slice(0, four ? 3 : 2) == kc.sizes().slice(0, four ? 3 : 2) &&
+                          (!four || ks.size(3) * 8 == kc.size(3)),
                       what, ": cache codes ", kc.sizes(), ", ", vc.sizes(), " and scales ", ks.sizes(), ", ",
                       vs.sizes(), " are not one cache");
-    pages = kc.size(0), heads = kc.size(1), page = kc.size(2), dim = kc.size(3);
+    pages = kc.size(0), heads = kc.size(1), page = kc.size(2), dim = kc.size(3) * (four ? 2 : 1);
     TORCH_CHECK_NOT_IMPLEMENTED((page == 32 || page == 64 || page == 128) && (dim == 64 || dim == 128), what,
                                 ": page in (32, 64, 128) and head_dim in (64, 128), not ", page, " and ", dim);
     TORCH_CHECK_VALUE(kc.is_contiguous() && vc.is_contiguous() && ks.is_contiguous() && vs.is_contiguous(), what,
                       ": the cache's tensors must be contiguous");
     TORCH_CHECK_VALUE(vc.device() == kc.device() && ks.device() == kc.device() && vs.device() == kc.device(), what,
                       ": the cache's tensors are on different devices");
+    if (four)
+      for (const Tensor* t : {&kf, &vf})
+        TORCH_CHECK_VALUE(t->scalar_type() == at::kFloat && t->dim() == 1 && t->size(0) == heads &&
+                              t->is_contiguous() && t->device() == kc.device(),
+                          what, ": the factors must be contiguous float32 [", heads, "] on ", kc.device());
   }
 };
 
@@ -235,21 +247,33 @@ Tensor heads_of(const Tensor& t) {
   return t.clone(at::MemoryFormat::Contiguous);
 }
 
+// A norm's weight [dim] in x's type, 16-byte aligned.
+Tensor norm_weight(PyObject* o, const char* name, const char* what, const Tensor& x, int64_t dim) {
+  Tensor w = optional(o, name);
+  if (!w.defined()) return w;
+  TORCH_CHECK_VALUE(w.scalar_type() == x.scalar_type() && w.dim() == 1 && w.size(0) == dim && w.device() == x.device(),
+                    what, ": ", name, " must be ", x.scalar_type(), " [", dim, "] on ", x.device());
+  if (w.stride(0) == 1 && ((uintptr_t)w.data_ptr() & 15) == 0) return w;
+  return w.clone(at::MemoryFormat::Contiguous);
+}
+
 // q, k, v, table, k_codes, v_codes, k_scale, v_scale, block_table, lengths,
-// counts or None, interleaved -> q turned
+// counts or None, interleaved, k_factor, v_factor (or None: E4M3), q_norm or
+// None, k_norm or None, eps -> q turned
 PyObject* rope_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const char* what = "rope_append";
-  TORCH_CHECK_TYPE(n == 12, "rope_append takes 12 arguments");
+  TORCH_CHECK_TYPE(n == 17, "rope_append takes 17 arguments");
   Tensor q = tensor(args[0], "q"), k = tensor(args[1], "k"), v = tensor(args[2], "v");
   const Tensor table = tensor(args[3], "table");
   const int interleaved = PyObject_IsTrue(args[11]);
-  if (interleaved < 0) return nullptr;
+  const double eps = PyFloat_AsDouble(args[16]);
+  if (interleaved < 0 || PyErr_Occurred()) return nullptr;
   const int code = float_code(q.scalar_type());
   TORCH_CHECK_NOT_IMPLEMENTED(code >= 0 && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
                               what, ": q, k and v of one type, bfloat16 or float32");
   TORCH_CHECK_NOT_IMPLEMENTED(q.is_cuda(), what, ": the CUDA kernel needs CUDA tensors");
-  const Cache c(args + 4, what);
+  const Cache c(args + 4, args + 12, what);
   TORCH_CHECK_VALUE(q.dim() == 4 && q.size(3) == c.dim && k.dim() == 4 && k.size(0) == q.size(0) &&
                         k.size(1) == q.size(1) && k.size(2) == c.heads && k.size(3) == c.dim && v.sizes() == k.sizes(),
                     what, ": q ", q.sizes(), ", k ", k.sizes(), ", v ", v.sizes(), " do not match a cache of ",
@@ -269,17 +293,26 @@ PyObject* rope_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   TORCH_CHECK_VALUE(table.size(0) >= width * c.page, what, ": the table's ", table.size(0),
                     " positions do not cover the block table's ", width * c.page, " tokens");
   On on(q);
+  const Tensor qn = norm_weight(args[14], "q_norm", what, q, c.dim), kn = norm_weight(args[15], "k_norm", what, q, c.dim);
   q = heads_of(q), k = heads_of(k), v = heads_of(v);
   Tensor out = output({B, T, H, c.dim}, q.scalar_type(), q);
   const int64_t strides[9] = {q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1),
                               k.stride(2), v.stride(0), v.stride(1), v.stride(2)};
-  const int st = vq_rope_append_kv8(
-      q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, code, table.data_ptr<float>(), table.size(0), (int)rot,
-      interleaved, B, T, (int)H, (int)c.heads, (int)c.dim, plan.table.data_ptr(), width, plan.lengths.data_ptr(),
-      ptr(plan.counts), c.pages, (int)c.page, out.data_ptr(), c.kc.data_ptr(), c.vc.data_ptr(),
-      c.ks.data_ptr<float>(), c.vs.data_ptr<float>(), stream_of(q));
+  const int st =
+      c.four ? vq_rope_append_kv4(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, code, table.data_ptr<float>(),
+                                  table.size(0), (int)rot, interleaved, B, T, (int)H, (int)c.heads, (int)c.dim,
+                                  plan.table.data_ptr(), width, plan.lengths.data_ptr(), ptr(plan.counts), c.pages,
+                                  (int)c.page, ptr(qn), ptr(kn), (float)eps, out.data_ptr(), c.kc.data_ptr(),
+                                  c.vc.data_ptr(), c.ks.data_ptr(), c.vs.data_ptr(), c.kf.data_ptr<float>(),
+                                  c.vf.data_ptr<float>(), stream_of(q))
+             : vq_rope_append_kv8_norm(q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, code,
+                                       table.data_ptr<float>(), table.size(0), (int)rot, interleaved, B, T, (int)H,
+                                       (int)c.heads, (int)c.dim, plan.table.data_ptr(), width,
+                                       plan.lengths.data_ptr(), ptr(plan.counts), c.pages, (int)c.page, ptr(qn),
+                                       ptr(kn), (float)eps, out.data_ptr(), c.kc.data_ptr(), c.vc.data_ptr(),
+                                       c.ks.data_ptr<float>(), c.vs.data_ptr<float>(), stream_of(q));
   if (failed(st, what)) return nullptr;
-  no_derivative(what, {&q, &k, &v, &table}, {&out});
+  no_derivative(what, {&q, &k, &v, &table, &qn, &kn}, {&out});
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
@@ -304,15 +337,15 @@ Tensor join_counters(const Tensor& q, int64_t n) {
 }
 
 // q, k_codes, v_codes, k_scale, v_scale, block_table, lengths, counts or
-// None, scale or None -> out
+// None, scale or None, k_factor, v_factor (or None: E4M3) -> out
 PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const char* what = "attend";
-  TORCH_CHECK_TYPE(n == 9, "attend takes 9 arguments");
+  TORCH_CHECK_TYPE(n == 11, "attend takes 11 arguments");
   Tensor q = tensor(args[0], "q");
   TORCH_CHECK_NOT_IMPLEMENTED(q.scalar_type() == at::kBFloat16, what, ": q must be bfloat16, not ", q.scalar_type());
   TORCH_CHECK_NOT_IMPLEMENTED(q.is_cuda(), what, ": the CUDA kernel needs CUDA tensors");
-  const Cache c(args + 1, what);
+  const Cache c(args + 1, args + 9, what);
   TORCH_CHECK_VALUE(q.dim() == 4 && q.size(3) == c.dim && q.size(2) > 0 && c.heads > 0 && q.size(2) % c.heads == 0,
                     what, ": q ", q.sizes(), " does not match a cache of ", c.heads, " heads of ", c.dim);
   TORCH_CHECK_VALUE(q.device() == c.kc.device(), what, ": operands on different devices");
@@ -325,20 +358,50 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   q = heads_of(q);
   Tensor out = output({B, T, H, c.dim}, q.scalar_type(), q);
   int64_t floats = 0, counters = 0;
-  if (failed(vq_attn_kv8_workspace(B, T, (int)H, (int)c.heads, (int)c.dim, (int)c.page, width, &floats, &counters),
+  if (failed((c.four ? vq_attn_kv4_workspace : vq_attn_kv8_workspace)(B, T, (int)H, (int)c.heads, (int)c.dim,
+                                                                      (int)c.page, width, &floats, &counters),
              what))
     return nullptr;
   const Tensor done = join_counters(q, counters);
   const Tensor part = output({floats}, at::kFloat, q);
   const int64_t strides[3] = {q.stride(0), q.stride(1), q.stride(2)};
-  const int st = vq_attn_kv8(q.data_ptr(), strides, B, T, (int)H, (int)c.heads, (int)c.dim, c.kc.data_ptr(),
-                             c.vc.data_ptr(), c.ks.data_ptr<float>(), c.vs.data_ptr<float>(), c.pages, (int)c.page,
-                             plan.table.data_ptr(), width, plan.lengths.data_ptr(), ptr(plan.counts), (float)scale,
-                             part.data_ptr<float>(), floats, done.data_ptr<int>(), done.numel(), out.data_ptr(),
-                             stream_of(q));
+  const int st =
+      c.four ? vq_attn_kv4(q.data_ptr(), strides, B, T, (int)H, (int)c.heads, (int)c.dim, c.kc.data_ptr(),
+                           c.vc.data_ptr(), c.ks.data_ptr(), c.vs.data_ptr(), c.kf.data_ptr<float>(),
+                           c.vf.data_ptr<float>(), c.pages, (int)c.page, plan.table.data_ptr(), width,
+                           plan.lengths.data_ptr(), ptr(plan.counts), (float)scale, part.data_ptr<float>(), floats,
+                           done.data_ptr<int>(), done.numel(), out.data_ptr(), stream_of(q))
+             : vq_attn_kv8(q.data_ptr(), strides, B, T, (int)H, (int)c.heads, (int)c.dim, c.kc.data_ptr(),
+                           c.vc.data_ptr(), c.ks.data_ptr<float>(), c.vs.data_ptr<float>(), c.pages, (int)c.page,
+                           plan.table.data_ptr(), width, plan.lengths.data_ptr(), ptr(plan.counts), (float)scale,
+                           part.data_ptr<float>(), floats, done.data_ptr<int>(), done.numel(), out.data_ptr(),
+                           stream_of(q));
   if (failed(st, what)) return nullptr;
-  no_derivative(what, {&q, &c.kc, &c.vc, &c.ks, &c.vs}, {&out});
+  no_derivative(what, {&q, &c.kc, &c.vc, &c.ks, &c.vs, &c.kf, &c.vf}, {&out});
   return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// k_codes, v_codes, k_scale, v_scale, k_factor, v_factor -> (k, v) float8_e4m3fn
+PyObject* unpack(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const char* what = "unpack";
+  TORCH_CHECK_TYPE(n == 6, "unpack takes 6 arguments");
+  const Cache c(args, args + 4, what);
+  TORCH_CHECK_TYPE(c.four, what, " takes a 4-bit cache");
+  TORCH_CHECK_NOT_IMPLEMENTED(c.kc.is_cuda(), what, ": the CUDA kernel needs CUDA tensors");
+  On on(c.kc);
+  Tensor k = output({c.pages, c.heads, c.page, c.dim}, at::kFloat8_e4m3fn, c.kc);
+  Tensor v = output({c.pages, c.heads, c.page, c.dim}, at::kFloat8_e4m3fn, c.kc);
+  if (failed(vq_kv4_unpack(c.kc.data_ptr(), c.vc.data_ptr(), c.kc.numel(), k.data_ptr(), v.data_ptr(),
+                           stream_of(c.kc)),
+             what))
+    return nullptr;
+  PyObject* out = PyTuple_New(2);
+  if (!out) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(k)));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(v)));
+  return out;
   END_HANDLE_TH_ERRORS
 }
 
@@ -353,6 +416,7 @@ PyMethodDef kMethods[] = {
     {"norm_quantize", (PyCFunction)(void (*)(void))norm_quantize, METH_FASTCALL, nullptr},
     {"linear", (PyCFunction)(void (*)(void))linear, METH_FASTCALL, nullptr},
     {"rope_append", (PyCFunction)(void (*)(void))rope_append, METH_FASTCALL, nullptr},
+    {"unpack", (PyCFunction)(void (*)(void))unpack, METH_FASTCALL, nullptr},
     {"attend", (PyCFunction)(void (*)(void))attend, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_decode", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -41,6 +41,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "voyager_b200.h"
 #include "vq_e4m3.cuh"
@@ -64,7 +65,8 @@ struct Args {
   const uint16_t* q;  // bf16, strides in elements
   int64_t qb, qt, qh;
   uint16_t* out;  // bf16 [B, T, H, D]
-  const float *k_scale, *v_scale;
+  const float *k_scale, *v_scale;  // per page and head; in 4 bits per head: the factors
+  const uint8_t *k_bscale, *v_bscale;  // in 4 bits: E4M3 [pages, Hkv, page, D / 16]
   const int32_t *block_table, *lengths, *counts;
   float* part;        // [CTAs][2][ROWS * (D + 3)]: pieces of heads that were cut
   int32_t* done;      // [B * groups * Hkv] zero before, zero after
@@ -78,18 +80,24 @@ struct Args {
 // keys: 130 us against 149 with two, in deeper rings than now); otherwise the third CTA costs more in
 // joins and shallower rings than its warps give (heads of 128, 32 sequences:
 // 66 us against 55).
-constexpr int ctas_per_sm(int head_dim, int nt) { return head_dim == 64 && nt == 1 ? 3 : 2; }
+constexpr int ctas_per_sm(int head_dim, int nt, bool fp4) {
+  return (head_dim == 64 || fp4) && nt == 1 ? 3 : 2;
+}
 
-template <int D, int NT>
+template <int D, int NT, bool FP4>
 struct Cfg {
   static constexpr int ROWS = 8 * NT;
-  static constexpr int TILE_BYTES = TILE * D;
+  // a stage holds codes of K, codes of V; in 4 bits then their scales
+  static constexpr int TILE_BYTES = FP4 ? TILE * D / 2 : TILE * D, SCALE_BYTES = FP4 ? TILE * D / 16 : 0;
+  static constexpr int STAGE = 2 * (TILE_BYTES + SCALE_BYTES);
+  static constexpr int STRIDE = (STAGE + 511) / 512 * 512;  // the swizzle's period
   // Two stages a warp: 128 KB in flight an SM (96 KB at heads of 64) fill HBM, and
   // more only lengthens the queue that every other access waits in (4 sequences
   // of 131000 keys: 168 us, with three 178; heads of 64, 24 sequences of 28631:
   // 118, with four 126).
-  static constexpr int PER_SM = ctas_per_sm(D, NT), STAGES = D == 128 || PER_SM == 3 ? 2 : 3;
-  static constexpr int RING = STAGES * 2 * TILE_BYTES;  // per warp
+  static constexpr int PER_SM = ctas_per_sm(D, NT, FP4);
+  static constexpr int STAGES = FP4 ? (D == 128 ? 3 : 4) : D == 128 || PER_SM == 3 ? 2 : 3;
+  static constexpr int RING = STAGES * STRIDE;  // per warp
   static constexpr int SMEM_RING = WARPS * RING;
   // the warps' O meet in SUMS buffers, rows LD floats apart
   static constexpr int SUMS = NT == 1 ? 2 : 1, LD = D + 4;
@@ -136,6 +144,44 @@ __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
 }
 // Bits 0x80 of it: the word's bytes that are an E4M3 NaN (0x7F or 0xFF).
 __device__ __forceinline__ uint32_t nan_bits(uint32_t w) { return (w & 0x7F7F7F7Fu) + 0x01010101u; }
+
+// Four bytes of two E2M1 codes each as f16 pairs (exact), the low halves first.
+__device__ __forceinline__ void e2m1_f16(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+}
+// A code times a scale: 2 by 4 significant bits within 2^-10 .. 2688, exact in f16.
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+  uint16_t v;
+  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds8(uint32_t a) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
+}
+// In 4 bits: the key, of each 8, that index i of the products stands for.  The
+// keys 2t of lanes t, and those of two neighbouring g, then lie in different
+// banks.
+__device__ __forceinline__ int key4(int i) { return (i & 12) | (0x9C >> ((i & 3) * 2) & 3); }
+// Byte offset of 16-byte chunk c of row r of a 4-bit tile: SWIZZLE_64B at 64 bytes a row, plain at 32.
+template <int D>
+__device__ __forceinline__ uint32_t swz4(int r, int c) {
+  return D == 128 ? (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4)) : (uint32_t)(r * 32 + (c << 4));
+}
 
 // Byte offset of 16-byte chunk c of row r in a TMA-swizzled tile of D-byte rows.
 template <int D>
@@ -184,11 +230,11 @@ __device__ __forceinline__ Entry entry_of(const Args& a, int e, const int2* plan
 }
 __device__ __forceinline__ int units_of(const Entry& x) { return (x.end + UNIT - 1) / UNIT; }
 
-template <int D, int NT>
-__global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
-    k_attn_kv8(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+template <int D, int NT, bool FP4>
+__global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
+    k_attn_kv(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                const __grid_constant__ Args a) {
-  using C = Cfg<D, NT>;
+  using C = Cfg<D, NT, FP4>;
   constexpr int KS = D / 16;   // k steps of the scores, and m tiles of the output
   constexpr int PART = C::ROWS * (D + 3);  // O, then m, l and w of each row
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -328,17 +374,25 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
       if (outside) note_err(nullptr, ERR_PAGE);
       const int blk = (outside ? 0 : pid_next) * a.Hkv + sg.kvh;
       n_row = (blk << a.page_log2) + (key_of(issued + lane) & ((1 << a.page_log2) - 1) & ~(TILE - 1));
-      n_ks = a.k_scale[blk];
-      n_v = a.v_scale[blk];
+      if constexpr (FP4) {
+        n_v = 1.0f;
+      } else {
+        n_ks = a.k_scale[blk];
+        n_v = a.v_scale[blk];
+      }
       n_v = outside ? -1.0f : n_v >= 0.0f ? n_v : -NEG_INF;  // no logarithm: the output is NaN
       pid_next = pid_of(issued + lane + 32);
     }
     const int y = __shfl_sync(FULL, n_row, issued & 31);
     if (lane == 0) {
-      const uint32_t bar = bar0 + 8 * wstage, dst = ring + wstage * 2 * C::TILE_BYTES;
-      mbar_expect_tx(bar, 2 * C::TILE_BYTES);
+      const uint32_t bar = bar0 + 8 * wstage, dst = ring + wstage * C::STRIDE;
+      mbar_expect_tx(bar, C::STAGE);
       tma_load_2d(dst, &map_k, 0, y, bar);
       tma_load_2d(dst + C::TILE_BYTES, &map_v, 0, y, bar);
+      if constexpr (FP4) {
+        bulk_load(dst + 2 * C::TILE_BYTES, a.k_bscale + (int64_t)y * (D / 16), C::SCALE_BYTES, bar);
+        bulk_load(dst + 2 * C::TILE_BYTES + C::SCALE_BYTES, a.v_bscale + (int64_t)y * (D / 16), C::SCALE_BYTES, bar);
+      }
     }
     ++issued;
     if (++wstage == C::STAGES) wstage = 0;
@@ -407,6 +461,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
   float* sl = sm + WARPS * C::ROWS;
   float* sw = sl + WARPS * C::ROWS;
   float* fin = sw + WARPS * C::ROWS;                            // [ROWS] m, l, w, the output's factor
+  const float factor = FP4 ? __ldg(a.v_scale + cur.kvh) : 1.0f;
   __syncthreads();  // the last join's readers are done
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -416,6 +471,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
       l += __shfl_xor_sync(FULL, l, 4);
       l += __shfl_xor_sync(FULL, l, 8);
       l += __shfl_xor_sync(FULL, l, 16);
+      if (FP4) l *= 1.0f / 32768.0f;  // sums of weights, which are 2^15 times the probabilities
       if (g == 0) {
         const int r = warp * C::ROWS + n * 8 + 2 * t + c;
         sm[r] = mx[n][c], sl[r] = l, sw[r] = wx[n][c];
@@ -434,7 +490,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
     for (int k = 0; k < WARPS; ++k)
       l = fmaf(sl[k * C::ROWS + threadIdx.x], ex2(sm[k * C::ROWS + threadIdx.x] - ref), l);
     fin[threadIdx.x] = m, fin[C::ROWS + threadIdx.x] = l, fin[2 * C::ROWS + threadIdx.x] = w;
-    fin[3 * C::ROWS + threadIdx.x] = (int)threadIdx.x < cur.nrows ? out_scale(m, l, w) : 0.0f;
+    fin[3 * C::ROWS + threadIdx.x] = (int)threadIdx.x < cur.nrows ? out_scale(m, l, w) * factor : 0.0f;
   }
   // every warp's O relative to the CTA's w, added in the warps' order.  Column
   // d = D/8 g + 2j + i of a row lies at place 16 j + 2 g + i of it: the lanes of
@@ -593,7 +649,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
       }
     }
     if (sub == 0) {
-      const float f = out_scale(m, l, w);
+      const float f = out_scale(m, l, w) * factor;
       // places 4 gl .. and D/2 + 4 gl ..: columns D/8 g2 + 2j of g2 = 2 gl % 8
       // and the next, j = gl / 4 and D/32 more
 #pragma unroll
@@ -667,7 +723,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      cs[n][c] = __shfl_sync(FULL, qs[n], (2 * t + c) * 4) * a.sm_log2;
+      cs[n][c] = __shfl_sync(FULL, qs[n], (2 * t + c) * 4) * (FP4 ? a.sm_log2 * __ldg(a.k_scale + sg.kvh) : a.sm_log2);
       lim[n][c] = held + row_of(sg, n * 8 + 2 * t + c).x;
     }
   const int free_end = held + sg.tok0 + 1;  // keys below: every row sees them
@@ -689,11 +745,13 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
   for (; i < mine; ++i, advance()) {
     const int key0 = k0 + (warp + i * WARPS) * TILE;
     if ((i & 31) == 0) c_ks = n_ks, c_lv = log2f(n_v);
-    const float ks = __shfl_sync(FULL, c_ks, i & 31), lv = __shfl_sync(FULL, c_lv, i & 31);
+    const float ks = FP4 ? 1.0f : __shfl_sync(FULL, c_ks, i & 31), lv = __shfl_sync(FULL, c_lv, i & 31);
     ok = mbar_wait_warp(bar0 + 8 * stage, phase, nullptr, ERR_WAIT);
     if (!ok) break;
     if (lv != lv) continue;  // a page outside the cache
-    const uint32_t kb = ring + stage * 2 * C::TILE_BYTES, vb = kb + C::TILE_BYTES;
+    const uint32_t kb = ring + stage * C::STRIDE, vb = kb + C::TILE_BYTES;
+    // the key that index r of the products stands for
+    auto place = [](int r) { return FP4 ? key4(r) : r; };
     const bool tail = key0 + TILE > free_end;
 
     // scores: two m tiles of 16 keys
@@ -702,21 +760,52 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
     for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) s[n][mt][0] = s[n][mt][1] = s[n][mt][2] = s[n][mt][3] = 0.0f;
-      uint32_t ka[D / 16], kc[D / 16];  // rows g and g + 8 of the tile, D / 4 columns
-      const int r = mt * 16 + g;
+      const int r = mt * 16 + place(g);
+      if constexpr (FP4) {
+        // rows r and r + 8 of the tile, D / 4 columns, in D / 64 blocks of 16
+        const uint32_t sb = vb + C::TILE_BYTES;
+        uint32_t x[D / 32], y[D / 32], sx[D / 64], sy[D / 64];
+        if constexpr (D == 128) {
+          const uint4 p = lds128(kb + swz4<D>(r, t)), q = lds128(kb + swz4<D>(r + 8, t));
+          x[0] = p.x, x[1] = p.y, x[D / 32 - 2] = p.z, x[D / 32 - 1] = p.w;
+          y[0] = q.x, y[1] = q.y, y[D / 32 - 2] = q.z, y[D / 32 - 1] = q.w;
+          const uint32_t u = unpack2(lds16(sb + r * 8 + 2 * t)), w = unpack2(lds16(sb + (r + 8) * 8 + 2 * t));
+          sx[0] = __byte_perm(u, u, 0x1010), sx[D / 64 - 1] = __byte_perm(u, u, 0x3232);
+          sy[0] = __byte_perm(w, w, 0x1010), sy[D / 64 - 1] = __byte_perm(w, w, 0x3232);
+        } else {
+          const uint2 p = lds64(kb + swz4<D>(r, 0) + 8 * t), q = lds64(kb + swz4<D>(r + 8, 0) + 8 * t);
+          x[0] = p.x, x[1] = p.y, y[0] = q.x, y[1] = q.y;
+          sx[0] = unpack2(lds8(sb + r * 4 + t) * 0x0101u), sy[0] = unpack2(lds8(sb + (r + 8) * 4 + t) * 0x0101u);
+        }
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        const uint4 x = lds128(kb + swz<D>(r, t * (D / 64) + c));
-        const uint4 y = lds128(kb + swz<D>(r + 8, t * (D / 64) + c));
-        ka[4 * c] = x.x, ka[4 * c + 1] = x.y, ka[4 * c + 2] = x.z, ka[4 * c + 3] = x.w;
-        kc[4 * c] = y.x, kc[4 * c + 1] = y.y, kc[4 * c + 2] = y.z, kc[4 * c + 3] = y.w;
-      }
+        for (int w = 0; w < D / 32; ++w) {
+          uint32_t hx[4], hy[4];
+          e2m1_f16(x[w], hx);
+          e2m1_f16(y[w], hy);
 #pragma unroll
-      for (int w = 0; w < KS; ++w) {
-        const uint32_t a0 = unpack2(ka[w]), a2 = unpack2_hi(ka[w]);
-        const uint32_t a1 = unpack2(kc[w]), a3 = unpack2_hi(kc[w]);
+          for (int j = 0; j < 4; ++j) hx[j] = mul_f16x2(hx[j], sx[w >> 1]), hy[j] = mul_f16x2(hy[j], sy[w >> 1]);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma(s[n][mt], a0, a1, a2, a3, qf[n][w][0], qf[n][w][1]);
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              mma(s[n][mt], hx[2 * j], hy[2 * j], hx[2 * j + 1], hy[2 * j + 1], qf[n][2 * w + j][0], qf[n][2 * w + j][1]);
+        }
+      } else {
+        uint32_t ka[D / 16], kc[D / 16];  // rows g and g + 8 of the tile, D / 4 columns
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          const uint4 x = lds128(kb + swz<D>(r, t * (D / 64) + c));
+          const uint4 y = lds128(kb + swz<D>(r + 8, t * (D / 64) + c));
+          ka[4 * c] = x.x, ka[4 * c + 1] = x.y, ka[4 * c + 2] = x.z, ka[4 * c + 3] = x.w;
+          kc[4 * c] = y.x, kc[4 * c + 1] = y.y, kc[4 * c + 2] = y.z, kc[4 * c + 3] = y.w;
+        }
+#pragma unroll
+        for (int w = 0; w < KS; ++w) {
+          const uint32_t a0 = unpack2(ka[w]), a2 = unpack2_hi(ka[w]);
+          const uint32_t a1 = unpack2(kc[w]), a3 = unpack2_hi(kc[w]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma(s[n][mt], a0, a1, a2, a3, qf[n][w][0], qf[n][w][1]);
+        }
       }
     }
 
@@ -732,7 +821,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
         s[n][mt][0] *= f0, s[n][mt][2] *= f0;
         s[n][mt][1] *= f1, s[n][mt][3] *= f1;
         if (tail) {
-          const int key = key0 + mt * 16 + g;
+          const int key = key0 + mt * 16 + place(g);
           if (key > lim[n][0]) s[n][mt][0] = NEG_INF;
           if (key > lim[n][1]) s[n][mt][1] = NEG_INF;
           if (key + 8 > lim[n][0]) s[n][mt][2] = NEG_INF;
@@ -754,10 +843,16 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
         grew |= w != wx[n][c];
         mx[n][c] = m;
         wx[n][c] = w;
-        const float pref = wref - lv - P_EXP;
+        const float pref = FP4 ? ref - P_EXP : wref - lv - P_EXP;
         float add = 0.0f;
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
+          if constexpr (FP4) {  // one page's values weigh as another's: the weights are their own sum's terms
+            s[n][mt][c] = ex2(s[n][mt][c] - pref);
+            s[n][mt][c + 2] = ex2(s[n][mt][c + 2] - pref);
+            add += s[n][mt][c] + s[n][mt][c + 2];
+            continue;
+          }
           add += ex2(s[n][mt][c] - ref) + ex2(s[n][mt][c + 2] - ref);
           s[n][mt][c] = ex2(s[n][mt][c] - pref);
           s[n][mt][c + 2] = ex2(s[n][mt][c + 2] - pref);
@@ -782,6 +877,87 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT))
 
     // output: lane (g, t) holds columns D/8 * g .. of keys 2t, 2t+1, 2t+8, 2t+9
     // of each half tile
+    if constexpr (FP4) {
+      constexpr int VW = D / 64;  // words of D / 8 columns
+      const uint32_t sb = vb + C::TILE_BYTES + C::SCALE_BYTES;
+      // the pairs of keys (2t, 2t+1) and (2t+8, 2t+9): words whose bytes are one
+      // column's two codes, even columns and odd, and the two scales
+      uint32_t ev[2][2][VW], od[2][2][VW], sp[2][2];
+      uint32_t odd = 0;
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int r0 = mt * 16 + p * 8 + key4(2 * t), r1 = mt * 16 + p * 8 + key4(2 * t + 1);
+          uint32_t x[VW], y[VW], e0, e1;
+          if constexpr (D == 128) {
+            const uint2 u = lds64(vb + swz4<D>(r0, g >> 1) + (g & 1) * 8), w = lds64(vb + swz4<D>(r1, g >> 1) + (g & 1) * 8);
+            x[0] = u.x, x[VW - 1] = u.y, y[0] = w.x, y[VW - 1] = w.y;
+            e0 = lds8(sb + r0 * 8 + g), e1 = lds8(sb + r1 * 8 + g);
+          } else {
+            x[0] = lds32(vb + swz4<D>(r0, 0) + 4 * g), y[0] = lds32(vb + swz4<D>(r1, 0) + 4 * g);
+            e0 = lds8(sb + r0 * 4 + (g >> 1)), e1 = lds8(sb + r1 * 4 + (g >> 1));
+          }
+          if (tail) {
+            if (key0 + r0 >= end) e0 = 0;  // slots that hold no token of this sequence
+            if (key0 + r1 >= end) e1 = 0;
+            odd |= nan_bits(e0) | nan_bits(e1);
+          }
+          sp[mt][p] = unpack2(e0 | e1 << 8);
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            ev[mt][p][w] = (x[w] & 0x0F0F0F0Fu) | (y[w] << 4 & 0xF0F0F0F0u);
+            od[mt][p][w] = (x[w] >> 4 & 0x0F0F0F0Fu) | (y[w] & 0xF0F0F0F0u);
+          }
+        }
+      auto product = [&](int n, int mt, int w, const uint32_t (&sc)[2], float (&acc)[4][4]) {
+        uint32_t a0[4], a1[4], a2[4], a3[4];
+        e2m1_f16(ev[mt][0][w], a0), e2m1_f16(od[mt][0][w], a1), e2m1_f16(ev[mt][1][w], a2), e2m1_f16(od[mt][1][w], a3);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          mma(acc[j], mul_f16x2(a0[j], sc[0]), mul_f16x2(a1[j], sc[0]), mul_f16x2(a2[j], sc[1]), mul_f16x2(a3[j], sc[1]),
+              pf[n][mt][0], pf[n][mt][1]);
+      };
+      if (tail) odd = __any_sync(FULL, (odd & 0x80u) != 0);
+      if (!odd) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int w = 0; w < VW; ++w)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              product(n, mt, w, sp[mt], *reinterpret_cast<float(*)[4][4]>(&o[n][4 * w]));
+      } else {  // as below: each row with the values it does not see taken as 0
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll 1
+          for (int r = 0; r < 8; ++r) {
+            const int last = held + row_of(sg, n * 8 + r).x;
+            const bool c0 = r == 2 * t, c1 = r == 2 * t + 1;
+            uint32_t sc[2][2];
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int p = 0; p < 2; ++p) {
+                const int at = key0 + mt * 16 + p * 8;
+                sc[mt][p] = (at + key4(2 * t) > last ? 0u : sp[mt][p] & 0xFFFFu) |
+                            (at + key4(2 * t + 1) > last ? 0u : sp[mt][p] & 0xFFFF0000u);
+              }
+#pragma unroll
+            for (int w = 0; w < VW; ++w) {
+              float acc[4][4] = {};
+#pragma unroll
+              for (int mt = 0; mt < 2; ++mt) product(n, mt, w, sc[mt], acc);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if (c0) o[n][4 * w + j][0] += acc[j][0], o[n][4 * w + j][2] += acc[j][2];
+                if (c1) o[n][4 * w + j][1] += acc[j][1], o[n][4 * w + j][3] += acc[j][3];
+              }
+            }
+          }
+      }
+      continue;
+    }
     constexpr int VW = D / 32;  // words of D / 8 columns
     uint32_t v[2][4][VW];
 #pragma unroll
@@ -888,7 +1064,7 @@ constexpr int64_t max_width(int32_t page) { return ((1ll << 31) - (1 << 14)) / p
 struct Cut {
   int nt, groups, ctas;
 };
-Cut cut_of(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim, int64_t capacity) {
+Cut cut_of(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim, int64_t capacity, bool fp4) {
   Cut c;
   // Row tiles per group: two.  Three, which fit the registers at heads of 64,
   // where the tiles come out even (96 rows: 120 us against 129, 24 rows 48
@@ -898,17 +1074,17 @@ Cut cut_of(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim,
   c.groups = (int)((tiles + most - 1) / most);
   c.nt = (int)((tiles + c.groups - 1) / c.groups);
   const int64_t units = std::max<int64_t>(1, (capacity + UNIT - 1) / UNIT);
-  c.ctas = (int)std::min<int64_t>(ctas_per_sm(head_dim, c.nt) * vq::mx::sm_count(), batch * c.groups * kv_heads * units);
+  c.ctas = (int)std::min<int64_t>(ctas_per_sm(head_dim, c.nt, fp4) * vq::mx::sm_count(), batch * c.groups * kv_heads * units);
   return c;
 }
 
-template <int D, int NT>
+template <int D, int NT, bool FP4>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int ctas, cudaStream_t st) {
-  using C = Cfg<D, NT>;
+  using C = Cfg<D, NT, FP4>;
   static_assert(WARPS * C::STAGES * 8 <= 256, "barrier area");
-  if (!allow_smem<k_attn_kv8<D, NT>>(C::SMEM))
+  if (!allow_smem<k_attn_kv<D, NT, FP4>>(C::SMEM))
     return VQ_ERR_CUDA;
-  return pdl::launch<k_attn_kv8<D, NT>>(ctas, THREADS, C::SMEM, st, 1, mk, mv, a) ? VQ_OK : VQ_ERR_CUDA;
+  return pdl::launch<k_attn_kv<D, NT, FP4>>(ctas, THREADS, C::SMEM, st, 1, mk, mv, a) ? VQ_OK : VQ_ERR_CUDA;
 }
 
 int sticky_kva(int* out, int clear, cudaStream_t st) { return vq::tc::sticky_read(out, clear, st); }
@@ -918,28 +1094,27 @@ int sticky_kva(int* out, int clear, cudaStream_t st) { return vq::tc::sticky_rea
 
 using namespace vq::kva;
 
-extern "C" {
-
-int vq_attn_kv8_workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_heads,
-                          int32_t head_dim, int32_t page, int64_t table_width, int64_t* floats,
-                          int64_t* counters) {
+static int workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t page,
+                     int64_t table_width, int64_t* floats, int64_t* counters, bool fp4) {
   if (!floats || !counters) return VQ_ERR_NULL;
   if (batch < 0 || tokens < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0 ||
       page <= 0 || table_width < 0 || table_width > max_width(page))
     return VQ_ERR_INVALID;
   const Cut c = cut_of(std::max<int64_t>(batch, 1), std::max<int64_t>(tokens, 1), heads, kv_heads,
-                       head_dim, table_width * page);
+                       head_dim, table_width * page, fp4);
   *counters = batch * kv_heads * c.groups;
   *floats = (int64_t)c.ctas * 2 * 8 * c.nt * (head_dim + 3);
   return VQ_OK;
 }
 
-int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t tokens, int32_t heads,
-                int32_t kv_heads, int32_t head_dim, const void* k_codes, const void* v_codes,
-                const float* k_scale, const float* v_scale, int64_t pages, int32_t page,
-                const void* block_table, int64_t table_width, const void* lengths, const void* counts,
-                float sm_scale, float* workspace, int64_t workspace_floats, int32_t* counters,
-                int64_t counters_len, void* out, void* stream) {
+// In E4M3 k_scale and v_scale are float32 per page and head; in 4 bits the
+// bytes of a block each, and k_factor and v_factor float32 per head.
+static int attention(const void* q, const int64_t* q_strides, int64_t batch, int64_t tokens, int32_t heads,
+                     int32_t kv_heads, int32_t head_dim, const void* k_codes, const void* v_codes,
+                     const void* k_scale, const void* v_scale, const float* k_factor, const float* v_factor,
+                     int64_t pages, int32_t page, const void* block_table, int64_t table_width, const void* lengths,
+                     const void* counts, float sm_scale, float* workspace, int64_t workspace_floats,
+                     int32_t* counters, int64_t counters_len, void* out, void* stream, bool fp4) {
   if (head_dim != 64 && head_dim != 128) return VQ_ERR_UNSUPPORTED;
   if (page != 32 && page != 64 && page != 128) return VQ_ERR_UNSUPPORTED;
   if (batch < 0 || tokens < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || table_width < 0 ||
@@ -963,14 +1138,14 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
     return vq::pdl::launch<k_attn_none>((unsigned)ctas, THREADS, 0, st, 1, a, chunks) ? VQ_OK : VQ_ERR_CUDA;
   }
   if (!q || !q_strides || !k_codes || !v_codes || !k_scale || !v_scale || !block_table || !lengths ||
-      !counters || !out)
+      !counters || !out || (fp4 && (!k_factor || !v_factor)))
     return VQ_ERR_NULL;
-  const void* p16[5] = {q, k_codes, v_codes, out, workspace};
+  const void* p16[7] = {q, k_codes, v_codes, out, workspace, fp4 ? k_scale : nullptr, fp4 ? v_scale : nullptr};
   for (const void* p : p16)
     if (reinterpret_cast<uintptr_t>(p) & 15) return VQ_ERR_ALIGNMENT;
   for (int i = 0; i < 3; ++i)
     if (q_strides[i] % 8) return VQ_ERR_ALIGNMENT;
-  const Cut c = cut_of(batch, tokens, heads, kv_heads, head_dim, table_width * page);
+  const Cut c = cut_of(batch, tokens, heads, kv_heads, head_dim, table_width * page, fp4);
   const int64_t pairs = batch * kv_heads * c.groups;
   // the units of all heads, counted in 32 bits
   if (pairs * ((table_width * page + UNIT - 1) / UNIT + 8) >= (1ll << 31) || counters_len < pairs)
@@ -978,23 +1153,66 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
   if (!workspace || workspace_floats < (int64_t)c.ctas * 2 * 8 * c.nt * (head_dim + 3)) return VQ_ERR_INVALID;
   CUtensorMap mk, mv;
   const uint64_t rows = (uint64_t)pages * kv_heads * page;
-  if (!vq::mx::make_map_box(&mk, k_codes, rows, head_dim, head_dim, TILE, head_dim) ||
-      !vq::mx::make_map_box(&mv, v_codes, rows, head_dim, head_dim, TILE, head_dim))
-    return VQ_ERR_CUDA;
+  const uint32_t bytes = fp4 ? head_dim / 2 : head_dim;
+  auto map = [&](CUtensorMap* m, const void* p) {
+    return bytes == 32 ? vq::mx::make_map_plain(m, p, rows, bytes, bytes, TILE)
+                       : vq::mx::make_map_box(m, p, rows, bytes, bytes, TILE, bytes);
+  };
+  if (!map(&mk, k_codes) || !map(&mv, v_codes)) return VQ_ERR_CUDA;
   a.q = (const uint16_t*)q;
   a.qb = q_strides[0], a.qt = q_strides[1], a.qh = q_strides[2];
-  a.k_scale = k_scale, a.v_scale = v_scale;
+  a.k_scale = fp4 ? k_factor : (const float*)k_scale, a.v_scale = fp4 ? v_factor : (const float*)v_scale;
+  a.k_bscale = fp4 ? (const uint8_t*)k_scale : nullptr, a.v_bscale = fp4 ? (const uint8_t*)v_scale : nullptr;
   a.block_table = (const int32_t*)block_table;
   a.part = workspace;
   a.done = counters;
   a.groups = c.groups;
   a.by_g = (uint32_t)(((1ll << 31) + a.G - 1) / a.G);
   a.sm_log2 = sm_scale * 1.4426950408889634f;
-  if (head_dim == 128)
-    return c.nt == 1 ? launch<128, 1>(mk, mv, a, c.ctas, st) : launch<128, 2>(mk, mv, a, c.ctas, st);
-  return c.nt == 1   ? launch<64, 1>(mk, mv, a, c.ctas, st)
-         : c.nt == 2 ? launch<64, 2>(mk, mv, a, c.ctas, st)
-                     : launch<64, 3>(mk, mv, a, c.ctas, st);
+  auto run = [&](auto four) {
+    constexpr bool F = decltype(four)::value;
+    if (head_dim == 128)
+      return c.nt == 1 ? launch<128, 1, F>(mk, mv, a, c.ctas, st) : launch<128, 2, F>(mk, mv, a, c.ctas, st);
+    return c.nt == 1   ? launch<64, 1, F>(mk, mv, a, c.ctas, st)
+           : c.nt == 2 ? launch<64, 2, F>(mk, mv, a, c.ctas, st)
+                       : launch<64, 3, F>(mk, mv, a, c.ctas, st);
+  };
+  return fp4 ? run(std::true_type()) : run(std::false_type());
+}
+
+extern "C" {
+
+int vq_attn_kv8_workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_heads,
+                          int32_t head_dim, int32_t page, int64_t table_width, int64_t* floats,
+                          int64_t* counters) {
+  return workspace(batch, tokens, heads, kv_heads, head_dim, page, table_width, floats, counters, false);
+}
+int vq_attn_kv4_workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_heads,
+                          int32_t head_dim, int32_t page, int64_t table_width, int64_t* floats,
+                          int64_t* counters) {
+  return workspace(batch, tokens, heads, kv_heads, head_dim, page, table_width, floats, counters, true);
+}
+
+int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t tokens, int32_t heads,
+                int32_t kv_heads, int32_t head_dim, const void* k_codes, const void* v_codes,
+                const float* k_scale, const float* v_scale, int64_t pages, int32_t page,
+                const void* block_table, int64_t table_width, const void* lengths, const void* counts,
+                float sm_scale, float* workspace, int64_t workspace_floats, int32_t* counters,
+                int64_t counters_len, void* out, void* stream) {
+  return attention(q, q_strides, batch, tokens, heads, kv_heads, head_dim, k_codes, v_codes, k_scale, v_scale, nullptr,
+                   nullptr, pages, page, block_table, table_width, lengths, counts, sm_scale, workspace,
+                   workspace_floats, counters, counters_len, out, stream, false);
+}
+
+int vq_attn_kv4(const void* q, const int64_t* q_strides, int64_t batch, int64_t tokens, int32_t heads,
+                int32_t kv_heads, int32_t head_dim, const void* k_codes, const void* v_codes,
+                const void* k_scale, const void* v_scale, const float* k_factor, const float* v_factor,
+                int64_t pages, int32_t page, const void* block_table, int64_t table_width, const void* lengths,
+                const void* counts, float sm_scale, float* workspace, int64_t workspace_floats,
+                int32_t* counters, int64_t counters_len, void* out, void* stream) {
+  return attention(q, q_strides, batch, tokens, heads, kv_heads, head_dim, k_codes, v_codes, k_scale, v_scale,
+                   k_factor, v_factor, pages, page, block_table, table_width, lengths, counts, sm_scale, workspace,
+                   workspace_floats, counters, counters_len, out, stream, true);
 }
 
 }  // extern "C"

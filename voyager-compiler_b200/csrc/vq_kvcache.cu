@@ -55,6 +55,11 @@ struct Args {
   int B, T, H, Hkv, rot, page, width, pages, interleaved;
   int q_blocks, W;  // CTAs of the q part; pages that T tokens can touch
   int hq, hc;       // heads per thread of the q part, per CTA of the cache part
+  const void *q_norm, *k_norm;  // [D] in q's type, or null: that part has no norm
+  float eps;
+  // the 4-bit cache: E4M3 bytes [pages, Hkv, page, D / 16], and a factor for each head
+  uint8_t *k_bscale, *v_bscale;
+  const float *k_factor, *v_factor;
 };
 
 // One thread's 16 columns of a head as 8 pairs: unit u of D / 16 is pairs
@@ -103,6 +108,24 @@ __device__ __forceinline__ void turn(float (&x0)[8], float (&x1)[8], const float
       x1[i] = a * s[i] + b * c[i];
     }
   }
+}
+
+// A head's RMSNorm: its U lanes, side by side in a warp, hold 16 columns each.
+template <typename T, int U>
+__device__ __forceinline__ void head_norm(float (&x0)[8], float (&x1)[8], const void* weight, int c0, int c1,
+                                          float eps) {
+  float w0[8], w1[8];
+  T::load8(reinterpret_cast<const typename T::type*>(weight) + c0, w0);
+  T::load8(reinterpret_cast<const typename T::type*>(weight) + c1, w1);
+  float s = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s = fmaf(x0[j], x0[j], fmaf(x1[j], x1[j], s));
+  const uint32_t lanes = ((1u << U) - 1) << (threadIdx.x & 31 & ~(U - 1));
+#pragma unroll
+  for (int d = U / 2; d; d >>= 1) s += __shfl_xor_sync(lanes, s, d);
+  const float f = rsqrtf(fmaf(s, 1.0f / (16 * U), eps));
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x0[j] = x0[j] * f * w0[j], x1[j] = x1[j] * f * w1[j];
 }
 
 // New tokens of sequence b that fit the plan, and the tokens it holds.
@@ -173,7 +196,7 @@ __device__ __forceinline__ QUnit q_unit(const Args& a, int64_t i) {
   unit_cols<IL>(x.u, a.rot, x.c0, x.c1);
   return x;
 }
-template <typename T, bool IL, int D>
+template <typename T, bool IL, int D, bool NORM>
 __device__ __forceinline__ void turn_q(const Args& a, int64_t i) {
   using E = typename T::type;
   const QUnit x = q_unit<IL, D>(a, i);
@@ -193,6 +216,7 @@ __device__ __forceinline__ void turn_q(const Args& a, int64_t i) {
 #pragma unroll
   for (int q = 0; q < QH; ++q)
     if (x.h0 + q < x.h1) {
+      if (NORM && a.q_norm) head_norm<T, D / 16>(x0[q], x1[q], a.q_norm, x.c0, x.c1, a.eps);
       if (turns) turn<IL>(x0[q], x1[q], c, s);
       if (!live) {
 #pragma unroll
@@ -242,7 +266,7 @@ struct Ring {
 
 // The q part alone, beside k_rope_append.
 constexpr int Q_THREADS = 256;
-template <typename T, bool IL, int D>
+template <typename T, bool IL, int D, bool NORM>
 __global__ void __launch_bounds__(Q_THREADS) k_turn_q(const __grid_constant__ Args a) {
   using E = typename T::type;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -280,6 +304,7 @@ __global__ void __launch_bounds__(Q_THREADS) k_turn_q(const __grid_constant__ Ar
       float x0[8], x1[8];
       ring.read(k, 2 * q, x0);
       ring.read(k, 2 * q + 1, x1);
+      if (NORM && a.q_norm) head_norm<T, D / 16>(x0, x1, a.q_norm, x.c0, x.c1, a.eps);
       if (turns) turn<IL>(x0, x1, c, s);
       if (!live) {
 #pragma unroll
@@ -357,7 +382,7 @@ __device__ __forceinline__ void rescale16(uint4* p, float f) {
 // while the next two blocks' loads are in flight.  768 threads an SM: 8 prompts
 // of 2048 tokens, 32 heads of 128, q included: 132 us (5.1 TB/s); with 512, 140,
 // with 1024 and spilled registers 162.
-template <typename T, bool IL, int D, int TH>
+template <typename T, bool IL, int D, int TH, bool NORM>
 __global__ void __launch_bounds__(TH, TH > 512 ? 1 : 768 / TH) k_rope_append(const __grid_constant__ Args a) {
   using E = typename T::type;
   constexpr int U = D / 16, ROWS = TH / U, IT = 2;  // threads per token, tokens per pass, passes
@@ -416,6 +441,7 @@ __global__ void __launch_bounds__(TH, TH > 512 ? 1 : 768 / TH) k_rope_append(con
 #pragma unroll
     for (int it = 0; it < IT; ++it)
       if (it * ROWS + r0 < k.tokens) {
+        if (NORM && !is_v && a.k_norm) head_norm<T, U>(x0[it], x1[it], a.k_norm, c0, c1, a.eps);
         if (turns) {
           float c[8], s[8];
           load_angles(a.table + (k.pos + it * ROWS + r0) * (a.rot >> 1), u, a.rot, c, s);
@@ -449,14 +475,14 @@ __global__ void __launch_bounds__(TH, TH > 512 ? 1 : 768 / TH) k_rope_append(con
 // by latency (plan, block table, the block's scale): one token 2.3 us, 64
 // sequences 2.6, of which the bytes take 0.2.
 constexpr int FEW_THREADS = 128;
-template <typename T, bool IL, int D, int G>
+template <typename T, bool IL, int D, int G, bool NORM>
 __global__ void __launch_bounds__(FEW_THREADS) k_rope_append_few(const __grid_constant__ Args a) {
   using E = typename T::type;
   constexpr int U = D / 16, L = G * U;  // lanes per block
   pdl::trigger();
   pdl::wait();
   if ((int)blockIdx.x < a.q_blocks) {
-    turn_q<T, IL, D>(a, (int64_t)blockIdx.x * FEW_THREADS + threadIdx.x);
+    turn_q<T, IL, D, NORM>(a, (int64_t)blockIdx.x * FEW_THREADS + threadIdx.x);
     return;
   }
   int i = (((int)blockIdx.x - a.q_blocks) * FEW_THREADS + (int)threadIdx.x) / L;
@@ -480,6 +506,7 @@ __global__ void __launch_bounds__(FEW_THREADS) k_rope_append_few(const __grid_co
     const E* p = reinterpret_cast<const E*>(is_v ? a.v : a.k) + b * st.b + (k.t0 + r) * st.t + h * st.h;
     T::load8(p + c0, x0);
     T::load8(p + c1, x1);
+    if (NORM && !is_v && a.k_norm) head_norm<T, U>(x0, x1, a.k_norm, c0, c1, a.eps);
     if (!is_v && u * 16 < a.rot) {
       float c[8], s[8];
       load_angles(a.table + (k.pos + r) * (a.rot >> 1), u, a.rot, c, s);
@@ -500,14 +527,14 @@ __global__ void __launch_bounds__(FEW_THREADS) k_rope_append_few(const __grid_co
   }
 }
 
-template <typename T, bool IL, int D, int TH>
+template <typename T, bool IL, int D, int TH, bool NORM>
 void launch_cache(const Args& a, unsigned n, int64_t& blocks, cudaStream_t st) {
-  if (!tc::allow_smem<k_rope_append<T, IL, D, TH>>(Ring<T, TH>::BYTES) ||
-      !pdl::launch<k_rope_append<T, IL, D, TH>>(n, TH, Ring<T, TH>::BYTES, st, 1, a))
+  if (!tc::allow_smem<k_rope_append<T, IL, D, TH, NORM>>(Ring<T, TH>::BYTES) ||
+      !pdl::launch<k_rope_append<T, IL, D, TH, NORM>>(n, TH, Ring<T, TH>::BYTES, st, 1, a))
     blocks = -1;
 }
 // blocks: of the largest launch (2^31 or more: nothing launched), -1: a CUDA call failed.
-template <typename T, bool IL, int D>
+template <typename T, bool IL, int D, bool NORM>
 void launch_d(Args& a, int64_t& blocks, cudaStream_t st) {
   const int64_t items = (int64_t)a.B * a.W * 2 * a.Hkv;
   auto q_ctas = [&](int th) {
@@ -521,10 +548,10 @@ void launch_d(Args& a, int64_t& blocks, cudaStream_t st) {
     if (blocks >= (1ll << 31)) return;
     a.q_blocks = (int)q_ctas(FEW_THREADS);
     const unsigned n = (unsigned)blocks;
-    const bool ok = g == 1   ? pdl::launch<k_rope_append_few<T, IL, D, 1>>(n, FEW_THREADS, 0, st, 1, a)
-                    : g == 2 ? pdl::launch<k_rope_append_few<T, IL, D, 2>>(n, FEW_THREADS, 0, st, 1, a)
-                    : g == 4 ? pdl::launch<k_rope_append_few<T, IL, D, 4>>(n, FEW_THREADS, 0, st, 1, a)
-                             : pdl::launch<k_rope_append_few<T, IL, D, 512 / D>>(n, FEW_THREADS, 0, st, 1, a);
+    const bool ok = g == 1   ? pdl::launch<k_rope_append_few<T, IL, D, 1, NORM>>(n, FEW_THREADS, 0, st, 1, a)
+                    : g == 2 ? pdl::launch<k_rope_append_few<T, IL, D, 2, NORM>>(n, FEW_THREADS, 0, st, 1, a)
+                    : g == 4 ? pdl::launch<k_rope_append_few<T, IL, D, 4, NORM>>(n, FEW_THREADS, 0, st, 1, a)
+                             : pdl::launch<k_rope_append_few<T, IL, D, 512 / D, NORM>>(n, FEW_THREADS, 0, st, 1, a);
     if (!ok) blocks = -1;
     return;
   }
@@ -536,25 +563,324 @@ void launch_d(Args& a, int64_t& blocks, cudaStream_t st) {
   while (a.hc < 4 && a.hc < a.Hkv && items / (2 * a.hc) >= 8 * sms) a.hc *= 2;
   blocks = std::max(q_ctas(Q_THREADS), (int64_t)a.B * a.W * 2 * ((a.Hkv + a.hc - 1) / a.hc));
   if (blocks >= (1ll << 31)) return;
-  if (!tc::allow_smem<k_turn_q<T, IL, D>>(Ring<T, Q_THREADS>::BYTES) ||
-      !pdl::launch<k_turn_q<T, IL, D>, false>((unsigned)q_ctas(Q_THREADS), Q_THREADS, Ring<T, Q_THREADS>::BYTES, st, 1, a)) {
+  if (!tc::allow_smem<k_turn_q<T, IL, D, NORM>>(Ring<T, Q_THREADS>::BYTES) ||
+      !pdl::launch<k_turn_q<T, IL, D, NORM>, false>((unsigned)q_ctas(Q_THREADS), Q_THREADS, Ring<T, Q_THREADS>::BYTES, st, 1, a)) {
     blocks = -1;
     return;
   }
   const unsigned n = (unsigned)(a.B * a.W * 2 * ((a.Hkv + a.hc - 1) / a.hc));
   if (a.page == 32)
-    launch_cache<T, IL, D, D>(a, n, blocks, st);
+    launch_cache<T, IL, D, D, NORM>(a, n, blocks, st);
   else if (a.page == 64)
-    launch_cache<T, IL, D, 2 * D>(a, n, blocks, st);
+    launch_cache<T, IL, D, 2 * D, NORM>(a, n, blocks, st);
   else
-    launch_cache<T, IL, D, 4 * D>(a, n, blocks, st);
+    launch_cache<T, IL, D, 4 * D, NORM>(a, n, blocks, st);
+}
+template <typename T, bool NORM>
+void launch_norm(Args& a, int D, int64_t& blocks, cudaStream_t st) {
+  if (D == 128)
+    a.interleaved ? launch_d<T, true, 128, NORM>(a, blocks, st) : launch_d<T, false, 128, NORM>(a, blocks, st);
+  else
+    a.interleaved ? launch_d<T, true, 64, NORM>(a, blocks, st) : launch_d<T, false, 64, NORM>(a, blocks, st);
 }
 template <typename T>
 void launch(Args& a, int D, int64_t& blocks, cudaStream_t st) {
+  a.q_norm || a.k_norm ? launch_norm<T, true>(a, D, blocks, st) : launch_norm<T, false>(a, D, blocks, st);
+}
+
+// ---- the cache in 4 bits ----------------------------------------------------
+//
+// Codes [pages, kv_heads, page, D / 2], two E2M1 values a byte (the even column
+// in the low half), and one E4M3 scale per 16 columns of a token [pages,
+// kv_heads, page, D / 16]; a value is code * scale * the head's float32 factor f.
+//
+//   scale = E4M3(max|x| / (6 f)), at least 2^-9;  code = E2M1(x / (scale f))
+//
+// Both round to nearest, ties to even, and saturate; a NaN makes its block's
+// scale NaN.  A token's blocks are its own: nothing that the cache holds is read
+// or changed, and a thread needs no more than its neighbour's maximum.
+//
+// The quotient is x r, r = 1 / (scale f), with one correction by its remainder
+// (Markstein 1990: the result is the rounded quotient), so that a quotient that
+// lies between two codes is taken as what it is; bf16 values meet such ties often.
+
+// Two floats times or plus two, rounded to nearest, in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+
+// 8 values, their quotients by d, as codes: 4 bytes.
+__device__ __forceinline__ uint32_t e2m1_codes(const float (&x)[8], float d, float r, bool plain) {
+  float y[8];
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const float2 v = make_float2(x[j], x[j + 1]), rr = make_float2(r, r), nd = make_float2(-d, -d);
+    float2 q = __fmul2_rn(v, rr);
+    if (plain) q = fma2(fma2(q, nd, v), rr, q);
+    y[j] = q.x, y[j + 1] = q.y;
+  }
+  uint32_t w;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(w)
+      : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
+  return w;
+}
+// The largest magnitude; NaN where one is.
+__device__ __forceinline__ float amax_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float amax8(const float (&x)[8]) {
+  float m = fabsf(x[0]);
+#pragma unroll
+  for (int j = 1; j < 8; ++j) m = amax_nan(m, fabsf(x[j]));
+  return m;
+}
+// A block's scale byte, and what its values are divided by.
+__device__ __forceinline__ uint32_t block_scale4(float amax, float f, float& d) {
+  const uint32_t b = max(pack2(__fdiv_rn(amax, 6.0f * f), 0.0f) & 0xFFu, 1u);
+  d = half2f(unpack2(b)).x * f;
+  return b;
+}
+// One unit's 16 columns of a key or value head to its token's place.  `split`:
+// the unit's two groups of 8 lie in two blocks, whose other halves are the
+// units of other lanes of the head (group g of a turned head is the first of
+// lane g, or the second of lane g - R).
+template <int U>
+__device__ __forceinline__ void store4(uint8_t* codes, uint8_t* scale, const float (&x0)[8], const float (&x1)[8],
+                                       float f, int u, int rot, bool split, bool store) {
+  float m0 = amax8(x0), m1 = amax8(x1);
+  const int R = rot >> 4;
+  if (split) {
+    const int lane = threadIdx.x & 31, first = lane & ~(U - 1);
+    const uint32_t lanes = ((1u << U) - 1) << first;
+    // every lane of the head asks; those past the turned columns keep their own
+    const bool turned = u < R;
+    const int p0 = turned ? u ^ 1 : 0, p1 = turned ? (u + R) ^ 1 : 0;
+    const int s0 = first + (p0 < R ? p0 : p0 - R), s1 = first + (p1 < R ? p1 : p1 - R);
+    const float a0 = __shfl_sync(lanes, m0, s0), a1 = __shfl_sync(lanes, m1, s0);
+    const float b0 = __shfl_sync(lanes, m0, s1), b1 = __shfl_sync(lanes, m1, s1);
+    const float n0 = amax_nan(m0, p0 < R ? a0 : a1), n1 = amax_nan(m1, p1 < R ? b0 : b1), n = amax_nan(m0, m1);
+    m0 = turned ? n0 : n, m1 = turned ? n1 : n;
+    split = turned;
+  } else {
+    m0 = m1 = amax_nan(m0, m1);
+  }
+  if (!store) return;
+  float d0, d1;
+  const uint32_t e0 = block_scale4(m0, f, d0);
+  const uint32_t e1 = split ? block_scale4(m1, f, d1) : (d1 = d0, e0);
+  // the correction's products leave float32 only where the values saturate all the same
+  const uint32_t w0 = e2m1_codes(x0, d0, __fdiv_rn(1.0f, d0), m0 < 1e30f);
+  const uint32_t w1 = e2m1_codes(x1, d1, split ? __fdiv_rn(1.0f, d1) : __fdiv_rn(1.0f, d0), m1 < 1e30f);
+  if (split) {
+    const int g1 = u + R;
+    reinterpret_cast<uint32_t*>(codes)[u] = w0;
+    reinterpret_cast<uint32_t*>(codes)[g1] = w1;
+    if (!(u & 1)) scale[u >> 1] = (uint8_t)e0;
+    if (!(g1 & 1)) scale[g1 >> 1] = (uint8_t)e1;
+  } else {
+    reinterpret_cast<uint2*>(codes)[u] = make_uint2(w0, w1);
+    scale[u] = (uint8_t)e0;
+  }
+}
+
+// The query, key and value heads alike: thread `i` takes its unit of a.hq heads
+// of a token, the heads of q, k and v counted on; the tokens of a warp are
+// neighbours, so that their codes and scales fill sectors.
+struct Unit4 {
+  int u, h0, h1, b, t;
+  int64_t row;
+};
+template <int D>
+__device__ __forceinline__ Unit4 unit4(const Args& a, int64_t i) {
+  constexpr int U = D / 16;
+  Unit4 x;
+  x.u = (int)(i % U);
+  const int64_t rows = (int64_t)a.B * a.T, r = i / U, hg = r / rows;
+  x.row = r - hg * rows;
+  const int all = a.H + 2 * a.Hkv;
+  x.h0 = (int)min(hg * a.hq, (int64_t)all), x.h1 = min(all, x.h0 + a.hq);
+  x.b = (int)(x.row / a.T), x.t = (int)(x.row - (int64_t)x.b * a.T);
+  return x;
+}
+// Where a head's unit lies: its row, and the first columns of its two groups.
+// Values do not turn, so their units are 16 columns that lie side by side.
+template <typename T, bool IL>
+__device__ __forceinline__ const typename T::type* head_row(const Args& a, const Unit4& x, int h, int& c0, int& c1) {
+  using E = typename T::type;
+  const bool is_v = h >= a.H + a.Hkv, is_k = h >= a.H && !is_v;
+  unit_cols<IL>(x.u, is_v ? 0 : a.rot, c0, c1);
+  const Strides& s = is_v ? a.sv : is_k ? a.sk : a.sq;
+  const E* p = reinterpret_cast<const E*>(is_v ? a.v : is_k ? a.k : a.q);
+  return p + x.b * s.b + x.t * s.t + (h - (is_v ? a.H + a.Hkv : is_k ? a.H : 0)) * s.h;
+}
+// A token's place: live, its slot of the cache (-1: none) and its angles.
+struct Token4 {
+  bool live, turns;
+  int64_t slot;  // (page * Hkv) * page size + place in it
+  float c[8], s[8];
+};
+__device__ __forceinline__ Token4 token4(const Args& a, const Unit4& x) {
+  Token4 k;
+  int held;
+  k.live = x.t < plan(a, x.b, held);
+  k.turns = k.live && x.u * 16 < a.rot;
+  k.slot = -1;
+  if (k.turns) load_angles(a.table + (int64_t)(held + x.t) * (a.rot >> 1), x.u, a.rot, k.c, k.s);
+  if (k.live && x.h1 > a.H) {
+    const int pos = held + x.t, at = pos / a.page;
+    const int pid = a.block_table[(int64_t)x.b * a.width + at];
+    if (pid < 0 || pid >= a.pages)
+      tc::note_err(nullptr, ERR_PAGE);
+    else
+      k.slot = (int64_t)pid * a.Hkv * a.page + (pos - at * a.page);
+  }
+  return k;
+}
+template <typename T, bool IL, int D, bool NORM>
+__device__ __forceinline__ void finish4(const Args& a, const Unit4& x, const Token4& k, int h, int c0, int c1,
+                                        float (&x0)[8], float (&x1)[8]) {
+  constexpr int U = D / 16;
+  const bool is_q = h < a.H, is_v = h >= a.H + a.Hkv;
+  if (!is_v) {
+    const void* w = is_q ? a.q_norm : a.k_norm;
+    if (NORM && w) head_norm<T, U>(x0, x1, w, c0, c1, a.eps);
+    if (k.turns) turn<IL>(x0, x1, k.c, k.s);
+  }
+  if (is_q) {
+    if (!k.live) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x0[j] = x1[j] = 0.0f;
+    }
+    store_unit<T>(reinterpret_cast<typename T::type*>(a.q_out) + (x.row * a.H + h) * D, c0, c1, x0, x1);
+  } else {
+    const int kvh = h - a.H - (is_v ? a.Hkv : 0);
+    const int64_t at = (k.slot < 0 ? 0 : k.slot) + (int64_t)kvh * a.page;
+    store4<U>((is_v ? a.v_codes : a.k_codes) + at * (D / 2), (is_v ? a.v_bscale : a.k_bscale) + at * U, x0, x1,
+              __ldg((is_v ? a.v_factor : a.k_factor) + kvh), x.u, a.rot, !IL && !is_v, k.slot >= 0);
+  }
+}
+
+// Few heads in all: one head a thread.
+template <typename T, bool IL, int D, bool NORM>
+__global__ void __launch_bounds__(FEW_THREADS) k_append4_few(const __grid_constant__ Args a) {
+  pdl::trigger();
+  pdl::wait();
+  const Unit4 x = unit4<D>(a, (int64_t)blockIdx.x * FEW_THREADS + threadIdx.x);
+  if (x.h0 >= x.h1) return;
+  int c0, c1;
+  const typename T::type* p = head_row<T, IL>(a, x, x.h0, c0, c1);
+  float x0[8], x1[8];
+  T::load8(p + c0, x0);
+  T::load8(p + c1, x1);
+  const Token4 k = token4(a, x);
+  finish4<T, IL, D, NORM>(a, x, k, x.h0, c0, c1, x0, x1);
+}
+
+// Many: a.hq heads a thread, QH at a time, whose loads travel through a ring.
+template <typename T, bool IL, int D, bool NORM>
+__global__ void __launch_bounds__(Q_THREADS) k_append4(const __grid_constant__ Args a) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const Ring<T, Q_THREADS> ring(smem);
+  pdl::wait();
+  const Unit4 x = unit4<D>(a, (int64_t)blockIdx.x * Q_THREADS + threadIdx.x);
+  if (x.h0 >= x.h1) return;
+  const int steps = (x.h1 - x.h0 + QH - 1) / QH;
+  auto fetch = [&](int k) {
+    if (k < steps) {
+#pragma unroll
+      for (int q = 0; q < QH; ++q) {
+        int c0, c1;
+        const typename T::type* p = head_row<T, IL>(a, x, min(x.h0 + k * QH + q, x.h1 - 1), c0, c1);
+        ring.fetch(k, 2 * q, p + c0);
+        ring.fetch(k, 2 * q + 1, p + c1);
+      }
+    }
+    ring.commit();
+  };
+#pragma unroll
+  for (int k = 0; k < Ring<T, Q_THREADS>::DEPTH - 1; ++k) fetch(k);
+  const Token4 tok = token4(a, x);
+  for (int k = 0; k < steps; ++k) {
+    fetch(k + Ring<T, Q_THREADS>::DEPTH - 1);
+    ring.wait();
+#pragma unroll
+    for (int q = 0; q < QH; ++q) {
+      const int h = x.h0 + k * QH + q;
+      float x0[8], x1[8];
+      ring.read(k, 2 * q, x0);
+      ring.read(k, 2 * q + 1, x1);
+      int c0, c1;
+      unit_cols<IL>(x.u, h >= a.H + a.Hkv ? 0 : a.rot, c0, c1);
+      if (h < x.h1) finish4<T, IL, D, NORM>(a, x, tok, h, c0, c1, x0, x1);
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+template <typename T, bool IL, int D, bool NORM>
+void launch4_d(Args& a, int64_t& blocks, cudaStream_t st) {
+  const int all = a.H + 2 * a.Hkv;
+  auto ctas = [&](int th) { return ((int64_t)a.B * a.T * ((all + a.hq - 1) / a.hq) * (D / 16) + th - 1) / th; };
+  a.hq = 1;
+  if (ctas(FEW_THREADS) <= 16 * vq::mx::sm_count()) {
+    blocks = ctas(FEW_THREADS);
+    if (!pdl::launch<k_append4_few<T, IL, D, NORM>>((unsigned)blocks, FEW_THREADS, 0, st, 1, a)) blocks = -1;
+    return;
+  }
+  a.hq = QH;
+  while (a.hq < all && ctas(Q_THREADS) >= 12 * vq::mx::sm_count()) a.hq *= 2;
+  blocks = ctas(Q_THREADS);
+  if (blocks >= (1ll << 31)) return;
+  if (!tc::allow_smem<k_append4<T, IL, D, NORM>>(Ring<T, Q_THREADS>::BYTES) ||
+      !pdl::launch<k_append4<T, IL, D, NORM>, false>((unsigned)blocks, Q_THREADS, Ring<T, Q_THREADS>::BYTES, st, 1, a))
+    blocks = -1;
+}
+template <typename T, bool IL, int D>
+void launch4_n(Args& a, int64_t& blocks, cudaStream_t st) {
+  a.q_norm || a.k_norm ? launch4_d<T, IL, D, true>(a, blocks, st) : launch4_d<T, IL, D, false>(a, blocks, st);
+}
+template <typename T>
+void launch4(Args& a, int D, int64_t& blocks, cudaStream_t st) {
   if (D == 128)
-    a.interleaved ? launch_d<T, true, 128>(a, blocks, st) : launch_d<T, false, 128>(a, blocks, st);
+    a.interleaved ? launch4_n<T, true, 128>(a, blocks, st) : launch4_n<T, false, 128>(a, blocks, st);
   else
-    a.interleaved ? launch_d<T, true, 64>(a, blocks, st) : launch_d<T, false, 64>(a, blocks, st);
+    a.interleaved ? launch4_n<T, true, 64>(a, blocks, st) : launch4_n<T, false, 64>(a, blocks, st);
+}
+
+// E2M1 codes as E4M3 codes of the same values: the magnitudes from a table of
+// eight bytes (0, .5, 1, 1.5, 2, 3, 4, 6), the sign moved.  16 bytes in, 32 out
+// a thread and turn.
+__device__ __forceinline__ uint32_t e2m1_to_e4m3(uint32_t nib4) {  // four codes, one in each byte's low half
+  const uint32_t lo = 0x3C383000u, hi = 0x4C484440u;
+  const uint32_t sel = nib4 & 0x07070707u;
+  const uint32_t s16 = (sel & 0x7u) | ((sel >> 4) & 0x70u) | ((sel >> 8) & 0x700u) | ((sel >> 12) & 0x7000u);
+  return __byte_perm(lo, hi, s16) | ((nib4 & 0x08080808u) << 4);
+}
+constexpr int UNPACK_THREADS = 256;
+__global__ void __launch_bounds__(UNPACK_THREADS)
+    k_unpack4(const uint4* k, const uint4* v, uint4* ko, uint4* vo, int64_t chunks) {
+  pdl::trigger();
+  pdl::wait();
+  const int64_t step = (int64_t)gridDim.x * UNPACK_THREADS;
+  for (int64_t i = (int64_t)blockIdx.x * UNPACK_THREADS + threadIdx.x; i < 2 * chunks; i += step) {
+    const bool second = i >= chunks;
+    const int64_t j = second ? i - chunks : i;
+    const uint4 w = __ldg((second ? v : k) + j);
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+    uint32_t o[8];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t even = e2m1_to_e4m3(in[q] & 0x0F0F0F0Fu), odd = e2m1_to_e4m3((in[q] >> 4) & 0x0F0F0F0Fu);
+      o[2 * q] = __byte_perm(even, odd, 0x5140), o[2 * q + 1] = __byte_perm(even, odd, 0x7362);
+    }
+    uint4* p = (second ? vo : ko) + 2 * j;
+    p[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    p[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  }
 }
 
 // This file's sticky word (vq_device_errors).
@@ -565,13 +891,13 @@ int sticky_kv(int* out, int clear, cudaStream_t st) { return vq::tc::sticky_read
 
 using namespace vq::kv;
 
-extern "C" int vq_rope_append_kv8(const void* q, const void* k, const void* v, const int64_t* strides,
-                                  int32_t dtype, const float* table, int64_t positions, int32_t rot,
-                                  int32_t interleaved, int64_t batch, int64_t tokens, int32_t heads,
-                                  int32_t kv_heads, int32_t head_dim, const void* block_table,
-                                  int64_t table_width, const void* lengths, const void* counts,
-                                  int64_t pages, int32_t page, void* q_out, void* k_codes,
-                                  void* v_codes, float* k_scale, float* v_scale, void* stream) {
+// What both caches' entry points check and take alike.  `align_v`: the codes'.
+static int arguments(Args& a, const void* q, const void* k, const void* v, const int64_t* strides, int32_t dtype,
+                     const float* table, int64_t positions, int32_t rot, int32_t interleaved, int64_t batch,
+                     int64_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, const void* block_table,
+                     int64_t table_width, const void* lengths, const void* counts, int64_t pages, int32_t page,
+                     const void* q_norm, const void* k_norm, float eps, void* q_out, void* k_codes, void* v_codes,
+                     const void* k_scale, const void* v_scale, bool& none) {
   if (dtype != VQ_BF16 && dtype != VQ_F32) return VQ_ERR_UNSUPPORTED;
   if (head_dim != 64 && head_dim != 128) return VQ_ERR_UNSUPPORTED;
   if (page != 32 && page != 64 && page != 128) return VQ_ERR_UNSUPPORTED;
@@ -579,21 +905,21 @@ extern "C" int vq_rope_append_kv8(const void* q, const void* k, const void* v, c
       rot > head_dim || rot % 16 || table_width < 0 || pages < 0 || batch > (1 << 24) ||
       tokens > (1 << 24) || table_width > (1 << 24) || pages * kv_heads * page >= (1ll << 31))
     return VQ_ERR_INVALID;
-  if (batch == 0 || tokens == 0) return VQ_OK;
+  none = batch == 0 || tokens == 0;
+  if (none) return VQ_OK;
   if (!q || !k || !v || !strides || !lengths || !q_out) return VQ_ERR_NULL;
   // a table of no columns and a cache of no pages are not read: may be null
   if (table_width && (!table || !block_table)) return VQ_ERR_NULL;
   if (pages && (!k_codes || !v_codes || !k_scale || !v_scale)) return VQ_ERR_NULL;
   if (positions < table_width * page) return VQ_ERR_SHAPE;  // every position the plan can name
   const int eb = dtype == VQ_BF16 ? 2 : 4;
-  const void* p16[6] = {q, k, v, q_out, k_codes, v_codes};
+  const void* p16[9] = {q, k, v, q_out, k_codes, v_codes, table, q_norm, k_norm};
   for (const void* p : p16)
     if (reinterpret_cast<uintptr_t>(p) & 15) return VQ_ERR_ALIGNMENT;
-  if ((reinterpret_cast<uintptr_t>(table) & 15) || (reinterpret_cast<uintptr_t>(q_out) & 31))
-    return VQ_ERR_ALIGNMENT;
+  if (reinterpret_cast<uintptr_t>(q_out) & 31) return VQ_ERR_ALIGNMENT;
   for (int i = 0; i < 9; ++i)
     if (strides[i] * eb % 16) return VQ_ERR_ALIGNMENT;
-  Args a;
+  a = {};
   a.q = q, a.k = k, a.v = v;
   a.sq = {strides[0], strides[1], strides[2]};
   a.sk = {strides[3], strides[4], strides[5]};
@@ -601,13 +927,33 @@ extern "C" int vq_rope_append_kv8(const void* q, const void* k, const void* v, c
   a.table = reinterpret_cast<const float2*>(table);
   a.q_out = q_out;
   a.k_codes = (uint8_t*)k_codes, a.v_codes = (uint8_t*)v_codes;
-  a.k_scale = k_scale, a.v_scale = v_scale;
   a.block_table = (const int32_t*)block_table;
   a.lengths = (const int32_t*)lengths;
   a.counts = (const int32_t*)counts;
   a.B = (int)batch, a.T = (int)tokens, a.H = heads, a.Hkv = kv_heads;
   a.rot = rot, a.page = page, a.width = (int)table_width, a.pages = (int)pages;
   a.interleaved = interleaved;
+  a.q_norm = q_norm, a.k_norm = k_norm, a.eps = eps;
+  return VQ_OK;
+}
+
+extern "C" {
+
+int vq_rope_append_kv8_norm(const void* q, const void* k, const void* v, const int64_t* strides,
+                            int32_t dtype, const float* table, int64_t positions, int32_t rot,
+                            int32_t interleaved, int64_t batch, int64_t tokens, int32_t heads,
+                            int32_t kv_heads, int32_t head_dim, const void* block_table,
+                            int64_t table_width, const void* lengths, const void* counts,
+                            int64_t pages, int32_t page, const void* q_norm, const void* k_norm, float eps,
+                            void* q_out, void* k_codes, void* v_codes, float* k_scale, float* v_scale,
+                            void* stream) {
+  Args a;
+  bool none;
+  const int bad = arguments(a, q, k, v, strides, dtype, table, positions, rot, interleaved, batch, tokens, heads,
+                            kv_heads, head_dim, block_table, table_width, lengths, counts, pages, page, q_norm,
+                            k_norm, eps, q_out, k_codes, v_codes, k_scale, v_scale, none);
+  if (bad || none) return bad;
+  a.k_scale = k_scale, a.v_scale = v_scale;
   a.W = (int)((tokens - 1 + page - 1) / page) + 1;
   if (batch * a.W * 2 * kv_heads >= (1ll << 26)) return VQ_ERR_INVALID;  // items times 32 lanes in 31 bits
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
@@ -620,3 +966,61 @@ extern "C" int vq_rope_append_kv8(const void* q, const void* k, const void* v, c
   if (blocks >= (1ll << 31)) return VQ_ERR_INVALID;
   return VQ_OK;
 }
+
+int vq_rope_append_kv8(const void* q, const void* k, const void* v, const int64_t* strides,
+                       int32_t dtype, const float* table, int64_t positions, int32_t rot,
+                       int32_t interleaved, int64_t batch, int64_t tokens, int32_t heads,
+                       int32_t kv_heads, int32_t head_dim, const void* block_table,
+                       int64_t table_width, const void* lengths, const void* counts, int64_t pages,
+                       int32_t page, void* q_out, void* k_codes, void* v_codes, float* k_scale,
+                       float* v_scale, void* stream) {
+  return vq_rope_append_kv8_norm(q, k, v, strides, dtype, table, positions, rot, interleaved, batch, tokens, heads,
+                                 kv_heads, head_dim, block_table, table_width, lengths, counts, pages, page, nullptr,
+                                 nullptr, 0.0f, q_out, k_codes, v_codes, k_scale, v_scale, stream);
+}
+
+int vq_rope_append_kv4(const void* q, const void* k, const void* v, const int64_t* strides,
+                       int32_t dtype, const float* table, int64_t positions, int32_t rot,
+                       int32_t interleaved, int64_t batch, int64_t tokens, int32_t heads,
+                       int32_t kv_heads, int32_t head_dim, const void* block_table,
+                       int64_t table_width, const void* lengths, const void* counts, int64_t pages,
+                       int32_t page, const void* q_norm, const void* k_norm, float eps, void* q_out,
+                       void* k_codes, void* v_codes, void* k_scale, void* v_scale, const float* k_factor,
+                       const float* v_factor, void* stream) {
+  Args a;
+  bool none;
+  const int bad = arguments(a, q, k, v, strides, dtype, table, positions, rot, interleaved, batch, tokens, heads,
+                            kv_heads, head_dim, block_table, table_width, lengths, counts, pages, page, q_norm,
+                            k_norm, eps, q_out, k_codes, v_codes, k_scale, v_scale, none);
+  if (bad || none) return bad;
+  if (!k_factor || !v_factor) return VQ_ERR_NULL;
+  a.k_bscale = (uint8_t*)k_scale, a.v_bscale = (uint8_t*)v_scale;
+  a.k_factor = k_factor, a.v_factor = v_factor;
+  if (heads > (1 << 20) || batch * tokens >= (1ll << 31)) return VQ_ERR_INVALID;  // heads and tokens in 31 bits
+  int64_t blocks = 0;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == VQ_BF16)
+    launch4<BF16>(a, head_dim, blocks, st);
+  else
+    launch4<F32>(a, head_dim, blocks, st);
+  if (blocks < 0) return VQ_ERR_CUDA;
+  if (blocks >= (1ll << 31)) return VQ_ERR_INVALID;
+  return VQ_OK;
+}
+
+int vq_kv4_unpack(const void* k_codes, const void* v_codes, int64_t bytes, void* k_out, void* v_out, void* stream) {
+  if (bytes < 0 || bytes % 16) return VQ_ERR_INVALID;
+  if (bytes == 0) return VQ_OK;
+  if (!k_codes || !v_codes || !k_out || !v_out) return VQ_ERR_NULL;
+  const void* p16[4] = {k_codes, v_codes, k_out, v_out};
+  for (const void* p : p16)
+    if (reinterpret_cast<uintptr_t>(p) & 15) return VQ_ERR_ALIGNMENT;
+  const int64_t chunks = bytes / 16, ctas = (2 * chunks + UNPACK_THREADS - 1) / UNPACK_THREADS;
+  const unsigned n = (unsigned)std::min<int64_t>(ctas, 8 * vq::mx::sm_count());
+  return vq::pdl::launch<k_unpack4>(n, UNPACK_THREADS, 0, reinterpret_cast<cudaStream_t>(stream), 1,
+                                    (const uint4*)k_codes, (const uint4*)v_codes, (uint4*)k_out, (uint4*)v_out, chunks)
+             ? VQ_OK
+             : VQ_ERR_CUDA;
+}
+
+}  // extern "C"

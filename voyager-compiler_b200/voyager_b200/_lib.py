@@ -258,6 +258,31 @@ _SIGNATURES = {
                                                ctypes.c_float, ctypes.c_void_p, ctypes.c_int64,
                                                ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
                                                ctypes.c_void_p]),
+    "vq_rope_append_kv8_norm": (ctypes.c_int, [ctypes.c_void_p] * 3
+                                + [P(ctypes.c_int64), ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64,
+                                   ctypes.c_int32, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64,
+                                   ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+                                   ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                   ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_float]
+                                + [ctypes.c_void_p] * 6),
+    "vq_rope_append_kv4": (ctypes.c_int, [ctypes.c_void_p] * 3
+                           + [P(ctypes.c_int64), ctypes.c_int32, ctypes.c_void_p, ctypes.c_int64,
+                              ctypes.c_int32, ctypes.c_int32, ctypes.c_int64, ctypes.c_int64,
+                              ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p,
+                              ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                              ctypes.c_int32, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_float]
+                           + [ctypes.c_void_p] * 8),
+    "vq_kv4_unpack": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64]
+                      + [ctypes.c_void_p] * 3),
+    "vq_attn_kv4_workspace": (ctypes.c_int, [ctypes.c_int64] * 2 + [ctypes.c_int32] * 4
+                              + [ctypes.c_int64, P(ctypes.c_int64), P(ctypes.c_int64)]),
+    "vq_attn_kv4": (ctypes.c_int, [ctypes.c_void_p, P(ctypes.c_int64), ctypes.c_int64,
+                                   ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32]
+                    + [ctypes.c_void_p] * 6 + [ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p,
+                                               ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+                                               ctypes.c_float, ctypes.c_void_p, ctypes.c_int64,
+                                               ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                               ctypes.c_void_p]),
     "vq_codebook_lookup": (ctypes.c_int, [P(VqTensor), P(ctypes.c_int64), ctypes.c_int32,
                                           ctypes.c_void_p, ctypes.c_int64, P(VqTensor),
                                           ctypes.c_void_p]),

@@ -1,8 +1,10 @@
-"""A paged key / value cache in E4M3, and the operators that fill and read it.
+"""A paged key / value cache in E4M3 or in 4 bits, and the operators that fill and read it.
 
-The cache keeps E4M3 codes [pages, kv_heads, page, head_dim] and one
+``KVCache`` keeps E4M3 codes [pages, kv_heads, page, head_dim] and one
 power-of-two float32 scale per block (page, head), for the keys and for the
-values.  Which page holds which tokens is the caller's plan:
+values.  ``KVCache4`` keeps E2M1 codes, two a byte, and one E4M3 scale per 16
+columns of a token: 9/16 of a byte a value.  The operators take either.  Which
+page holds which tokens is the caller's plan:
 
   block_table  int32 [B, width]  the cache page of each page of a sequence
   lengths      int32 [B]         tokens the cache holds before the step
@@ -17,13 +19,14 @@ cache) leaves the tokens concerned out and is reported by
 reaches an output raises.
 
   rotary_table  cos / sin of every position, with the scalings for long contexts
-  rope_append   rotary positions + append
+  rope_append   (norms of the query and key heads +) rotary positions + append
   attend        causal attention of the newest tokens over the cache
+  unpack        the codes of a 4-bit cache, one a byte
 """
 
 import math
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Tuple, Union
 
 import torch
 
@@ -53,6 +56,41 @@ class KVCache:
              for _ in range(2)]
         s = [torch.ones((pages, kv_heads), dtype=torch.float32, device=device) for _ in range(2)]
         return cls(c[0], c[1], s[0], s[1])
+
+
+@dataclass
+class KVCache4:
+    """Codes uint8 [pages, kv_heads, page, head_dim / 2], two E2M1 codes a byte with
+    the even column in the low half, scales float8_e4m3fn [pages, kv_heads, page,
+    head_dim / 16], factors float32 [kv_heads], positive.  A value is code x scale
+    x its head's factor.  Scales reach from 2^-9 to 448, codes to 6: a factor of
+    max|x| / 2688 over a head uses the scales' whole range, and 1 holds values up
+    to 2688 with blocks below 0.01 losing bits."""
+
+    k_codes: torch.Tensor
+    v_codes: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    k_factor: torch.Tensor
+    v_factor: torch.Tensor
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, head_dim: int, page: int = 64, device="cuda",
+              k_factor: Optional[torch.Tensor] = None, v_factor: Optional[torch.Tensor] = None) -> "KVCache4":
+        """A cache that holds no token; a factor of None is 1 for every head."""
+        if page not in PAGES or head_dim not in HEAD_DIMS:
+            raise ValueError(f"KVCache4: page in {PAGES} and head_dim in {HEAD_DIMS}, not {page} and {head_dim}")
+        c = [torch.zeros((pages, kv_heads, page, head_dim // 2), dtype=torch.uint8, device=device) for _ in range(2)]
+        s = [torch.ones((pages, kv_heads, page, head_dim // 16), device=device).to(E4M3) for _ in range(2)]
+        f = [torch.ones(kv_heads, device=device) if f is None else f for f in (k_factor, v_factor)]
+        return cls(*c, *s, *f)
+
+
+Cache = Union[KVCache, KVCache4]
+
+
+def _factors(cache: Cache):
+    return (cache.k_factor, cache.v_factor) if isinstance(cache, KVCache4) else (None, None)
 
 
 def rotary_table(positions: int, rotary_dim: int, theta: float = 10000.0, *, scaling: Optional[str] = None,
@@ -104,9 +142,10 @@ def rotary_table(positions: int, rotary_dim: int, theta: float = 10000.0, *, sca
     return (torch.stack([angle.cos(), angle.sin()], -1) * amp).float()
 
 
-def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, cache: KVCache,
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, cache: Cache,
                 block_table: torch.Tensor, lengths: torch.Tensor, counts: Optional[torch.Tensor] = None,
-                interleaved: bool = False) -> torch.Tensor:
+                interleaved: bool = False, *, q_norm: Optional[torch.Tensor] = None,
+                k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
     """Turn q [B, T, H, D] and k [B, T, Hkv, D] by ``table`` (``rotary_table``,
     at least block_table.shape[1] * page positions) at the positions
     lengths[b] + t, append k and v [B, T, Hkv, D] to the cache (in place), and
@@ -114,18 +153,31 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.
     views such as the parts of one fused projection are read as they are.
 
     ``interleaved``: pairs are columns (2i, 2i + 1), otherwise (i, i +
-    rotary_dim / 2); columns past rotary_dim stay.  A block's scale is the
-    least power of two under which its tokens fit E4M3; it grows when a new
-    token needs it, and the codes it holds are brought to the new scale."""
+    rotary_dim / 2); columns past rotary_dim stay.  ``q_norm`` / ``k_norm`` [D] in
+    q's type: the heads of q / k are normalised first, ``x * rsqrt(mean(x^2) +
+    eps) * weight`` over D in float32, unrounded before they turn.
+
+    E4M3: a block's scale is the least power of two under which its tokens fit;
+    it grows when a new token needs it, and the codes it holds are brought to the
+    new scale.  4 bits: per 16 columns of a token ``scale = E4M3(max|x| / (6
+    factor))``, at least 2^-9, and ``code = E2M1(x / (scale factor))``, to nearest
+    even and saturating; what the cache holds is not touched."""
     return native.rope_append(q, k, v, table, cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale,
-                              block_table, lengths, counts, interleaved)
+                              block_table, lengths, counts, interleaved, *_factors(cache), q_norm, k_norm, eps)
 
 
-def attend(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, lengths: torch.Tensor,
+def attend(q: torch.Tensor, cache: Cache, block_table: torch.Tensor, lengths: torch.Tensor,
            counts: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
     """Causal attention of the step's tokens over the cache, which holds their
     keys and values already (``rope_append`` with the same plan): q bfloat16
     [B, T, H, D] -> [B, T, H, D], row (b, t) over the keys 0 .. lengths[b] + t.
     ``scale`` defaults to 1 / sqrt(D).  Tokens past counts get 0."""
     return native.attend(q, cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale, block_table, lengths,
-                         counts, scale)
+                         counts, scale, *_factors(cache))
+
+
+def unpack(cache: KVCache4) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The key and value codes of a 4-bit cache as float8_e4m3fn [pages,
+    kv_heads, page, head_dim], which holds every E2M1 value; scales and factors
+    are not in them."""
+    return native.unpack(cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale, *_factors(cache))
