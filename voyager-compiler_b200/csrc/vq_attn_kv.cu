@@ -49,6 +49,15 @@
 #include "vq_tc.cuh"
 
 namespace vq {
+namespace kv4 {  // vq_attn_kv4.cu
+void workspace(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim, int64_t capacity, int64_t* floats,
+               int64_t* counters);
+int attend(const void* q, const int64_t* q_strides, int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim,
+           const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, const float* k_factor,
+           const float* v_factor, int64_t pages, int page, const void* block_table, int64_t table_width,
+           const void* lengths, const void* counts, float sm_scale, float* workspace, int64_t workspace_floats,
+           int32_t* counters, int64_t counters_len, void* out, cudaStream_t st);
+}  // namespace kv4
 namespace kva {
 
 using namespace vq::e4;
@@ -145,19 +154,6 @@ __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
 // Bits 0x80 of it: the word's bytes that are an E4M3 NaN (0x7F or 0xFF).
 __device__ __forceinline__ uint32_t nan_bits(uint32_t w) { return (w & 0x7F7F7F7Fu) + 0x01010101u; }
 
-// Four bytes of two E2M1 codes each as f16 pairs (exact), the low halves first.
-__device__ __forceinline__ void e2m1_f16(uint32_t w, uint32_t (&h)[4]) {
-  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
-}
-// A code times a scale: 2 by 4 significant bits within 2^-10 .. 2688, exact in f16.
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
   uint32_t v;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
@@ -1094,12 +1090,19 @@ int sticky_kva(int* out, int clear, cudaStream_t st) { return vq::tc::sticky_rea
 
 using namespace vq::kva;
 
+// The 4-bit cache under more rows a kv head than this is vq_attn_kv4.cu's.
+constexpr int64_t FEW_ROWS = 16;
+
 static int workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t page,
                      int64_t table_width, int64_t* floats, int64_t* counters, bool fp4) {
   if (!floats || !counters) return VQ_ERR_NULL;
   if (batch < 0 || tokens < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0 ||
       page <= 0 || table_width < 0 || table_width > max_width(page))
     return VQ_ERR_INVALID;
+  if (fp4 && tokens * (heads / kv_heads) > FEW_ROWS) {
+    vq::kv4::workspace(batch, tokens, heads, kv_heads, head_dim, table_width * page, floats, counters);
+    return VQ_OK;
+  }
   const Cut c = cut_of(std::max<int64_t>(batch, 1), std::max<int64_t>(tokens, 1), heads, kv_heads,
                        head_dim, table_width * page, fp4);
   *counters = batch * kv_heads * c.groups;
@@ -1145,6 +1148,10 @@ static int attention(const void* q, const int64_t* q_strides, int64_t batch, int
     if (reinterpret_cast<uintptr_t>(p) & 15) return VQ_ERR_ALIGNMENT;
   for (int i = 0; i < 3; ++i)
     if (q_strides[i] % 8) return VQ_ERR_ALIGNMENT;
+  if (fp4 && tokens * a.G > FEW_ROWS)
+    return vq::kv4::attend(q, q_strides, batch, tokens, heads, kv_heads, head_dim, k_codes, v_codes, k_scale, v_scale,
+                           k_factor, v_factor, pages, page, block_table, table_width, lengths, counts, sm_scale,
+                           workspace, workspace_floats, counters, counters_len, out, st);
   const Cut c = cut_of(batch, tokens, heads, kv_heads, head_dim, table_width * page, fp4);
   const int64_t pairs = batch * kv_heads * c.groups;
   // the units of all heads, counted in 32 bits

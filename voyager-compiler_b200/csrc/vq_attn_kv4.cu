@@ -1,0 +1,1044 @@
+// Attention of many query rows over the paged 4-bit key / value cache: prompts,
+// pieces of prompts, and drafts of more than 16 rows a kv head.
+//
+//   o[b, t, h] = sum_j softmax_j(q . k_j * sm_scale) v_j,  j <= held[b] + t,
+//   k_j = code * scale * factor, v_j likewise (vq_rope_append_kv4's cache)
+//
+// The T tokens and the G query heads that share a kv head are the rows of one
+// product: row r = t * G + g.
+//
+// Mathematics: S = Q K^T and O += P V on tcgen05 in f16, float32 accumulators in
+// tensor memory.  code * scale has at most 6 significant bits within 2^-10 ..
+// 2688, so a cache tile is exact in f16; q is scaled per row by a power of two to
+// a largest value of 2^14 .. 2^15, so that f16 holds every bf16 down to 2^-31 of
+// it exactly.  Scores are base-2 exponents s (float32); P = 2^(s - m + 7) in f16,
+// m a running reference that is at most 8 below the row's maximum: P <= 2^15, and
+// O is scaled anew only where the maximum has left m by more than that.
+// l = sum of the unrounded P in float32; the output is O / l * factor of V.
+//
+// A value whose scale is NaN enters the product as 0, and the smallest key of each
+// block of 16 columns that has one is noted: the rows that see it get NaN there at
+// the end, the others nothing (0 * NaN would reach every row of the tile).
+//
+// Work: two streams of 128 rows, each with a warpgroup for its softmax (a thread
+// is a row) and its own S and O in tensor memory; P lies in place of S and is the
+// second product's first operand.  While one stream's softmax runs, the tensor
+// cores work for the other.  PAIR: the streams are 256 rows of a head and share
+// the keys.  Otherwise a head has at most 128 rows: both streams have them and
+// take every other tile of keys; their sums meet in shared memory.  Four warps
+// each turn 128 keys' K and V from codes to f16 in shared memory, in the
+// SWIZZLE_128B layout that serves K as K-major and V as MN-major operand; the
+// next tile's codes are on their way in registers meanwhile.
+//
+// The tiles of every (sequence, row tile, kv head) lie end to end and are cut into
+// equal runs, one per CTA, one CTA per SM; the pieces of a head that was cut are
+// joined by the CTA that finishes last, in the CTAs' order.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "voyager_b200.h"
+#include "vq_e4m3.cuh"
+#include "vq_pdl.cuh"
+#include "vq_tc.cuh"
+
+namespace vq {
+namespace kv4 {
+
+using namespace vq::e4;
+using namespace vq::tc;
+
+enum { ERR_WAIT = 331, ERR_PAGE = 332, ERR_CAPACITY = 333, ERR_COUNT = 334 };
+
+constexpr int TILE = 128;  // keys
+constexpr int PLANS = 128;
+// warps: 0-7 softmax (a stream's four each), 8-11 codes to f16, 12 the MMAs, 13-15 none (a warpgroup's registers are
+// split together)
+constexpr int SM_WARPS = 8, W_DQ = 8, W_MMA = 12, WARPS = 16, THREADS = WARPS * 32;
+// registers a thread: launched with 128; a warpgroup of 4 warps gives some up or takes them
+constexpr int R_LAUNCH = 128, R_SOFT = 184, R_DQ = 80, R_REST = 64;
+static_assert(2 * R_SOFT + R_DQ + R_REST <= 4 * R_LAUNCH, "a register taken was given up before");
+constexpr int SOFT = SM_WARPS * 32;
+constexpr float NEG_INF = -__builtin_huge_valf();
+constexpr float P_EXP = 7.0f, LAG = 8.0f;
+constexpr int NAN_SETS = 3;  // a segment's, of which the epilogue of one and the loads of two more can be under way
+
+enum { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_VEMPTY = 6, B_QFULL = 8, B_SFULL = 10, B_PFULL = 12, B_OFULL = 14,
+       B_SOFT = 16, B_DRAIN = 18, NBARS = 19 };
+
+constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_O = 256;  // stream i: S at 128 i, O at 256 + 128 i
+
+template <int D>
+struct Lay {
+  static constexpr int TILE_BYTES = TILE * D * 2, HALF = TILE * 128;
+  static constexpr int OFF_Q = 0, OFF_K = 2 * TILE_BYTES, OFF_V = 4 * TILE_BYTES, OFF_BAR = 6 * TILE_BYTES;
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;
+};
+
+struct Args {
+  const uint16_t* q;
+  int64_t qb, qt, qh;
+  uint16_t* out;
+  const uint8_t *k_codes, *v_codes, *k_scale, *v_scale;
+  const float *k_factor, *v_factor;
+  const int32_t *block_table, *lengths, *counts;
+  float* part;    // [CTAs][2][streams with rows of their own][D + 2][128]: pieces of heads that were cut
+  int32_t* done;  // [B * groups * Hkv][streams ..] zero before, zero after
+  int B, T, H, Hkv, G, page_log2, width, pages, groups;
+  float sm_log2;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+  __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// 16 words of this warp's 32 TMEM lanes (lane = thread) to columns taddr ..
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// f16 x f16 -> float32; b_mn: the second operand is MN-major.
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t n, bool b_mn) {
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// MN-major SWIZZLE_128B: 64 columns (128 bytes) a row, 8 rows of K 1024 bytes
+// apart, the next 64 columns `half` bytes on.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr, uint32_t half) {
+  return (sw128_desc(saddr) & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(half >> 4) << 16);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accum));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accum));
+}
+
+// One lane of a converged warp, the same each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// A sequence's tokens held and new tokens, brought to what fits.
+__device__ __forceinline__ int2 plan_of(const Args& a, int b, int& err) {
+  int held = a.lengths[b], cnt = a.counts ? a.counts[b] : a.T;
+  if (held < 0 || cnt < 0 || cnt > a.T) {
+    err = ERR_COUNT;
+    cnt = held < 0 ? 0 : min(max(cnt, 0), a.T);
+    held = max(held, 0);
+  }
+  const int64_t cap = (int64_t)a.width << a.page_log2;
+  if (held + (int64_t)cnt > cap) {
+    err = ERR_CAPACITY;
+    cnt = held >= cap ? 0 : (int)(cap - held);
+  }
+  return make_int2(held, cnt);
+}
+// Entry e = (sequence, row tile): its rows that have a query, the tokens held,
+// and the keys that some of its rows sees.
+struct Entry {
+  int b, row0, nrows, held, end;
+};
+template <int ROWS>
+__device__ __forceinline__ Entry entry_of(const Args& a, int e, const int2* plans) {
+  Entry x;
+  x.b = a.groups == 1 ? e : e / a.groups;
+  x.row0 = (e - x.b * a.groups) * ROWS;
+  int err;
+  const int2 plan = x.b < PLANS ? plans[x.b] : plan_of(a, x.b, err);
+  x.held = plan.x;
+  x.nrows = min(ROWS, plan.y * a.G - x.row0);
+  x.end = x.nrows > 0 ? x.held + (x.row0 + x.nrows - 1) / a.G + 1 : 0;
+  return x;
+}
+__device__ __forceinline__ int tiles_of(const Entry& x) { return (x.end + TILE - 1) / TILE; }
+
+// The fewest tiles of a run: a piece more of a head costs its join about as much
+// time as a tile, and pieces' joins run one after the other.
+__device__ __forceinline__ float run_least(int tiles, int heads) {
+  return heads ? fmaxf(1.0f, sqrtf((float)tiles / (float)heads)) : 1.0f;
+}
+
+// What opening and ending a head costs, in tiles: the cuts count it.
+template <bool PAIR>
+struct Cost {
+  static constexpr int HEAD = PAIR ? 2 : 1;
+};
+
+// This CTA's run lies from lo to hi; its first head is of `entry`, which begins
+// at `before`.  Heads lie end to end, HEAD + tiles each; a cut within the first
+// HEAD of one moves to its begin.
+struct Run {
+  int lo, hi, entry, before, base, rest;  // the first `rest` runs are base + 1 long
+};
+// Segments, one after the other: the part of one head (entry, kv head) in the run.
+struct Seg {
+  int b, row0, nrows, held, end, kvh, t0, t1, tiles, slot, pair, ps;
+  bool whole;
+};
+template <int ROWS, int HEAD>
+struct Segments {
+  const Args& a;
+  const int2* plans;
+  Run r;
+  int pos, ebase, e, tiles;
+  Entry x;
+  __device__ __forceinline__ Segments(const Args& a_, const int2* p, const Run& run)
+      : a(a_), plans(p), r(run), pos(run.lo), ebase(run.before), e(run.entry - 1), tiles(0), x() {}
+  __device__ __forceinline__ bool next(Seg& s) {
+    if (pos >= r.hi) return false;
+#pragma unroll 1
+    while (tiles == 0 || pos >= ebase + (tiles + HEAD) * a.Hkv) {
+      if (tiles) ebase += (tiles + HEAD) * a.Hkv;
+      x = entry_of<ROWS>(a, ++e, plans);
+      tiles = tiles_of(x);
+    }
+    s.b = x.b, s.row0 = x.row0, s.nrows = x.nrows, s.held = x.held, s.end = x.end, s.tiles = tiles;
+    s.kvh = (pos - ebase) / (tiles + HEAD);
+    s.pair = e * a.Hkv + s.kvh;
+    s.ps = ebase + s.kvh * (tiles + HEAD);
+    s.t0 = max(0, pos - s.ps - HEAD);
+    s.t1 = min(tiles, r.hi - s.ps - HEAD);
+    s.whole = s.t0 == 0 && s.t1 == tiles;
+    s.slot = pos == r.lo ? 0 : 1;
+    pos = min(r.hi, s.ps + HEAD + tiles);
+    return true;
+  }
+  // the run that holds this place, by the cuts as they were before they moved
+  __device__ __forceinline__ int run_of(int at) const {
+    const int far = at - r.rest * (r.base + 1);
+    return (far < 0 ? 0 : r.rest) + (far < 0 ? at : far) / (far < 0 ? r.base + 1 : r.base);
+  }
+  // the runs that a head's pieces come from, and which of its first run's pieces is the head's
+  __device__ __forceinline__ void pieces_of(const Seg& s, int& c0, int& c1, int& slot0) const {
+    c0 = run_of(s.ps + HEAD), c1 = run_of(s.ps + HEAD + s.tiles - 1);
+    slot0 = c0 * r.base + min(c0, r.rest) >= s.ps ? 0 : 1;
+  }
+};
+
+// The weights of 32 scores and their sum; masked scores are -infinity.
+__device__ __forceinline__ void weights32(const uint32_t (&v)[32], float f, float bias, float2& sum, uint32_t (&p)[16]) {
+  const float2 ff = make_float2(f, f), bb = make_float2(bias, bias);
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    float2 x = __ffma2_rn(make_float2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])), ff, bb);
+    x.x = ex2(x.x), x.y = ex2(x.y);
+    sum = __fadd2_rn(sum, x);
+    p[q] = f16x2(x.x, x.y);
+  }
+}
+__device__ __forceinline__ float max32(const uint32_t (&v)[32], float m) {
+#pragma unroll
+  for (int q = 0; q < 32; q += 2) m = fmaxf(fmaxf(__uint_as_float(v[q]), __uint_as_float(v[q + 1])), m);
+  return m;
+}
+// 32 bytes, a whole sector.
+__device__ __forceinline__ void stg256(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+template <int D, bool PAIR>
+__global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__ Args a) {
+  using L = Lay<D>;
+  constexpr int ROWS = PAIR ? 256 : 128, KS = D / 16, HEAD = Cost<PAIR>::HEAD;
+  constexpr int PIECE = 128 * (D + 2);  // of a stream
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem =
+      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_last[2], s_nan[SM_WARPS][NAN_SETS][D / 16];
+  __shared__ long long s_sum[WARPS];
+  __shared__ int2 s_plan[PLANS];
+  __shared__ Run s_run;
+  // of a tile, in turns of four (the loads are at most two ahead): a byte per 32 keys, not 0: outside the cache
+  __shared__ uint32_t s_bad[4];
+  __shared__ float s_ml[2 * 128];     // not PAIR: the second stream's m and l
+  const uint32_t sbase = smem_u32(smem);
+  auto bar = [&](int i) { return smem_u32(bars + i); };
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      // one arrival a warp, or a commit
+      mbar_init(bar(B_KFULL + i), 4), mbar_init(bar(B_KEMPTY + i), 1);
+      mbar_init(bar(B_VFULL + i), 4), mbar_init(bar(B_VEMPTY + i), 1);
+      mbar_init(bar(B_QFULL + i), 4), mbar_init(bar(B_SFULL + i), 1);
+      mbar_init(bar(B_PFULL + i), 4), mbar_init(bar(B_OFULL + i), 1);
+      mbar_init(bar(B_SOFT + i), PAIR ? 4 : 8);
+    }
+    mbar_init(bar(B_DRAIN), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == W_MMA) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+                 "r"(TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  for (int i = threadIdx.x; i < SM_WARPS * NAN_SETS * (D / 16); i += THREADS) (&s_nan[0][0][0])[i] = 0x7FFFFFFF;
+  if (threadIdx.x == 0) s_run.lo = s_run.hi = 0;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  pdl::trigger();  // every CTA holds its tensor memory before the next kernel's can ask for it
+  pdl::wait();
+
+  // ---- this CTA's run of tiles ----
+  for (int b = threadIdx.x; b < (blockIdx.x == 0 ? a.B : min(a.B, PLANS)); b += THREADS) {
+    int err = 0;
+    const int2 plan = plan_of(a, b, err);
+    if (b < PLANS) s_plan[b] = plan;
+    if (err && blockIdx.x == 0) note_err(nullptr, err);
+  }
+  __syncthreads();
+  const int entries = a.B * a.groups, per = (entries + THREADS - 1) / THREADS;
+  const int e0 = min(entries, (int)threadIdx.x * per), e1 = min(entries, e0 + per);
+  long long own = 0;  // tiles, and in the upper half entries that have any
+#pragma unroll 1
+  for (int e = e0; e < e1; ++e) {
+    const int u = tiles_of(entry_of<ROWS>(a, e, s_plan));
+    own += u ? u + (1ll << 32) : 0;
+  }
+  long long scan = own;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long y = __shfl_up_sync(FULL, scan, d);
+    if (lane >= d) scan += y;
+  }
+  if (lane == 31) s_sum[warp] = scan;
+  __syncthreads();
+  long long total = 0, before = scan - own;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    if (w < warp) before += s_sum[w];
+    total += s_sum[w];
+  }
+  {
+    const int heads = (int)(total >> 32) * a.Hkv, real = (int)total * a.Hkv, all = real + HEAD * heads;
+    const int runs = min((int)gridDim.x, (int)ceilf((float)real / run_least(real, heads)));
+    const int base = runs ? all / runs : 0, rest = all - base * runs;
+    const int cut0 = blockIdx.x * base + min((int)blockIdx.x, rest), cut1 = cut0 + base + ((int)blockIdx.x < rest);
+    int at = ((int)before + HEAD * (int)(before >> 32)) * a.Hkv;
+    const int to = at + ((int)own + HEAD * (int)(own >> 32)) * a.Hkv;
+    if ((int)blockIdx.x < runs) {
+      if ((at <= cut0 && cut0 < to) || (at <= cut1 && cut1 < to)) {
+#pragma unroll 1
+        for (int e = e0; e < e1; ++e) {
+          const int w = tiles_of(entry_of<ROWS>(a, e, s_plan)) + HEAD;
+          if (w == HEAD) continue;
+          auto moved = [&](int cut) {
+            const int ps = at + (cut - at) / w * w;
+            return cut - ps <= HEAD ? ps : cut;
+          };
+          const int next = at + w * a.Hkv;
+          if (at <= cut0 && cut0 < next)
+            s_run.entry = e, s_run.before = at, s_run.base = base, s_run.rest = rest, s_run.lo = moved(cut0);
+          if (at <= cut1 && cut1 < next) s_run.hi = moved(cut1);
+          at = next;
+        }
+      }
+      if (threadIdx.x == 0 && cut1 == all) s_run.hi = all;
+    }
+  }
+  __syncthreads();
+  Segments<ROWS, HEAD> segs(a, s_plan, s_run);
+  Seg sg;
+  // a warp's arrival, its threads' writes before it
+  auto arrive = [&](int b) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(b));
+  };
+
+  if (warp >= W_DQ && warp < W_MMA) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R_DQ));
+    // ---------------- codes to f16: a warp takes 32 keys, K and V in turn ----------------
+    constexpr int LPR = D / 32, PASS = LPR, KPP = 32 / LPR;  // lanes a key, passes, keys a pass
+    const int wq = warp & 3, c = lane % LPR, kr = lane / LPR;
+    uint4 rk[PASS], rv[PASS];
+    uint32_t sk[PASS], sv[PASS];
+    // one tile after the other over all segments: the tile whose page is known (next),
+    // and the one whose codes are on their way (now)
+    bool more = segs.next(sg);
+    int t = sg.t0, set = 0, pid = 0;
+    auto page_of = [&]() {  // of this warp's 32 keys of tile t
+      const int key = min(t * TILE + wq * 32, sg.end - 1);
+      return a.block_table[(int64_t)sg.b * a.width + (key >> a.page_log2)];
+    };
+    struct Now {
+      int64_t row;
+      int key0, end, set;
+      bool bad;
+    } now = {}, nxt = {};
+    auto place = [&](Now& x) {
+      x.key0 = t * TILE + wq * 32, x.end = sg.end, x.set = set;
+      const bool out = pid < 0 || pid >= a.pages;
+      x.bad = out && x.key0 < x.end;
+      if (x.bad) note_err(nullptr, ERR_PAGE);
+      x.row = (((int64_t)(out ? 0 : pid) * a.Hkv + sg.kvh) << a.page_log2) + (x.key0 & ((1 << a.page_log2) - 1));
+      // the caches' lines on their way to L2 a tile ahead of the loads
+      if (lane < 4) {
+        const uint8_t* p = lane == 0   ? a.k_codes + x.row * (D / 2)
+                           : lane == 1 ? a.v_codes + x.row * (D / 2)
+                           : lane == 2 ? a.k_scale + x.row * (D / 16)
+                                       : a.v_scale + x.row * (D / 16);
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(lane < 2 ? 16 * D : 2 * D) : "memory");
+      }
+    };
+    auto step = [&]() {  // on to the next tile
+      if (++t == sg.t1) {
+        more = segs.next(sg);
+        if (more) t = sg.t0;
+        set = set == NAN_SETS - 1 ? 0 : set + 1;
+      }
+      if (more) pid = page_of();
+    };
+    auto load = [&](const Now& x, const uint8_t* codes, const uint8_t* scales, uint4 (&raw)[PASS], uint32_t (&sc)[PASS]) {
+#pragma unroll
+      for (int p = 0; p < PASS; ++p) {
+        const int k = p * KPP + kr;
+        // volatile: issued here, a tile's time before they are used
+        asm volatile("ld.global.nc.v4.b32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(raw[p].x), "=r"(raw[p].y), "=r"(raw[p].z), "=r"(raw[p].w)
+                     : "l"(codes + (x.row + k) * (D / 2) + 16 * c));
+        uint16_t e;
+        asm volatile("ld.global.nc.b16 %0, [%1];" : "=h"(e) : "l"(scales + (x.row + k) * (D / 16) + 2 * c));
+        sc[p] = e;
+      }
+    };
+    auto convert = [&](uint32_t dst, const uint4& raw, uint32_t s2, int k) {
+      const int r = wq * 32 + k;
+      uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+      const uint32_t ss = unpack2(s2);
+      uint32_t s0 = __byte_perm(ss, ss, 0x1010), s1 = __byte_perm(ss, ss, 0x3232);
+      // lanes of the row's second half go through their chunks in another order:
+      // the eight lanes that store together then meet eight different groups of banks
+      const int turn = D == 128 ? c & 2 : 0;
+      if (turn) {
+        uint32_t x = w[0];
+        w[0] = w[2], w[2] = x;
+        x = w[1], w[1] = w[3], w[3] = x;
+        x = s0, s0 = s1, s1 = x;
+      }
+      const uint32_t rowp = dst + (D == 128 ? (c >> 1) * L::HALF : 0) + r * 128;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t h[4];
+        e2m1_f16(w[i], h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = mul_f16x2(h[j], i < 2 ? s0 : s1);
+        const int chunk = (c & 1) * 4 + (i ^ turn);
+        sts128(rowp + ((chunk ^ (r & 7)) << 4), h[0], h[1], h[2], h[3]);
+      }
+    };
+    if (more) {
+      int buf = 0, turn4 = 0;
+      uint32_t phase = 0;
+      pid = page_of();
+      place(now);
+      load(now, a.k_codes, a.k_scale, rk, sk);
+      load(now, a.v_codes, a.v_scale, rv, sv);
+      step();
+      bool last = !more;
+      if (!last) place(nxt), step();
+      while (true) {
+        if (!mbar_wait_warp(bar(B_KEMPTY + buf), phase ^ 1, nullptr, ERR_WAIT)) break;
+        if (lane == 0) reinterpret_cast<uint8_t*>(s_bad + turn4)[wq] = now.bad;
+        turn4 = (turn4 + 1) & 3;
+#pragma unroll
+        for (int p = 0; p < PASS; ++p) convert(sbase + L::OFF_K + buf * L::TILE_BYTES, rk[p], sk[p], p * KPP + kr);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        arrive(B_KFULL + buf);
+        if (!last) load(nxt, a.k_codes, a.k_scale, rk, sk);
+
+        if (!mbar_wait_warp(bar(B_VEMPTY + buf), phase ^ 1, nullptr, ERR_WAIT)) break;
+#pragma unroll
+        for (int p = 0; p < PASS; ++p) {
+          const int k = p * KPP + kr;
+          uint32_t s2 = sv[p];
+          if (now.key0 + k >= now.end || now.bad) s2 = 0;  // no token of this sequence
+          const uint32_t odd = ((s2 & 0x7F7Fu) + 0x0101u) & 0x8080u;
+          if (odd) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (odd >> (8 * h) & 0x80u) {
+                for (int w = 0; w < SM_WARPS; ++w) atomicMin(&s_nan[w][now.set][2 * c + h], now.key0 + k);
+                s2 &= ~(0xFFu << (8 * h));
+              }
+          }
+          convert(sbase + L::OFF_V + buf * L::TILE_BYTES, rv[p], s2, k);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        arrive(B_VFULL + buf);
+        if (last) break;
+        load(nxt, a.v_codes, a.v_scale, rv, sv);
+        now = nxt;
+        last = !more;
+        if (!last) place(nxt), step();
+        if (++buf == 2) buf = 0, phase ^= 1;
+      }
+    }
+  } else if (warp >= W_MMA) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R_REST));
+    if (warp == W_MMA) {
+      // ---------------- MMA issuer ----------------
+      // The whole warp runs the loop and one lane issues: the operands then stay in
+      // uniform registers.
+      constexpr uint32_t ID_S = idesc_f16(128, false), ID_O = idesc_f16(D, true);
+      const uint64_t dq = sw128_desc(sbase + L::OFF_Q), dk = sw128_desc(sbase + L::OFF_K),
+                     dv = mn_desc(sbase + L::OFF_V, L::HALF);
+      constexpr uint32_t TILE16 = L::TILE_BYTES / 16;
+      int kb = 0, vb = 0;
+      uint32_t kph = 0, vph = 0, qph = 0, pph = 0;  // of the streams: bits 0 and 1
+      bool ok = true;
+      // S of stream i from K buffer kb; `release`: its last reader
+      auto scores = [&](int i, bool release) {
+        if (elect_one()) {
+          const uint64_t q = desc_at(dq, i * TILE16), k = desc_at(dk, kb * TILE16);
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            const uint32_t off = ((s >> 2) * L::HALF + (s & 3) * 32) / 16;
+            mma_ss(tmem + COL_S + i * 128, desc_at(q, off), desc_at(k, off), ID_S, s > 0);
+          }
+          tc_commit(bar(B_SFULL + i));
+          if (release) tc_commit(bar(B_KEMPTY + kb));
+        }
+        __syncwarp();
+        if (release && ++kb == 2) kb = 0, kph ^= 1;
+      };
+      // O of stream i from V buffer vb; `last`: of the segment
+      auto values = [&](int i, bool first, bool release, bool last) {
+        if (elect_one()) {
+          const uint64_t v = desc_at(dv, vb * TILE16);
+#pragma unroll
+          for (int s = 0; s < TILE / 16; ++s)
+            mma_ts(tmem + COL_O + i * 128, tmem + COL_S + i * 128 + s * 8, desc_at(v, s * 128), ID_O, !first || s > 0);
+          if (release) tc_commit(bar(B_VEMPTY + vb));
+          if (last) tc_commit(bar(B_OFULL + i));
+        }
+        __syncwarp();
+        if (release && ++vb == 2) vb = 0, vph ^= 1;
+      };
+      auto wait = [&](int b, uint32_t ph) {
+        ok = ok && mbar_wait_warp(bar(b), ph, nullptr, ERR_WAIT);
+        tc_fence_after();
+        return ok;
+      };
+      auto take = [&](int b, int i, uint32_t& ph) {
+        const bool r = wait(b + i, ph >> i & 1);
+        ph ^= 1u << i;
+        return r;
+      };
+      while (ok && segs.next(sg)) {
+        const int n = sg.t1 - sg.t0;
+        if (PAIR) {
+          if (!wait(B_KFULL + kb, kph) || !take(B_QFULL, 0, qph)) break;
+          scores(0, false);
+          if (!take(B_QFULL, 1, qph)) break;
+          scores(1, true);
+          for (int j = 0; j < n; ++j) {
+            const bool again = j + 1 < n;
+            if (!take(B_PFULL, 0, pph) || !wait(B_VFULL + vb, vph)) break;
+            values(0, j == 0, false, !again);
+            if (again) {
+              if (!wait(B_KFULL + kb, kph)) break;
+              scores(0, false);
+            }
+            if (!take(B_PFULL, 1, pph)) break;
+            values(1, j == 0, true, !again);
+            if (again) scores(1, true);
+          }
+        } else {
+          if (!take(B_QFULL, 0, qph) || !take(B_QFULL, 1, qph)) break;
+          for (int j = 0; j < min(n, 2); ++j) {
+            if (!wait(B_KFULL + kb, kph)) break;
+            scores(j, true);
+          }
+          for (int j = 0; j < n && ok; ++j) {
+            const int i = j & 1;
+            if (!take(B_PFULL, i, pph) || !wait(B_VFULL + vb, vph)) break;
+            values(i, j < 2, true, j + 2 >= n);
+            if (j + 2 < n) {
+              if (!wait(B_KFULL + kb, kph)) break;
+              scores(i, true);
+            }
+          }
+        }
+      }
+      // every MMA issued has completed before the TMEM is released
+      if (elect_one()) {
+        tc_commit(bar(B_DRAIN));
+        mbar_wait(bar(B_DRAIN), 0, nullptr, ERR_WAIT);
+      }
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R_SOFT));
+    // ---------------- softmax, and the ends of segments ----------------
+    const int i = warp >> 2, wq = warp & 3, r = wq * 32 + lane;  // stream, its row
+    const int first = PAIR ? i * 128 : 0;                        // of the stream's rows in the tile
+    const uint32_t tq = tmem + ((uint32_t)(wq * 32) << 16);
+    const uint32_t ts = tq + COL_S + i * 128, to = tq + COL_O + i * 128;
+    const uint32_t sq = sbase + L::OFF_Q + i * L::TILE_BYTES;
+    uint32_t sph = 0, oph = 0, softph = 0;
+    int set = 0, turn4 = 0;  // of s_nan; of s_bad, at the segment's first tile
+    bool ok = true;
+    // the threads that end a segment together: a stream's, or both streams'; bounded, as every wait
+    auto soft_sync = [&]() {
+      arrive(B_SOFT + (PAIR ? i : 0));
+      ok = mbar_wait_warp(bar(B_SOFT + (PAIR ? i : 0)), softph, nullptr, ERR_WAIT);
+      softph ^= 1;
+      return ok;
+    };
+    // A segment's rows: this thread's token and head, and whether they are there.
+    struct Row {
+      int tok, head;
+      bool live, exists;
+    };
+    auto row_of = [&](const Seg& s) {
+      Row x;
+      const int at = s.row0 + first + r;
+      x.tok = at / a.G, x.head = s.kvh * a.G + at - x.tok * a.G;
+      x.live = first + r < s.nrows, x.exists = at < a.T * a.G;
+      return x;
+    };
+    // The queries as they lie, to their place in shared memory: a warp's 32 rows,
+    // some at a time, 16 bytes a lane.
+    auto fetch_q = [&](const Seg& s, const Row& x) {
+      const int64_t off = (int64_t)s.b * a.qb + (int64_t)x.tok * a.qt + (int64_t)x.head * a.qh;
+      constexpr int CH = D / 8, PER = 32 / CH;  // chunks a row, rows a step
+      const int ch = lane % CH;
+      const uint32_t there = __ballot_sync(FULL, x.live);
+#pragma unroll
+      for (int k = 0; k < 32 / PER; ++k) {
+        const int rr = k * PER + lane / CH;
+        const int64_t o = __shfl_sync(FULL, off, rr);
+        const uint32_t dst = sq + (ch >> 3) * L::HALF + (wq * 32 + rr) * 128 + (((ch & 7) ^ (rr & 7)) << 4);
+        if (there >> rr & 1u)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(a.q + o + ch * 8) : "memory");
+        else
+          sts128(dst, 0, 0, 0, 0);
+      }
+    };
+    // ... and in f16, scaled by the row's power of two; a negative scale turns them.
+    // Returns the scores' factor: that power of two, the scale and the keys' factor;
+    // never 0, so that a masked score stays -infinity.
+    auto finish_q = [&](float scale) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
+      uint32_t m = 0;
+#pragma unroll
+      for (int q = 0; q < D / 8; ++q) {
+        const uint4 v = lds128(sq + (q >> 3) * L::HALF + r * 128 + (((q & 7) ^ (r & 7)) << 4));
+        m = __vmaxu2(m, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu),
+                                 __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
+      }
+      m = max(m & 0xFFFFu, m >> 16);
+      const int e = min(max((int)(m >> 7), 15), 253);  // the largest value's exponent field
+      const float up = copysignf(__uint_as_float((uint32_t)(254 + 14 - e) << 23), scale);
+#pragma unroll
+      for (int q = 0; q < D / 8; ++q) {
+        const uint32_t at = sq + (q >> 3) * L::HALF + r * 128 + (((q & 7) ^ (r & 7)) << 4);
+        const uint4 v = lds128(at);
+        sts128(at, f16x2(bf_lo(v.x) * up, bf_hi(v.x) * up), f16x2(bf_lo(v.y) * up, bf_hi(v.y) * up),
+               f16x2(bf_lo(v.z) * up, bf_hi(v.z) * up), f16x2(bf_lo(v.w) * up, bf_hi(v.w) * up));
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      arrive(B_QFULL + i);
+      const float f = fmaxf(__uint_as_float((uint32_t)(e - 14) << 23) * fabsf(scale), 1.17549435e-38f);
+      return scale != scale ? scale : f;
+    };
+
+    // row tiles without a query are written here: no tile of keys belongs to them
+#pragma unroll 1
+    for (int e = blockIdx.x; e < entries; e += gridDim.x) {
+      const Entry x = entry_of<ROWS>(a, e, s_plan);
+      if (x.nrows > 0) continue;
+      const int rows = min(ROWS, a.T * a.G - x.row0);
+      for (int64_t n = threadIdx.x; n < (int64_t)rows * a.Hkv * (D / 8); n += SOFT) {
+        const int q = (int)(n / (D / 8)), rr = x.row0 + q % rows, h = q / rows;
+        reinterpret_cast<uint4*>(a.out + (((int64_t)x.b * a.T + rr / a.G) * a.H + h * a.G + rr % a.G) * D)[n % (D / 8)] =
+            make_uint4(0, 0, 0, 0);
+      }
+    }
+
+    bool more = segs.next(sg);
+    Row x = {};
+    float f = 0.0f, scale = 0.0f;
+    if (more) {
+      x = row_of(sg);
+      scale = a.sm_log2 * __ldg(a.k_factor + sg.kvh);
+      fetch_q(sg, x);
+      f = finish_q(scale);
+    }
+    while (more) {
+      const Seg cur = sg;
+      const Row now = x;
+      const float vf = __ldg(a.v_factor + cur.kvh);
+      more = segs.next(sg);
+      if (more) {
+        x = row_of(sg);
+        scale = a.sm_log2 * __ldg(a.k_factor + sg.kvh);
+      }
+      const int limit = now.live ? cur.held + now.tok : -1;  // the last key that the row sees
+      // keys below: every row of the warp sees them (rows without a query do not count)
+      const int free_end = min(__reduce_min_sync(FULL, now.live ? limit : 0x7FFFFFFE), 0x7FFFFFFE) + 1;
+      const bool any_live = __any_sync(FULL, now.live);
+      float m = NEG_INF, l = 0.0f;
+      const int n = cur.t1 - cur.t0;
+      bool any = false;  // this stream has had a tile
+      for (int j = PAIR ? 0 : i; j < n; j += PAIR ? 1 : 2) {
+        if (!(ok = mbar_wait_warp(bar(B_SFULL + i), sph, nullptr, ERR_WAIT))) break;
+        sph ^= 1;
+        tc_fence_after();
+        // the last scores are there, so the queries' place is free: the next ones travel under this tile
+        if (PAIR && j + 1 == n && more) fetch_q(sg, x);
+        if (any_live) {
+          uint32_t va[32], vb[32], vc[32], vd[32], p[16];
+          tmem_ld32(ts, va);
+          tmem_ld32(ts + 32, vb);
+          const int key0 = (cur.t0 + j) * TILE;
+          const uint32_t bad = s_bad[(turn4 + j) & 3];
+          const bool masked = key0 + TILE > free_end || bad;
+          // -infinity where the key lies past the row's last, or in no page
+          auto mask32 = [&](uint32_t (&v)[32], int c) {
+            const int stay = bad >> (8 * c) & 0xFFu ? 0 : limit + 1 - key0 - 32 * c;
+#pragma unroll
+            for (int q = 0; q < 32; ++q) v[q] = q < stay ? v[q] : 0xFF800000u;
+          };
+          tmem_ld_wait();
+          tmem_ld32(ts + 64, vc);
+          tmem_ld32(ts + 96, vd);
+          if (masked) mask32(va, 0), mask32(vb, 1);
+          float mx = fmaxf(max32(va, NEG_INF), max32(vb, NEG_INF));
+          tmem_ld_wait();
+          if (masked) mask32(vc, 2), mask32(vd, 3);
+          mx = fmaxf(mx, fmaxf(max32(vc, NEG_INF), max32(vd, NEG_INF)));
+          const float top = mx == NEG_INF ? NEG_INF : mx * f;
+          if (__any_sync(FULL, top > m + LAG)) {
+            const float mn = fmaxf(m, top), corr = mn == NEG_INF ? 1.0f : ex2(m - mn);
+            m = mn;
+            l *= corr;
+            if (any) {
+#pragma unroll 1
+              for (int c = 0; c < D / 16; ++c) {
+                uint32_t o[16];
+                tmem_ld16(to + 16 * c, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int q = 0; q < 16; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * corr);
+                tmem_st16(to + 16 * c, o);
+              }
+            }
+          }
+          const float bias = m == NEG_INF ? P_EXP : P_EXP - m;
+          float2 sum = make_float2(0.0f, 0.0f);
+          weights32(va, f, bias, sum, p);
+          tmem_st16(ts, p);
+          weights32(vb, f, bias, sum, p);
+          tmem_st16(ts + 16, p);
+          weights32(vc, f, bias, sum, p);
+          tmem_st16(ts + 32, p);
+          weights32(vd, f, bias, sum, p);
+          tmem_st16(ts + 48, p);
+          l += sum.x + sum.y;
+          tmem_st_wait();
+          any = true;
+        }
+        tc_fence_before();
+        arrive(B_PFULL + i);
+      }
+      if (!ok) break;
+      if (PAIR && more) f = finish_q(scale);  // while the last product runs
+      turn4 = (turn4 + n) & 3;
+      const bool had = PAIR || i < n;  // this stream's O has been written
+      if (had) {
+        if (!(ok = mbar_wait_warp(bar(B_OFULL + i), oph, nullptr, ERR_WAIT))) break;
+        oph ^= 1;
+        tc_fence_after();
+      }
+      // ---- the end of a segment ----
+      uint16_t* orow = a.out + (((int64_t)cur.b * a.T + now.tok) * a.H + now.head) * D;
+      const bool writer = PAIR || i == 0;
+      float ow = 1.0f, xw = 0.0f;  // weights of this stream's O and of the other's
+      const float4* other = reinterpret_cast<const float4*>(smem + L::OFF_Q);
+      if (!PAIR) {  // the second stream's sums to the first, through the queries' place
+        if (i == 1) {
+          s_ml[r] = m, s_ml[128 + r] = l;
+          if (had && any_live)
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t v[32];
+              tmem_ld32(to + 32 * c, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                sts128(smem_u32(other + r * (D / 4) + ((8 * c + q) ^ (r & 7))), v[4 * q], v[4 * q + 1], v[4 * q + 2],
+                       v[4 * q + 3]);
+            }
+        }
+        if (!soft_sync()) break;
+        if (i == 0 && n > 1) {
+          const float m1 = s_ml[r], mn = fmaxf(m, m1), ref = mn == NEG_INF ? 0.0f : mn;
+          ow = ex2(m - ref), xw = ex2(m1 - ref);
+          l = l * ow + s_ml[128 + r] * xw;
+          m = mn;
+        }
+      }
+      const float of = l == 0.0f ? 0.0f : __fdiv_rn(vf, l);
+      float* piece = a.part + (((int64_t)blockIdx.x * 2 + cur.slot) * (PAIR ? 2 : 1) + (PAIR ? i : 0)) * PIECE;
+      if (writer && any_live) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t v[32];
+          tmem_ld32(to + 32 * c, v);
+          tmem_ld_wait();
+          if (!PAIR && n > 1) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+              const float4 y = other[r * (D / 4) + ((8 * c + q) ^ (r & 7))];
+              v[4 * q] = __float_as_uint(__uint_as_float(v[4 * q]) * ow + y.x * xw);
+              v[4 * q + 1] = __float_as_uint(__uint_as_float(v[4 * q + 1]) * ow + y.y * xw);
+              v[4 * q + 2] = __float_as_uint(__uint_as_float(v[4 * q + 2]) * ow + y.z * xw);
+              v[4 * q + 3] = __float_as_uint(__uint_as_float(v[4 * q + 3]) * ow + y.w * xw);
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (s_nan[warp][set][2 * c + h] <= limit)
+#pragma unroll
+              for (int q = 0; q < 16; ++q) v[16 * h + q] = 0x7FC00000u;
+          if (now.live) {
+            if (cur.whole) {
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                uint32_t w[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  w[k] = bf_pack(__uint_as_float(v[16 * q + 2 * k]) * of, __uint_as_float(v[16 * q + 2 * k + 1]) * of);
+                stg256(orow + 32 * c + 16 * q, w);
+              }
+            } else {
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                reinterpret_cast<uint4*>(piece)[(8 * c + q) * 128 + r] =
+                    make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+            }
+          }
+        }
+      }
+      auto blank = [&]() {  // a row without a query
+#pragma unroll
+        for (int q = 0; q < D / 8; ++q) reinterpret_cast<uint4*>(orow)[q] = make_uint4(0, 0, 0, 0);
+      };
+      if (cur.whole) {
+        if (writer && !now.live && now.exists) blank();
+      } else {
+        if (writer && now.live) piece[128 * D + r] = m, piece[128 * (D + 1) + r] = l;
+        // the stream that finishes last reads the head's pieces in the CTAs' order
+        int c0, c1, slot0;
+        segs.pieces_of(cur, c0, c1, slot0);
+        const int pieces = c1 - c0 + 1, me = PAIR ? i : 0;
+        int* done = a.done + (PAIR ? 2 * cur.pair + i : cur.pair);
+        if (!soft_sync()) break;
+        if (threadIdx.x == (PAIR ? 128 * i : 0)) {
+          int k;  // releases every thread's stores, which the barrier has ordered before it
+          asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(k) : "l"(done) : "memory");
+          s_last[me] = k == pieces - 1;
+        }
+        if (!soft_sync()) break;
+        if (s_last[me]) {
+          auto at_piece = [&](int p) {
+            return a.part + (((int64_t)(c0 + p) * 2 + (p == 0 ? slot0 : 0)) * (PAIR ? 2 : 1) + me) * PIECE;
+          };
+          // A warp takes 32 rows and every WPB-th group of four columns, four groups at a time.
+          const int rows = min(128, cur.nrows - first), blocks = max(1, (rows + 31) / 32);
+          constexpr int W = PAIR ? 4 : 8;
+          const int w = PAIR ? wq : warp, wpb = W / (blocks == 3 ? 4 : blocks), blk = w / wpb;
+          const int rr = blk * 32 + lane, at = cur.row0 + first + rr;
+          const bool there = rr < rows;
+          const int tok = at / a.G, head = cur.kvh * a.G + at - tok * a.G;
+          uint16_t* dst = a.out + (((int64_t)cur.b * a.T + tok) * a.H + head) * D;
+          if (there) {
+            float mm = NEG_INF, ll = 0.0f;
+            for (int p0 = 0; p0 < pieces; p0 += 4) {
+              float pm[4], pl[4], mn = mm;
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {  // beyond the last: that one's maximum again, no sum
+                const float* src = at_piece(min(p0 + q, pieces - 1)) + 128 * D + rr;
+                pm[q] = __ldcg(src), pl[q] = p0 + q < pieces ? __ldcg(src + 128) : 0.0f;
+              }
+#pragma unroll
+              for (int q = 0; q < 4; ++q) mn = fmaxf(mn, pm[q]);
+              const float ref = mn == NEG_INF ? 0.0f : mn;
+              ll *= ex2(mm - ref);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) ll = fmaf(pl[q], ex2(pm[q] - ref), ll);
+              mm = mn;
+            }
+            const float ref = mm == NEG_INF ? 0.0f : mm, g = ll == 0.0f ? 0.0f : __fdiv_rn(vf, ll);
+#pragma unroll 1
+            for (int g0 = w % wpb; g0 < D / 4; g0 += 4 * wpb) {
+              float4 acc[4] = {};
+#pragma unroll 1
+              for (int p0 = 0; p0 < pieces; p0 += 2) {
+                float4 y[2][4];
+                float pm[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  const float* src = at_piece(min(p0 + k, pieces - 1));
+                  pm[k] = __ldcg(src + 128 * D + rr);
+#pragma unroll
+                  for (int q = 0; q < 4; ++q)
+                    y[k][q] = __ldcg(reinterpret_cast<const float4*>(src) + min(g0 + q * wpb, D / 4 - 1) * 128 + rr);
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                  if (p0 + k < pieces) {
+                    const float e = ex2(pm[k] - ref);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                      acc[q].x = fmaf(y[k][q].x, e, acc[q].x), acc[q].y = fmaf(y[k][q].y, e, acc[q].y);
+                      acc[q].z = fmaf(y[k][q].z, e, acc[q].z), acc[q].w = fmaf(y[k][q].w, e, acc[q].w);
+                    }
+                  }
+              }
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                if (g0 + q * wpb < D / 4)
+                  *reinterpret_cast<uint2*>(dst + 4 * (g0 + q * wpb)) =
+                      make_uint2(bf_pack(acc[q].x * g, acc[q].y * g), bf_pack(acc[q].z * g, acc[q].w * g));
+            }
+          }
+          if (writer && !now.live && now.exists) blank();
+          if (threadIdx.x == (PAIR ? 128 * i : 0)) *done = 0;
+        }
+      }
+      // the set of NaNs is for another segment
+      __syncwarp();
+      if (lane < D / 16) s_nan[warp][set][lane] = 0x7FFFFFFF;
+      set = set == NAN_SETS - 1 ? 0 : set + 1;
+      if (!PAIR) {
+        if (!soft_sync()) break;  // the queries' place was read
+        if (more) {
+          fetch_q(sg, x);
+          f = finish_q(scale);
+        }
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == W_MMA) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
+  }
+}
+
+// How a call's work is cut: rows a tile, row tiles of a sequence, and CTAs.
+struct Cut {
+  int rows, groups, ctas;
+};
+static Cut cut_of(int64_t batch, int64_t tokens, int heads, int kv_heads, int64_t capacity) {
+  const int64_t rows = tokens * (heads / kv_heads);
+  Cut c;
+  c.rows = rows > 128 ? 256 : 128;
+  c.groups = (int)((rows + c.rows - 1) / c.rows);
+  const int64_t tiles = std::max<int64_t>(1, (capacity + TILE - 1) / TILE);
+  c.ctas = (int)std::min<int64_t>(vq::mx::sm_count(), std::max<int64_t>(1, batch) * c.groups * kv_heads * tiles);
+  return c;
+}
+
+void workspace(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim, int64_t capacity, int64_t* floats,
+               int64_t* counters) {
+  const Cut c = cut_of(batch, tokens, heads, kv_heads, capacity);
+  *counters = batch * kv_heads * c.groups * (c.rows / 128);
+  *floats = (int64_t)c.ctas * 2 * c.rows * (head_dim + 2);
+}
+
+template <int D, bool PAIR>
+static int launch(const Args& a, int ctas, cudaStream_t st) {
+  if (!allow_smem<k_attn_kv4<D, PAIR>>(Lay<D>::SMEM)) return VQ_ERR_CUDA;
+  // the registers that the split takes up have to be there at the launch
+  static const int regs = [] {
+    cudaFuncAttributes at;
+    return cudaFuncGetAttributes(&at, k_attn_kv4<D, PAIR>) == cudaSuccess ? at.numRegs : 0;
+  }();
+  if (regs < R_LAUNCH) return VQ_ERR_CUDA;
+  return pdl::launch<k_attn_kv4<D, PAIR>>(ctas, THREADS, Lay<D>::SMEM, st, 1, a) ? VQ_OK : VQ_ERR_CUDA;
+}
+
+// Checked arguments (vq_attn_kv4), but for the sizes of the workspaces.
+int attend(const void* q, const int64_t* q_strides, int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim,
+           const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, const float* k_factor,
+           const float* v_factor, int64_t pages, int page, const void* block_table, int64_t table_width,
+           const void* lengths, const void* counts, float sm_scale, float* workspace, int64_t workspace_floats,
+           int32_t* counters, int64_t counters_len, void* out, cudaStream_t st) {
+  const int64_t capacity = table_width * page;
+  const Cut c = cut_of(batch, tokens, heads, kv_heads, capacity);
+  const int64_t pairs = batch * kv_heads * c.groups;
+  // the tiles of all heads, counted in 32 bits
+  if (pairs * ((capacity + TILE - 1) / TILE + 3) >= (1ll << 31) || counters_len < pairs * (c.rows / 128)) return VQ_ERR_INVALID;
+  if (!workspace || workspace_floats < (int64_t)c.ctas * 2 * c.rows * (head_dim + 2)) return VQ_ERR_INVALID;
+  Args a;
+  a.q = (const uint16_t*)q;
+  a.qb = q_strides[0], a.qt = q_strides[1], a.qh = q_strides[2];
+  a.out = (uint16_t*)out;
+  a.k_codes = (const uint8_t*)k_codes, a.v_codes = (const uint8_t*)v_codes;
+  a.k_scale = (const uint8_t*)k_scale, a.v_scale = (const uint8_t*)v_scale;
+  a.k_factor = k_factor, a.v_factor = v_factor;
+  a.block_table = (const int32_t*)block_table;
+  a.lengths = (const int32_t*)lengths;
+  a.counts = (const int32_t*)counts;
+  a.part = workspace;
+  a.done = counters;
+  a.B = (int)batch, a.T = (int)tokens, a.H = heads, a.Hkv = kv_heads, a.G = heads / kv_heads;
+  a.page_log2 = page == 32 ? 5 : page == 64 ? 6 : 7;
+  a.width = (int)table_width, a.pages = (int)pages, a.groups = c.groups;
+  a.sm_log2 = sm_scale * 1.4426950408889634f;
+  if (head_dim == 128) return c.rows == 256 ? launch<128, true>(a, c.ctas, st) : launch<128, false>(a, c.ctas, st);
+  return c.rows == 256 ? launch<64, true>(a, c.ctas, st) : launch<64, false>(a, c.ctas, st);
+}
+
+// This file's sticky word (vq_device_errors).
+int sticky_kv4(int* out, int clear, cudaStream_t st) { return vq::tc::sticky_read(out, clear, st); }
+
+}  // namespace kv4
+}  // namespace vq

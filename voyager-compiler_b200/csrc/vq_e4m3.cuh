@@ -1,5 +1,5 @@
-// E4M3 bytes to and from float, and the small reductions shared by the
-// float32-scaled E4M3 kernels (norm, linear, key / value cache).
+// E4M3 bytes to and from float, E2M1 codes to f16, and the element types shared
+// by the kernels of a decoding step (norm, linear, key / value caches).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -35,6 +35,19 @@ __device__ __forceinline__ uint32_t unpack2_hi(uint32_t w) {
   asm("{\n\t.reg .b16 t, u;\n\tmov.b32 {t, u}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, u;\n\t}"
       : "=r"(h) : "r"(w));
   return h;
+}
+// Four bytes of two E2M1 codes each as f16 pairs (exact), the low halves first.
+__device__ __forceinline__ void e2m1_f16(uint32_t w, uint32_t (&h)[4]) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+}
+// A code times a scale: 2 by 4 significant bits within 2^-10 .. 2688, exact in f16.
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 __device__ __forceinline__ float2 half2f(uint32_t h) {
   return __half22float2(*reinterpret_cast<__half2*>(&h));

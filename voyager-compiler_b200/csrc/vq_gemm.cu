@@ -1265,6 +1265,9 @@ int sticky_kv(int* out, int clear, cudaStream_t st);
 namespace kva {
 int sticky_kva(int* out, int clear, cudaStream_t st);
 }
+namespace kv4 {
+int sticky_kv4(int* out, int clear, cudaStream_t st);
+}
 namespace f8 {
 int sticky_f8(int* out, int clear, cudaStream_t st);
 }
@@ -1546,17 +1549,18 @@ int vq_linear_mxf8_noalloc_status(int32_t* code, void* stream) {
 int vq_device_errors(int32_t* code, int32_t clear, void* stream) {
   if (!code) return VQ_ERR_NULL;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  int v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  int v[9] = {};
   if (vq::tc::sticky_read(&v[0], clear, s) || vq::dq::sticky_dq(&v[1], clear, s) ||
       vq::tp::sticky_tp(&v[2], clear, s) || vq::attn::sticky_attn(&v[3], clear, s) ||
       vq::w4::sticky_w4(&v[4], clear, s) || vq::kv::sticky_kv(&v[5], clear, s) ||
-      vq::kva::sticky_kva(&v[6], clear, s) || vq::f8::sticky_f8(&v[7], clear, s))
+      vq::kva::sticky_kva(&v[6], clear, s) || vq::f8::sticky_f8(&v[7], clear, s) ||
+      vq::kv4::sticky_kv4(&v[8], clear, s))
     return VQ_ERR_CUDA;
   // the first nonzero word: MXFP8 GEMM 1-4, bf16 GEMM 11-14, W4A8 21-23,
   // tensor-parallel barrier 100 + rank, attention 200 + its code, key / value
-  // cache 301-303 and 311-314, E4M3 linear 321-324
+  // cache 301-303, 311-314 and 331-334, E4M3 linear 321-324
   *code = v[0] ? v[0] : (v[1] ? v[1] : (v[4] ? v[4] : (v[2] ? v[2] : (v[3] ? 200 + v[3] : 0))));
-  for (int i = 5; i < 8; ++i)
+  for (int i = 5; i < 9; ++i)
     if (!*code) *code = v[i];
   return VQ_OK;
 }

@@ -39,6 +39,6 @@ def check_errors(device=None, clear: bool = True) -> None:
                    "vq_device_errors")
     if code.value:
         what = ("a key / value cache plan did not fit (a length, count or page out of range)"
-                if code.value in (301, 302, 303, 312, 313, 314) else "a bounded device wait gave up")
+                if code.value in (301, 302, 303, 312, 313, 314, 332, 333, 334) else "a bounded device wait gave up")
         raise _lib.VqError(f"{what} on {dev} (code {code.value}): "
                            "the results of that launch are incomplete")
