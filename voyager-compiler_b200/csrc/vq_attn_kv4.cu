@@ -56,9 +56,9 @@ enum { ERR_WAIT = 331, ERR_PAGE = 332, ERR_CAPACITY = 333, ERR_COUNT = 334 };
 
 constexpr int TILE = 128;  // keys
 constexpr int PLANS = 128;
-// warps: 0-7 softmax (a stream's four each), 8-11 codes to f16, 12 the MMAs, 13-15 none (a warpgroup's registers are
-// split together)
-constexpr int SM_WARPS = 8, W_DQ = 8, W_MMA = 12, WARPS = 16, THREADS = WARPS * 32;
+// warps: 0-7 softmax (a stream's four each), 8-11 codes to f16, 12 the MMAs, 13 where the tiles lie, 14 and 15 none
+// (a warpgroup's registers are split together)
+constexpr int SM_WARPS = 8, W_DQ = 8, W_MMA = 12, W_SCOUT = 13, WARPS = 16, THREADS = WARPS * 32;
 // registers a thread: launched with 128; a warpgroup of 4 warps gives some up or takes them
 constexpr int R_LAUNCH = 128, R_SOFT = 184, R_DQ = 80, R_REST = 64;
 static_assert(2 * R_SOFT + R_DQ + R_REST <= 4 * R_LAUNCH, "a register taken was given up before");
@@ -68,7 +68,11 @@ constexpr float P_EXP = 7.0f, LAG = 8.0f;
 constexpr int NAN_SETS = 3;  // a segment's, of which the epilogue of one and the loads of two more can be under way
 
 enum { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_VEMPTY = 6, B_QFULL = 8, B_SFULL = 10, B_PFULL = 12, B_OFULL = 14,
-       B_SOFT = 16, B_DRAIN = 18, NBARS = 19 };
+       B_SOFT = 16, B_DRAIN = 18, B_TFULL = 20, B_TEMPTY = 24, NBARS = 28 };
+// tiles whose places are known, and words of pages outside the cache (of a tile until its softmax has begun: the two in
+// the buffers and those known)
+constexpr int TURNS = 4, BAD_TURNS = 16;
+constexpr uint32_t NO_TILE = 0xFFFFFFFFu;
 
 constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_O = 256;  // stream i: S at 128 i, O at 256 + 128 i
 
@@ -246,15 +250,21 @@ struct Segments {
   }
 };
 
-// The weights of 32 scores and their sum; masked scores are -infinity.
-__device__ __forceinline__ void weights32(const uint32_t (&v)[32], float f, float bias, float2& sum, uint32_t (&p)[16]) {
+// The weights of 32 scores and their sum; masked scores are -infinity.  All the
+// exponentials first: their results come some 40 cycles after they are asked for.
+__device__ __forceinline__ void weights32(uint32_t (&v)[32], float f, float bias, float2& sum, uint32_t (&p)[16]) {
   const float2 ff = make_float2(f, f), bb = make_float2(bias, bias);
+  float e[32];
+#pragma unroll
+  for (int q = 0; q < 32; q += 2) {
+    const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[q]), __uint_as_float(v[q + 1])), ff, bb);
+    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[q]) : "f"(x.x));
+    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[q + 1]) : "f"(x.y));
+  }
 #pragma unroll
   for (int q = 0; q < 16; ++q) {
-    float2 x = __ffma2_rn(make_float2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])), ff, bb);
-    x.x = ex2(x.x), x.y = ex2(x.y);
-    sum = __fadd2_rn(sum, x);
-    p[q] = f16x2(x.x, x.y);
+    sum = __fadd2_rn(sum, make_float2(e[2 * q], e[2 * q + 1]));
+    asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[q]) : "f"(e[2 * q + 1]), "f"(e[2 * q]));
   }
 }
 __device__ __forceinline__ float max32(const uint32_t (&v)[32], float m) {
@@ -287,8 +297,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
   __shared__ long long s_sum[WARPS];
   __shared__ int2 s_plan[PLANS];
   __shared__ Run s_run;
-  // of a tile, in turns of four (the loads are at most two ahead): a byte per 32 keys, not 0: outside the cache
-  __shared__ uint32_t s_bad[4];
+  __shared__ uint32_t s_bad[BAD_TURNS];        // of a tile: a byte per 32 keys, not 0: outside the cache
+  __shared__ uint4 s_tile[TURNS][4];
   __shared__ float s_ml[2 * 128];     // not PAIR: the second stream's m and l
   const uint32_t sbase = smem_u32(smem);
   auto bar = [&](int i) { return smem_u32(bars + i); };
@@ -303,6 +313,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
       mbar_init(bar(B_PFULL + i), 4), mbar_init(bar(B_OFULL + i), 1);
       mbar_init(bar(B_SOFT + i), PAIR ? 4 : 8);
     }
+    for (int i = 0; i < TURNS; ++i) mbar_init(bar(B_TFULL + i), 1), mbar_init(bar(B_TEMPTY + i), 4);
     mbar_init(bar(B_DRAIN), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -391,65 +402,31 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
     // ---------------- codes to f16: a warp takes 32 keys, K and V in turn ----------------
     constexpr int LPR = D / 32, PASS = LPR, KPP = 32 / LPR;  // lanes a key, passes, keys a pass
     const int wq = warp & 3, c = lane % LPR, kr = lane / LPR;
+    const int64_t at = (int64_t)kr * (D / 2) + 16 * c;  // of this lane in 32 keys' codes; an eighth of it in the scales
+    const uint8_t *kc = a.k_codes + at, *vc = a.v_codes + at, *ks = a.k_scale + at / 8, *vs = a.v_scale + at / 8;
     uint4 rk[PASS], rv[PASS];
     uint32_t sk[PASS], sv[PASS];
-    // one tile after the other over all segments: the tile whose page is known (next),
-    // and the one whose codes are on their way (now)
-    bool more = segs.next(sg);
-    int t = sg.t0, set = 0, pid = 0;
-    auto page_of = [&]() {  // of this warp's 32 keys of tile t
-      const int key = min(t * TILE + wq * 32, sg.end - 1);
-      return a.block_table[(int64_t)sg.b * a.width + (key >> a.page_log2)];
-    };
-    struct Now {
-      int64_t row;
-      int key0, end, set;
-      bool bad;
-    } now = {}, nxt = {};
-    auto place = [&](Now& x) {
-      x.key0 = t * TILE + wq * 32, x.end = sg.end, x.set = set;
-      const bool out = pid < 0 || pid >= a.pages;
-      x.bad = out && x.key0 < x.end;
-      if (x.bad) note_err(nullptr, ERR_PAGE);
-      x.row = (((int64_t)(out ? 0 : pid) * a.Hkv + sg.kvh) << a.page_log2) + (x.key0 & ((1 << a.page_log2) - 1));
-      // the caches' lines on their way to L2 a tile ahead of the loads
-      if (lane < 4) {
-        const uint8_t* p = lane == 0   ? a.k_codes + x.row * (D / 2)
-                           : lane == 1 ? a.v_codes + x.row * (D / 2)
-                           : lane == 2 ? a.k_scale + x.row * (D / 16)
-                                       : a.v_scale + x.row * (D / 16);
-        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(lane < 2 ? 16 * D : 2 * D) : "memory");
-      }
-    };
-    auto step = [&]() {  // on to the next tile
-      if (++t == sg.t1) {
-        more = segs.next(sg);
-        if (more) t = sg.t0;
-        set = set == NAN_SETS - 1 ? 0 : set + 1;
-      }
-      if (more) pid = page_of();
-    };
-    auto load = [&](const Now& x, const uint8_t* codes, const uint8_t* scales, uint4 (&raw)[PASS], uint32_t (&sc)[PASS]) {
+    auto load = [&](int row, const uint8_t* codes, const uint8_t* scales, uint4 (&raw)[PASS], uint32_t (&sc)[PASS]) {
+      const uint8_t *x = codes + (int64_t)row * (D / 2), *y = scales + (int64_t)row * (D / 16);
 #pragma unroll
       for (int p = 0; p < PASS; ++p) {
-        const int k = p * KPP + kr;
         // volatile: issued here, a tile's time before they are used
         asm volatile("ld.global.nc.v4.b32 {%0,%1,%2,%3}, [%4];"
                      : "=r"(raw[p].x), "=r"(raw[p].y), "=r"(raw[p].z), "=r"(raw[p].w)
-                     : "l"(codes + (x.row + k) * (D / 2) + 16 * c));
+                     : "l"(x + p * KPP * (D / 2)));
         uint16_t e;
-        asm volatile("ld.global.nc.b16 %0, [%1];" : "=h"(e) : "l"(scales + (x.row + k) * (D / 16) + 2 * c));
+        asm volatile("ld.global.nc.b16 %0, [%1];" : "=h"(e) : "l"(y + p * KPP * (D / 16)));
         sc[p] = e;
       }
     };
+    // lanes of the row's second half go through their chunks in another order: the
+    // eight lanes that store together then meet eight different groups of banks
+    const int turn = D == 128 ? c & 2 : 0;
     auto convert = [&](uint32_t dst, const uint4& raw, uint32_t s2, int k) {
       const int r = wq * 32 + k;
       uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
       const uint32_t ss = unpack2(s2);
       uint32_t s0 = __byte_perm(ss, ss, 0x1010), s1 = __byte_perm(ss, ss, 0x3232);
-      // lanes of the row's second half go through their chunks in another order:
-      // the eight lanes that store together then meet eight different groups of banks
-      const int turn = D == 128 ? c & 2 : 0;
       if (turn) {
         uint32_t x = w[0];
         w[0] = w[2], w[2] = x;
@@ -467,56 +444,104 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
         sts128(rowp + ((chunk ^ (r & 7)) << 4), h[0], h[1], h[2], h[3]);
       }
     };
+    int slot = 0;
+    uint32_t sphase = 0;
+    uint4 now = {}, nxt = {};  // row, key, keys that hold a token, set; no keys at all: no tile
+    auto next_tile = [&](uint4& d) {
+      const bool ok = mbar_wait_warp(bar(B_TFULL + slot), sphase, nullptr, ERR_WAIT);
+      d = s_tile[slot][wq];
+      arrive(B_TEMPTY + slot);
+      if (++slot == TURNS) slot = 0, sphase ^= 1;
+      return ok && d.x != NO_TILE;
+    };
+    bool more = next_tile(now);
     if (more) {
-      int buf = 0, turn4 = 0;
-      uint32_t phase = 0;
-      pid = page_of();
-      place(now);
-      load(now, a.k_codes, a.k_scale, rk, sk);
-      load(now, a.v_codes, a.v_scale, rv, sv);
-      step();
-      bool last = !more;
-      if (!last) place(nxt), step();
-      while (true) {
-        if (!mbar_wait_warp(bar(B_KEMPTY + buf), phase ^ 1, nullptr, ERR_WAIT)) break;
-        if (lane == 0) reinterpret_cast<uint8_t*>(s_bad + turn4)[wq] = now.bad;
-        turn4 = (turn4 + 1) & 3;
+      load(now.x, kc, ks, rk, sk);
+      load(now.x, vc, vs, rv, sv);
+    }
+    int buf = 0;
+    uint32_t phase = 1;
+    while (more) {
+      if (!mbar_wait_warp(bar(B_KEMPTY + buf), phase, nullptr, ERR_WAIT)) break;
 #pragma unroll
-        for (int p = 0; p < PASS; ++p) convert(sbase + L::OFF_K + buf * L::TILE_BYTES, rk[p], sk[p], p * KPP + kr);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        arrive(B_KFULL + buf);
-        if (!last) load(nxt, a.k_codes, a.k_scale, rk, sk);
+      for (int p = 0; p < PASS; ++p) convert(sbase + L::OFF_K + buf * L::TILE_BYTES, rk[p], sk[p], p * KPP + kr);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      arrive(B_KFULL + buf);
+      more = next_tile(nxt);
+      if (more) load(nxt.x, kc, ks, rk, sk);
 
-        if (!mbar_wait_warp(bar(B_VEMPTY + buf), phase ^ 1, nullptr, ERR_WAIT)) break;
+      if (!mbar_wait_warp(bar(B_VEMPTY + buf), phase, nullptr, ERR_WAIT)) break;
+      uint32_t odd = 0;
 #pragma unroll
-        for (int p = 0; p < PASS; ++p) {
-          const int k = p * KPP + kr;
-          uint32_t s2 = sv[p];
-          if (now.key0 + k >= now.end || now.bad) s2 = 0;  // no token of this sequence
-          const uint32_t odd = ((s2 & 0x7F7Fu) + 0x0101u) & 0x8080u;
-          if (odd) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              if (odd >> (8 * h) & 0x80u) {
-                for (int w = 0; w < SM_WARPS; ++w) atomicMin(&s_nan[w][now.set][2 * c + h], now.key0 + k);
-                s2 &= ~(0xFFu << (8 * h));
-              }
-          }
-          convert(sbase + L::OFF_V + buf * L::TILE_BYTES, rv[p], s2, k);
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        arrive(B_VFULL + buf);
-        if (last) break;
-        load(nxt, a.v_codes, a.v_scale, rv, sv);
-        now = nxt;
-        last = !more;
-        if (!last) place(nxt), step();
-        if (++buf == 2) buf = 0, phase ^= 1;
+      for (int p = 0; p < PASS; ++p) {
+        if (p * KPP + kr >= (int)now.z) sv[p] = 0;  // no token of this sequence
+        odd |= (sv[p] & 0x7F7Fu) + 0x0101u;
       }
+      if (odd & 0x8080u) {  // a NaN: its key noted, its values 0
+#pragma unroll
+        for (int p = 0; p < PASS; ++p)
+#pragma unroll 1
+          for (int h = 0; h < 16; h += 8)
+            if ((sv[p] >> h & 0x7Fu) == 0x7Fu) {
+#pragma unroll 1
+              for (int w = 0; w < SM_WARPS; ++w)
+                atomicMin(&s_nan[w][now.w][2 * c + (h >> 3)], (int)now.y + p * KPP + kr);
+              sv[p] &= ~(0xFFu << h);
+            }
+      }
+#pragma unroll
+      for (int p = 0; p < PASS; ++p)
+        convert(sbase + L::OFF_V + buf * L::TILE_BYTES, rv[p], sv[p], p * KPP + kr);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      arrive(B_VFULL + buf);
+      if (more) load(nxt.x, vc, vs, rv, sv);
+      now = nxt;
+      if (++buf == 2) buf = 0, phase ^= 1;
     }
   } else if (warp >= W_MMA) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R_REST));
-    if (warp == W_MMA) {
+    if (warp == W_SCOUT) {
+      // ---------------- where the tiles lie, some ahead: lane g < 4 for 32 keys each ----------------
+      int slot = 0, set = 0;
+      uint32_t phase = 1, bturn = 0;
+      bool ok = true;
+      while (ok && segs.next(sg)) {
+        for (int t = sg.t0; t < sg.t1; ++t) {
+          const int key0 = t * TILE + (lane & 3) * 32, left = sg.end - key0;
+          const int key = min(key0, sg.end - 1);
+          const int pid = __ldg(a.block_table + (int64_t)sg.b * a.width + (key >> a.page_log2));
+          const bool out = pid < 0 || pid >= a.pages, bad = out && left > 0;
+          const int row = (((out ? 0 : pid) * a.Hkv + sg.kvh) << a.page_log2) + (key0 & ((1 << a.page_log2) - 1));
+          if (bad && lane < 4) note_err(nullptr, ERR_PAGE);
+          if (!(ok = mbar_wait_warp(bar(B_TEMPTY + slot), phase, nullptr, ERR_WAIT))) break;
+          if (lane < 4) {
+            s_tile[slot][lane] = make_uint4(row, key0, bad ? 0 : max(0, min(32, left)), set);
+            reinterpret_cast<uint8_t*>(s_bad + bturn)[lane] = bad;
+          }
+          arrive(B_TFULL + slot);
+          // its lines to L2: a lane a line of 128 bytes
+          constexpr int LINES = 32 * D / 2 / 128;  // of 32 keys' codes
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int64_t r = __shfl_sync(FULL, row, g);
+            const int i = lane % LINES;
+            const uint8_t* p = (lane < LINES ? a.k_codes : a.v_codes) + r * (D / 2) + i * 128;
+            if (lane < 2 * LINES) asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+            if (lane < 4) {
+              p = (lane < 2 ? a.k_scale : a.v_scale) + r * (D / 16) + (lane & 1) * 128;
+              if (D == 128 || !(lane & 1)) asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+            }
+          }
+          if (++slot == TURNS) slot = 0, phase ^= 1;
+          bturn = (bturn + 1) & (BAD_TURNS - 1);
+        }
+        set = set == NAN_SETS - 1 ? 0 : set + 1;
+      }
+      if (ok && mbar_wait_warp(bar(B_TEMPTY + slot), phase, nullptr, ERR_WAIT)) {
+        if (lane < 4) s_tile[slot][lane] = make_uint4(NO_TILE, 0, 0, 0);
+        arrive(B_TFULL + slot);
+      }
+    } else if (warp == W_MMA) {
       // ---------------- MMA issuer ----------------
       // The whole warp runs the loop and one lane issues: the operands then stay in
       // uniform registers.
@@ -574,12 +599,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
           scores(1, true);
           for (int j = 0; j < n; ++j) {
             const bool again = j + 1 < n;
-            if (!take(B_PFULL, 0, pph) || !wait(B_VFULL + vb, vph)) break;
+            // the tiles are there before the weights are: the products then follow each other
+            if (!wait(B_VFULL + vb, vph) || (again && !wait(B_KFULL + kb, kph)) || !take(B_PFULL, 0, pph)) break;
             values(0, j == 0, false, !again);
-            if (again) {
-              if (!wait(B_KFULL + kb, kph)) break;
-              scores(0, false);
-            }
+            if (again) scores(0, false);
             if (!take(B_PFULL, 1, pph)) break;
             values(1, j == 0, true, !again);
             if (again) scores(1, true);
@@ -592,12 +615,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
           }
           for (int j = 0; j < n && ok; ++j) {
             const int i = j & 1;
-            if (!take(B_PFULL, i, pph) || !wait(B_VFULL + vb, vph)) break;
+            if (!wait(B_VFULL + vb, vph) || (j + 2 < n && !wait(B_KFULL + kb, kph)) || !take(B_PFULL, i, pph)) break;
             values(i, j < 2, true, j + 2 >= n);
-            if (j + 2 < n) {
-              if (!wait(B_KFULL + kb, kph)) break;
-              scores(i, true);
-            }
+            if (j + 2 < n) scores(i, true);
           }
         }
       }
@@ -617,7 +637,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
     const uint32_t ts = tq + COL_S + i * 128, to = tq + COL_O + i * 128;
     const uint32_t sq = sbase + L::OFF_Q + i * L::TILE_BYTES;
     uint32_t sph = 0, oph = 0, softph = 0;
-    int set = 0, turn4 = 0;  // of s_nan; of s_bad, at the segment's first tile
+    int set = 0, bturn = 0;  // of s_nan; of s_bad, at the segment's first tile
     bool ok = true;
     // the threads that end a segment together: a stream's, or both streams'; bounded, as every wait
     auto soft_sync = [&]() {
@@ -730,53 +750,72 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
         // the last scores are there, so the queries' place is free: the next ones travel under this tile
         if (PAIR && j + 1 == n && more) fetch_q(sg, x);
         if (any_live) {
-          uint32_t va[32], vb[32], vc[32], vd[32], p[16];
-          tmem_ld32(ts, va);
-          tmem_ld32(ts + 32, vb);
           const int key0 = (cur.t0 + j) * TILE;
-          const uint32_t bad = s_bad[(turn4 + j) & 3];
-          const bool masked = key0 + TILE > free_end || bad;
-          // -infinity where the key lies past the row's last, or in no page
-          auto mask32 = [&](uint32_t (&v)[32], int c) {
-            const int stay = bad >> (8 * c) & 0xFFu ? 0 : limit + 1 - key0 - 32 * c;
-#pragma unroll
-            for (int q = 0; q < 32; ++q) v[q] = q < stay ? v[q] : 0xFF800000u;
-          };
-          tmem_ld_wait();
-          tmem_ld32(ts + 64, vc);
-          tmem_ld32(ts + 96, vd);
-          if (masked) mask32(va, 0), mask32(vb, 1);
-          float mx = fmaxf(max32(va, NEG_INF), max32(vb, NEG_INF));
-          tmem_ld_wait();
-          if (masked) mask32(vc, 2), mask32(vd, 3);
-          mx = fmaxf(mx, fmaxf(max32(vc, NEG_INF), max32(vd, NEG_INF)));
-          const float top = mx == NEG_INF ? NEG_INF : mx * f;
-          if (__any_sync(FULL, top > m + LAG)) {
-            const float mn = fmaxf(m, top), corr = mn == NEG_INF ? 1.0f : ex2(m - mn);
-            m = mn;
-            l *= corr;
-            if (any) {
+          const uint32_t bad = s_bad[(bturn + j) & (BAD_TURNS - 1)];
+          float2 sum = make_float2(0.0f, 0.0f);
+          // the reference m after scores whose largest is mx, and O and l with it
+          auto refer = [&](float mx) {
+            const float top = mx == NEG_INF ? NEG_INF : mx * f;
+            if (__any_sync(FULL, top > m + LAG)) {
+              const float mn = fmaxf(m, top), corr = mn == NEG_INF ? 1.0f : ex2(m - mn);
+              m = mn;
+              l *= corr;
+              if (any) {
 #pragma unroll 1
-              for (int c = 0; c < D / 16; ++c) {
-                uint32_t o[16];
-                tmem_ld16(to + 16 * c, o);
-                tmem_ld_wait();
+                for (int c = 0; c < D / 16; ++c) {
+                  uint32_t o[16];
+                  tmem_ld16(to + 16 * c, o);
+                  tmem_ld_wait();
 #pragma unroll
-                for (int q = 0; q < 16; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * corr);
-                tmem_st16(to + 16 * c, o);
+                  for (int q = 0; q < 16; ++q) o[q] = __float_as_uint(__uint_as_float(o[q]) * corr);
+                  tmem_st16(to + 16 * c, o);
+                }
               }
             }
+            return m == NEG_INF ? P_EXP : P_EXP - m;
+          };
+          if (key0 + TILE <= free_end && !bad) {
+            uint32_t va[32], vb[32], vc[32], vd[32], p[16];
+            tmem_ld32(ts, va);
+            tmem_ld32(ts + 32, vb);
+            tmem_ld_wait();
+            tmem_ld32(ts + 64, vc);
+            tmem_ld32(ts + 96, vd);
+            float mx = fmaxf(max32(va, NEG_INF), max32(vb, NEG_INF));
+            tmem_ld_wait();
+            mx = fmaxf(mx, fmaxf(max32(vc, NEG_INF), max32(vd, NEG_INF)));
+            const float bias = refer(mx);
+            weights32(va, f, bias, sum, p);
+            tmem_st16(ts, p);
+            weights32(vb, f, bias, sum, p);
+            tmem_st16(ts + 16, p);
+            weights32(vc, f, bias, sum, p);
+            tmem_st16(ts + 32, p);
+            weights32(vd, f, bias, sum, p);
+            tmem_st16(ts + 48, p);
+          } else {  // some scores are -infinity: their key lies past the row's last, or in no page
+            auto masked32 = [&](int c, uint32_t (&v)[32]) {
+              tmem_ld32(ts + 32 * c, v);
+              tmem_ld_wait();
+              const int stay = bad >> (8 * c) & 0xFFu ? 0 : limit + 1 - key0 - 32 * c;
+#pragma unroll
+              for (int q = 0; q < 32; ++q) v[q] = q < stay ? v[q] : 0xFF800000u;
+            };
+            uint32_t v[32], p[16];
+            float mx = NEG_INF;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              masked32(c, v);
+              mx = max32(v, mx);
+            }
+            const float bias = refer(mx);
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              masked32(c, v);
+              weights32(v, f, bias, sum, p);
+              tmem_st16(ts + 16 * c, p);
+            }
           }
-          const float bias = m == NEG_INF ? P_EXP : P_EXP - m;
-          float2 sum = make_float2(0.0f, 0.0f);
-          weights32(va, f, bias, sum, p);
-          tmem_st16(ts, p);
-          weights32(vb, f, bias, sum, p);
-          tmem_st16(ts + 16, p);
-          weights32(vc, f, bias, sum, p);
-          tmem_st16(ts + 32, p);
-          weights32(vd, f, bias, sum, p);
-          tmem_st16(ts + 48, p);
           l += sum.x + sum.y;
           tmem_st_wait();
           any = true;
@@ -786,7 +825,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
       }
       if (!ok) break;
       if (PAIR && more) f = finish_q(scale);  // while the last product runs
-      turn4 = (turn4 + n) & 3;
+      bturn = (bturn + n) & (BAD_TURNS - 1);
       const bool had = PAIR || i < n;  // this stream's O has been written
       if (had) {
         if (!(ok = mbar_wait_warp(bar(B_OFULL + i), oph, nullptr, ERR_WAIT))) break;
