@@ -179,6 +179,13 @@ __device__ __forceinline__ uint32_t swz4(int r, int c) {
   return D == 128 ? (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4)) : (uint32_t)(r * 32 + (c << 4));
 }
 
+// One lane of a converged warp: the copies' operands stay in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, P;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // Byte offset of 16-byte chunk c of row r in a TMA-swizzled tile of D-byte rows.
 template <int D>
 __device__ __forceinline__ uint32_t swz(int r, int c) {
@@ -380,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
       pid_next = pid_of(issued + lane + 32);
     }
     const int y = __shfl_sync(FULL, n_row, issued & 31);
-    if (lane == 0) {
+    if (FP4 ? elect_one() : lane == 0) {
       const uint32_t bar = bar0 + 8 * wstage, dst = ring + wstage * C::STRIDE;
       mbar_expect_tx(bar, C::STAGE);
       tma_load_2d(dst, &map_k, 0, y, bar);
@@ -690,6 +697,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
   if (!more) break;
   const int held = sg.held, end = sg.end, k0 = sg.k0;
 
+  const float sm_head = FP4 ? a.sm_log2 * __ldg(a.k_scale + sg.kvh) : a.sm_log2;
   // Q as the second operand of S^T = K Q^T: k step w takes the lane's 4
   // columns D/4 * t + 4 w ...
   uint32_t qf[NT][KS][2];
@@ -705,7 +713,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
     m = max(m, __shfl_xor_sync(FULL, m, 1));
     m = max(m, __shfl_xor_sync(FULL, m, 2));
     const int e = min(max((int)(m >> 7), 15), 253);  // the largest value's exponent field
-    const float up = __uint_as_float((uint32_t)(254 + 14 - e) << 23);
+    float up = __uint_as_float((uint32_t)(254 + 14 - e) << 23);
+    if (FP4) up = copysignf(up, sm_head);  // a negative scale turns the query
     qs[n] = __uint_as_float((uint32_t)(e - 14) << 23);
 #pragma unroll
     for (int i = 0; i < D / 8; ++i)
@@ -719,7 +728,9 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      cs[n][c] = __shfl_sync(FULL, qs[n], (2 * t + c) * 4) * (FP4 ? a.sm_log2 * __ldg(a.k_scale + sg.kvh) : a.sm_log2);
+      cs[n][c] = __shfl_sync(FULL, qs[n], (2 * t + c) * 4) * (FP4 ? fabsf(sm_head) : sm_head);
+      // never 0, so that a masked score stays -infinity; NaN stays
+      if (FP4 && cs[n][c] < 1.17549435e-38f) cs[n][c] = 1.17549435e-38f;
       lim[n][c] = held + row_of(sg, n * 8 + 2 * t + c).x;
     }
   const int free_end = held + sg.tok0 + 1;  // keys below: every row sees them
@@ -733,6 +744,8 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
   }
 
   int i = 0;
+  int nan_key = 0x7FFFFFFF;  // in 4 bits: the first key whose values in this lane's block are NaN
+  uint32_t c_outside = 0;  // in 4 bits: of the batch, the tiles in no page
   auto advance = [&]() {
     __syncwarp();  // every lane has read the stage
     if (issued < mine) issue();
@@ -740,11 +753,12 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
   };
   for (; i < mine; ++i, advance()) {
     const int key0 = k0 + (warp + i * WARPS) * TILE;
-    if ((i & 31) == 0) c_ks = n_ks, c_lv = log2f(n_v);
-    const float ks = FP4 ? 1.0f : __shfl_sync(FULL, c_ks, i & 31), lv = __shfl_sync(FULL, c_lv, i & 31);
+    if ((i & 31) == 0) c_ks = n_ks, c_lv = FP4 ? n_v : log2f(n_v);
+    if constexpr (FP4) c_outside = (i & 31) == 0 ? __ballot_sync(FULL, n_v < 0.0f) : c_outside;
+    const float ks = FP4 ? 1.0f : __shfl_sync(FULL, c_ks, i & 31), lv = FP4 ? 0.0f : __shfl_sync(FULL, c_lv, i & 31);
     ok = mbar_wait_warp(bar0 + 8 * stage, phase, nullptr, ERR_WAIT);
     if (!ok) break;
-    if (lv != lv) continue;  // a page outside the cache
+    if (FP4 ? c_outside >> (i & 31) & 1u : lv != lv) continue;  // a page outside the cache
     const uint32_t kb = ring + stage * C::STRIDE, vb = kb + C::TILE_BYTES;
     // the key that index r of the products stands for
     auto place = [](int r) { return FP4 ? key4(r) : r; };
@@ -811,49 +825,85 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
     bool grew = false;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float f0 = cs[n][0] * ks, f1 = cs[n][1] * ks;
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-        s[n][mt][0] *= f0, s[n][mt][2] *= f0;
-        s[n][mt][1] *= f1, s[n][mt][3] *= f1;
+      if constexpr (FP4) {
+        // One page's values weigh as another's: w is m, the weights are their sum's terms.
+        // The lanes of a column meet only where one of them has found a larger score.
         if (tail) {
-          const int key = key0 + mt * 16 + place(g);
-          if (key > lim[n][0]) s[n][mt][0] = NEG_INF;
-          if (key > lim[n][1]) s[n][mt][1] = NEG_INF;
-          if (key + 8 > lim[n][0]) s[n][mt][2] = NEG_INF;
-          if (key + 8 > lim[n][1]) s[n][mt][3] = NEG_INF;
-        }
-      }
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        float m = fmaxf(fmaxf(s[n][0][c], s[n][0][c + 2]), fmaxf(s[n][1][c], s[n][1][c + 2]));
-        m = fmaxf(m, __shfl_xor_sync(FULL, m, 4));
-        m = fmaxf(m, __shfl_xor_sync(FULL, m, 8));
-        m = fmaxf(m, __shfl_xor_sync(FULL, m, 16));
-        const float w = fmaxf(m + lv, wx[n][c]);
-        m = fmaxf(m, mx[n][c]);
-        // nothing seen yet (or every v_scale 0): every weight is 0
-        const float ref = m == NEG_INF ? 0.0f : m, wref = w == NEG_INF ? 0.0f : w;
-        const float lower = ex2(mx[n][c] - ref);
-        corr[n][c] = ex2(wx[n][c] - wref);
-        grew |= w != wx[n][c];
-        mx[n][c] = m;
-        wx[n][c] = w;
-        const float pref = FP4 ? ref - P_EXP : wref - lv - P_EXP;
-        float add = 0.0f;
+          for (int mt = 0; mt < 2; ++mt) {
+            const int key = key0 + mt * 16 + place(g);
+            if (key > lim[n][0]) s[n][mt][0] = NEG_INF;
+            if (key > lim[n][1]) s[n][mt][1] = NEG_INF;
+            if (key + 8 > lim[n][0]) s[n][mt][2] = NEG_INF;
+            if (key + 8 > lim[n][1]) s[n][mt][3] = NEG_INF;
+          }
+        }
+        float top[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)  // cs > 0: -infinity stays
+          top[c] = fmaxf(fmaxf(s[n][0][c], s[n][0][c + 2]), fmaxf(s[n][1][c], s[n][1][c + 2])) * cs[n][c];
+        corr[n][0] = corr[n][1] = 1.0f;
+        if (__any_sync(FULL, top[0] > mx[n][0] || top[1] > mx[n][1])) {
+          grew = true;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float m = fmaxf(top[c], __shfl_xor_sync(FULL, top[c], 4));
+            m = fmaxf(m, __shfl_xor_sync(FULL, m, 8));
+            m = fmaxf(fmaxf(m, __shfl_xor_sync(FULL, m, 16)), mx[n][c]);
+            corr[n][c] = m == NEG_INF ? 1.0f : ex2(mx[n][c] - m);
+            mx[n][c] = wx[n][c] = m;
+            sum[n][c] *= corr[n][c];
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float bias = P_EXP - (mx[n][c] == NEG_INF ? 0.0f : mx[n][c]);
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            s[n][mt][c] = ex2(fmaf(s[n][mt][c], cs[n][c], bias));
+            s[n][mt][c + 2] = ex2(fmaf(s[n][mt][c + 2], cs[n][c], bias));
+          }
+          sum[n][c] += (s[n][0][c] + s[n][0][c + 2]) + (s[n][1][c] + s[n][1][c + 2]);
+        }
+      } else {
+        const float f0 = cs[n][0] * ks, f1 = cs[n][1] * ks;
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
-          if constexpr (FP4) {  // one page's values weigh as another's: the weights are their own sum's terms
+          s[n][mt][0] *= f0, s[n][mt][2] *= f0;
+          s[n][mt][1] *= f1, s[n][mt][3] *= f1;
+          if (tail) {
+            const int key = key0 + mt * 16 + place(g);
+            if (key > lim[n][0]) s[n][mt][0] = NEG_INF;
+            if (key > lim[n][1]) s[n][mt][1] = NEG_INF;
+            if (key + 8 > lim[n][0]) s[n][mt][2] = NEG_INF;
+            if (key + 8 > lim[n][1]) s[n][mt][3] = NEG_INF;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float m = fmaxf(fmaxf(s[n][0][c], s[n][0][c + 2]), fmaxf(s[n][1][c], s[n][1][c + 2]));
+          m = fmaxf(m, __shfl_xor_sync(FULL, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(FULL, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(FULL, m, 16));
+          const float w = fmaxf(m + lv, wx[n][c]);
+          m = fmaxf(m, mx[n][c]);
+          // nothing seen yet (or every v_scale 0): every weight is 0
+          const float ref = m == NEG_INF ? 0.0f : m, wref = w == NEG_INF ? 0.0f : w;
+          const float lower = ex2(mx[n][c] - ref);
+          corr[n][c] = ex2(wx[n][c] - wref);
+          grew |= w != wx[n][c];
+          mx[n][c] = m;
+          wx[n][c] = w;
+          const float pref = wref - lv - P_EXP;
+          float add = 0.0f;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            add += ex2(s[n][mt][c] - ref) + ex2(s[n][mt][c + 2] - ref);
             s[n][mt][c] = ex2(s[n][mt][c] - pref);
             s[n][mt][c + 2] = ex2(s[n][mt][c + 2] - pref);
-            add += s[n][mt][c] + s[n][mt][c + 2];
-            continue;
           }
-          add += ex2(s[n][mt][c] - ref) + ex2(s[n][mt][c + 2] - ref);
-          s[n][mt][c] = ex2(s[n][mt][c] - pref);
-          s[n][mt][c + 2] = ex2(s[n][mt][c + 2] - pref);
+          sum[n][c] = fmaf(sum[n][c], lower, add);
         }
-        sum[n][c] = fmaf(sum[n][c], lower, add);
       }
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
@@ -861,7 +911,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
         pf[n][mt][1] = transpose8x8(f16x2(s[n][mt][2], s[n][mt][3]));
       }
     }
-    if (__any_sync(FULL, grew)) {
+    if (FP4 ? grew : __any_sync(FULL, grew)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -897,60 +947,40 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
           if (tail) {
             if (key0 + r0 >= end) e0 = 0;  // slots that hold no token of this sequence
             if (key0 + r1 >= end) e1 = 0;
-            odd |= nan_bits(e0) | nan_bits(e1);
           }
-          sp[mt][p] = unpack2(e0 | e1 << 8);
+          sp[mt][p] = e0 | e1 << 8;
+          odd |= nan_bits(sp[mt][p]);
 #pragma unroll
           for (int w = 0; w < VW; ++w) {
             ev[mt][p][w] = (x[w] & 0x0F0F0F0Fu) | (y[w] << 4 & 0xF0F0F0F0u);
             od[mt][p][w] = (x[w] >> 4 & 0x0F0F0F0Fu) | (y[w] & 0xF0F0F0F0u);
           }
         }
-      auto product = [&](int n, int mt, int w, const uint32_t (&sc)[2], float (&acc)[4][4]) {
-        uint32_t a0[4], a1[4], a2[4], a3[4];
-        e2m1_f16(ev[mt][0][w], a0), e2m1_f16(od[mt][0][w], a1), e2m1_f16(ev[mt][1][w], a2), e2m1_f16(od[mt][1][w], a3);
+      // 0 * NaN is NaN, also for a row that may not see the value: a NaN enters as 0,
+      // its key is noted, and the rows that see it get NaN at the segment's end
+      if (odd & 0x8080u) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          mma(acc[j], mul_f16x2(a0[j], sc[0]), mul_f16x2(a1[j], sc[0]), mul_f16x2(a2[j], sc[1]), mul_f16x2(a3[j], sc[1]),
-              pf[n][mt][0], pf[n][mt][1]);
-      };
-      if (tail) odd = __any_sync(FULL, (odd & 0x80u) != 0);
-      if (!odd) {
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int w = 0; w < VW; ++w)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-              product(n, mt, w, sp[mt], *reinterpret_cast<float(*)[4][4]>(&o[n][4 * w]));
-      } else {  // as below: each row with the values it does not see taken as 0
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll 1
-          for (int r = 0; r < 8; ++r) {
-            const int last = held + row_of(sg, n * 8 + r).x;
-            const bool c0 = r == 2 * t, c1 = r == 2 * t + 1;
-            uint32_t sc[2][2];
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-              for (int p = 0; p < 2; ++p) {
-                const int at = key0 + mt * 16 + p * 8;
-                sc[mt][p] = (at + key4(2 * t) > last ? 0u : sp[mt][p] & 0xFFFFu) |
-                            (at + key4(2 * t + 1) > last ? 0u : sp[mt][p] & 0xFFFF0000u);
-              }
-#pragma unroll
-            for (int w = 0; w < VW; ++w) {
-              float acc[4][4] = {};
-#pragma unroll
-              for (int mt = 0; mt < 2; ++mt) product(n, mt, w, sc[mt], acc);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                if (c0) o[n][4 * w + j][0] += acc[j][0], o[n][4 * w + j][2] += acc[j][2];
-                if (c1) o[n][4 * w + j][1] += acc[j][1], o[n][4 * w + j][3] += acc[j][3];
-              }
-            }
+        for (int q = 0; q < 8; ++q)
+          if ((sp[q >> 2][q >> 1 & 1] >> (8 * (q & 1)) & 0x7Fu) == 0x7Fu) {
+            nan_key = min(nan_key, key0 + (q >> 2) * 16 + (q >> 1 & 1) * 8 + key4(2 * t + (q & 1)));
+            sp[q >> 2][q >> 1 & 1] &= ~(0xFFu << (8 * (q & 1)));
           }
+      }
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+        const uint32_t s0 = unpack2(sp[mt][0]), s1 = unpack2(sp[mt][1]);
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          uint32_t a0[4], a1[4], a2[4], a3[4];
+          e2m1_f16(ev[mt][0][w], a0), e2m1_f16(od[mt][0][w], a1), e2m1_f16(ev[mt][1][w], a2), e2m1_f16(od[mt][1][w], a3);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            a0[j] = mul_f16x2(a0[j], s0), a1[j] = mul_f16x2(a1[j], s0);
+            a2[j] = mul_f16x2(a2[j], s1), a3[j] = mul_f16x2(a3[j], s1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma(o[n][4 * w + j], a0[j], a1[j], a2[j], a3[j], pf[n][mt][0], pf[n][mt][1]);
+          }
+        }
       }
       continue;
     }
@@ -1025,6 +1055,19 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
             if (c1) o[n][j][1] += acc[1], o[n][j][3] += acc[3];
           }
         }
+    }
+  }
+  if (FP4) {
+    nan_key = min(nan_key, __shfl_xor_sync(FULL, nan_key, 1));
+    nan_key = min(nan_key, __shfl_xor_sync(FULL, nan_key, 2));
+    if (nan_key != 0x7FFFFFFF) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          if (nan_key <= lim[n][c])
+#pragma unroll
+            for (int j = 0; j < KS; ++j) o[n][j][c] = o[n][j][c + 2] = __uint_as_float(0x7FC00000u);
     }
   }
   // after a wait that gave up: the loads in flight land before the ring is reused
