@@ -75,7 +75,7 @@ struct Args {
   int64_t qb, qt, qh;
   uint16_t* out;  // bf16 [B, T, H, D]
   const float *k_scale, *v_scale;  // per page and head; in 4 bits per head: the factors
-  const uint8_t *k_bscale, *v_bscale;  // in 4 bits: E4M3 [pages, Hkv, page, D / 16]
+  const uint8_t *k_codes, *v_codes, *k_bscale, *v_bscale;  // in 4 bits: the codes, E4M3 [pages, Hkv, page, D / 16]
   const int32_t *block_table, *lengths, *counts;
   float* part;        // [CTAs][2][ROWS * (D + 3)]: pieces of heads that were cut
   int32_t* done;      // [B * groups * Hkv] zero before, zero after
@@ -99,13 +99,13 @@ struct Cfg {
   // a stage holds codes of K, codes of V; in 4 bits then their scales
   static constexpr int TILE_BYTES = FP4 ? TILE * D / 2 : TILE * D, SCALE_BYTES = FP4 ? TILE * D / 16 : 0;
   static constexpr int STAGE = 2 * (TILE_BYTES + SCALE_BYTES);
-  static constexpr int STRIDE = (STAGE + 511) / 512 * 512;  // the swizzle's period
+  static constexpr int STRIDE = STAGE;
   // Two stages a warp: 128 KB in flight an SM (96 KB at heads of 64) fill HBM, and
   // more only lengthens the queue that every other access waits in (4 sequences
   // of 131000 keys: 168 us, with three 178; heads of 64, 24 sequences of 28631:
   // 118, with four 126).
   static constexpr int PER_SM = ctas_per_sm(D, NT, FP4);
-  static constexpr int STAGES = FP4 ? (D == 128 ? 3 : 4) : D == 128 || PER_SM == 3 ? 2 : 3;
+  static constexpr int STAGES = FP4 ? (D == 128 ? 2 : 3) : D == 128 || PER_SM == 3 ? 2 : 3;
   static constexpr int RING = STAGES * STRIDE;  // per warp
   static constexpr int SMEM_RING = WARPS * RING;
   // the warps' O meet in SUMS buffers, rows LD floats apart
@@ -173,12 +173,6 @@ __device__ __forceinline__ uint32_t lds8(uint32_t a) {
 // keys 2t of lanes t, and those of two neighbouring g, then lie in different
 // banks.
 __device__ __forceinline__ int key4(int i) { return (i & 12) | (0x9C >> ((i & 3) * 2) & 3); }
-// Byte offset of 16-byte chunk c of row r of a 4-bit tile: SWIZZLE_64B at 64 bytes a row, plain at 32.
-template <int D>
-__device__ __forceinline__ uint32_t swz4(int r, int c) {
-  return D == 128 ? (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4)) : (uint32_t)(r * 32 + (c << 4));
-}
-
 // One lane of a converged warp: the copies' operands stay in uniform registers.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -256,7 +250,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
 
-  if (threadIdx.x == 0) {
+  if (!FP4 && threadIdx.x == 0) {
     prefetch_map(&map_k);
     prefetch_map(&map_v);
   }
@@ -355,6 +349,15 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
   int pos = lo, ebase = s_before, e = s_entry - 1, units = 0;
   Entry x = {};
 
+  // In 4 bits: where this lane's parts of a stage's first 8 keys lie: rows of K by
+  // g and of V by t, and their scales.
+  const uint32_t at_k = key4(g) * (D / 2) + t * (D / 8);
+  const uint32_t at_ks = 2 * C::TILE_BYTES + key4(g) * (D / 16) + (D == 128 ? 2 * t : t);
+  const uint32_t at_v0 = C::TILE_BYTES + key4(2 * t) * (D / 2) + g * (D / 16);
+  const uint32_t at_v1 = C::TILE_BYTES + key4(2 * t + 1) * (D / 2) + g * (D / 16);
+  const uint32_t at_vs0 = 2 * C::TILE_BYTES + C::SCALE_BYTES + key4(2 * t) * (D / 16) + (D == 128 ? g : g >> 1);
+  const uint32_t at_vs1 = 2 * C::TILE_BYTES + C::SCALE_BYTES + key4(2 * t + 1) * (D / 16) + (D == 128 ? g : g >> 1);
+
   // A segment: the part of one head (entry, kv head) in this run.
   struct Seg {
     int b, row0, nrows, held, end, kvh, k0, k1, units, slot, pair;
@@ -390,9 +393,12 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
     if (FP4 ? elect_one() : lane == 0) {
       const uint32_t bar = bar0 + 8 * wstage, dst = ring + wstage * C::STRIDE;
       mbar_expect_tx(bar, C::STAGE);
-      tma_load_2d(dst, &map_k, 0, y, bar);
-      tma_load_2d(dst + C::TILE_BYTES, &map_v, 0, y, bar);
-      if constexpr (FP4) {
+      if constexpr (!FP4) {
+        tma_load_2d(dst, &map_k, 0, y, bar);
+        tma_load_2d(dst + C::TILE_BYTES, &map_v, 0, y, bar);
+      } else {  // 32 keys lie side by side
+        bulk_load(dst, a.k_codes + (int64_t)y * (D / 2), C::TILE_BYTES, bar);
+        bulk_load(dst + C::TILE_BYTES, a.v_codes + (int64_t)y * (D / 2), C::TILE_BYTES, bar);
         bulk_load(dst + 2 * C::TILE_BYTES, a.k_bscale + (int64_t)y * (D / 16), C::SCALE_BYTES, bar);
         bulk_load(dst + 2 * C::TILE_BYTES + C::SCALE_BYTES, a.v_bscale + (int64_t)y * (D / 16), C::SCALE_BYTES, bar);
       }
@@ -773,19 +779,19 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
       const int r = mt * 16 + place(g);
       if constexpr (FP4) {
         // rows r and r + 8 of the tile, D / 4 columns, in D / 64 blocks of 16
-        const uint32_t sb = vb + C::TILE_BYTES;
         uint32_t x[D / 32], y[D / 32], sx[D / 64], sy[D / 64];
+        const uint32_t ka = kb + at_k + mt * (16 * D / 2), kc = kb + at_ks + mt * D;  // 8 rows on: half of that
         if constexpr (D == 128) {
-          const uint4 p = lds128(kb + swz4<D>(r, t)), q = lds128(kb + swz4<D>(r + 8, t));
+          const uint4 p = lds128(ka), q = lds128(ka + 512);
           x[0] = p.x, x[1] = p.y, x[D / 32 - 2] = p.z, x[D / 32 - 1] = p.w;
           y[0] = q.x, y[1] = q.y, y[D / 32 - 2] = q.z, y[D / 32 - 1] = q.w;
-          const uint32_t u = unpack2(lds16(sb + r * 8 + 2 * t)), w = unpack2(lds16(sb + (r + 8) * 8 + 2 * t));
+          const uint32_t u = unpack2(lds16(kc)), w = unpack2(lds16(kc + 64));
           sx[0] = __byte_perm(u, u, 0x1010), sx[D / 64 - 1] = __byte_perm(u, u, 0x3232);
           sy[0] = __byte_perm(w, w, 0x1010), sy[D / 64 - 1] = __byte_perm(w, w, 0x3232);
         } else {
-          const uint2 p = lds64(kb + swz4<D>(r, 0) + 8 * t), q = lds64(kb + swz4<D>(r + 8, 0) + 8 * t);
+          const uint2 p = lds64(ka), q = lds64(ka + 256);
           x[0] = p.x, x[1] = p.y, y[0] = q.x, y[1] = q.y;
-          sx[0] = unpack2(lds8(sb + r * 4 + t) * 0x0101u), sy[0] = unpack2(lds8(sb + (r + 8) * 4 + t) * 0x0101u);
+          sx[0] = unpack2(lds8(kc) * 0x0101u), sy[0] = unpack2(lds8(kc + 32) * 0x0101u);
         }
 #pragma unroll
         for (int w = 0; w < D / 32; ++w) {
@@ -925,7 +931,6 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
     // of each half tile
     if constexpr (FP4) {
       constexpr int VW = D / 64;  // words of D / 8 columns
-      const uint32_t sb = vb + C::TILE_BYTES + C::SCALE_BYTES;
       // the pairs of keys (2t, 2t+1) and (2t+8, 2t+9): words whose bytes are one
       // column's two codes, even columns and odd, and the two scales
       uint32_t ev[2][2][VW], od[2][2][VW], sp[2][2];
@@ -936,14 +941,14 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
         for (int p = 0; p < 2; ++p) {
           const int r0 = mt * 16 + p * 8 + key4(2 * t), r1 = mt * 16 + p * 8 + key4(2 * t + 1);
           uint32_t x[VW], y[VW], e0, e1;
+          const uint32_t on = (mt * 16 + p * 8) * (D / 2), ons = on / 8;
           if constexpr (D == 128) {
-            const uint2 u = lds64(vb + swz4<D>(r0, g >> 1) + (g & 1) * 8), w = lds64(vb + swz4<D>(r1, g >> 1) + (g & 1) * 8);
+            const uint2 u = lds64(kb + at_v0 + on), w = lds64(kb + at_v1 + on);
             x[0] = u.x, x[VW - 1] = u.y, y[0] = w.x, y[VW - 1] = w.y;
-            e0 = lds8(sb + r0 * 8 + g), e1 = lds8(sb + r1 * 8 + g);
           } else {
-            x[0] = lds32(vb + swz4<D>(r0, 0) + 4 * g), y[0] = lds32(vb + swz4<D>(r1, 0) + 4 * g);
-            e0 = lds8(sb + r0 * 4 + (g >> 1)), e1 = lds8(sb + r1 * 4 + (g >> 1));
+            x[0] = lds32(kb + at_v0 + on), y[0] = lds32(kb + at_v1 + on);
           }
+          e0 = lds8(kb + at_vs0 + ons), e1 = lds8(kb + at_vs1 + ons);
           if (tail) {
             if (key0 + r0 >= end) e0 = 0;  // slots that hold no token of this sequence
             if (key0 + r1 >= end) e1 = 0;
@@ -1203,12 +1208,12 @@ static int attention(const void* q, const int64_t* q_strides, int64_t batch, int
   if (!workspace || workspace_floats < (int64_t)c.ctas * 2 * 8 * c.nt * (head_dim + 3)) return VQ_ERR_INVALID;
   CUtensorMap mk, mv;
   const uint64_t rows = (uint64_t)pages * kv_heads * page;
-  const uint32_t bytes = fp4 ? head_dim / 2 : head_dim;
-  auto map = [&](CUtensorMap* m, const void* p) {
-    return bytes == 32 ? vq::mx::make_map_plain(m, p, rows, bytes, bytes, TILE)
-                       : vq::mx::make_map_box(m, p, rows, bytes, bytes, TILE, bytes);
-  };
-  if (!map(&mk, k_codes) || !map(&mv, v_codes)) return VQ_ERR_CUDA;
+  if (fp4)
+    mk = mv = {};  // not used
+  else if (!vq::mx::make_map_box(&mk, k_codes, rows, head_dim, head_dim, TILE, head_dim) ||
+           !vq::mx::make_map_box(&mv, v_codes, rows, head_dim, head_dim, TILE, head_dim))
+    return VQ_ERR_CUDA;
+  a.k_codes = fp4 ? (const uint8_t*)k_codes : nullptr, a.v_codes = fp4 ? (const uint8_t*)v_codes : nullptr;
   a.q = (const uint16_t*)q;
   a.qb = q_strides[0], a.qt = q_strides[1], a.qh = q_strides[2];
   a.k_scale = fp4 ? k_factor : (const float*)k_scale, a.v_scale = fp4 ? v_factor : (const float*)v_scale;
