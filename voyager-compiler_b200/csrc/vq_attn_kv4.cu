@@ -68,19 +68,21 @@ constexpr float P_EXP = 7.0f, LAG = 8.0f;
 constexpr int NAN_SETS = 3;  // a segment's, of which the epilogue of one and the loads of two more can be under way
 
 enum { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_VEMPTY = 6, B_QFULL = 8, B_SFULL = 10, B_PFULL = 12, B_OFULL = 14,
-       B_SOFT = 16, B_DRAIN = 18, B_TFULL = 20, B_TEMPTY = 24, NBARS = 28 };
+       B_SOFT = 16, B_DRAIN = 18, B_TFULL = 20, B_TEMPTY = 24, B_GFULL = 28, B_GEMPTY = 32, NBARS = 36 };
+static_assert(NBARS * 8 <= 512, "barrier area");
 // tiles whose places are known, and words of pages outside the cache (of a tile until its softmax has begun: the two in
 // the buffers and those known)
-constexpr int TURNS = 4, BAD_TURNS = 16;
+constexpr int TURNS = 4, BAD_TURNS = 16, SEGS = 4;
 constexpr uint32_t NO_TILE = 0xFFFFFFFFu;
 
 constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_O = 256;  // stream i: S at 128 i, O at 256 + 128 i
+constexpr uint32_t COL_P = 64;  // P lies in the upper half of S
 
 template <int D>
 struct Lay {
   static constexpr int TILE_BYTES = TILE * D * 2, HALF = TILE * 128;
   static constexpr int OFF_Q = 0, OFF_K = 2 * TILE_BYTES, OFF_V = 4 * TILE_BYTES, OFF_BAR = 6 * TILE_BYTES;
-  static constexpr int SMEM = OFF_BAR + 256 + 1024;
+  static constexpr int SMEM = OFF_BAR + 512 + 1024;
 };
 
 struct Args {
@@ -205,6 +207,7 @@ struct Cost {
 struct Run {
   int lo, hi, entry, before, base, rest;  // the first `rest` runs are base + 1 long
 };
+__device__ __forceinline__ int run_of(const Run& r, int at);
 // Segments, one after the other: the part of one head (entry, kv head) in the run.
 struct Seg {
   int b, row0, nrows, held, end, kvh, t0, t1, tiles, slot, pair, ps;
@@ -238,17 +241,12 @@ struct Segments {
     pos = min(r.hi, s.ps + HEAD + tiles);
     return true;
   }
-  // the run that holds this place, by the cuts as they were before they moved
-  __device__ __forceinline__ int run_of(int at) const {
-    const int far = at - r.rest * (r.base + 1);
-    return (far < 0 ? 0 : r.rest) + (far < 0 ? at : far) / (far < 0 ? r.base + 1 : r.base);
-  }
-  // the runs that a head's pieces come from, and which of its first run's pieces is the head's
-  __device__ __forceinline__ void pieces_of(const Seg& s, int& c0, int& c1, int& slot0) const {
-    c0 = run_of(s.ps + HEAD), c1 = run_of(s.ps + HEAD + s.tiles - 1);
-    slot0 = c0 * r.base + min(c0, r.rest) >= s.ps ? 0 : 1;
-  }
 };
+// The run that holds this place, by the cuts as they were before they moved.
+__device__ __forceinline__ int run_of(const Run& r, int at) {
+  const int far = at - r.rest * (r.base + 1);
+  return (far < 0 ? 0 : r.rest) + (far < 0 ? at : far) / (far < 0 ? r.base + 1 : r.base);
+}
 
 // The weights of 32 scores and their sum; masked scores are -infinity.  All the
 // exponentials first: their results come some 40 cycles after they are asked for.
@@ -299,6 +297,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
   __shared__ Run s_run;
   __shared__ uint32_t s_bad[BAD_TURNS];        // of a tile: a byte per 32 keys, not 0: outside the cache
   __shared__ uint4 s_tile[TURNS][4];
+  __shared__ Seg s_seg[SEGS];                   // the segments under way; no tiles: the end
   __shared__ float s_ml[2 * 128];     // not PAIR: the second stream's m and l
   const uint32_t sbase = smem_u32(smem);
   auto bar = [&](int i) { return smem_u32(bars + i); };
@@ -314,6 +313,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
       mbar_init(bar(B_SOFT + i), PAIR ? 4 : 8);
     }
     for (int i = 0; i < TURNS; ++i) mbar_init(bar(B_TFULL + i), 1), mbar_init(bar(B_TEMPTY + i), 4);
+    for (int i = 0; i < SEGS; ++i) mbar_init(bar(B_GFULL + i), 1), mbar_init(bar(B_GEMPTY + i), SM_WARPS + 1);
     mbar_init(bar(B_DRAIN), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -389,8 +389,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
     }
   }
   __syncthreads();
-  Segments<ROWS, HEAD> segs(a, s_plan, s_run);
-  Seg sg;
   // a warp's arrival, its threads' writes before it
   auto arrive = [&](int b) {
     __syncwarp();
@@ -411,11 +409,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
 #pragma unroll
       for (int p = 0; p < PASS; ++p) {
         // volatile: issued here, a tile's time before they are used
-        asm volatile("ld.global.nc.v4.b32 {%0,%1,%2,%3}, [%4];"
+        asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
                      : "=r"(raw[p].x), "=r"(raw[p].y), "=r"(raw[p].z), "=r"(raw[p].w)
                      : "l"(x + p * KPP * (D / 2)));
         uint16_t e;
-        asm volatile("ld.global.nc.b16 %0, [%1];" : "=h"(e) : "l"(y + p * KPP * (D / 16)));
+        asm volatile("ld.global.nc.L1::no_allocate.b16 %0, [%1];" : "=h"(e) : "l"(y + p * KPP * (D / 16)));
         sc[p] = e;
       }
     };
@@ -502,10 +500,20 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R_REST));
     if (warp == W_SCOUT) {
       // ---------------- where the tiles lie, some ahead: lane g < 4 for 32 keys each ----------------
-      int slot = 0, set = 0;
-      uint32_t phase = 1, bturn = 0;
+      int slot = 0, set = 0, turn = 0;
+      uint32_t phase = 1, bturn = 0, gphase = 1;
       bool ok = true;
+      Segments<ROWS, HEAD> segs(a, s_plan, s_run);
+      Seg sg;
+      auto publish = [&]() {
+        ok = mbar_wait_warp(bar(B_GEMPTY + turn), gphase, nullptr, ERR_WAIT);
+        if (ok && lane == 0) s_seg[turn] = sg;
+        if (ok) arrive(B_GFULL + turn);
+        if (++turn == SEGS) turn = 0, gphase ^= 1;
+        return ok;
+      };
       while (ok && segs.next(sg)) {
+        if (!publish()) break;
         for (int t = sg.t0; t < sg.t1; ++t) {
           const int key0 = t * TILE + (lane & 3) * 32, left = sg.end - key0;
           const int key = min(key0, sg.end - 1);
@@ -537,7 +545,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
         }
         set = set == NAN_SETS - 1 ? 0 : set + 1;
       }
-      if (ok && mbar_wait_warp(bar(B_TEMPTY + slot), phase, nullptr, ERR_WAIT)) {
+      sg.t0 = sg.t1 = 0;
+      if (ok && publish() && mbar_wait_warp(bar(B_TEMPTY + slot), phase, nullptr, ERR_WAIT)) {
         if (lane < 4) s_tile[slot][lane] = make_uint4(NO_TILE, 0, 0, 0);
         arrive(B_TFULL + slot);
       }
@@ -573,7 +582,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
           const uint64_t v = desc_at(dv, vb * TILE16);
 #pragma unroll
           for (int s = 0; s < TILE / 16; ++s)
-            mma_ts(tmem + COL_O + i * 128, tmem + COL_S + i * 128 + s * 8, desc_at(v, s * 128), ID_O, !first || s > 0);
+            mma_ts(tmem + COL_O + i * 128, tmem + COL_S + COL_P + i * 128 + s * 8, desc_at(v, s * 128), ID_O, !first || s > 0);
           if (release) tc_commit(bar(B_VEMPTY + vb));
           if (last) tc_commit(bar(B_OFULL + i));
         }
@@ -590,8 +599,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
         ph ^= 1u << i;
         return r;
       };
-      while (ok && segs.next(sg)) {
-        const int n = sg.t1 - sg.t0;
+      int turn = 0;
+      uint32_t gphase = 0;
+      while (wait(B_GFULL + turn, gphase)) {
+        const int n = s_seg[turn].t1 - s_seg[turn].t0;
+        arrive(B_GEMPTY + turn);
+        if (n == 0) break;
+        if (++turn == SEGS) turn = 0, gphase ^= 1;
         if (PAIR) {
           if (!wait(B_KFULL + kb, kph) || !take(B_QFULL, 0, qph)) break;
           scores(0, false);
@@ -634,7 +648,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
     const int i = warp >> 2, wq = warp & 3, r = wq * 32 + lane;  // stream, its row
     const int first = PAIR ? i * 128 : 0;                        // of the stream's rows in the tile
     const uint32_t tq = tmem + ((uint32_t)(wq * 32) << 16);
-    const uint32_t ts = tq + COL_S + i * 128, to = tq + COL_O + i * 128;
+    const uint32_t ts = tq + COL_S + i * 128, tp = ts + COL_P, to = tq + COL_O + i * 128;
     const uint32_t sq = sbase + L::OFF_Q + i * L::TILE_BYTES;
     uint32_t sph = 0, oph = 0, softph = 0;
     int set = 0, bturn = 0;  // of s_nan; of s_bad, at the segment's first tile
@@ -718,39 +732,43 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
       }
     }
 
-    bool more = segs.next(sg);
-    Row x = {};
-    float f = 0.0f, scale = 0.0f;
+    int turn = 0;
+    uint32_t gphase = 0;
+    // the segment of this turn: whether there is one
+    auto segment = [&]() {
+      ok = mbar_wait_warp(bar(B_GFULL + turn), gphase, nullptr, ERR_WAIT);
+      return ok && s_seg[turn].t1 > 0;
+    };
+    auto scale_of = [&](const Seg& g) { return a.sm_log2 * __ldg(a.k_factor + g.kvh); };
+    bool more = segment();
+    float f = 0.0f;
     if (more) {
-      x = row_of(sg);
-      scale = a.sm_log2 * __ldg(a.k_factor + sg.kvh);
-      fetch_q(sg, x);
-      f = finish_q(scale);
+      fetch_q(s_seg[turn], row_of(s_seg[turn]));
+      f = finish_q(scale_of(s_seg[turn]));
     }
     while (more) {
-      const Seg cur = sg;
-      const Row now = x;
-      const float vf = __ldg(a.v_factor + cur.kvh);
-      more = segs.next(sg);
-      if (more) {
-        x = row_of(sg);
-        scale = a.sm_log2 * __ldg(a.k_factor + sg.kvh);
+      const Seg& cur = s_seg[turn];  // stays until this warp has let it go
+      const int mine = turn;
+      if (++turn == SEGS) turn = 0, gphase ^= 1;
+      int limit;  // the last key that the row sees
+      {
+        const Row x = row_of(cur);
+        limit = x.live ? cur.held + x.tok : -1;
       }
-      const int limit = now.live ? cur.held + now.tok : -1;  // the last key that the row sees
       // keys below: every row of the warp sees them (rows without a query do not count)
-      const int free_end = min(__reduce_min_sync(FULL, now.live ? limit : 0x7FFFFFFE), 0x7FFFFFFE) + 1;
-      const bool any_live = __any_sync(FULL, now.live);
+      const int free_end = min(__reduce_min_sync(FULL, limit >= 0 ? limit : 0x7FFFFFFE), 0x7FFFFFFE) + 1;
+      const bool any_live = __any_sync(FULL, limit >= 0);
       float m = NEG_INF, l = 0.0f;
-      const int n = cur.t1 - cur.t0;
+      const int n = cur.t1 - cur.t0, key00 = cur.t0 * TILE;
       bool any = false;  // this stream has had a tile
       for (int j = PAIR ? 0 : i; j < n; j += PAIR ? 1 : 2) {
         if (!(ok = mbar_wait_warp(bar(B_SFULL + i), sph, nullptr, ERR_WAIT))) break;
         sph ^= 1;
         tc_fence_after();
         // the last scores are there, so the queries' place is free: the next ones travel under this tile
-        if (PAIR && j + 1 == n && more) fetch_q(sg, x);
+        if (PAIR && j + 1 == n && (more = segment())) fetch_q(s_seg[turn], row_of(s_seg[turn]));
         if (any_live) {
-          const int key0 = (cur.t0 + j) * TILE;
+          const int key0 = key00 + j * TILE;
           const uint32_t bad = s_bad[(bturn + j) & (BAD_TURNS - 1)];
           float2 sum = make_float2(0.0f, 0.0f);
           // the reference m after scores whose largest is mx, and O and l with it
@@ -775,24 +793,29 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
             return m == NEG_INF ? P_EXP : P_EXP - m;
           };
           if (key0 + TILE <= free_end && !bad) {
-            uint32_t va[32], vb[32], vc[32], vd[32], p[16];
+            // the upper half stays in registers; its weights free the place of the lower half's
+            uint32_t va[32], vb[32], p[16];
             tmem_ld32(ts, va);
             tmem_ld32(ts + 32, vb);
             tmem_ld_wait();
-            tmem_ld32(ts + 64, vc);
-            tmem_ld32(ts + 96, vd);
             float mx = fmaxf(max32(va, NEG_INF), max32(vb, NEG_INF));
+            tmem_ld32(ts + 64, va);
+            tmem_ld32(ts + 96, vb);
             tmem_ld_wait();
-            mx = fmaxf(mx, fmaxf(max32(vc, NEG_INF), max32(vd, NEG_INF)));
+            mx = fmaxf(mx, fmaxf(max32(va, NEG_INF), max32(vb, NEG_INF)));
             const float bias = refer(mx);
             weights32(va, f, bias, sum, p);
-            tmem_st16(ts, p);
+            tmem_ld32(ts, va);
+            tmem_st16(tp + 32, p);
             weights32(vb, f, bias, sum, p);
-            tmem_st16(ts + 16, p);
-            weights32(vc, f, bias, sum, p);
-            tmem_st16(ts + 32, p);
-            weights32(vd, f, bias, sum, p);
-            tmem_st16(ts + 48, p);
+            tmem_ld_wait();
+            tmem_ld32(ts + 32, vb);
+            tmem_st16(tp + 48, p);
+            weights32(va, f, bias, sum, p);
+            tmem_ld_wait();
+            tmem_st16(tp, p);
+            weights32(vb, f, bias, sum, p);
+            tmem_st16(tp + 16, p);
           } else {  // some scores are -infinity: their key lies past the row's last, or in no page
             auto masked32 = [&](int c, uint32_t (&v)[32]) {
               tmem_ld32(ts + 32 * c, v);
@@ -810,10 +833,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
             }
             const float bias = refer(mx);
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 3; c >= 0; --c) {  // from above, as the places free up
               masked32(c, v);
               weights32(v, f, bias, sum, p);
-              tmem_st16(ts + 16 * c, p);
+              tmem_st16(tp + 16 * c, p);
             }
           }
           l += sum.x + sum.y;
@@ -824,7 +847,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
         arrive(B_PFULL + i);
       }
       if (!ok) break;
-      if (PAIR && more) f = finish_q(scale);  // while the last product runs
+      if (PAIR && more) f = finish_q(scale_of(s_seg[turn]));  // while the last product runs
       bturn = (bturn + n) & (BAD_TURNS - 1);
       const bool had = PAIR || i < n;  // this stream's O has been written
       if (had) {
@@ -833,6 +856,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
         tc_fence_after();
       }
       // ---- the end of a segment ----
+      const Row now = row_of(cur);
+      const float vf = __ldg(a.v_factor + cur.kvh);
       uint16_t* orow = a.out + (((int64_t)cur.b * a.T + now.tok) * a.H + now.head) * D;
       const bool writer = PAIR || i == 0;
       float ow = 1.0f, xw = 0.0f;  // weights of this stream's O and of the other's
@@ -911,9 +936,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
       } else {
         if (writer && now.live) piece[128 * D + r] = m, piece[128 * (D + 1) + r] = l;
         // the stream that finishes last reads the head's pieces in the CTAs' order
-        int c0, c1, slot0;
-        segs.pieces_of(cur, c0, c1, slot0);
-        const int pieces = c1 - c0 + 1, me = PAIR ? i : 0;
+        const int c0 = run_of(s_run, cur.ps + HEAD), pieces = run_of(s_run, cur.ps + HEAD + cur.tiles - 1) - c0 + 1;
+        // which of its first run's pieces is the head's
+        const int slot0 = c0 * s_run.base + min(c0, s_run.rest) >= cur.ps ? 0 : 1, me = PAIR ? i : 0;
         int* done = a.done + (PAIR ? 2 * cur.pair + i : cur.pair);
         if (!soft_sync()) break;
         if (threadIdx.x == (PAIR ? 128 * i : 0)) {
@@ -993,11 +1018,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
       __syncwarp();
       if (lane < D / 16) s_nan[warp][set][lane] = 0x7FFFFFFF;
       set = set == NAN_SETS - 1 ? 0 : set + 1;
+      arrive(B_GEMPTY + mine);
       if (!PAIR) {
         if (!soft_sync()) break;  // the queries' place was read
+        more = segment();
         if (more) {
-          fetch_q(sg, x);
-          f = finish_q(scale);
+          fetch_q(s_seg[turn], row_of(s_seg[turn]));
+          f = finish_q(scale_of(s_seg[turn]));
         }
       }
     }
