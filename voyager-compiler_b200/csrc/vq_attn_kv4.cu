@@ -68,7 +68,7 @@ constexpr float P_EXP = 7.0f, LAG = 8.0f;
 constexpr int NAN_SETS = 3;  // a segment's, of which the epilogue of one and the loads of two more can be under way
 
 enum { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_VEMPTY = 6, B_QFULL = 8, B_SFULL = 10, B_PFULL = 12, B_OFULL = 14,
-       B_SOFT = 16, B_DRAIN = 18, B_TFULL = 20, B_TEMPTY = 24, B_GFULL = 28, B_GEMPTY = 32, NBARS = 36 };
+       B_SOFT = 16, B_DRAIN = 18, B_TFULL = 20, B_TEMPTY = 24, B_GFULL = 28, B_GEMPTY = 32, B_PHALF = 36, NBARS = 38 };
 static_assert(NBARS * 8 <= 512, "barrier area");
 // tiles whose places are known, and words of pages outside the cache (of a tile until its softmax has begun: the two in
 // the buffers and those known)
@@ -94,6 +94,7 @@ struct Args {
   const int32_t *block_table, *lengths, *counts;
   float* part;    // [CTAs][2][streams with rows of their own][D + 2][128]: pieces of heads that were cut
   int32_t* done;  // [B * groups * Hkv][streams ..] zero before, zero after
+  int32_t* next;  // heads taken whole so far: zero before, zero after
   int B, T, H, Hkv, G, page_log2, width, pages, groups;
   float sm_log2;
 };
@@ -200,18 +201,24 @@ template <bool PAIR>
 struct Cost {
   static constexpr int HEAD = PAIR ? 2 : 1;
 };
+constexpr float CUT = 5.0f;
 
 // This CTA's run lies from lo to hi; its first head is of `entry`, which begins
 // at `before`.  Heads lie end to end, HEAD + tiles each; a cut within the first
 // HEAD of one moves to its begin.
 struct Run {
   int lo, hi, entry, before, base, rest;  // the first `rest` runs are base + 1 long
+  int uncut;                              // no cuts: heads are taken whole, one after the other
 };
 __device__ __forceinline__ int run_of(const Run& r, int at);
 // Segments, one after the other: the part of one head (entry, kv head) in the run.
 struct Seg {
   int b, row0, nrows, held, end, kvh, t0, t1, tiles, slot, pair, ps;
   bool whole;
+  __device__ __forceinline__ void set(const Entry& x, int e, int kv_heads, int h, int n) {
+    b = x.b, row0 = x.row0, nrows = x.nrows, held = x.held, end = x.end, tiles = n;
+    kvh = h, pair = e * kv_heads + h;
+  }
 };
 template <int ROWS, int HEAD>
 struct Segments {
@@ -230,9 +237,7 @@ struct Segments {
       x = entry_of<ROWS>(a, ++e, plans);
       tiles = tiles_of(x);
     }
-    s.b = x.b, s.row0 = x.row0, s.nrows = x.nrows, s.held = x.held, s.end = x.end, s.tiles = tiles;
-    s.kvh = (pos - ebase) / (tiles + HEAD);
-    s.pair = e * a.Hkv + s.kvh;
+    s.set(x, e, a.Hkv, (pos - ebase) / (tiles + HEAD), tiles);
     s.ps = ebase + s.kvh * (tiles + HEAD);
     s.t0 = max(0, pos - s.ps - HEAD);
     s.t1 = min(tiles, r.hi - s.ps - HEAD);
@@ -295,6 +300,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
   __shared__ long long s_sum[WARPS];
   __shared__ int2 s_plan[PLANS];
   __shared__ Run s_run;
+  __shared__ int s_top;
   __shared__ uint32_t s_bad[BAD_TURNS];        // of a tile: a byte per 32 keys, not 0: outside the cache
   __shared__ uint4 s_tile[TURNS][4];
   __shared__ Seg s_seg[SEGS];                   // the segments under way; no tiles: the end
@@ -309,7 +315,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
       mbar_init(bar(B_KFULL + i), 4), mbar_init(bar(B_KEMPTY + i), 1);
       mbar_init(bar(B_VFULL + i), 4), mbar_init(bar(B_VEMPTY + i), 1);
       mbar_init(bar(B_QFULL + i), 4), mbar_init(bar(B_SFULL + i), 1);
-      mbar_init(bar(B_PFULL + i), 4), mbar_init(bar(B_OFULL + i), 1);
+      mbar_init(bar(B_PFULL + i), 4), mbar_init(bar(B_PHALF + i), 4), mbar_init(bar(B_OFULL + i), 1);
       mbar_init(bar(B_SOFT + i), PAIR ? 4 : 8);
     }
     for (int i = 0; i < TURNS; ++i) mbar_init(bar(B_TFULL + i), 1), mbar_init(bar(B_TEMPTY + i), 4);
@@ -323,7 +329,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   for (int i = threadIdx.x; i < SM_WARPS * NAN_SETS * (D / 16); i += THREADS) (&s_nan[0][0][0])[i] = 0x7FFFFFFF;
-  if (threadIdx.x == 0) s_run.lo = s_run.hi = 0;
+  if (threadIdx.x == 0) s_run.lo = s_run.hi = s_top = 0;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -342,10 +348,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
   const int entries = a.B * a.groups, per = (entries + THREADS - 1) / THREADS;
   const int e0 = min(entries, (int)threadIdx.x * per), e1 = min(entries, e0 + per);
   long long own = 0;  // tiles, and in the upper half entries that have any
+  int top = 0;
 #pragma unroll 1
   for (int e = e0; e < e1; ++e) {
     const int u = tiles_of(entry_of<ROWS>(a, e, s_plan));
     own += u ? u + (1ll << 32) : 0;
+    top = max(top, u);
   }
   long long scan = own;
 #pragma unroll
@@ -361,9 +369,24 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
     if (w < warp) before += s_sum[w];
     total += s_sum[w];
   }
+  // The longest head, for the choice between cut and uncut heads.
+  top = __reduce_max_sync(FULL, top);
+  if (lane == 0) atomicMax(&s_top, top);
+  __syncthreads();
+  top = s_top;
   {
     const int heads = (int)(total >> 32) * a.Hkv, real = (int)total * a.Hkv, all = real + HEAD * heads;
-    const int runs = min((int)gridDim.x, (int)ceilf((float)real / run_least(real, heads)));
+    // Uncut, CTAs idle at the end for about a quarter of an average head where
+    // lengths differ (the long ones come first), and for what a whole number of equal
+    // heads leaves where they do not; a cut costs its pieces' way through memory and
+    // their join, about CUT tiles a CTA.
+    const int ctas = (int)gridDim.x;
+    const float mean = heads ? (float)all / (float)heads : 0.0f;
+    const float idle = 2.0f * (top + HEAD) <= 3.0f * mean
+                           ? (float)((heads + ctas - 1) / ctas) * mean - (float)all / (float)ctas : 0.25f * mean;
+    const bool uncut = PAIR && heads >= 2 * ctas && idle <= CUT;
+    if (threadIdx.x == 0) s_run.uncut = uncut;
+    const int runs = uncut ? 0 : min(ctas, (int)ceilf((float)real / run_least(real, heads)));
     const int base = runs ? all / runs : 0, rest = all - base * runs;
     const int cut0 = blockIdx.x * base + min((int)blockIdx.x, rest), cut1 = cut0 + base + ((int)blockIdx.x < rest);
     int at = ((int)before + HEAD * (int)(before >> 32)) * a.Hkv;
@@ -512,7 +535,28 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
         if (++turn == SEGS) turn = 0, gphase ^= 1;
         return ok;
       };
-      while (ok && segs.next(sg)) {
+      const int heads = a.B * a.groups * a.Hkv;
+      auto next = [&]() {
+        if (!s_run.uncut) return segs.next(sg);
+        // the next head that no CTA has taken, sequences' last row tiles (the longest) first
+        while (true) {
+          int k = 0;
+          if (lane == 0) k = atomicAdd(a.next, 1);
+          k = __shfl_sync(FULL, k, 0);
+          if (k >= heads) {  // each CTA comes here once; the last of them leaves 0
+            if (k == heads + (int)gridDim.x - 1 && lane == 0) *a.next = 0;
+            return false;
+          }
+          const int kvh = k % a.Hkv, b = k / a.Hkv % a.B, e = b * a.groups + a.groups - 1 - k / a.Hkv / a.B;
+          const Entry x = entry_of<ROWS>(a, e, s_plan);
+          const int n = tiles_of(x);
+          if (n == 0) continue;
+          sg.set(x, e, a.Hkv, kvh, n);
+          sg.ps = sg.slot = sg.t0 = 0, sg.t1 = n, sg.whole = true;
+          return true;
+        }
+      };
+      while (ok && next()) {
         if (!publish()) break;
         for (int t = sg.t0; t < sg.t1; ++t) {
           const int key0 = t * TILE + (lane & 3) * 32, left = sg.end - key0;
@@ -559,7 +603,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
                      dv = mn_desc(sbase + L::OFF_V, L::HALF);
       constexpr uint32_t TILE16 = L::TILE_BYTES / 16;
       int kb = 0, vb = 0;
-      uint32_t kph = 0, vph = 0, qph = 0, pph = 0;  // of the streams: bits 0 and 1
+      uint32_t kph = 0, vph = 0, qph = 0, hph = 0, pph = 0;  // of the streams: bits 0 and 1
       bool ok = true;
       // S of stream i from K buffer kb; `release`: its last reader
       auto scores = [&](int i, bool release) {
@@ -576,13 +620,24 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
         __syncwarp();
         if (release && ++kb == 2) kb = 0, kph ^= 1;
       };
-      // O of stream i from V buffer vb; `last`: of the segment
-      auto values = [&](int i, bool first, bool release, bool last) {
+      // O of stream i from V buffer vb: the upper half of the keys, whose weights are
+      // there first, then the lower; `last`: of the segment
+      auto upper = [&](int i, bool first) {
         if (elect_one()) {
           const uint64_t v = desc_at(dv, vb * TILE16);
 #pragma unroll
-          for (int s = 0; s < TILE / 16; ++s)
-            mma_ts(tmem + COL_O + i * 128, tmem + COL_S + COL_P + i * 128 + s * 8, desc_at(v, s * 128), ID_O, !first || s > 0);
+          for (int s = TILE / 32; s < TILE / 16; ++s)
+            mma_ts(tmem + COL_O + i * 128, tmem + COL_S + COL_P + i * 128 + s * 8, desc_at(v, s * 128), ID_O,
+                   !first || s > TILE / 32);
+        }
+        __syncwarp();
+      };
+      auto lower = [&](int i, bool release, bool last) {
+        if (elect_one()) {
+          const uint64_t v = desc_at(dv, vb * TILE16);
+#pragma unroll
+          for (int s = 0; s < TILE / 32; ++s)
+            mma_ts(tmem + COL_O + i * 128, tmem + COL_S + COL_P + i * 128 + s * 8, desc_at(v, s * 128), ID_O, 1);
           if (release) tc_commit(bar(B_VEMPTY + vb));
           if (last) tc_commit(bar(B_OFULL + i));
         }
@@ -614,11 +669,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
           for (int j = 0; j < n; ++j) {
             const bool again = j + 1 < n;
             // the tiles are there before the weights are: the products then follow each other
-            if (!wait(B_VFULL + vb, vph) || (again && !wait(B_KFULL + kb, kph)) || !take(B_PFULL, 0, pph)) break;
-            values(0, j == 0, false, !again);
+            if (!wait(B_VFULL + vb, vph) || (again && !wait(B_KFULL + kb, kph)) || !take(B_PHALF, 0, hph)) break;
+            upper(0, j == 0);
+            if (!take(B_PFULL, 0, pph)) break;
+            lower(0, false, !again);
             if (again) scores(0, false);
+            if (!take(B_PHALF, 1, hph)) break;
+            upper(1, j == 0);
             if (!take(B_PFULL, 1, pph)) break;
-            values(1, j == 0, true, !again);
+            lower(1, true, !again);
             if (again) scores(1, true);
           }
         } else {
@@ -629,8 +688,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
           }
           for (int j = 0; j < n && ok; ++j) {
             const int i = j & 1;
-            if (!wait(B_VFULL + vb, vph) || (j + 2 < n && !wait(B_KFULL + kb, kph)) || !take(B_PFULL, i, pph)) break;
-            values(i, j < 2, true, j + 2 >= n);
+            if (!wait(B_VFULL + vb, vph) || (j + 2 < n && !wait(B_KFULL + kb, kph)) || !take(B_PHALF, i, hph)) break;
+            upper(i, j < 2);
+            if (!take(B_PFULL, i, pph)) break;
+            lower(i, true, j + 2 >= n);
             if (j + 2 < n) scores(i, true);
           }
         }
@@ -811,6 +872,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
             tmem_ld_wait();
             tmem_ld32(ts + 32, vb);
             tmem_st16(tp + 48, p);
+            tmem_st_wait();
+            tc_fence_before();
+            arrive(B_PHALF + i);
             weights32(va, f, bias, sum, p);
             tmem_ld_wait();
             tmem_st16(tp, p);
@@ -837,11 +901,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
               masked32(c, v);
               weights32(v, f, bias, sum, p);
               tmem_st16(tp + 16 * c, p);
+              if (c == 2) {
+                tmem_st_wait();
+                tc_fence_before();
+                arrive(B_PHALF + i);
+              }
             }
           }
           l += sum.x + sum.y;
           tmem_st_wait();
           any = true;
+        } else {
+          arrive(B_PHALF + i);
         }
         tc_fence_before();
         arrive(B_PFULL + i);
@@ -1055,7 +1126,7 @@ static Cut cut_of(int64_t batch, int64_t tokens, int heads, int kv_heads, int64_
 void workspace(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim, int64_t capacity, int64_t* floats,
                int64_t* counters) {
   const Cut c = cut_of(batch, tokens, heads, kv_heads, capacity);
-  *counters = batch * kv_heads * c.groups * (c.rows / 128);
+  *counters = batch * kv_heads * c.groups * (c.rows / 128) + 1;
   *floats = (int64_t)c.ctas * 2 * c.rows * (head_dim + 2);
 }
 
@@ -1081,7 +1152,7 @@ int attend(const void* q, const int64_t* q_strides, int64_t batch, int64_t token
   const Cut c = cut_of(batch, tokens, heads, kv_heads, capacity);
   const int64_t pairs = batch * kv_heads * c.groups;
   // the tiles of all heads, counted in 32 bits
-  if (pairs * ((capacity + TILE - 1) / TILE + 3) >= (1ll << 31) || counters_len < pairs * (c.rows / 128)) return VQ_ERR_INVALID;
+  if (pairs * ((capacity + TILE - 1) / TILE + 3) >= (1ll << 31) || counters_len < pairs * (c.rows / 128) + 1) return VQ_ERR_INVALID;
   if (!workspace || workspace_floats < (int64_t)c.ctas * 2 * c.rows * (head_dim + 2)) return VQ_ERR_INVALID;
   Args a;
   a.q = (const uint16_t*)q;
@@ -1094,7 +1165,7 @@ int attend(const void* q, const int64_t* q_strides, int64_t batch, int64_t token
   a.lengths = (const int32_t*)lengths;
   a.counts = (const int32_t*)counts;
   a.part = workspace;
-  a.done = counters;
+  a.next = counters, a.done = counters + 1;
   a.B = (int)batch, a.T = (int)tokens, a.H = heads, a.Hkv = kv_heads, a.G = heads / kv_heads;
   a.page_log2 = page == 32 ? 5 : page == 64 ? 6 : 7;
   a.width = (int)table_width, a.pages = (int)pages, a.groups = c.groups;
