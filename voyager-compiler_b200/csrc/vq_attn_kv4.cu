@@ -65,6 +65,7 @@ static_assert(2 * R_SOFT + R_DQ + R_REST <= 4 * R_LAUNCH, "a register taken was 
 constexpr int SOFT = SM_WARPS * 32;
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr float P_EXP = 7.0f, LAG = 8.0f;
+constexpr int FMA_PAIRS = 0;  // of 16 pairs of exponentials, those of the FMA pipe
 constexpr int NAN_SETS = 3;  // a segment's, of which the epilogue of one and the loads of two more can be under way
 
 enum { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_VEMPTY = 6, B_QFULL = 8, B_SFULL = 10, B_PFULL = 12, B_OFULL = 14,
@@ -253,26 +254,55 @@ __device__ __forceinline__ int run_of(const Run& r, int at) {
   return (far < 0 ? 0 : r.rest) + (far < 0 ? at : far) / (far < 0 ? r.base + 1 : r.base);
 }
 
-// The weights of 32 scores and their sum; masked scores are -infinity.  All the
-// exponentials first: their results come some 40 cycles after they are asked for.
+// 2^x of two values in [-126, 127] by the FMA pipe: 2^n 2^r with n the nearest
+// integer, which x + 1.5 * 2^23 has in its low bits, and a cubic whose relative
+// error over r in [-1/2, 1/2] is least, 2^-13.7 (its coefficients are the solution
+// of that minimax problem).  Smaller x give 2^-126.
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
+  const float2 big = make_float2(12582912.0f, 12582912.0f), t = __fadd2_rn(x, big);
+  const float2 n = __fadd2_rn(t, make_float2(-12582912.0f, -12582912.0f));
+  const float2 r = __ffma2_rn(n, make_float2(-1.0f, -1.0f), x);
+  float2 p = __ffma2_rn(make_float2(0.0551716685f, 0.0551716685f), r, make_float2(0.242611125f, 0.242611125f));
+  p = __ffma2_rn(p, r, make_float2(0.693260968f, 0.693260968f));
+  p = __ffma2_rn(p, r, make_float2(0.999928057f, 0.999928057f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+// The weights of 32 scores and their sum, FMA of the 16 pairs by exp2_fma: the
+// special function unit gives 4 results a cycle and scheduler, and would be what
+// the tile takes longest for.  The other exponentials are asked for first.  Masked
+// scores, -infinity, need FMA = 0.
+template <int FMA>
 __device__ __forceinline__ void weights32(uint32_t (&v)[32], float f, float bias, float2& sum, uint32_t (&p)[16]) {
   const float2 ff = make_float2(f, f), bb = make_float2(bias, bias);
-  float e[32];
-#pragma unroll
-  for (int q = 0; q < 32; q += 2) {
-    const float2 x = __ffma2_rn(make_float2(__uint_as_float(v[q]), __uint_as_float(v[q + 1])), ff, bb);
-    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[q]) : "f"(x.x));
-    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[q + 1]) : "f"(x.y));
-  }
+  float2 e[16];
 #pragma unroll
   for (int q = 0; q < 16; ++q) {
-    sum = __fadd2_rn(sum, make_float2(e[2 * q], e[2 * q + 1]));
-    asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[q]) : "f"(e[2 * q + 1]), "f"(e[2 * q]));
+    e[q] = __ffma2_rn(make_float2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])), ff, bb);
+    if ((q + 1) * FMA / 16 == q * FMA / 16) {
+      asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[q].x));
+      asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[q].y));
+    }
   }
+#pragma unroll
+  for (int q = 0; q < 16; ++q)
+    if ((q + 1) * FMA / 16 != q * FMA / 16) e[q] = exp2_fma(e[q]);
+#pragma unroll
+  for (int q = 0; q < 16; ++q) {
+    sum = __fadd2_rn(sum, e[q]);
+    asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[q]) : "f"(e[q].y), "f"(e[q].x));
+  }
+}
+// The largest of m and 32 scores; NaN where one is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 __device__ __forceinline__ float max32(const uint32_t (&v)[32], float m) {
 #pragma unroll
-  for (int q = 0; q < 32; q += 2) m = fmaxf(fmaxf(__uint_as_float(v[q]), __uint_as_float(v[q + 1])), m);
+  for (int q = 0; q < 32; q += 2) m = max_nan(max_nan(__uint_as_float(v[q]), __uint_as_float(v[q + 1])), m);
   return m;
 }
 // 32 bytes, a whole sector.
@@ -819,6 +849,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
       // keys below: every row of the warp sees them (rows without a query do not count)
       const int free_end = min(__reduce_min_sync(FULL, limit >= 0 ? limit : 0x7FFFFFFE), 0x7FFFFFFE) + 1;
       const bool any_live = __any_sync(FULL, limit >= 0);
+      const float vf = __ldg(a.v_factor + cur.kvh);
       float m = NEG_INF, l = 0.0f;
       const int n = cur.t1 - cur.t0, key00 = cur.t0 * TILE;
       bool any = false;  // this stream has had a tile
@@ -859,26 +890,27 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
             tmem_ld32(ts, va);
             tmem_ld32(ts + 32, vb);
             tmem_ld_wait();
-            float mx = fmaxf(max32(va, NEG_INF), max32(vb, NEG_INF));
+            float mx = max_nan(max32(va, NEG_INF), max32(vb, NEG_INF));
             tmem_ld32(ts + 64, va);
             tmem_ld32(ts + 96, vb);
             tmem_ld_wait();
-            mx = fmaxf(mx, fmaxf(max32(va, NEG_INF), max32(vb, NEG_INF)));
+            mx = max_nan(mx, max_nan(max32(va, NEG_INF), max32(vb, NEG_INF)));
+            if (mx != mx) l = mx;  // a score is NaN: so is the row
             const float bias = refer(mx);
-            weights32(va, f, bias, sum, p);
+            weights32<FMA_PAIRS>(va, f, bias, sum, p);
             tmem_ld32(ts, va);
             tmem_st16(tp + 32, p);
-            weights32(vb, f, bias, sum, p);
+            weights32<FMA_PAIRS>(vb, f, bias, sum, p);
             tmem_ld_wait();
             tmem_ld32(ts + 32, vb);
             tmem_st16(tp + 48, p);
             tmem_st_wait();
             tc_fence_before();
             arrive(B_PHALF + i);
-            weights32(va, f, bias, sum, p);
+            weights32<FMA_PAIRS>(va, f, bias, sum, p);
             tmem_ld_wait();
             tmem_st16(tp, p);
-            weights32(vb, f, bias, sum, p);
+            weights32<FMA_PAIRS>(vb, f, bias, sum, p);
             tmem_st16(tp + 16, p);
           } else {  // some scores are -infinity: their key lies past the row's last, or in no page
             auto masked32 = [&](int c, uint32_t (&v)[32]) {
@@ -899,7 +931,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
 #pragma unroll 1
             for (int c = 3; c >= 0; --c) {  // from above, as the places free up
               masked32(c, v);
-              weights32(v, f, bias, sum, p);
+              weights32<0>(v, f, bias, sum, p);
               tmem_st16(tp + 16 * c, p);
               if (c == 2) {
                 tmem_st_wait();
@@ -928,7 +960,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
       }
       // ---- the end of a segment ----
       const Row now = row_of(cur);
-      const float vf = __ldg(a.v_factor + cur.kvh);
       uint16_t* orow = a.out + (((int64_t)cur.b * a.T + now.tok) * a.H + now.head) * D;
       const bool writer = PAIR || i == 0;
       float ow = 1.0f, xw = 0.0f;  // weights of this stream's O and of the other's
@@ -1022,7 +1053,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
           auto at_piece = [&](int p) {
             return a.part + (((int64_t)(c0 + p) * 2 + (p == 0 ? slot0 : 0)) * (PAIR ? 2 : 1) + me) * PIECE;
           };
-          // A warp takes 32 rows and every WPB-th group of four columns, four groups at a time.
+          // A warp takes 32 rows and every wpb-th 16 columns of them, two at a time.
           const int rows = min(128, cur.nrows - first), blocks = max(1, (rows + 31) / 32);
           constexpr int W = PAIR ? 4 : 8;
           const int w = PAIR ? wq : warp, wpb = W / (blocks == 3 ? 4 : blocks), blk = w / wpb;
@@ -1049,36 +1080,45 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
             }
             const float ref = mm == NEG_INF ? 0.0f : mm, g = ll == 0.0f ? 0.0f : __fdiv_rn(vf, ll);
 #pragma unroll 1
-            for (int g0 = w % wpb; g0 < D / 4; g0 += 4 * wpb) {
-              float4 acc[4] = {};
+            for (int c = w % wpb; c < D / 16; c += 2 * wpb) {
+              float4 acc[2][4] = {};
 #pragma unroll 1
-              for (int p0 = 0; p0 < pieces; p0 += 2) {
-                float4 y[2][4];
+              for (int p0 = 0; p0 < pieces; p0 += 2) {  // all loads of two pieces in flight together
+                float4 y[2][2][4];
                 float pm[2];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                   const float* src = at_piece(min(p0 + k, pieces - 1));
                   pm[k] = __ldcg(src + 128 * D + rr);
 #pragma unroll
-                  for (int q = 0; q < 4; ++q)
-                    y[k][q] = __ldcg(reinterpret_cast<const float4*>(src) + min(g0 + q * wpb, D / 4 - 1) * 128 + rr);
+                  for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                      y[k][h][q] = __ldcg(reinterpret_cast<const float4*>(src) +
+                                          (4 * min(c + h * wpb, D / 16 - 1) + q) * 128 + rr);
                 }
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
                   if (p0 + k < pieces) {
                     const float e = ex2(pm[k] - ref);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                      acc[q].x = fmaf(y[k][q].x, e, acc[q].x), acc[q].y = fmaf(y[k][q].y, e, acc[q].y);
-                      acc[q].z = fmaf(y[k][q].z, e, acc[q].z), acc[q].w = fmaf(y[k][q].w, e, acc[q].w);
-                    }
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                      for (int q = 0; q < 4; ++q) {
+                        float4 &t = acc[h][q], z = y[k][h][q];
+                        t.x = fmaf(z.x, e, t.x), t.y = fmaf(z.y, e, t.y), t.z = fmaf(z.z, e, t.z), t.w = fmaf(z.w, e, t.w);
+                      }
                   }
               }
 #pragma unroll
-              for (int q = 0; q < 4; ++q)
-                if (g0 + q * wpb < D / 4)
-                  *reinterpret_cast<uint2*>(dst + 4 * (g0 + q * wpb)) =
-                      make_uint2(bf_pack(acc[q].x * g, acc[q].y * g), bf_pack(acc[q].z * g, acc[q].w * g));
+              for (int h = 0; h < 2; ++h)
+                if (c + h * wpb < D / 16) {
+                  uint32_t o[8];
+#pragma unroll
+                  for (int q = 0; q < 4; ++q)
+                    o[2 * q] = bf_pack(acc[h][q].x * g, acc[h][q].y * g), o[2 * q + 1] = bf_pack(acc[h][q].z * g, acc[h][q].w * g);
+                  stg256(dst + 16 * (c + h * wpb), o);
+                }
             }
           }
           if (writer && !now.live && now.exists) blank();
