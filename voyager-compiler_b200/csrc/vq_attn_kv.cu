@@ -1138,8 +1138,17 @@ int sticky_kva(int* out, int clear, cudaStream_t st) { return vq::tc::sticky_rea
 
 using namespace vq::kva;
 
-// The 4-bit cache under more rows a kv head than this is vq_attn_kv4.cu's.
-constexpr int64_t FEW_ROWS = 16;
+// Whether a call on the 4-bit cache is this file's, or vq_attn_kv4.cu's.  There a
+// tile of 128 keys costs the same for 1 to 128 rows a kv head, here once for every
+// group of 16; the start there costs 10 us more.  With t tiles in the block table and
+// g groups that makes about 12 + 0.0052 t g us here and 22 + 0.0119 t there (heads of
+// 128: 3768 tiles, 32 rows 58 us here and 63 there, 35 rows 74 and 64, 128 rows 171
+// and 68; 128 tiles, 128 rows 21 and 32; heads of 64: 43, 53, 121 here, 49 to 51
+// there; 16 and 23).  Tables are as wide as the longest sequence: 1.6 times that t.
+static bool few_rows(int64_t batch, int64_t rows, int kv_heads, int64_t capacity) {
+  const int64_t g = (rows + 15) / 16, t = batch * kv_heads * ((capacity + 127) / 128);
+  return g <= 2 || (g <= 8 && t * (4 * g - 9) <= 12000);
+}
 
 static int workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t page,
                      int64_t table_width, int64_t* floats, int64_t* counters, bool fp4) {
@@ -1147,7 +1156,7 @@ static int workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_he
   if (batch < 0 || tokens < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0 ||
       page <= 0 || table_width < 0 || table_width > max_width(page))
     return VQ_ERR_INVALID;
-  if (fp4 && tokens * (heads / kv_heads) > FEW_ROWS) {
+  if (fp4 && !few_rows(batch, tokens * (heads / kv_heads), kv_heads, table_width * page)) {
     vq::kv4::workspace(batch, tokens, heads, kv_heads, head_dim, table_width * page, floats, counters);
     return VQ_OK;
   }
@@ -1196,7 +1205,7 @@ static int attention(const void* q, const int64_t* q_strides, int64_t batch, int
     if (reinterpret_cast<uintptr_t>(p) & 15) return VQ_ERR_ALIGNMENT;
   for (int i = 0; i < 3; ++i)
     if (q_strides[i] % 8) return VQ_ERR_ALIGNMENT;
-  if (fp4 && tokens * a.G > FEW_ROWS)
+  if (fp4 && !few_rows(batch, tokens * a.G, kv_heads, table_width * page))
     return vq::kv4::attend(q, q_strides, batch, tokens, heads, kv_heads, head_dim, k_codes, v_codes, k_scale, v_scale,
                            k_factor, v_factor, pages, page, block_table, table_width, lengths, counts, sm_scale,
                            workspace, workspace_floats, counters, counters_len, out, st);

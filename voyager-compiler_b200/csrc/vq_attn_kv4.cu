@@ -56,20 +56,20 @@ enum { ERR_WAIT = 331, ERR_PAGE = 332, ERR_CAPACITY = 333, ERR_COUNT = 334 };
 
 constexpr int TILE = 128;  // keys
 constexpr int PLANS = 128;
-// warps: 0-7 softmax (a stream's four each), 8-11 codes to f16, 12 the MMAs, 13 where the tiles lie, 14 and 15 none
-// (a warpgroup's registers are split together)
-constexpr int SM_WARPS = 8, W_DQ = 8, W_MMA = 12, W_SCOUT = 13, WARPS = 16, THREADS = WARPS * 32;
-// registers a thread: launched with 128; a warpgroup of 4 warps gives some up or takes them
-constexpr int R_LAUNCH = 128, R_SOFT = 184, R_DQ = 80, R_REST = 64;
-static_assert(2 * R_SOFT + R_DQ + R_REST <= 4 * R_LAUNCH, "a register taken was given up before");
+// warps: 0-7 softmax (a stream's four each), 8-11 K and 12-15 V from codes to f16, 16 the MMAs, 17 where the tiles
+// lie, 18 and 19 none (a warpgroup's registers are split together)
+constexpr int SM_WARPS = 8, W_DQ = 8, W_MMA = 16, W_SCOUT = 17, WARPS = 20, THREADS = WARPS * 32;
+// registers a thread: launched with 96; a warpgroup of 4 warps gives some up or takes them
+constexpr int R_LAUNCH = 96, R_SOFT = 144, R_DQ = 56, R_REST = 80;
+static_assert(2 * R_SOFT + 2 * R_DQ + R_REST <= 5 * R_LAUNCH, "a register taken was given up before");
 constexpr int SOFT = SM_WARPS * 32;
 constexpr float NEG_INF = -__builtin_huge_valf();
 constexpr float P_EXP = 7.0f, LAG = 8.0f;
-constexpr int FMA_PAIRS = 0;  // of 16 pairs of exponentials, those of the FMA pipe
 constexpr int NAN_SETS = 3;  // a segment's, of which the epilogue of one and the loads of two more can be under way
 
-enum { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_VEMPTY = 6, B_QFULL = 8, B_SFULL = 10, B_PFULL = 12, B_OFULL = 14,
-       B_SOFT = 16, B_DRAIN = 18, B_TFULL = 20, B_TEMPTY = 24, B_GFULL = 28, B_GEMPTY = 32, B_PHALF = 36, NBARS = 38 };
+// S and P: two of each stream, for the halves of a tile
+enum { B_KFULL = 0, B_KEMPTY = 2, B_VFULL = 4, B_VEMPTY = 6, B_QFULL = 8, B_ODONE = 10, B_SFULL = 12, B_PFULL = 36,
+       B_SOFT = 16, B_DRAIN = 18, B_TFULL = 20, B_TEMPTY = 24, B_GFULL = 28, B_GEMPTY = 32, B_OFULL = 40, NBARS = 42 };
 static_assert(NBARS * 8 <= 512, "barrier area");
 // tiles whose places are known, and words of pages outside the cache (of a tile until its softmax has begun: the two in
 // the buffers and those known)
@@ -77,7 +77,6 @@ constexpr int TURNS = 4, BAD_TURNS = 16, SEGS = 4;
 constexpr uint32_t NO_TILE = 0xFFFFFFFFu;
 
 constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_O = 256;  // stream i: S at 128 i, O at 256 + 128 i
-constexpr uint32_t COL_P = 64;  // P lies in the upper half of S
 
 template <int D>
 struct Lay {
@@ -254,55 +253,25 @@ __device__ __forceinline__ int run_of(const Run& r, int at) {
   return (far < 0 ? 0 : r.rest) + (far < 0 ? at : far) / (far < 0 ? r.base + 1 : r.base);
 }
 
-// 2^x of two values in [-126, 127] by the FMA pipe: 2^n 2^r with n the nearest
-// integer, which x + 1.5 * 2^23 has in its low bits, and a cubic whose relative
-// error over r in [-1/2, 1/2] is least, 2^-13.7 (its coefficients are the solution
-// of that minimax problem).  Smaller x give 2^-126.
-__device__ __forceinline__ float2 exp2_fma(float2 x) {
-  x.x = fmaxf(x.x, -126.0f), x.y = fmaxf(x.y, -126.0f);
-  const float2 big = make_float2(12582912.0f, 12582912.0f), t = __fadd2_rn(x, big);
-  const float2 n = __fadd2_rn(t, make_float2(-12582912.0f, -12582912.0f));
-  const float2 r = __ffma2_rn(n, make_float2(-1.0f, -1.0f), x);
-  float2 p = __ffma2_rn(make_float2(0.0551716685f, 0.0551716685f), r, make_float2(0.242611125f, 0.242611125f));
-  p = __ffma2_rn(p, r, make_float2(0.693260968f, 0.693260968f));
-  p = __ffma2_rn(p, r, make_float2(0.999928057f, 0.999928057f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
-}
-// The weights of 32 scores and their sum, FMA of the 16 pairs by exp2_fma: the
-// special function unit gives 4 results a cycle and scheduler, and would be what
-// the tile takes longest for.  The other exponentials are asked for first.  Masked
-// scores, -infinity, need FMA = 0.
-template <int FMA>
+// The weights of 32 scores and their sum; masked scores are -infinity.
 __device__ __forceinline__ void weights32(uint32_t (&v)[32], float f, float bias, float2& sum, uint32_t (&p)[16]) {
   const float2 ff = make_float2(f, f), bb = make_float2(bias, bias);
   float2 e[16];
 #pragma unroll
   for (int q = 0; q < 16; ++q) {
     e[q] = __ffma2_rn(make_float2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1])), ff, bb);
-    if ((q + 1) * FMA / 16 == q * FMA / 16) {
-      asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[q].x));
-      asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[q].y));
-    }
+    asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[q].x));
+    asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(e[q].y));
   }
-#pragma unroll
-  for (int q = 0; q < 16; ++q)
-    if ((q + 1) * FMA / 16 != q * FMA / 16) e[q] = exp2_fma(e[q]);
 #pragma unroll
   for (int q = 0; q < 16; ++q) {
     sum = __fadd2_rn(sum, e[q]);
-    asm volatile("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(p[q]) : "f"(e[q].y), "f"(e[q].x));
+    p[q] = f16x2(e[q].x, e[q].y);
   }
-}
-// The largest of m and 32 scores; NaN where one is.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
 }
 __device__ __forceinline__ float max32(const uint32_t (&v)[32], float m) {
 #pragma unroll
-  for (int q = 0; q < 32; q += 2) m = max_nan(max_nan(__uint_as_float(v[q]), __uint_as_float(v[q + 1])), m);
+  for (int q = 0; q < 32; q += 2) m = fmaxf(fmaxf(__uint_as_float(v[q]), __uint_as_float(v[q + 1])), m);
   return m;
 }
 // 32 bytes, a whole sector.
@@ -344,11 +313,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
       // one arrival a warp, or a commit
       mbar_init(bar(B_KFULL + i), 4), mbar_init(bar(B_KEMPTY + i), 1);
       mbar_init(bar(B_VFULL + i), 4), mbar_init(bar(B_VEMPTY + i), 1);
-      mbar_init(bar(B_QFULL + i), 4), mbar_init(bar(B_SFULL + i), 1);
-      mbar_init(bar(B_PFULL + i), 4), mbar_init(bar(B_PHALF + i), 4), mbar_init(bar(B_OFULL + i), 1);
+      mbar_init(bar(B_QFULL + i), 4), mbar_init(bar(B_ODONE + i), 1), mbar_init(bar(B_OFULL + i), 1);
+      mbar_init(bar(B_SFULL + i), 1), mbar_init(bar(B_SFULL + 2 + i), 1);
+      mbar_init(bar(B_PFULL + i), 4), mbar_init(bar(B_PFULL + 2 + i), 4);
       mbar_init(bar(B_SOFT + i), PAIR ? 4 : 8);
     }
-    for (int i = 0; i < TURNS; ++i) mbar_init(bar(B_TFULL + i), 1), mbar_init(bar(B_TEMPTY + i), 4);
+    for (int i = 0; i < TURNS; ++i) mbar_init(bar(B_TFULL + i), 1), mbar_init(bar(B_TEMPTY + i), 8);
     for (int i = 0; i < SEGS; ++i) mbar_init(bar(B_GFULL + i), 1), mbar_init(bar(B_GEMPTY + i), SM_WARPS + 1);
     mbar_init(bar(B_DRAIN), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -450,18 +420,21 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
 
   if (warp >= W_DQ && warp < W_MMA) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R_DQ));
-    // ---------------- codes to f16: a warp takes 32 keys, K and V in turn ----------------
+    // ---------------- codes to f16: a warp takes 32 keys of a tile ----------------
     constexpr int LPR = D / 32, PASS = LPR, KPP = 32 / LPR;  // lanes a key, passes, keys a pass
+    const bool is_v = warp >= W_DQ + 4;
     const int wq = warp & 3, c = lane % LPR, kr = lane / LPR;
     const int64_t at = (int64_t)kr * (D / 2) + 16 * c;  // of this lane in 32 keys' codes; an eighth of it in the scales
-    const uint8_t *kc = a.k_codes + at, *vc = a.v_codes + at, *ks = a.k_scale + at / 8, *vs = a.v_scale + at / 8;
-    uint4 rk[PASS], rv[PASS];
-    uint32_t sk[PASS], sv[PASS];
-    auto load = [&](int row, const uint8_t* codes, const uint8_t* scales, uint4 (&raw)[PASS], uint32_t (&sc)[PASS]) {
+    const uint8_t *codes = (is_v ? a.v_codes : a.k_codes) + at, *scales = (is_v ? a.v_scale : a.k_scale) + at / 8;
+    const int b_full = is_v ? B_VFULL : B_KFULL, b_empty = is_v ? B_VEMPTY : B_KEMPTY;
+    const uint32_t buf0 = sbase + (is_v ? L::OFF_V : L::OFF_K);
+    uint4 raw[PASS];
+    uint32_t sc[PASS];
+    auto load = [&](int row) {
       const uint8_t *x = codes + (int64_t)row * (D / 2), *y = scales + (int64_t)row * (D / 16);
 #pragma unroll
       for (int p = 0; p < PASS; ++p) {
-        // volatile: issued here, a tile's time before they are used
+        // volatile: issued here, before the wait for the buffer
         asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
                      : "=r"(raw[p].x), "=r"(raw[p].y), "=r"(raw[p].z), "=r"(raw[p].w)
                      : "l"(x + p * KPP * (D / 2)));
@@ -473,9 +446,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
     // lanes of the row's second half go through their chunks in another order: the
     // eight lanes that store together then meet eight different groups of banks
     const int turn = D == 128 ? c & 2 : 0;
-    auto convert = [&](uint32_t dst, const uint4& raw, uint32_t s2, int k) {
+    auto convert = [&](uint32_t dst, const uint4& v, uint32_t s2, int k) {
       const int r = wq * 32 + k;
-      uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+      uint32_t w[4] = {v.x, v.y, v.z, v.w};
       const uint32_t ss = unpack2(s2);
       uint32_t s0 = __byte_perm(ss, ss, 0x1010), s1 = __byte_perm(ss, ss, 0x3232);
       if (turn) {
@@ -497,56 +470,43 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
     };
     int slot = 0;
     uint32_t sphase = 0;
-    uint4 now = {}, nxt = {};  // row, key, keys that hold a token, set; no keys at all: no tile
-    auto next_tile = [&](uint4& d) {
+    uint4 now = {};  // row, key, keys that hold a token, set
+    auto next_tile = [&]() {
       const bool ok = mbar_wait_warp(bar(B_TFULL + slot), sphase, nullptr, ERR_WAIT);
-      d = s_tile[slot][wq];
+      now = s_tile[slot][wq];
       arrive(B_TEMPTY + slot);
       if (++slot == TURNS) slot = 0, sphase ^= 1;
-      return ok && d.x != NO_TILE;
+      return ok && now.x != NO_TILE;
     };
-    bool more = next_tile(now);
-    if (more) {
-      load(now.x, kc, ks, rk, sk);
-      load(now.x, vc, vs, rv, sv);
-    }
     int buf = 0;
     uint32_t phase = 1;
-    while (more) {
-      if (!mbar_wait_warp(bar(B_KEMPTY + buf), phase, nullptr, ERR_WAIT)) break;
+    while (next_tile()) {
+      load(now.x);
+      if (!mbar_wait_warp(bar(b_empty + buf), phase, nullptr, ERR_WAIT)) break;
+      if (is_v) {
+        uint32_t odd = 0;
 #pragma unroll
-      for (int p = 0; p < PASS; ++p) convert(sbase + L::OFF_K + buf * L::TILE_BYTES, rk[p], sk[p], p * KPP + kr);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      arrive(B_KFULL + buf);
-      more = next_tile(nxt);
-      if (more) load(nxt.x, kc, ks, rk, sk);
-
-      if (!mbar_wait_warp(bar(B_VEMPTY + buf), phase, nullptr, ERR_WAIT)) break;
-      uint32_t odd = 0;
+        for (int p = 0; p < PASS; ++p) {
+          if (p * KPP + kr >= (int)now.z) sc[p] = 0;  // no token of this sequence
+          odd |= (sc[p] & 0x7F7Fu) + 0x0101u;
+        }
+        if (odd & 0x8080u) {  // a NaN: its key noted, its values 0
 #pragma unroll
-      for (int p = 0; p < PASS; ++p) {
-        if (p * KPP + kr >= (int)now.z) sv[p] = 0;  // no token of this sequence
-        odd |= (sv[p] & 0x7F7Fu) + 0x0101u;
-      }
-      if (odd & 0x8080u) {  // a NaN: its key noted, its values 0
-#pragma unroll
-        for (int p = 0; p < PASS; ++p)
+          for (int p = 0; p < PASS; ++p)
 #pragma unroll 1
-          for (int h = 0; h < 16; h += 8)
-            if ((sv[p] >> h & 0x7Fu) == 0x7Fu) {
+            for (int h = 0; h < 16; h += 8)
+              if ((sc[p] >> h & 0x7Fu) == 0x7Fu) {
 #pragma unroll 1
-              for (int w = 0; w < SM_WARPS; ++w)
-                atomicMin(&s_nan[w][now.w][2 * c + (h >> 3)], (int)now.y + p * KPP + kr);
-              sv[p] &= ~(0xFFu << h);
-            }
+                for (int w = 0; w < SM_WARPS; ++w)
+                  atomicMin(&s_nan[w][now.w][2 * c + (h >> 3)], (int)now.y + p * KPP + kr);
+                sc[p] &= ~(0xFFu << h);
+              }
+        }
       }
 #pragma unroll
-      for (int p = 0; p < PASS; ++p)
-        convert(sbase + L::OFF_V + buf * L::TILE_BYTES, rv[p], sv[p], p * KPP + kr);
+      for (int p = 0; p < PASS; ++p) convert(buf0 + buf * L::TILE_BYTES, raw[p], sc[p], p * KPP + kr);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      arrive(B_VFULL + buf);
-      if (more) load(nxt.x, vc, vs, rv, sv);
-      now = nxt;
+      arrive(b_full + buf);
       if (++buf == 2) buf = 0, phase ^= 1;
     }
   } else if (warp >= W_MMA) {
@@ -628,102 +588,97 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
       // ---------------- MMA issuer ----------------
       // The whole warp runs the loop and one lane issues: the operands then stay in
       // uniform registers.
-      constexpr uint32_t ID_S = idesc_f16(128, false), ID_O = idesc_f16(D, true);
+      constexpr uint32_t ID_S = idesc_f16(64, false), ID_O = idesc_f16(D, true);
       const uint64_t dq = sw128_desc(sbase + L::OFF_Q), dk = sw128_desc(sbase + L::OFF_K),
                      dv = mn_desc(sbase + L::OFF_V, L::HALF);
       constexpr uint32_t TILE16 = L::TILE_BYTES / 16;
-      int kb = 0, vb = 0;
-      uint32_t kph = 0, vph = 0, qph = 0, hph = 0, pph = 0;  // of the streams: bits 0 and 1
+      uint32_t kph = 0, vph = 0, qph = 0, pph = 0;  // bits: of the buffers, the streams, streams' halves (2 i + half)
+      int kb = 0, vb = 0;                           // buffers of the segment's next tile
       bool ok = true;
-      // S of stream i from K buffer kb; `release`: its last reader
-      auto scores = [&](int i, bool release) {
+      // S of a half tile (64 keys) of stream i from K buffer b; `release`: its last reader
+      auto scores = [&](int i, int half, int b, bool release) {
         if (elect_one()) {
-          const uint64_t q = desc_at(dq, i * TILE16), k = desc_at(dk, kb * TILE16);
+          const uint64_t q = desc_at(dq, i * TILE16), k = desc_at(dk, b * TILE16 + half * (64 * 128 / 16));
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
             const uint32_t off = ((s >> 2) * L::HALF + (s & 3) * 32) / 16;
-            mma_ss(tmem + COL_S + i * 128, desc_at(q, off), desc_at(k, off), ID_S, s > 0);
+            mma_ss(tmem + COL_S + i * 128 + half * 64, desc_at(q, off), desc_at(k, off), ID_S, s > 0);
           }
-          tc_commit(bar(B_SFULL + i));
-          if (release) tc_commit(bar(B_KEMPTY + kb));
-        }
-        __syncwarp();
-        if (release && ++kb == 2) kb = 0, kph ^= 1;
-      };
-      // O of stream i from V buffer vb: the upper half of the keys, whose weights are
-      // there first, then the lower; `last`: of the segment
-      auto upper = [&](int i, bool first) {
-        if (elect_one()) {
-          const uint64_t v = desc_at(dv, vb * TILE16);
-#pragma unroll
-          for (int s = TILE / 32; s < TILE / 16; ++s)
-            mma_ts(tmem + COL_O + i * 128, tmem + COL_S + COL_P + i * 128 + s * 8, desc_at(v, s * 128), ID_O,
-                   !first || s > TILE / 32);
+          tc_commit(bar(B_SFULL + 2 * i + half));
+          if (release) tc_commit(bar(B_KEMPTY + b));
         }
         __syncwarp();
       };
-      auto lower = [&](int i, bool release, bool last) {
+      // O of stream i and that half's values from V buffer b
+      auto values = [&](int i, int half, int b, bool first, bool release, bool last) {
         if (elect_one()) {
-          const uint64_t v = desc_at(dv, vb * TILE16);
+          const uint64_t v = desc_at(dv, b * TILE16 + half * (64 * 128 / 16));
+          const uint32_t p = tmem + COL_S + i * 128 + half * 64;
 #pragma unroll
-          for (int s = 0; s < TILE / 32; ++s)
-            mma_ts(tmem + COL_O + i * 128, tmem + COL_S + COL_P + i * 128 + s * 8, desc_at(v, s * 128), ID_O, 1);
-          if (release) tc_commit(bar(B_VEMPTY + vb));
+          for (int s = 0; s < 4; ++s)
+            mma_ts(tmem + COL_O + i * 128, p + s * 8, desc_at(v, s * 128), ID_O, !first || s > 0);
+          tc_commit(bar(B_ODONE + i));
           if (last) tc_commit(bar(B_OFULL + i));
+          if (release) tc_commit(bar(B_VEMPTY + b));
         }
         __syncwarp();
-        if (release && ++vb == 2) vb = 0, vph ^= 1;
       };
-      auto wait = [&](int b, uint32_t ph) {
-        ok = ok && mbar_wait_warp(bar(b), ph, nullptr, ERR_WAIT);
+      auto take = [&](int b, int i, uint32_t& ph) {
+        ok = ok && mbar_wait_warp(bar(b + i), ph >> i & 1, nullptr, ERR_WAIT);
+        ph ^= 1u << i;
         tc_fence_after();
         return ok;
       };
-      auto take = [&](int b, int i, uint32_t& ph) {
-        const bool r = wait(b + i, ph >> i & 1);
-        ph ^= 1u << i;
-        return r;
-      };
       int turn = 0;
       uint32_t gphase = 0;
-      while (wait(B_GFULL + turn, gphase)) {
+      while (true) {
+        ok = mbar_wait_warp(bar(B_GFULL + turn), gphase, nullptr, ERR_WAIT);
+        if (!ok) break;
         const int n = s_seg[turn].t1 - s_seg[turn].t0;
         arrive(B_GEMPTY + turn);
         if (n == 0) break;
         if (++turn == SEGS) turn = 0, gphase ^= 1;
         if (PAIR) {
-          if (!wait(B_KFULL + kb, kph) || !take(B_QFULL, 0, qph)) break;
-          scores(0, false);
-          if (!take(B_QFULL, 1, qph)) break;
-          scores(1, true);
-          for (int j = 0; j < n; ++j) {
-            const bool again = j + 1 < n;
-            // the tiles are there before the weights are: the products then follow each other
-            if (!wait(B_VFULL + vb, vph) || (again && !wait(B_KFULL + kb, kph)) || !take(B_PHALF, 0, hph)) break;
-            upper(0, j == 0);
-            if (!take(B_PFULL, 0, pph)) break;
-            lower(0, false, !again);
-            if (again) scores(0, false);
-            if (!take(B_PHALF, 1, hph)) break;
-            upper(1, j == 0);
-            if (!take(B_PFULL, 1, pph)) break;
-            lower(1, true, !again);
-            if (again) scores(1, true);
+          // both streams take every tile; a half's scores are asked for when the
+          // weights in their place have been used, two halves ahead of the softmax
+          if (!take(B_KFULL, kb, kph)) break;
+          for (int i = 0; i < 2; ++i) {
+            if (!take(B_QFULL, i, qph)) break;
+            scores(i, 0, kb, false);
+            scores(i, 1, kb, i == 1);
+          }
+          if (!ok) break;
+          kb ^= 1;
+          for (int h = 0; h < 2 * n && ok; ++h) {
+            const int half = h & 1;
+            const bool again = h + 2 < 2 * n;
+            if (!half && (!take(B_VFULL, vb, vph) || (again && !take(B_KFULL, kb, kph)))) break;
+            for (int i = 0; i < 2; ++i) {
+              if (!take(B_PFULL, 2 * i + half, pph)) break;
+              values(i, half, vb, h == 0, half && i == 1, h + 1 == 2 * n);
+              if (again) scores(i, half, kb, half && i == 1);
+            }
+            if (half) vb ^= 1, kb ^= again;
           }
         } else {
+          // tile t is stream t % 2's, in buffers that stay its own for the segment
           if (!take(B_QFULL, 0, qph) || !take(B_QFULL, 1, qph)) break;
-          for (int j = 0; j < min(n, 2); ++j) {
-            if (!wait(B_KFULL + kb, kph)) break;
-            scores(j, true);
+          for (int i = 0; i < min(n, 2); ++i) {
+            if (!take(B_KFULL, kb ^ i, kph)) break;
+            scores(i, 0, kb ^ i, false);
+            scores(i, 1, kb ^ i, true);
           }
-          for (int j = 0; j < n && ok; ++j) {
-            const int i = j & 1;
-            if (!wait(B_VFULL + vb, vph) || (j + 2 < n && !wait(B_KFULL + kb, kph)) || !take(B_PHALF, i, hph)) break;
-            upper(i, j < 2);
-            if (!take(B_PFULL, i, pph)) break;
-            lower(i, true, j + 2 >= n);
-            if (j + 2 < n) scores(i, true);
-          }
+          for (int h = 0; h < n + (n & 1) && ok; ++h)  // halves of stream 0
+            for (int i = 0; i < 2 && ok; ++i) {
+              const int half = h & 1, t = (h >> 1) * 2 + i;
+              if (t >= n) continue;
+              if (!half && !take(B_VFULL, vb ^ i, vph)) break;
+              if (!half && t + 2 < n && !take(B_KFULL, kb ^ i, kph)) break;
+              if (!take(B_PFULL, 2 * i + half, pph)) break;
+              values(i, half, vb ^ i, h == 0, half, half && t + 2 >= n);
+              if (t + 2 < n) scores(i, half, kb ^ i, half);
+            }
+          kb ^= n & 1, vb ^= n & 1;
         }
       }
       // every MMA issued has completed before the TMEM is released
@@ -739,9 +694,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
     const int i = warp >> 2, wq = warp & 3, r = wq * 32 + lane;  // stream, its row
     const int first = PAIR ? i * 128 : 0;                        // of the stream's rows in the tile
     const uint32_t tq = tmem + ((uint32_t)(wq * 32) << 16);
-    const uint32_t ts = tq + COL_S + i * 128, tp = ts + COL_P, to = tq + COL_O + i * 128;
+    const uint32_t ts = tq + COL_S + i * 128, to = tq + COL_O + i * 128;
     const uint32_t sq = sbase + L::OFF_Q + i * L::TILE_BYTES;
-    uint32_t sph = 0, oph = 0, softph = 0;
+    uint32_t sph = 0, oph = 0, softph = 0, given = 0;  // sph: bits of the halves; given: weights so far, in halves
     int set = 0, bturn = 0;  // of s_nan; of s_bad, at the segment's first tile
     bool ok = true;
     // the threads that end a segment together: a stream's, or both streams'; bounded, as every wait
@@ -853,24 +808,40 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
       float m = NEG_INF, l = 0.0f;
       const int n = cur.t1 - cur.t0, key00 = cur.t0 * TILE;
       bool any = false;  // this stream has had a tile
-      for (int j = PAIR ? 0 : i; j < n; j += PAIR ? 1 : 2) {
-        if (!(ok = mbar_wait_warp(bar(B_SFULL + i), sph, nullptr, ERR_WAIT))) break;
-        sph ^= 1;
-        tc_fence_after();
-        // the last scores are there, so the queries' place is free: the next ones travel under this tile
-        if (PAIR && j + 1 == n && (more = segment())) fetch_q(s_seg[turn], row_of(s_seg[turn]));
-        if (any_live) {
-          const int key0 = key00 + j * TILE;
-          const uint32_t bad = s_bad[(bturn + j) & (BAD_TURNS - 1)];
-          float2 sum = make_float2(0.0f, 0.0f);
-          // the reference m after scores whose largest is mx, and O and l with it
-          auto refer = [&](float mx) {
-            const float top = mx == NEG_INF ? NEG_INF : mx * f;
-            if (__any_sync(FULL, top > m + LAG)) {
+      // The products of all weights given so far are done.  The scores that were just
+      // read were asked for after the product before the last, so that only the last
+      // can be under way and the parity is of its phase.
+      auto products = [&]() { return mbar_wait_warp(bar(B_ODONE + i), (given - 1) & 1, nullptr, ERR_WAIT); };
+      for (int j = PAIR ? 0 : i; j < n && ok; j += PAIR ? 1 : 2)
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          if (!(ok = mbar_wait_warp(bar(B_SFULL + 2 * i + half), sph >> half & 1, nullptr, ERR_WAIT))) break;
+          sph ^= 1u << half;
+          tc_fence_after();
+          // the last scores are there, so the queries' place is free: the next ones travel under this tile
+          if (PAIR && half && j + 1 == n && (more = segment())) fetch_q(s_seg[turn], row_of(s_seg[turn]));
+          if (any_live) {
+            const int key0 = key00 + j * TILE + half * 64;
+            const uint32_t th = ts + half * 64, bad = s_bad[(bturn + j) & (BAD_TURNS - 1)] >> (16 * half) & 0xFFFFu;
+            uint32_t va[32], vb[32], p[16];
+            float2 sum = make_float2(0.0f, 0.0f);
+            tmem_ld32(th, va);
+            tmem_ld32(th + 32, vb);
+            tmem_ld_wait();
+            if (key0 + 64 > free_end || bad) {
+              // -infinity where the key lies past the row's last, or in no page
+              const int stay = limit + 1 - key0, na = bad & 0xFFu ? 0 : stay, nb = bad >> 8 ? 0 : stay - 32;
+#pragma unroll
+              for (int q = 0; q < 32; ++q) va[q] = q < na ? va[q] : 0xFF800000u, vb[q] = q < nb ? vb[q] : 0xFF800000u;
+            }
+            const float mx = fmaxf(max32(va, NEG_INF), max32(vb, NEG_INF)), top = mx == NEG_INF ? NEG_INF : mx * f;
+            if (__any_sync(FULL, top > m + LAG)) {  // the reference moves, O and l with it
               const float mn = fmaxf(m, top), corr = mn == NEG_INF ? 1.0f : ex2(m - mn);
               m = mn;
               l *= corr;
               if (any) {
+                if (!(ok = products())) break;
+                tc_fence_after();
 #pragma unroll 1
                 for (int c = 0; c < D / 16; ++c) {
                   uint32_t o[16];
@@ -882,73 +853,19 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
                 }
               }
             }
-            return m == NEG_INF ? P_EXP : P_EXP - m;
-          };
-          if (key0 + TILE <= free_end && !bad) {
-            // the upper half stays in registers; its weights free the place of the lower half's
-            uint32_t va[32], vb[32], p[16];
-            tmem_ld32(ts, va);
-            tmem_ld32(ts + 32, vb);
-            tmem_ld_wait();
-            float mx = max_nan(max32(va, NEG_INF), max32(vb, NEG_INF));
-            tmem_ld32(ts + 64, va);
-            tmem_ld32(ts + 96, vb);
-            tmem_ld_wait();
-            mx = max_nan(mx, max_nan(max32(va, NEG_INF), max32(vb, NEG_INF)));
-            if (mx != mx) l = mx;  // a score is NaN: so is the row
-            const float bias = refer(mx);
-            weights32<FMA_PAIRS>(va, f, bias, sum, p);
-            tmem_ld32(ts, va);
-            tmem_st16(tp + 32, p);
-            weights32<FMA_PAIRS>(vb, f, bias, sum, p);
-            tmem_ld_wait();
-            tmem_ld32(ts + 32, vb);
-            tmem_st16(tp + 48, p);
+            const float bias = m == NEG_INF ? P_EXP : P_EXP - m;
+            weights32(va, f, bias, sum, p);
+            tmem_st16(th, p);
+            weights32(vb, f, bias, sum, p);
+            tmem_st16(th + 16, p);
+            l += sum.x + sum.y;
             tmem_st_wait();
-            tc_fence_before();
-            arrive(B_PHALF + i);
-            weights32<FMA_PAIRS>(va, f, bias, sum, p);
-            tmem_ld_wait();
-            tmem_st16(tp, p);
-            weights32<FMA_PAIRS>(vb, f, bias, sum, p);
-            tmem_st16(tp + 16, p);
-          } else {  // some scores are -infinity: their key lies past the row's last, or in no page
-            auto masked32 = [&](int c, uint32_t (&v)[32]) {
-              tmem_ld32(ts + 32 * c, v);
-              tmem_ld_wait();
-              const int stay = bad >> (8 * c) & 0xFFu ? 0 : limit + 1 - key0 - 32 * c;
-#pragma unroll
-              for (int q = 0; q < 32; ++q) v[q] = q < stay ? v[q] : 0xFF800000u;
-            };
-            uint32_t v[32], p[16];
-            float mx = NEG_INF;
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              masked32(c, v);
-              mx = max32(v, mx);
-            }
-            const float bias = refer(mx);
-#pragma unroll 1
-            for (int c = 3; c >= 0; --c) {  // from above, as the places free up
-              masked32(c, v);
-              weights32<0>(v, f, bias, sum, p);
-              tmem_st16(tp + 16 * c, p);
-              if (c == 2) {
-                tmem_st_wait();
-                tc_fence_before();
-                arrive(B_PHALF + i);
-              }
-            }
+            any = true;
           }
-          l += sum.x + sum.y;
-          tmem_st_wait();
-          any = true;
-        } else {
-          arrive(B_PHALF + i);
+          tc_fence_before();
+          arrive(B_PFULL + 2 * i + half);
+          ++given;
         }
-        tc_fence_before();
-        arrive(B_PFULL + i);
-      }
       if (!ok) break;
       if (PAIR && more) f = finish_q(scale_of(s_seg[turn]));  // while the last product runs
       bturn = (bturn + n) & (BAD_TURNS - 1);
@@ -1189,6 +1106,7 @@ int attend(const void* q, const int64_t* q_strides, int64_t batch, int64_t token
            const void* lengths, const void* counts, float sm_scale, float* workspace, int64_t workspace_floats,
            int32_t* counters, int64_t counters_len, void* out, cudaStream_t st) {
   const int64_t capacity = table_width * page;
+  if (reinterpret_cast<uintptr_t>(out) & 31) return VQ_ERR_ALIGNMENT;
   const Cut c = cut_of(batch, tokens, heads, kv_heads, capacity);
   const int64_t pairs = batch * kv_heads * c.groups;
   // the tiles of all heads, counted in 32 bits
