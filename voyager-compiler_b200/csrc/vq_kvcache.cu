@@ -600,21 +600,26 @@ void launch(Args& a, int D, int64_t& blocks, cudaStream_t st) {
 // scale NaN.  A token's blocks are its own: nothing that the cache holds is read
 // or changed, and a thread needs no more than its neighbour's maximum.
 //
-// The quotient is x r, r = 1 / (scale f), with one correction by its remainder
-// (Markstein 1990: the result is the rounded quotient), so that a quotient that
-// lies between two codes is taken as what it is; bf16 values meet such ties often.
+// A quotient is x r with one correction by its remainder (Markstein 1990), r the
+// divisor's reciprocal after one step of Newton's iteration: one that float32 holds,
+// as ties between two codes are, comes out exactly, and bf16 values meet ties often.
+// Divisors lie within 2^-126 .. 2^126.
 
-// Two floats times or plus two, rounded to nearest, in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
-
-// 8 values, their quotients by d, as codes: 4 bytes.
-__device__ __forceinline__ uint32_t e2m1_codes(const float (&x)[8], float d, float r, bool plain) {
+__device__ __forceinline__ float reciprocal(float d) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return fmaf(fmaf(-d, r, 1.0f), r, r);
+}
+// 8 values, their quotients by d, as codes: 4 bytes.  `finite`: the products of the
+// correction stay in float32; beyond, the values saturate all the same.
+__device__ __forceinline__ uint32_t e2m1_codes(const float (&x)[8], float d, float r, bool finite) {
   float y[8];
+  const float2 rr = make_float2(r, r), nd = make_float2(-d, -d);
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
-    const float2 v = make_float2(x[j], x[j + 1]), rr = make_float2(r, r), nd = make_float2(-d, -d);
+    const float2 v = make_float2(x[j], x[j + 1]);
     float2 q = __fmul2_rn(v, rr);
-    if (plain) q = fma2(fma2(q, nd, v), rr, q);
+    if (finite) q = __ffma2_rn(__ffma2_rn(q, nd, v), rr, q);
     y[j] = q.x, y[j + 1] = q.y;
   }
   uint32_t w;
@@ -638,10 +643,16 @@ __device__ __forceinline__ float amax8(const float (&x)[8]) {
   for (int j = 1; j < 8; ++j) m = amax_nan(m, fabsf(x[j]));
   return m;
 }
-// A block's scale byte, and what its values are divided by.
-__device__ __forceinline__ uint32_t block_scale4(float amax, float f, float& d) {
-  const uint32_t b = max(pack2(__fdiv_rn(amax, 6.0f * f), 0.0f) & 0xFFu, 1u);
+// A block's scale byte, what its values are divided by, and that one's reciprocal.
+__device__ __forceinline__ uint32_t block_scale4(float amax, float f, float& d, float& r) {
+  const float six = 6.0f * f, r6 = reciprocal(six);
+  float a;  // an infinity saturates like any large value; NaN stays
+  asm("min.NaN.f32 %0, %1, 0f7CF0BDC2;" : "=f"(a) : "f"(amax));  // 1e37
+  float q = a * r6;
+  q = fmaf(fmaf(-q, six, a), r6, q);
+  const uint32_t b = max(pack2(q, 0.0f) & 0xFFu, 1u);
   d = half2f(unpack2(b)).x * f;
+  r = reciprocal(d);
   return b;
 }
 // One unit's 16 columns of a key or value head to its token's place.  `split`:
@@ -669,12 +680,14 @@ __device__ __forceinline__ void store4(uint8_t* codes, uint8_t* scale, const flo
     m0 = m1 = amax_nan(m0, m1);
   }
   if (!store) return;
-  float d0, d1;
-  const uint32_t e0 = block_scale4(m0, f, d0);
-  const uint32_t e1 = split ? block_scale4(m1, f, d1) : (d1 = d0, e0);
-  // the correction's products leave float32 only where the values saturate all the same
-  const uint32_t w0 = e2m1_codes(x0, d0, __fdiv_rn(1.0f, d0), m0 < 1e30f);
-  const uint32_t w1 = e2m1_codes(x1, d1, split ? __fdiv_rn(1.0f, d1) : __fdiv_rn(1.0f, d0), m1 < 1e30f);
+  float d0, d1, r0, r1;
+  const uint32_t e0 = block_scale4(m0, f, d0, r0);
+  uint32_t e1 = e0;
+  if (split)
+    e1 = block_scale4(m1, f, d1, r1);
+  else
+    d1 = d0, r1 = r0;
+  const uint32_t w0 = e2m1_codes(x0, d0, r0, m0 < 1e30f), w1 = e2m1_codes(x1, d1, r1, m1 < 1e30f);
   if (split) {
     const int g1 = u + R;
     reinterpret_cast<uint32_t*>(codes)[u] = w0;
@@ -687,11 +700,10 @@ __device__ __forceinline__ void store4(uint8_t* codes, uint8_t* scale, const flo
   }
 }
 
-// The query, key and value heads alike: thread `i` takes its unit of a.hq heads
-// of a token, the heads of q, k and v counted on; the tokens of a warp are
-// neighbours, so that their codes and scales fill sectors.
+// Few heads in all: thread `i` takes its unit of one head of a token, the heads of
+// q, k and v counted on.
 struct Unit4 {
-  int u, h0, h1, b, t;
+  int u, h, b, t;
   int64_t row;
 };
 template <int D>
@@ -699,10 +711,9 @@ __device__ __forceinline__ Unit4 unit4(const Args& a, int64_t i) {
   constexpr int U = D / 16;
   Unit4 x;
   x.u = (int)(i % U);
-  const int64_t rows = (int64_t)a.B * a.T, r = i / U, hg = r / rows;
-  x.row = r - hg * rows;
-  const int all = a.H + 2 * a.Hkv;
-  x.h0 = (int)min(hg * a.hq, (int64_t)all), x.h1 = min(all, x.h0 + a.hq);
+  const int64_t rows = (int64_t)a.B * a.T, r = i / U;
+  x.h = (int)min(r / rows, (int64_t)(a.H + 2 * a.Hkv));
+  x.row = r - r / rows * rows;
   x.b = (int)(x.row / a.T), x.t = (int)(x.row - (int64_t)x.b * a.T);
   return x;
 }
@@ -730,7 +741,7 @@ __device__ __forceinline__ Token4 token4(const Args& a, const Unit4& x) {
   k.turns = k.live && x.u * 16 < a.rot;
   k.slot = -1;
   if (k.turns) load_angles(a.table + (int64_t)(held + x.t) * (a.rot >> 1), x.u, a.rot, k.c, k.s);
-  if (k.live && x.h1 > a.H) {
+  if (k.live && x.h >= a.H) {
     const int pos = held + x.t, at = pos / a.page;
     const int pid = a.block_table[(int64_t)x.b * a.width + at];
     if (pid < 0 || pid >= a.pages)
@@ -764,79 +775,116 @@ __device__ __forceinline__ void finish4(const Args& a, const Unit4& x, const Tok
   }
 }
 
-// Few heads in all: one head a thread.
+// Bound by latency: the plan, the block table, the heads, the angles.
 template <typename T, bool IL, int D, bool NORM>
 __global__ void __launch_bounds__(FEW_THREADS) k_append4_few(const __grid_constant__ Args a) {
   pdl::trigger();
   pdl::wait();
   const Unit4 x = unit4<D>(a, (int64_t)blockIdx.x * FEW_THREADS + threadIdx.x);
-  if (x.h0 >= x.h1) return;
+  if (x.h >= a.H + 2 * a.Hkv) return;
   int c0, c1;
-  const typename T::type* p = head_row<T, IL>(a, x, x.h0, c0, c1);
+  const typename T::type* p = head_row<T, IL>(a, x, x.h, c0, c1);
   float x0[8], x1[8];
   T::load8(p + c0, x0);
   T::load8(p + c1, x1);
   const Token4 k = token4(a, x);
-  finish4<T, IL, D, NORM>(a, x, k, x.h0, c0, c1, x0, x1);
+  finish4<T, IL, D, NORM>(a, x, k, x.h, c0, c1, x0, x1);
 }
 
-// Many: a.hq heads a thread, QH at a time, whose loads travel through a ring.
+// Many: the keys and values beside k_turn_q, half of the CTAs each; a thread takes
+// its unit of a.hc heads of a token, QH at a time, whose loads travel through a ring.
+// The tokens of a warp are neighbours, so that their codes and scales fill sectors.
 template <typename T, bool IL, int D, bool NORM>
-__global__ void __launch_bounds__(Q_THREADS) k_append4(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(Q_THREADS, 3) k_append4(const __grid_constant__ Args a) {
+  using E = typename T::type;
+  constexpr int U = D / 16;
   extern __shared__ __align__(16) uint8_t smem[];
   const Ring<T, Q_THREADS> ring(smem);
-  pdl::wait();
-  const Unit4 x = unit4<D>(a, (int64_t)blockIdx.x * Q_THREADS + threadIdx.x);
-  if (x.h0 >= x.h1) return;
-  const int steps = (x.h1 - x.h0 + QH - 1) / QH;
-  auto fetch = [&](int k) {
-    if (k < steps) {
+  pdl::trigger();
+  const bool is_v = blockIdx.x & 1;
+  const int64_t i = (int64_t)(blockIdx.x >> 1) * Q_THREADS + threadIdx.x, rows = (int64_t)a.B * a.T, at = i / U;
+  const int u = (int)(i % U), h0 = (int)min(at / rows * a.hc, (int64_t)a.Hkv), h1 = min(a.Hkv, h0 + a.hc);
+  const int64_t row = at % rows;
+  const int b = (int)(row / a.T), t = (int)(row - (int64_t)b * a.T);
+  int held, pid = -1, pos = 0;
+  if (h0 < h1 && t < plan(a, b, held)) {
+    pos = held + t;
+    pid = a.block_table[(int64_t)b * a.width + pos / a.page];
+    if (pid < 0 || pid >= a.pages) tc::note_err(nullptr, ERR_PAGE), pid = -1;
+  }
+  // a token's U lanes go together; k_turn_q, launched before this kernel, shares
+  // nothing with it, so only the end waits
+  if (pid >= 0) {
+    const Strides st = is_v ? a.sv : a.sk;
+    const E* src = reinterpret_cast<const E*>(is_v ? a.v : a.k) + b * st.b + t * st.t;
+    int c0, c1;
+    unit_cols<IL>(u, is_v ? 0 : a.rot, c0, c1);
+    const int steps = (h1 - h0 + QH - 1) / QH;
+    auto fetch = [&](int k) {
+      if (k < steps) {
+#pragma unroll
+        for (int q = 0; q < QH; ++q) {
+          const E* p = src + min(h0 + k * QH + q, h1 - 1) * st.h;
+          ring.fetch(k, 2 * q, p + c0);
+          ring.fetch(k, 2 * q + 1, p + c1);
+        }
+      }
+      ring.commit();
+    };
+#pragma unroll
+    for (int k = 0; k < Ring<T, Q_THREADS>::DEPTH - 1; ++k) fetch(k);
+    const bool turns = !is_v && u * 16 < a.rot;
+    float c[8], s[8];
+    if (turns) load_angles(a.table + (int64_t)pos * (a.rot >> 1), u, a.rot, c, s);
+    const int64_t slot = (int64_t)pid * a.Hkv * a.page + pos % a.page;
+    uint8_t* codes = (is_v ? a.v_codes : a.k_codes) + slot * (D / 2);
+    uint8_t* scale = (is_v ? a.v_bscale : a.k_bscale) + slot * U;
+    const float* factor = is_v ? a.v_factor : a.k_factor;
+    for (int k = 0; k < steps; ++k) {
+      fetch(k + Ring<T, Q_THREADS>::DEPTH - 1);
+      ring.wait();
 #pragma unroll
       for (int q = 0; q < QH; ++q) {
-        int c0, c1;
-        const typename T::type* p = head_row<T, IL>(a, x, min(x.h0 + k * QH + q, x.h1 - 1), c0, c1);
-        ring.fetch(k, 2 * q, p + c0);
-        ring.fetch(k, 2 * q + 1, p + c1);
+        const int h = h0 + k * QH + q;
+        float x0[8], x1[8];
+        ring.read(k, 2 * q, x0);
+        ring.read(k, 2 * q + 1, x1);
+        if (h < h1) {
+          if (NORM && !is_v && a.k_norm) head_norm<T, U>(x0, x1, a.k_norm, c0, c1, a.eps);
+          if (turns) turn<IL>(x0, x1, c, s);
+          const int64_t on = (int64_t)h * a.page;
+          store4<U>(codes + on * (D / 2), scale + on * U, x0, x1, __ldg(factor + h), u, a.rot, !IL && !is_v, true);
+        }
       }
     }
-    ring.commit();
-  };
-#pragma unroll
-  for (int k = 0; k < Ring<T, Q_THREADS>::DEPTH - 1; ++k) fetch(k);
-  const Token4 tok = token4(a, x);
-  for (int k = 0; k < steps; ++k) {
-    fetch(k + Ring<T, Q_THREADS>::DEPTH - 1);
-    ring.wait();
-#pragma unroll
-    for (int q = 0; q < QH; ++q) {
-      const int h = x.h0 + k * QH + q;
-      float x0[8], x1[8];
-      ring.read(k, 2 * q, x0);
-      ring.read(k, 2 * q + 1, x1);
-      int c0, c1;
-      unit_cols<IL>(x.u, h >= a.H + a.Hkv ? 0 : a.rot, c0, c1);
-      if (h < x.h1) finish4<T, IL, D, NORM>(a, x, tok, h, c0, c1, x0, x1);
-    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  pdl::wait();
 }
 
 template <typename T, bool IL, int D, bool NORM>
 void launch4_d(Args& a, int64_t& blocks, cudaStream_t st) {
-  const int all = a.H + 2 * a.Hkv;
-  auto ctas = [&](int th) { return ((int64_t)a.B * a.T * ((all + a.hq - 1) / a.hq) * (D / 16) + th - 1) / th; };
+  const int all = a.H + 2 * a.Hkv, sms = vq::mx::sm_count();
+  auto ctas = [&](int heads, int each, int th) {
+    return ((int64_t)a.B * a.T * ((heads + each - 1) / each) * (D / 16) + th - 1) / th;
+  };
   a.hq = 1;
-  if (ctas(FEW_THREADS) <= 16 * vq::mx::sm_count()) {
-    blocks = ctas(FEW_THREADS);
+  blocks = ctas(all, 1, FEW_THREADS);
+  if (blocks <= 16 * sms) {
     if (!pdl::launch<k_append4_few<T, IL, D, NORM>>((unsigned)blocks, FEW_THREADS, 0, st, 1, a)) blocks = -1;
     return;
   }
-  a.hq = QH;
-  while (a.hq < all && ctas(Q_THREADS) >= 12 * vq::mx::sm_count()) a.hq *= 2;
-  blocks = ctas(Q_THREADS);
+  // more heads per thread while the SMs are filled all the same, twice over by each part
+  a.hq = a.hc = QH;
+  while (a.hq < a.H && ctas(a.H, a.hq, Q_THREADS) >= 12 * sms) a.hq *= 2;
+  while (a.hc < a.Hkv && ctas(a.Hkv, a.hc, Q_THREADS) >= 6 * sms) a.hc *= 2;
+  const int64_t nq = ctas(a.H, a.hq, Q_THREADS), nc = 2 * ctas(a.Hkv, a.hc, Q_THREADS);
+  blocks = std::max(nq, nc);
   if (blocks >= (1ll << 31)) return;
-  if (!tc::allow_smem<k_append4<T, IL, D, NORM>>(Ring<T, Q_THREADS>::BYTES) ||
-      !pdl::launch<k_append4<T, IL, D, NORM>, false>((unsigned)blocks, Q_THREADS, Ring<T, Q_THREADS>::BYTES, st, 1, a))
+  constexpr int BYTES = Ring<T, Q_THREADS>::BYTES;
+  if (!tc::allow_smem<k_turn_q<T, IL, D, NORM>>(BYTES) || !tc::allow_smem<k_append4<T, IL, D, NORM>>(BYTES) ||
+      !pdl::launch<k_turn_q<T, IL, D, NORM>, false>((unsigned)nq, Q_THREADS, BYTES, st, 1, a) ||
+      !pdl::launch<k_append4<T, IL, D, NORM>>((unsigned)nc, Q_THREADS, BYTES, st, 1, a))
     blocks = -1;
 }
 template <typename T, bool IL, int D>
@@ -860,26 +908,33 @@ __device__ __forceinline__ uint32_t e2m1_to_e4m3(uint32_t nib4) {  // four codes
   const uint32_t s16 = (sel & 0x7u) | ((sel >> 4) & 0x70u) | ((sel >> 8) & 0x700u) | ((sel >> 12) & 0x7000u);
   return __byte_perm(lo, hi, s16) | ((nib4 & 0x08080808u) << 4);
 }
-constexpr int UNPACK_THREADS = 256;
+constexpr int UNPACK_THREADS = 256, UNPACK = 4;  // chunks a thread and turn, all loads in flight together
 __global__ void __launch_bounds__(UNPACK_THREADS)
     k_unpack4(const uint4* k, const uint4* v, uint4* ko, uint4* vo, int64_t chunks) {
   pdl::trigger();
   pdl::wait();
-  const int64_t step = (int64_t)gridDim.x * UNPACK_THREADS;
-  for (int64_t i = (int64_t)blockIdx.x * UNPACK_THREADS + threadIdx.x; i < 2 * chunks; i += step) {
-    const bool second = i >= chunks;
-    const int64_t j = second ? i - chunks : i;
-    const uint4 w = __ldg((second ? v : k) + j);
-    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-    uint32_t o[8];
+  const bool second = blockIdx.x & 1;  // the values
+  const uint4* in = second ? v : k;
+  uint4* out = second ? vo : ko;
+  const int64_t step = (int64_t)(gridDim.x >> 1) * (UNPACK_THREADS * UNPACK);
+  for (int64_t i = (int64_t)(blockIdx.x >> 1) * (UNPACK_THREADS * UNPACK) + threadIdx.x; i < chunks; i += step) {
+    uint4 w[UNPACK];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const uint32_t even = e2m1_to_e4m3(in[q] & 0x0F0F0F0Fu), odd = e2m1_to_e4m3((in[q] >> 4) & 0x0F0F0F0Fu);
-      o[2 * q] = __byte_perm(even, odd, 0x5140), o[2 * q + 1] = __byte_perm(even, odd, 0x7362);
+    for (int n = 0; n < UNPACK; ++n)
+      w[n] = i + n * UNPACK_THREADS < chunks ? __ldg(in + i + n * UNPACK_THREADS) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int n = 0; n < UNPACK; ++n) {
+      const uint32_t x[4] = {w[n].x, w[n].y, w[n].z, w[n].w};
+      uint32_t o[8];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t even = e2m1_to_e4m3(x[q] & 0x0F0F0F0Fu), odd = e2m1_to_e4m3((x[q] >> 4) & 0x0F0F0F0Fu);
+        o[2 * q] = __byte_perm(even, odd, 0x5140), o[2 * q + 1] = __byte_perm(even, odd, 0x7362);
+      }
+      if (i + n * UNPACK_THREADS < chunks)
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + 2 * (i + n * UNPACK_THREADS)),
+                     "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
     }
-    uint4* p = (second ? vo : ko) + 2 * j;
-    p[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    p[1] = make_uint4(o[4], o[5], o[6], o[7]);
   }
 }
 
@@ -1015,8 +1070,9 @@ int vq_kv4_unpack(const void* k_codes, const void* v_codes, int64_t bytes, void*
   const void* p16[4] = {k_codes, v_codes, k_out, v_out};
   for (const void* p : p16)
     if (reinterpret_cast<uintptr_t>(p) & 15) return VQ_ERR_ALIGNMENT;
-  const int64_t chunks = bytes / 16, ctas = (2 * chunks + UNPACK_THREADS - 1) / UNPACK_THREADS;
-  const unsigned n = (unsigned)std::min<int64_t>(ctas, 8 * vq::mx::sm_count());
+  if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 31) return VQ_ERR_ALIGNMENT;
+  const int64_t chunks = bytes / 16, ctas = (chunks + UNPACK_THREADS * UNPACK - 1) / (UNPACK_THREADS * UNPACK);
+  const unsigned n = 2 * (unsigned)std::min<int64_t>(ctas, 4 * vq::mx::sm_count());
   return vq::pdl::launch<k_unpack4>(n, UNPACK_THREADS, 0, reinterpret_cast<cudaStream_t>(stream), 1,
                                     (const uint4*)k_codes, (const uint4*)v_codes, (uint4*)k_out, (uint4*)v_out, chunks)
              ? VQ_OK
