@@ -395,7 +395,8 @@ int vq_linear_mxf8_noalloc_status(int32_t* code, void* stream);
  * recorded since the last clear -- GEMM 1-4, bf16 GEMM 11-14, W4A8 21-23,
  * tensor-parallel barrier
  * 100 + rank, attention 200 + its code, key / value cache 301-303 and
- * 311-314, E4M3 linear 321-324.  The per-call error words report to
+ * 311-314, E4M3 linear 321-324, attention of many rows over the 4-bit cache
+ * 331-334.  The per-call error words report to
  * one caller; this one lets the host ask, after a batch of work, whether any
  * launch gave up.  clear != 0 resets the word.  Synchronises `stream`.  The
  * reference raises on the host and has no device waits; this has no
@@ -769,7 +770,7 @@ int vq_rope_append_kv4(const void* q, const void* k, const void* v, const int64_
                        const float* k_factor, const float* v_factor, void* stream);
 
 /* The codes of a 4-bit cache, `bytes` of each (a multiple of 16), as E4M3 codes
- * of the same values, one a byte: k_out and v_out [2 * bytes]. */
+ * of the same values, one a byte: k_out and v_out [2 * bytes], 32-byte aligned. */
 int vq_kv4_unpack(const void* k_codes, const void* v_codes, int64_t bytes, void* k_out, void* v_out,
                   void* stream);
 
@@ -798,7 +799,9 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
                 const void* counts, float sm_scale, float* workspace, int64_t workspace_floats,
                 int32_t* counters, int64_t counters_len, void* out, void* stream);
 
-/* vq_attn_kv8 over the 4-bit cache of vq_rope_append_kv4. */
+/* vq_attn_kv8 over the 4-bit cache of vq_rope_append_kv4; scales 16-byte and out
+ * 32-byte aligned.  Calls of many rows a kv head (tokens * heads / kv_heads) run
+ * another kernel, whose waits and plans set the sticky word to 331-334. */
 int vq_attn_kv4_workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_heads,
                           int32_t head_dim, int32_t page, int64_t table_width, int64_t* floats,
                           int64_t* counters);

@@ -1203,6 +1203,7 @@ static int attention(const void* q, const int64_t* q_strides, int64_t batch, int
   const void* p16[7] = {q, k_codes, v_codes, out, workspace, fp4 ? k_scale : nullptr, fp4 ? v_scale : nullptr};
   for (const void* p : p16)
     if (reinterpret_cast<uintptr_t>(p) & 15) return VQ_ERR_ALIGNMENT;
+  if (fp4 && (reinterpret_cast<uintptr_t>(out) & 31)) return VQ_ERR_ALIGNMENT;
   for (int i = 0; i < 3; ++i)
     if (q_strides[i] % 8) return VQ_ERR_ALIGNMENT;
   if (fp4 && !few_rows(batch, tokens * a.G, kv_heads, table_width * page))

@@ -1106,7 +1106,6 @@ int attend(const void* q, const int64_t* q_strides, int64_t batch, int64_t token
            const void* lengths, const void* counts, float sm_scale, float* workspace, int64_t workspace_floats,
            int32_t* counters, int64_t counters_len, void* out, cudaStream_t st) {
   const int64_t capacity = table_width * page;
-  if (reinterpret_cast<uintptr_t>(out) & 31) return VQ_ERR_ALIGNMENT;
   const Cut c = cut_of(batch, tokens, heads, kv_heads, capacity);
   const int64_t pairs = batch * kv_heads * c.groups;
   // the tiles of all heads, counted in 32 bits

@@ -600,15 +600,27 @@ void launch(Args& a, int D, int64_t& blocks, cudaStream_t st) {
 // scale NaN.  A token's blocks are its own: nothing that the cache holds is read
 // or changed, and a thread needs no more than its neighbour's maximum.
 //
-// A quotient is x r with one correction by its remainder (Markstein 1990), r the
-// divisor's reciprocal after one step of Newton's iteration: one that float32 holds,
-// as ties between two codes are, comes out exactly, and bf16 values meet ties often.
-// Divisors lie within 2^-126 .. 2^126.
+// A quotient is q = x r with one correction by its remainder, q + (x - q d) r
+// (Markstein 1990), r the divisor's reciprocal to about 2^-22: a quotient that
+// float32 holds, as ties between two codes are, comes out exactly, since its error
+// falls to 2^-44, and bf16 values meet ties often.  Divisors lie within 2^-126 .. 2^126.
 
 __device__ __forceinline__ float reciprocal(float d) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-  return fmaf(fmaf(-d, r, 1.0f), r, r);
+  return r;
+}
+// turn() with two columns an instruction.
+template <bool IL>
+__device__ __forceinline__ void turn4(float (&x0)[8], float (&x1)[8], const float (&c)[8], const float (&s)[8]) {
+  if (IL) return turn<IL>(x0, x1, c, s);
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const float2 a = make_float2(x0[i], x0[i + 1]), b = make_float2(x1[i], x1[i + 1]);
+    const float2 cc = make_float2(c[i], c[i + 1]), ss = make_float2(s[i], s[i + 1]), ns = make_float2(-s[i], -s[i + 1]);
+    const float2 p = __ffma2_rn(a, cc, __fmul2_rn(b, ns)), q = __ffma2_rn(a, ss, __fmul2_rn(b, cc));
+    x0[i] = p.x, x0[i + 1] = p.y, x1[i] = q.x, x1[i + 1] = q.y;
+  }
 }
 // 8 values, their quotients by d, as codes: 4 bytes.  `finite`: the products of the
 // correction stay in float32; beyond, the values saturate all the same.
@@ -759,7 +771,7 @@ __device__ __forceinline__ void finish4(const Args& a, const Unit4& x, const Tok
   if (!is_v) {
     const void* w = is_q ? a.q_norm : a.k_norm;
     if (NORM && w) head_norm<T, U>(x0, x1, w, c0, c1, a.eps);
-    if (k.turns) turn<IL>(x0, x1, k.c, k.s);
+    if (k.turns) turn4<IL>(x0, x1, k.c, k.s);
   }
   if (is_q) {
     if (!k.live) {
@@ -851,7 +863,7 @@ __global__ void __launch_bounds__(Q_THREADS, 3) k_append4(const __grid_constant_
         ring.read(k, 2 * q + 1, x1);
         if (h < h1) {
           if (NORM && !is_v && a.k_norm) head_norm<T, U>(x0, x1, a.k_norm, c0, c1, a.eps);
-          if (turns) turn<IL>(x0, x1, c, s);
+          if (turns) turn4<IL>(x0, x1, c, s);
           const int64_t on = (int64_t)h * a.page;
           store4<U>(codes + on * (D / 2), scale + on * U, x0, x1, __ldg(factor + h), u, a.rot, !IL && !is_v, true);
         }
@@ -874,10 +886,12 @@ void launch4_d(Args& a, int64_t& blocks, cudaStream_t st) {
     if (!pdl::launch<k_append4_few<T, IL, D, NORM>>((unsigned)blocks, FEW_THREADS, 0, st, 1, a)) blocks = -1;
     return;
   }
-  // more heads per thread while the SMs are filled all the same, twice over by each part
+  // more heads per thread while the SMs are filled all the same, twice over by each
+  // part; beyond 16 keys and values only lengthen the last CTAs (32 heads, 8 x 2048
+  // tokens: 133 us with 32 a thread, 128 with 16)
   a.hq = a.hc = QH;
   while (a.hq < a.H && ctas(a.H, a.hq, Q_THREADS) >= 12 * sms) a.hq *= 2;
-  while (a.hc < a.Hkv && ctas(a.Hkv, a.hc, Q_THREADS) >= 6 * sms) a.hc *= 2;
+  while (a.hc < std::min(a.Hkv, 16) && ctas(a.Hkv, a.hc, Q_THREADS) >= 6 * sms) a.hc *= 2;
   const int64_t nq = ctas(a.H, a.hq, Q_THREADS), nc = 2 * ctas(a.Hkv, a.hc, Q_THREADS);
   blocks = std::max(nq, nc);
   if (blocks >= (1ll << 31)) return;
