@@ -302,7 +302,9 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
   const int heads = (int)(total >> 32) * a.Hkv, real = (int)total * a.Hkv;
   const float least = heads ? fmaxf(1.0f, sqrtf(0.125f * (float)real / (float)heads)) : 1.0f;
   const int runs = min((int)gridDim.x, (int)ceilf((float)real / least));
-  const int HEAD = 6 * heads >= runs ? 5 : 0;
+  // (In 4 bits, whose units take half as long to read but not to multiply: 3; 32
+  // sequences to 8192 keys 46.3 us, with 5 47.7, with 1 47.5.)
+  const int HEAD = 6 * heads >= runs ? (FP4 ? 3 : 5) : 0;
   const int all = real + HEAD * heads;
   const int base = runs ? all / runs : 0, near_end = 4 * (top + HEAD) <= 5 * base ? HEAD : 0;
   const int rest = all - base * runs;  // the first `rest` runs have one more
@@ -372,6 +374,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
   // and are passed over.
   int n_row = 0, pid_next = 0, mine = 0, issued = 0, wstage = 0;
   float n_ks = 0.0f, n_v = 0.0f, c_ks = 0.0f, c_lv = 0.0f;
+  uint32_t skip = 0;  // in 4 bits: the stages whose tile is in no page
   auto key_of = [&](int tile) { return min(sg.k0 + (warp + tile * WARPS) * TILE, sg.k1 - 1); };
   auto pid_of = [&](int tile) { return a.block_table[(int64_t)sg.b * a.width + (key_of(tile) >> a.page_log2)]; };
   auto issue = [&]() {
@@ -387,9 +390,11 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
         n_v = a.v_scale[blk];
       }
       n_v = outside ? -1.0f : n_v >= 0.0f ? n_v : -NEG_INF;  // no logarithm: the output is NaN
+      if (FP4 && outside) n_row = -1;
       pid_next = pid_of(issued + lane + 32);
     }
-    const int y = __shfl_sync(FULL, n_row, issued & 31);
+    int y = __shfl_sync(FULL, n_row, issued & 31);
+    if (FP4 && y < 0) skip |= 1u << wstage, y = 0;
     if (FP4 ? elect_one() : lane == 0) {
       const uint32_t bar = bar0 + 8 * wstage, dst = ring + wstage * C::STRIDE;
       mbar_expect_tx(bar, C::STAGE);
@@ -751,7 +756,6 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
 
   int i = 0;
   int nan_key = 0x7FFFFFFF;  // in 4 bits: the first key whose values in this lane's block are NaN
-  uint32_t c_outside = 0;  // in 4 bits: of the batch, the tiles in no page
   auto advance = [&]() {
     __syncwarp();  // every lane has read the stage
     if (issued < mine) issue();
@@ -759,12 +763,14 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
   };
   for (; i < mine; ++i, advance()) {
     const int key0 = k0 + (warp + i * WARPS) * TILE;
-    if ((i & 31) == 0) c_ks = n_ks, c_lv = FP4 ? n_v : log2f(n_v);
-    if constexpr (FP4) c_outside = (i & 31) == 0 ? __ballot_sync(FULL, n_v < 0.0f) : c_outside;
+    if (!FP4 && (i & 31) == 0) c_ks = n_ks, c_lv = log2f(n_v);
     const float ks = FP4 ? 1.0f : __shfl_sync(FULL, c_ks, i & 31), lv = FP4 ? 0.0f : __shfl_sync(FULL, c_lv, i & 31);
     ok = mbar_wait_warp(bar0 + 8 * stage, phase, nullptr, ERR_WAIT);
     if (!ok) break;
-    if (FP4 ? c_outside >> (i & 31) & 1u : lv != lv) continue;  // a page outside the cache
+    if (FP4 ? skip >> stage & 1u : lv != lv) {  // a page outside the cache
+      skip &= ~(1u << stage);
+      continue;
+    }
     const uint32_t kb = ring + stage * C::STRIDE, vb = kb + C::TILE_BYTES;
     // the key that index r of the products stands for
     auto place = [](int r) { return FP4 ? key4(r) : r; };
@@ -954,16 +960,17 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
             if (key0 + r1 >= end) e1 = 0;
           }
           sp[mt][p] = e0 | e1 << 8;
-          odd |= nan_bits(sp[mt][p]);
+          if (tail) odd |= nan_bits(sp[mt][p]);
 #pragma unroll
           for (int w = 0; w < VW; ++w) {
             ev[mt][p][w] = (x[w] & 0x0F0F0F0Fu) | (y[w] << 4 & 0xF0F0F0F0u);
             od[mt][p][w] = (x[w] >> 4 & 0x0F0F0F0Fu) | (y[w] & 0xF0F0F0F0u);
           }
         }
-      // 0 * NaN is NaN, also for a row that may not see the value: a NaN enters as 0,
-      // its key is noted, and the rows that see it get NaN at the segment's end
-      if (odd & 0x8080u) {
+      // 0 * NaN is NaN, also for a row that may not see the value: where rows differ in
+      // what they see a NaN enters as 0, its key is noted, and the rows that see it get
+      // NaN at the segment's end
+      if (tail && (odd & 0x8080u)) {
 #pragma unroll
         for (int q = 0; q < 8; ++q)
           if ((sp[q >> 2][q >> 1 & 1] >> (8 * (q & 1)) & 0x7Fu) == 0x7Fu) {
