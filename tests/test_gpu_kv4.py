@@ -387,6 +387,68 @@ def test_attend4_prompts(D, Hkv, G, page):
     _check_attend(1, 513, Hkv, G, D, page, [127], seed=3)
 
 
+@pytest.mark.parametrize("B,T,Hkv,G,D", [(40, 130, 4, 2, 128), (200, 70, 2, 2, 64), (75, 129, 2, 2, 64), (3, 1100, 8, 4, 64)])
+def test_attend4_many_heads(B, T, Hkv, G, D):
+    """More row tiles than CTAs, of equal and of unequal sizes, some of them empty;
+    more sequences than a CTA keeps plans of."""
+    held = [(i * 37) % 150 for i in range(B)]
+    counts = [0 if i % 7 == 3 else T - (i * 29) % T for i in range(B)]
+    _check_attend(B, T, Hkv, G, D, 64, held, counts, seed=B)
+    _check_attend(B, T, Hkv, G, D, 64, [100] * B, seed=B + 1)
+
+
+@pytest.mark.parametrize("T,G", [(1, 4), (3, 8), (9, 8), (60, 4)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend4_growing_scores(T, G, D):
+    """Keys that grow along the sequence: the running maximum moves on and on."""
+    def grow(cache, bt):
+        raw = cache.k_scale.view(torch.uint8)
+        pos = torch.arange(bt.shape[1] * 32, device="cuda").view(-1, 32)
+        for p in range(bt.shape[1]):
+            raw[int(bt[0, p])] = (0x10 + pos[p] * 0x30 // pos.numel()).byte()[None, :, None]
+        cache.k_factor.fill_(0.2)
+
+    _check_attend(1, T, 2, G, D, 32, [2500], seed=11, edit=grow, stale=False)
+
+
+@pytest.mark.parametrize("T,G", [(2, 4), (40, 4), (90, 2)])
+def test_attend4_queries_that_are_no_numbers(T, G):
+    """A NaN or an infinity in a query stays in its row."""
+    from voyager_b200 import kvcache
+
+    bt, cache = _table(1, 16, 1), _cache(20, 2, 64, 128, 2)
+    q = torch.randn(1, T, 2 * G, 128, generator=_gen(3), device="cuda").bfloat16()
+    want = kvcache.attend(q, cache, bt, _i32([800]))
+    for bad in (float("nan"), float("inf")):
+        x = q.clone()
+        x[0, 1, 1, 7] = bad
+        out = kvcache.attend(x, cache, bt, _i32([800]))
+        assert bool(out[0, 1, 1].isnan().all())
+        keep = torch.ones(1, T, 2 * G, dtype=torch.bool, device="cuda")
+        keep[0, 1, 1] = False
+        assert torch.equal(out[keep], want[keep])
+
+
+def test_attend4_kernels_take_turns():
+    """Calls of few and of many rows on one stream, and captured together, share
+    their counters and leave them as they were."""
+    from voyager_b200 import kvcache
+
+    bt = _table(6, 70, 1)
+    cache = _cache(430, 4, 64, 128, 2)
+    held = _i32([4000, 10, 900, 0, 2000, 333])
+    qs = [torch.randn(6, T, 16, 128, generator=_gen(T), device="cuda").bfloat16() for T in (1, 200, 4, 60, 12)]
+    want = [kvcache.attend(q, cache, bt, held) for q in qs]
+    for _ in range(4):
+        assert all(torch.equal(kvcache.attend(q, cache, bt, held), w) for q, w in zip(qs, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [kvcache.attend(q, cache, bt, held) for q in qs]
+    for _ in range(3):
+        graph.replay()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
 def test_attend4_empty_sequences():
     """No key at all, no new token, and both beside ordinary sequences."""
     from voyager_b200 import kvcache
