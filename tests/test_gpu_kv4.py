@@ -200,6 +200,34 @@ def test_append4_specials():
     assert int(c.v_scale.float().isnan().sum()) == 1
 
 
+@pytest.mark.parametrize("tokens", [1, 40])
+@pytest.mark.parametrize("power", [-100, -30, -12, 0, 12, 100])
+def test_append4_saturates_under_any_factor(power, tokens):
+    """Infinities and the largest values saturate, and ordinary ones keep their codes, whatever the
+    factor; every quotient is a power of two's multiple that float32 holds, so nothing is rounded."""
+    from voyager_b200 import kvcache
+
+    f, top = 2.0 ** power, torch.finfo(torch.float32).max
+    rows = torch.tensor([[math.inf, 1.0, -1.0], [-math.inf, 0.0, top], [-top, top, 0.0], [6 * 448 * f, -448 * f, 0.0],
+                         [-6 * f, 5 * f, 1.25 * f], [6e4 * f, 448 * f, -224 * f]], device="cuda")
+    n = len(rows)
+    x = torch.zeros(n, tokens, 40, 128, device="cuda")
+    x[..., 16:19] = rows[:, None, None]
+    factor = torch.full((40,), f, device="cuda")
+    cache = kvcache.KVCache4.empty(n, 40, 128, 64, k_factor=factor, v_factor=factor)
+    bt = torch.arange(n, device="cuda").int()[:, None].contiguous()
+    held = torch.zeros(n, dtype=torch.int32, device="cuda")
+    table = kvcache.rotary_table(64, 16)  # columns from 16 on do not turn
+    kvcache.rope_append(x, x, x, table, cache, bt, held)
+    y = x[0:, :, 0, 16:32].double()
+    scale = block_scale(y.abs().amax(-1), f)
+    want = e2m1(y / (scale * f)[..., None])
+    for codes, scales in ((cache.k_codes, cache.k_scale), (cache.v_codes, cache.v_scale)):
+        got = codes_of(codes[:, :, :tokens].transpose(1, 2)).unflatten(-1, (8, 16))[..., 1, :]
+        assert torch.equal(scales.float()[:, :, :tokens, 1].transpose(1, 2).double(), scale[..., None].expand(-1, -1, 40))
+        assert torch.equal(got, want[:, :, None].expand_as(got))
+
+
 def test_append4_token_by_token_is_the_prompt():
     """Tokens do not touch each other's blocks: one at a time, in pieces and at
     once give the same bytes."""

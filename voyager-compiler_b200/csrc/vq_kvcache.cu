@@ -622,8 +622,9 @@ __device__ __forceinline__ void turn4(float (&x0)[8], float (&x1)[8], const floa
     x0[i] = p.x, x0[i + 1] = p.y, x1[i] = q.x, x1[i + 1] = q.y;
   }
 }
-// 8 values, their quotients by d, as codes: 4 bytes.  `finite`: the products of the
-// correction stay in float32; beyond, the values saturate all the same.
+// 8 values, their quotients by d, as codes: 4 bytes.  `finite`: the correction's
+// products stay in float32; a block with quotients beyond goes without it, and those
+// saturate all the same.
 __device__ __forceinline__ uint32_t e2m1_codes(const float (&x)[8], float d, float r, bool finite) {
   float y[8];
   const float2 rr = make_float2(r, r), nd = make_float2(-d, -d);
@@ -658,8 +659,8 @@ __device__ __forceinline__ float amax8(const float (&x)[8]) {
 // A block's scale byte, what its values are divided by, and that one's reciprocal.
 __device__ __forceinline__ uint32_t block_scale4(float amax, float f, float& d, float& r) {
   const float six = 6.0f * f, r6 = reciprocal(six);
-  float a;  // an infinity saturates like any large value; NaN stays
-  asm("min.NaN.f32 %0, %1, 0f7CF0BDC2;" : "=f"(a) : "f"(amax));  // 1e37
+  float a;  // from 464 on a quotient saturates, an infinity's too; NaN stays
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(amax), "f"(1024.0f * six));
   float q = a * r6;
   q = fmaf(fmaf(-q, six, a), r6, q);
   const uint32_t b = max(pack2(q, 0.0f) & 0xFFu, 1u);
@@ -699,7 +700,7 @@ __device__ __forceinline__ void store4(uint8_t* codes, uint8_t* scale, const flo
     e1 = block_scale4(m1, f, d1, r1);
   else
     d1 = d0, r1 = r0;
-  const uint32_t w0 = e2m1_codes(x0, d0, r0, m0 < 1e30f), w1 = e2m1_codes(x1, d1, r1, m1 < 1e30f);
+  const uint32_t w0 = e2m1_codes(x0, d0, r0, m0 < 0x1p100f * d0), w1 = e2m1_codes(x1, d1, r1, m1 < 0x1p100f * d1);
   if (split) {
     const int g1 = u + R;
     reinterpret_cast<uint32_t*>(codes)[u] = w0;

@@ -62,7 +62,7 @@ class KVCache:
 class KVCache4:
     """Codes uint8 [pages, kv_heads, page, head_dim / 2], two E2M1 codes a byte with
     the even column in the low half, scales float8_e4m3fn [pages, kv_heads, page,
-    head_dim / 16], factors float32 [kv_heads], positive.  A value is code x scale
+    head_dim / 16], factors float32 [kv_heads] within 2^-100 .. 2^100.  A value is code x scale
     x its head's factor.  Scales reach from 2^-9 to 448, codes to 6: a factor of
     max|x| / 2688 over a head uses the scales' whole range, and 1 holds values up
     to 2688 with blocks below 0.01 losing bits."""
