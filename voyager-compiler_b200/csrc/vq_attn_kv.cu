@@ -1,4 +1,4 @@
-// Attention of the newest tokens over a paged E4M3 key / value cache.
+// Attention of the newest tokens over a paged key / value cache, in E4M3 or in 4 bits.
 //
 //   o[b, t, h] = sum_j softmax_j(q . k_j * sm_scale) v_j,  j <= held[b] + t,
 //   k_j = code * k_scale[page of j, head], v_j likewise
@@ -35,6 +35,26 @@
 // heads of 128: 168 us, 6.4 TB/s); one short sequence by a chain of latencies
 // (99 keys: 7 us); several row tiles by the products (5 tokens x 7 heads of 64:
 // 24 us where the bytes take 2.5).
+//
+// FP4: the cache of vq_rope_append_kv4 (E2M1 codes, an E4M3 scale per 16 columns of
+// a token, a float32 factor per head), for calls with few rows a kv head; the others
+// are vq_attn_kv4.cu's.  The same work with these differences:
+//  - a tile's codes and scales lie side by side, so that four untiled copies fetch
+//    it; the fragment loads' bank conflicts are avoided by the order of the keys
+//    within the product (key4), which no sum depends on.
+//  - code * scale is exact in f16 (6 significant bits): two PRMTs a word of codes
+//    and a multiplication by the scale make the operands.  A key pair's codes lie in
+//    one word, so that V needs no shuffle.
+//  - no page has a factor of its own, so the weights are relative to m alone, and m
+//    and O move only where some score of the tile passes m (a vote): 2^(15 + s - m).
+//  - a NaN scale makes K's scores NaN as it is.  V's is looked for only in tiles whose
+//    keys some row does not see (0 * NaN); its key is noted, and the rows that see
+//    it get NaN at the end.
+// Bound by instructions: 676 a warp and tile of 32 keys and 8 rows, of which the
+// loads, conversions and products of 4.5 KB are most; HBM has 9/16 of E4M3's bytes.
+// 4 sequences of 131000 keys, 8 x 8 heads of 128: 134 us, 4.5 TB/s (143 over and over,
+// when the power cap takes the clock to 1.82 GHz); 32 sequences to 8192, 8 x 4 heads:
+// 45 us where E4M3 takes 53; 99 keys: 7.7 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -88,7 +108,7 @@ struct Args {
 // CTAs per SM.  Three with heads of 64 and one row tile (24 sequences of 28631
 // keys: 130 us against 149 with two, in deeper rings than now); otherwise the third CTA costs more in
 // joins and shallower rings than its warps give (heads of 128, 32 sequences:
-// 66 us against 55).
+// 66 us against 55).  In 4 bits, bound by instructions, three with one row tile.
 constexpr int ctas_per_sm(int head_dim, int nt, bool fp4) {
   return (head_dim == 64 || fp4) && nt == 1 ? 3 : 2;
 }
@@ -103,7 +123,8 @@ struct Cfg {
   // Two stages a warp: 128 KB in flight an SM (96 KB at heads of 64) fill HBM, and
   // more only lengthens the queue that every other access waits in (4 sequences
   // of 131000 keys: 168 us, with three 178; heads of 64, 24 sequences of 28631:
-  // 118, with four 126).
+  // 118, with four 126).  In 4 bits a stage is 9/16 as large: two of them at heads of
+  // 128 and three CTAs an SM (108 KB), three at heads of 64 (81 KB).
   static constexpr int PER_SM = ctas_per_sm(D, NT, FP4);
   static constexpr int STAGES = FP4 ? (D == 128 ? 2 : 3) : D == 128 || PER_SM == 3 ? 2 : 3;
   static constexpr int RING = STAGES * STRIDE;  // per warp

@@ -1,5 +1,6 @@
 // Attention of many query rows over the paged 4-bit key / value cache: prompts,
-// pieces of prompts, and drafts of more than 16 rows a kv head.
+// pieces of prompts, and drafts of many rows a kv head (vq_attn_kv.cu's
+// few_rows() says from where on).
 //
 //   o[b, t, h] = sum_j softmax_j(q . k_j * sm_scale) v_j,  j <= held[b] + t,
 //   k_j = code * scale * factor, v_j likewise (vq_rope_append_kv4's cache)
@@ -21,18 +22,33 @@
 // the end, the others nothing (0 * NaN would reach every row of the tile).
 //
 // Work: two streams of 128 rows, each with a warpgroup for its softmax (a thread
-// is a row) and its own S and O in tensor memory; P lies in place of S and is the
-// second product's first operand.  While one stream's softmax runs, the tensor
-// cores work for the other.  PAIR: the streams are 256 rows of a head and share
-// the keys.  Otherwise a head has at most 128 rows: both streams have them and
-// take every other tile of keys; their sums meet in shared memory.  Four warps
-// each turn 128 keys' K and V from codes to f16 in shared memory, in the
-// SWIZZLE_128B layout that serves K as K-major and V as MN-major operand; the
-// next tile's codes are on their way in registers meanwhile.
+// is a row) and its own S and O in tensor memory.  PAIR: the streams are 256 rows
+// of a head and share the keys.  Otherwise a head has at most 128 rows: both
+// streams have them and take every other tile of keys; their sums meet in shared
+// memory.  A tile of 128 keys goes in two halves of 64: S of a half is asked for
+// as soon as the weights in its place have been used, so that while one half is in
+// the softmax the tensor cores have the stream's other half and the other stream.
+// P lies in place of its half of S and is the second product's first operand.
+//
+// Warps: eight of softmax; four turn K and four V from codes to f16 in shared
+// memory, in the SWIZZLE_128B layout that serves K as K-major and V as MN-major
+// operand (a tile's codes travel to registers while its buffer is still in use);
+// one issues the MMAs; one looks up where the tiles lie, some ahead, and asks for
+// their lines in L2.  The softmax needs 144 registers, the conversion 56.
 //
 // The tiles of every (sequence, row tile, kv head) lie end to end and are cut into
 // equal runs, one per CTA, one CTA per SM; the pieces of a head that was cut are
-// joined by the CTA that finishes last, in the CTAs' order.
+// joined by the CTA that finishes last, in the CTAs' order.  With many heads of
+// PAIR rows, where the CTAs idle for less than a cut costs, they are not cut: a CTA
+// takes the next one off a counter, the long ones first.
+//
+// Bound by the round trips of a half tile: from its S over the softmax and P to the
+// next S take about 2000 cycles of a stream, two halves of two streams at a time;
+// the tensor pipe is 34 % active, issue slots 38 %, the exponentials' unit 34 %.
+// S at N = 64 reads the queries from shared memory anew for every half.  Pairs of
+// CTAs (cta_group::2) would share the conversion of a tile; not built.  500 tokens x
+// 5 heads on 16011 held, 8 kv heads of 128: 201 us, 830 TFLOP/s; 4 prompts of 2048
+// tokens, 8 x 4 heads: 195 us, 705.  Few tiles: start, ends and joins, about 22 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
