@@ -72,8 +72,8 @@ enum { ERR_WAIT = 331, ERR_PAGE = 332, ERR_CAPACITY = 333, ERR_COUNT = 334 };
 
 constexpr int TILE = 128;  // keys
 constexpr int PLANS = 128;
-// warps: 0-7 softmax (a stream's four each), 8-11 K and 12-15 V from codes to f16, 16 the MMAs, 17 where the tiles
-// lie, 18 and 19 none (a warpgroup's registers are split together)
+// warps: 0-7 softmax (a stream's four each), 8-11 K and 12-15 V from codes to f16, 16 and 18 the streams' MMAs, 17
+// where the tiles lie, 19 none (a warpgroup's registers are split together)
 constexpr int SM_WARPS = 8, W_DQ = 8, W_MMA = 16, W_SCOUT = 17, WARPS = 20, THREADS = WARPS * 32;
 // registers a thread: launched with 96; a warpgroup of 4 warps gives some up or takes them
 constexpr int R_LAUNCH = 96, R_SOFT = 144, R_DQ = 56, R_REST = 80;
@@ -327,16 +327,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
       // one arrival a warp, or a commit
-      mbar_init(bar(B_KFULL + i), 4), mbar_init(bar(B_KEMPTY + i), 1);
-      mbar_init(bar(B_VFULL + i), 4), mbar_init(bar(B_VEMPTY + i), 1);
+      mbar_init(bar(B_KFULL + i), 4), mbar_init(bar(B_KEMPTY + i), PAIR ? 2 : 1);
+      mbar_init(bar(B_VFULL + i), 4), mbar_init(bar(B_VEMPTY + i), PAIR ? 2 : 1);
       mbar_init(bar(B_QFULL + i), 4), mbar_init(bar(B_ODONE + i), 1), mbar_init(bar(B_OFULL + i), 1);
       mbar_init(bar(B_SFULL + i), 1), mbar_init(bar(B_SFULL + 2 + i), 1);
       mbar_init(bar(B_PFULL + i), 4), mbar_init(bar(B_PFULL + 2 + i), 4);
-      mbar_init(bar(B_SOFT + i), PAIR ? 4 : 8);
+      mbar_init(bar(B_SOFT + i), PAIR ? 4 : 8), mbar_init(bar(B_DRAIN + i), 1);
     }
     for (int i = 0; i < TURNS; ++i) mbar_init(bar(B_TFULL + i), 1), mbar_init(bar(B_TEMPTY + i), 8);
-    for (int i = 0; i < SEGS; ++i) mbar_init(bar(B_GFULL + i), 1), mbar_init(bar(B_GEMPTY + i), SM_WARPS + 1);
-    mbar_init(bar(B_DRAIN), 1);
+    for (int i = 0; i < SEGS; ++i) mbar_init(bar(B_GFULL + i), 1), mbar_init(bar(B_GEMPTY + i), SM_WARPS + 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == W_MMA) {
@@ -600,52 +599,53 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
         if (lane < 4) s_tile[slot][lane] = make_uint4(NO_TILE, 0, 0, 0);
         arrive(B_TFULL + slot);
       }
-    } else if (warp == W_MMA) {
-      // ---------------- MMA issuer ----------------
+    } else if (warp != W_MMA + 3) {
+      // ---------------- MMA issuers, one a stream ----------------
       // The whole warp runs the loop and one lane issues: the operands then stay in
       // uniform registers.
       constexpr uint32_t ID_S = idesc_f16(64, false), ID_O = idesc_f16(D, true);
-      const uint64_t dq = sw128_desc(sbase + L::OFF_Q), dk = sw128_desc(sbase + L::OFF_K),
-                     dv = mn_desc(sbase + L::OFF_V, L::HALF);
       constexpr uint32_t TILE16 = L::TILE_BYTES / 16;
-      uint32_t kph = 0, vph = 0, qph = 0, pph = 0;  // bits: of the buffers, the streams, streams' halves (2 i + half)
-      int kb = 0, vb = 0;                           // buffers of the segment's next tile
+      const int i = warp == W_MMA ? 0 : 1;
+      const uint64_t dq = sw128_desc(sbase + L::OFF_Q + i * L::TILE_BYTES), dk = sw128_desc(sbase + L::OFF_K),
+                     dv = mn_desc(sbase + L::OFF_V, L::HALF);
+      const uint32_t ts = tmem + COL_S + i * 128, to = tmem + COL_O + i * 128;
+      uint32_t qph = 0, pph = 0;  // pph: bits of the halves
       bool ok = true;
-      // S of a half tile (64 keys) of stream i from K buffer b; `release`: its last reader
-      auto scores = [&](int i, int half, int b, bool release) {
+      // S of a half (64 keys) of tile g; `release`: the stream's last use of its keys
+      auto scores = [&](int half, int g, bool release) {
         if (elect_one()) {
-          const uint64_t q = desc_at(dq, i * TILE16), k = desc_at(dk, b * TILE16 + half * (64 * 128 / 16));
+          const uint64_t k = desc_at(dk, (g & 1) * TILE16 + half * (64 * 128 / 16));
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
             const uint32_t off = ((s >> 2) * L::HALF + (s & 3) * 32) / 16;
-            mma_ss(tmem + COL_S + i * 128 + half * 64, desc_at(q, off), desc_at(k, off), ID_S, s > 0);
+            mma_ss(ts + half * 64, desc_at(dq, off), desc_at(k, off), ID_S, s > 0);
           }
           tc_commit(bar(B_SFULL + 2 * i + half));
-          if (release) tc_commit(bar(B_KEMPTY + b));
+          if (release) tc_commit(bar(B_KEMPTY + (g & 1)));
         }
         __syncwarp();
       };
-      // O of stream i and that half's values from V buffer b
-      auto values = [&](int i, int half, int b, bool first, bool release, bool last) {
+      // O and that half's values
+      auto values = [&](int half, int g, bool first, bool last) {
         if (elect_one()) {
-          const uint64_t v = desc_at(dv, b * TILE16 + half * (64 * 128 / 16));
-          const uint32_t p = tmem + COL_S + i * 128 + half * 64;
+          const uint64_t v = desc_at(dv, (g & 1) * TILE16 + half * (64 * 128 / 16));
+          const uint32_t p = ts + half * 64;
 #pragma unroll
-          for (int s = 0; s < 4; ++s)
-            mma_ts(tmem + COL_O + i * 128, p + s * 8, desc_at(v, s * 128), ID_O, !first || s > 0);
+          for (int s = 0; s < 4; ++s) mma_ts(to, p + s * 8, desc_at(v, s * 128), ID_O, !first || s > 0);
           tc_commit(bar(B_ODONE + i));
           if (last) tc_commit(bar(B_OFULL + i));
-          if (release) tc_commit(bar(B_VEMPTY + b));
+          if (half) tc_commit(bar(B_VEMPTY + (g & 1)));
         }
         __syncwarp();
       };
-      auto take = [&](int b, int i, uint32_t& ph) {
-        ok = ok && mbar_wait_warp(bar(b + i), ph >> i & 1, nullptr, ERR_WAIT);
-        ph ^= 1u << i;
+      auto take = [&](int b, uint32_t parity) {
+        ok = ok && mbar_wait_warp(bar(b), parity, nullptr, ERR_WAIT);
         tc_fence_after();
         return ok;
       };
-      int turn = 0;
+      // PAIR: every tile is both streams'; otherwise tile t of a segment is stream t % 2's
+      constexpr int STEP = PAIR ? 1 : 2;
+      int turn = 0, g0 = 0;  // g0: tiles before the segment
       uint32_t gphase = 0;
       while (true) {
         ok = mbar_wait_warp(bar(B_GFULL + turn), gphase, nullptr, ERR_WAIT);
@@ -654,53 +654,36 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
         arrive(B_GEMPTY + turn);
         if (n == 0) break;
         if (++turn == SEGS) turn = 0, gphase ^= 1;
-        if (PAIR) {
-          // both streams take every tile; a half's scores are asked for when the
-          // weights in their place have been used, two halves ahead of the softmax
-          if (!take(B_KFULL, kb, kph)) break;
-          for (int i = 0; i < 2; ++i) {
-            if (!take(B_QFULL, i, qph)) break;
-            scores(i, 0, kb, false);
-            scores(i, 1, kb, i == 1);
-          }
-          if (!ok) break;
-          kb ^= 1;
-          for (int h = 0; h < 2 * n && ok; ++h) {
-            const int half = h & 1;
-            const bool again = h + 2 < 2 * n;
-            if (!half && (!take(B_VFULL, vb, vph) || (again && !take(B_KFULL, kb, kph)))) break;
-            for (int i = 0; i < 2; ++i) {
-              if (!take(B_PFULL, 2 * i + half, pph)) break;
-              values(i, half, vb, h == 0, half && i == 1, h + 1 == 2 * n);
-              if (again) scores(i, half, kb, half && i == 1);
-            }
-            if (half) vb ^= 1, kb ^= again;
-          }
-        } else {
-          // tile t is stream t % 2's, in buffers that stay its own for the segment
-          if (!take(B_QFULL, 0, qph) || !take(B_QFULL, 1, qph)) break;
-          for (int i = 0; i < min(n, 2); ++i) {
-            if (!take(B_KFULL, kb ^ i, kph)) break;
-            scores(i, 0, kb ^ i, false);
-            scores(i, 1, kb ^ i, true);
-          }
-          for (int h = 0; h < n + (n & 1) && ok; ++h)  // halves of stream 0
-            for (int i = 0; i < 2 && ok; ++i) {
-              const int half = h & 1, t = (h >> 1) * 2 + i;
-              if (t >= n) continue;
-              if (!half && !take(B_VFULL, vb ^ i, vph)) break;
-              if (!half && t + 2 < n && !take(B_KFULL, kb ^ i, kph)) break;
-              if (!take(B_PFULL, 2 * i + half, pph)) break;
-              values(i, half, vb ^ i, h == 0, half, half && t + 2 >= n);
-              if (t + 2 < n) scores(i, half, kb ^ i, half);
-            }
-          kb ^= n & 1, vb ^= n & 1;
+        // a half's scores are asked for when the weights in their place have been
+        // used, two halves ahead of the softmax
+        const int j0 = PAIR ? 0 : i;
+        if (!take(B_QFULL + i, qph)) break;
+        qph ^= 1;
+        if (j0 < n) {
+          if (!take(B_KFULL + ((g0 + j0) & 1), (g0 + j0) >> 1 & 1)) break;
+          scores(0, g0 + j0, false);
+          scores(1, g0 + j0, true);
         }
+        for (int j = j0; j < n && ok; j += STEP) {
+          const int g = g0 + j;
+          const bool again = j + STEP < n;
+          if (!take(B_VFULL + (g & 1), g >> 1 & 1)) break;
+          if (again && !take(B_KFULL + ((g + STEP) & 1), (g + STEP) >> 1 & 1)) break;
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half) {
+            if (!take(B_PFULL + 2 * i + half, pph >> half & 1)) break;
+            pph ^= 1u << half;
+            values(half, g, j == j0 && half == 0, half && !again);
+            if (again) scores(half, g + STEP, half);
+          }
+        }
+        if (!ok) break;
+        g0 += n;
       }
       // every MMA issued has completed before the TMEM is released
       if (elect_one()) {
-        tc_commit(bar(B_DRAIN));
-        mbar_wait(bar(B_DRAIN), 0, nullptr, ERR_WAIT);
+        tc_commit(bar(B_DRAIN + i));
+        mbar_wait(bar(B_DRAIN + i), 0, nullptr, ERR_WAIT);
       }
       __syncwarp();
     }
