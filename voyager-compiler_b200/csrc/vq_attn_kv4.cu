@@ -33,8 +33,9 @@
 // Warps: eight of softmax; four turn K and four V from codes to f16 in shared
 // memory, in the SWIZZLE_128B layout that serves K as K-major and V as MN-major
 // operand (a tile's codes travel to registers while its buffer is still in use);
-// one issues the MMAs; one looks up where the tiles lie, some ahead, and asks for
-// their lines in L2.  The softmax needs 144 registers, the conversion 56.
+// one a stream issues its MMAs, so that neither stream waits for the other's weights;
+// one looks up where the tiles lie, some ahead, and asks for their lines in L2.  The
+// softmax needs 144 registers, the conversion 56.
 //
 // The tiles of every (sequence, row tile, kv head) lie end to end and are cut into
 // equal runs, one per CTA, one CTA per SM; the pieces of a head that was cut are
@@ -42,13 +43,16 @@
 // PAIR rows, where the CTAs idle for less than a cut costs, they are not cut: a CTA
 // takes the next one off a counter, the long ones first.
 //
-// Bound by the round trips of a half tile: from its S over the softmax and P to the
-// next S take about 2000 cycles of a stream, two halves of two streams at a time;
-// the tensor pipe is 34 % active, issue slots 38 %, the exponentials' unit 34 %.
-// S at N = 64 reads the queries from shared memory anew for every half.  Pairs of
-// CTAs (cta_group::2) would share the conversion of a tile; not built.  500 tokens x
-// 5 heads on 16011 held, 8 kv heads of 128: 201 us, 830 TFLOP/s; 4 prompts of 2048
-// tokens, 8 x 4 heads: 195 us, 705.  Few tiles: start, ends and joins, about 22 us.
+// Bound by the softmax warps' own chain, 2100 cycles a half tile: 200 to find the scores
+// there, 420 to read them and their maximum, 1250 for the weights (the exponentials'
+// unit is shared by the streams' warps, 1024 at its rate), 250 to store and hand over;
+// the tensor pipe has 1024 of work in that time (S at N = 64 reads the queries anew for
+// every half, 6 KB an MMA).  Slower were: sixteen warps of softmax at 88 registers
+// (208 us where this takes 190), the next half's scores read under this one's weights
+// (212: spills), weights of the two streams in turn (193), whole tiles.  Pairs of CTAs
+// (cta_group::2) would share the conversion of a tile; not built.  500 tokens x 5 heads
+// on 16011 held, 8 kv heads of 128: 193 us, 860 TFLOP/s; 4 prompts of 2048 tokens, 8 x 4
+// heads: 192 us, 716.  Few tiles: start, ends and joins, about 22 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
