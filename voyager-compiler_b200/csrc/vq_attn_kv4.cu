@@ -51,8 +51,8 @@
 // (208 us where this takes 190), the next half's scores read under this one's weights
 // (212: spills), weights of the two streams in turn (193), whole tiles.  Pairs of CTAs
 // (cta_group::2) would share the conversion of a tile; not built.  500 tokens x 5 heads
-// on 16011 held, 8 kv heads of 128: 193 us, 860 TFLOP/s; 4 prompts of 2048 tokens, 8 x 4
-// heads: 192 us, 716.  Few tiles: start, ends and joins, about 22 us.
+// on 16011 held, 8 kv heads of 128: 186 us, 895 TFLOP/s; 4 prompts of 2048 tokens, 8 x 4
+// heads: 189 us, 728.  Few tiles: start, ends and joins, about 22 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
