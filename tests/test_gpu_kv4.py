@@ -550,6 +550,42 @@ def test_attend4_offsets_past_32_bits(T):
     assert not torch.equal(before[1], cache.k_codes[3, :, 127])
 
 
+@pytest.mark.parametrize("T,G,D", [(40, 4, 128), (60, 4, 64), (30, 4, 128), (25, 5, 64), (3, 4, 64)])
+def test_attend4_many_heads_on_two_streams(T, G, D):
+    """Heads taken whole, cut and joined, or few rows: calls on two streams and two graphs at once
+    take theirs from counters of their own, and whoever takes a head computes the same."""
+    from voyager_b200 import kvcache
+
+    B, Hkv = 40, 8
+    bt = _table(B, 7, 1)
+    cache = _cache(B * 7 + 2, Hkv, 64, D, 2)
+    held = _i32([300 + 2 * b for b in range(B)])
+    qs = [torch.randn(B, T, Hkv * G, D, generator=_gen(i), device="cuda").bfloat16() for i in range(2)]
+    want = [kvcache.attend(q, cache, bt, held) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(kvcache.attend(qs[i], cache, bt, held))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph):
+            outs.append(kvcache.attend(qs[i], cache, bt, held))
+    for _ in range(5):
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    counts = [int(n) for n in torch.randint(0, T + 1, (B,), generator=torch.Generator().manual_seed(1))]
+    _check_attend(B, T, Hkv, G, D, 64, held.tolist(), counts, seed=T)
+
+
 @pytest.mark.parametrize("T", [1, 40])
 def test_attend4_streams_and_graphs(T):
     """Calls on two streams do not share their joins; a captured call replays."""

@@ -885,6 +885,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
       float ow = 1.0f, xw = 0.0f;  // weights of this stream's O and of the other's
       const float4* other = reinterpret_cast<const float4*>(smem + L::OFF_Q);
       if (!PAIR) {  // the second stream's sums to the first, through the queries' place
+        if (!soft_sync()) break;  // whose last reader may be the other stream: its last scores are there
         if (i == 1) {
           s_ml[r] = m, s_ml[128 + r] = l;
           if (had && any_live)
