@@ -801,7 +801,9 @@ int vq_attn_kv8(const void* q, const int64_t* q_strides, int64_t batch, int64_t 
 
 /* vq_attn_kv8 over the 4-bit cache of vq_rope_append_kv4; scales 16-byte and out
  * 32-byte aligned.  Calls of many rows a kv head (tokens * heads / kv_heads) run
- * another kernel, whose waits and plans set the sticky word to 331-334. */
+ * another kernel, whose waits and plans set the sticky word to 331-334; it takes its
+ * counters from the workspace, which may hold anything, and needs none here (0, may
+ * be NULL). */
 int vq_attn_kv4_workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_heads,
                           int32_t head_dim, int32_t page, int64_t table_width, int64_t* floats,
                           int64_t* counters);

@@ -362,7 +362,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
                                                                       (int)c.page, width, &floats, &counters),
              what))
     return nullptr;
-  const Tensor done = join_counters(q, counters);
+  const Tensor done = counters ? join_counters(q, counters) : Tensor();
   const Tensor part = output({floats}, at::kFloat, q);
   const int64_t strides[3] = {q.stride(0), q.stride(1), q.stride(2)};
   const int st =
@@ -370,11 +370,11 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
                            c.vc.data_ptr(), c.ks.data_ptr(), c.vs.data_ptr(), c.kf.data_ptr<float>(),
                            c.vf.data_ptr<float>(), c.pages, (int)c.page, plan.table.data_ptr(), width,
                            plan.lengths.data_ptr(), ptr(plan.counts), (float)scale, part.data_ptr<float>(), floats,
-                           done.data_ptr<int>(), done.numel(), out.data_ptr(), stream_of(q))
+                           (int32_t*)ptr(done), counters, out.data_ptr(), stream_of(q))
              : vq_attn_kv8(q.data_ptr(), strides, B, T, (int)H, (int)c.heads, (int)c.dim, c.kc.data_ptr(),
                            c.vc.data_ptr(), c.ks.data_ptr<float>(), c.vs.data_ptr<float>(), c.pages, (int)c.page,
                            plan.table.data_ptr(), width, plan.lengths.data_ptr(), ptr(plan.counts), (float)scale,
-                           part.data_ptr<float>(), floats, done.data_ptr<int>(), done.numel(), out.data_ptr(),
+                           part.data_ptr<float>(), floats, (int32_t*)ptr(done), counters, out.data_ptr(),
                            stream_of(q));
   if (failed(st, what)) return nullptr;
   no_derivative(what, {&q, &c.kc, &c.vc, &c.ks, &c.vs, &c.kf, &c.vf}, {&out});

@@ -70,13 +70,12 @@
 
 namespace vq {
 namespace kv4 {  // vq_attn_kv4.cu
-void workspace(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim, int64_t capacity, int64_t* floats,
-               int64_t* counters);
+int64_t workspace(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim, int64_t capacity);
 int attend(const void* q, const int64_t* q_strides, int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim,
            const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, const float* k_factor,
            const float* v_factor, int64_t pages, int page, const void* block_table, int64_t table_width,
            const void* lengths, const void* counts, float sm_scale, float* workspace, int64_t workspace_floats,
-           int32_t* counters, int64_t counters_len, void* out, cudaStream_t st);
+           void* out, cudaStream_t st);
 }  // namespace kv4
 namespace kva {
 
@@ -1185,7 +1184,8 @@ static int workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_he
       page <= 0 || table_width < 0 || table_width > max_width(page))
     return VQ_ERR_INVALID;
   if (fp4 && !few_rows(batch, tokens * (heads / kv_heads), kv_heads, table_width * page)) {
-    vq::kv4::workspace(batch, tokens, heads, kv_heads, head_dim, table_width * page, floats, counters);
+    *floats = vq::kv4::workspace(batch, tokens, heads, kv_heads, head_dim, table_width * page);
+    *counters = 0;
     return VQ_OK;
   }
   const Cut c = cut_of(std::max<int64_t>(batch, 1), std::max<int64_t>(tokens, 1), heads, kv_heads,
@@ -1225,8 +1225,9 @@ static int attention(const void* q, const int64_t* q_strides, int64_t batch, int
     const int64_t ctas = std::min<int64_t>((chunks + THREADS - 1) / THREADS, 8 * vq::mx::sm_count());
     return vq::pdl::launch<k_attn_none>((unsigned)ctas, THREADS, 0, st, 1, a, chunks) ? VQ_OK : VQ_ERR_CUDA;
   }
+  const bool few = !fp4 || few_rows(batch, tokens * a.G, kv_heads, table_width * page);
   if (!q || !q_strides || !k_codes || !v_codes || !k_scale || !v_scale || !block_table || !lengths ||
-      !counters || !out || (fp4 && (!k_factor || !v_factor)))
+      (few && !counters) || !out || (fp4 && (!k_factor || !v_factor)))
     return VQ_ERR_NULL;
   const void* p16[7] = {q, k_codes, v_codes, out, workspace, fp4 ? k_scale : nullptr, fp4 ? v_scale : nullptr};
   for (const void* p : p16)
@@ -1234,10 +1235,10 @@ static int attention(const void* q, const int64_t* q_strides, int64_t batch, int
   if (fp4 && (reinterpret_cast<uintptr_t>(out) & 31)) return VQ_ERR_ALIGNMENT;
   for (int i = 0; i < 3; ++i)
     if (q_strides[i] % 8) return VQ_ERR_ALIGNMENT;
-  if (fp4 && !few_rows(batch, tokens * a.G, kv_heads, table_width * page))
+  if (!few)
     return vq::kv4::attend(q, q_strides, batch, tokens, heads, kv_heads, head_dim, k_codes, v_codes, k_scale, v_scale,
                            k_factor, v_factor, pages, page, block_table, table_width, lengths, counts, sm_scale,
-                           workspace, workspace_floats, counters, counters_len, out, st);
+                           workspace, workspace_floats, out, st);
   const Cut c = cut_of(batch, tokens, heads, kv_heads, head_dim, table_width * page, fp4);
   const int64_t pairs = batch * kv_heads * c.groups;
   // the units of all heads, counted in 32 bits

@@ -113,8 +113,8 @@ struct Args {
   const float *k_factor, *v_factor;
   const int32_t *block_table, *lengths, *counts;
   float* part;    // [CTAs][2][streams with rows of their own][D + 2][128]: pieces of heads that were cut
-  int32_t* done;  // [B * groups * Hkv][streams ..] zero before, zero after
-  int32_t* next;  // heads taken whole so far: zero before, zero after
+  int32_t* done;  // [B * groups * Hkv][streams ..] pieces that are there: k_zero's zeros at the start
+  int32_t* next;  // heads taken whole so far, likewise
   int B, T, H, Hkv, G, page_log2, width, pages, groups;
   float sm_log2;
 };
@@ -552,10 +552,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
           int k = 0;
           if (lane == 0) k = atomicAdd(a.next, 1);
           k = __shfl_sync(FULL, k, 0);
-          if (k >= heads) {  // each CTA comes here once; the last of them leaves 0
-            if (k == heads + (int)gridDim.x - 1 && lane == 0) *a.next = 0;
-            return false;
-          }
+          if (k >= heads) return false;
           const int kvh = k % a.Hkv, b = k / a.Hkv % a.B, e = b * a.groups + a.groups - 1 - k / a.Hkv / a.B;
           const Entry x = entry_of<ROWS>(a, e, s_plan);
           const int n = tiles_of(x);
@@ -1043,7 +1040,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
             }
           }
           if (writer && !now.live && now.exists) blank();
-          if (threadIdx.x == (PAIR ? 128 * i : 0)) *done = 0;
         }
       }
       // the set of NaNs is for another segment
@@ -1070,25 +1066,38 @@ __global__ void __launch_bounds__(THREADS, 1) k_attn_kv4(const __grid_constant__
   }
 }
 
-// How a call's work is cut: rows a tile, row tiles of a sequence, and CTAs.
+// A launch's counters to 0, in the stream before it.  They are the call's own and lie in
+// its workspace: a launch whose waits gave up leaves them anywhere, and kept from call to
+// call they would have the next one skip heads.
+constexpr int ZERO_THREADS = 256;
+__global__ void __launch_bounds__(ZERO_THREADS) k_zero(int32_t* counters, int64_t n) {
+  pdl::trigger();
+  pdl::wait();
+  for (int64_t i = (int64_t)blockIdx.x * ZERO_THREADS + threadIdx.x; i < n; i += (int64_t)gridDim.x * ZERO_THREADS)
+    counters[i] = 0;
+}
+
+// How a call's work is cut: rows a tile, row tiles of a sequence, and CTAs; floats of
+// pieces and, behind them in the workspace, counters.
 struct Cut {
   int rows, groups, ctas;
+  int64_t floats, counters;
 };
-static Cut cut_of(int64_t batch, int64_t tokens, int heads, int kv_heads, int64_t capacity) {
+static Cut cut_of(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim, int64_t capacity) {
   const int64_t rows = tokens * (heads / kv_heads);
   Cut c;
   c.rows = rows > 128 ? 256 : 128;
   c.groups = (int)((rows + c.rows - 1) / c.rows);
   const int64_t tiles = std::max<int64_t>(1, (capacity + TILE - 1) / TILE);
   c.ctas = (int)std::min<int64_t>(vq::mx::sm_count(), std::max<int64_t>(1, batch) * c.groups * kv_heads * tiles);
+  c.floats = (int64_t)c.ctas * 2 * c.rows * (head_dim + 2);
+  c.counters = batch * kv_heads * c.groups * (c.rows / 128) + 1;
   return c;
 }
 
-void workspace(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim, int64_t capacity, int64_t* floats,
-               int64_t* counters) {
-  const Cut c = cut_of(batch, tokens, heads, kv_heads, capacity);
-  *counters = batch * kv_heads * c.groups * (c.rows / 128) + 1;
-  *floats = (int64_t)c.ctas * 2 * c.rows * (head_dim + 2);
+int64_t workspace(int64_t batch, int64_t tokens, int heads, int kv_heads, int head_dim, int64_t capacity) {
+  const Cut c = cut_of(batch, tokens, heads, kv_heads, head_dim, capacity);
+  return c.floats + c.counters;
 }
 
 template <int D, bool PAIR>
@@ -1108,13 +1117,13 @@ int attend(const void* q, const int64_t* q_strides, int64_t batch, int64_t token
            const void* k_codes, const void* v_codes, const void* k_scale, const void* v_scale, const float* k_factor,
            const float* v_factor, int64_t pages, int page, const void* block_table, int64_t table_width,
            const void* lengths, const void* counts, float sm_scale, float* workspace, int64_t workspace_floats,
-           int32_t* counters, int64_t counters_len, void* out, cudaStream_t st) {
+           void* out, cudaStream_t st) {
   const int64_t capacity = table_width * page;
-  const Cut c = cut_of(batch, tokens, heads, kv_heads, capacity);
+  const Cut c = cut_of(batch, tokens, heads, kv_heads, head_dim, capacity);
   const int64_t pairs = batch * kv_heads * c.groups;
   // the tiles of all heads, counted in 32 bits
-  if (pairs * ((capacity + TILE - 1) / TILE + 3) >= (1ll << 31) || counters_len < pairs * (c.rows / 128) + 1) return VQ_ERR_INVALID;
-  if (!workspace || workspace_floats < (int64_t)c.ctas * 2 * c.rows * (head_dim + 2)) return VQ_ERR_INVALID;
+  if (pairs * ((capacity + TILE - 1) / TILE + 3) >= (1ll << 31)) return VQ_ERR_INVALID;
+  if (!workspace || workspace_floats < c.floats + c.counters) return VQ_ERR_INVALID;
   Args a;
   a.q = (const uint16_t*)q;
   a.qb = q_strides[0], a.qt = q_strides[1], a.qh = q_strides[2];
@@ -1126,11 +1135,13 @@ int attend(const void* q, const int64_t* q_strides, int64_t batch, int64_t token
   a.lengths = (const int32_t*)lengths;
   a.counts = (const int32_t*)counts;
   a.part = workspace;
-  a.next = counters, a.done = counters + 1;
+  a.next = reinterpret_cast<int32_t*>(workspace + c.floats), a.done = a.next + 1;
   a.B = (int)batch, a.T = (int)tokens, a.H = heads, a.Hkv = kv_heads, a.G = heads / kv_heads;
   a.page_log2 = page == 32 ? 5 : page == 64 ? 6 : 7;
   a.width = (int)table_width, a.pages = (int)pages, a.groups = c.groups;
   a.sm_log2 = sm_scale * 1.4426950408889634f;
+  const unsigned zero_ctas = (unsigned)std::min<int64_t>((c.counters + ZERO_THREADS - 1) / ZERO_THREADS, vq::mx::sm_count());
+  if (!pdl::launch<k_zero>(zero_ctas, ZERO_THREADS, 0, st, 1, a.next, c.counters)) return VQ_ERR_CUDA;
   if (head_dim == 128) return c.rows == 256 ? launch<128, true>(a, c.ctas, st) : launch<128, false>(a, c.ctas, st);
   return c.rows == 256 ? launch<64, true>(a, c.ctas, st) : launch<64, false>(a, c.ctas, st);
 }
