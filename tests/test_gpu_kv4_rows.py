@@ -1,4 +1,5 @@
-"""Attention of many rows over the 4-bit cache: what a launch takes from earlier ones.
+"""Attention of many rows over the 4-bit cache: what a launch takes from earlier ones, and small
+weights.
 
 Tolerances as in test_gpu_kv4.py."""
 
@@ -58,3 +59,38 @@ def test_attend4_many_rows_start_from_any_workspace(B, T, Hkv, G, D, held):
     assert not bool(want.isnan().any())
     for fill in (0, 1, 7, 0x7F7F7F7F, -1):
         assert torch.equal(_raw_attend(q, cache, bt, lengths, fill), want)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T,G,B", [(1, 4, 1), (200, 2, 1), (30, 4, 40)])
+@pytest.mark.parametrize("less", [33, 36])
+def test_attend4_small_weights_on_large_values(T, G, B, D, less):
+    """Small weights on large values, where the large weight's values are 0.  The first key's score
+    is `less` above all others' in base 2; its weight is 1, the others' 2^-less each, and only they
+    have values.  The largest weight is at least 2^11 in f16 (2^15 with up to 16 rows a kv head),
+    whose steps are 2^-24 at the least, so a weight is off by at most 2^-25 there: 2^-36 (2^-40);
+    2^-11 relative where that is more, and one bf16 rounding.  Scores are sums of D products of few
+    bits, so exact."""
+    from voyager_b200 import kvcache
+
+    held, Hkv = 700, 8 if B > 1 else 1
+    width = -(-(held + T) // 64)
+    bt = _table(B, width, 1)
+    cache = _cache(int(bt.max()) + 1, Hkv, 64, D, 2, ones=True)
+    cache.k_scale.copy_(torch.ones(()))
+    cache.k_codes.fill_(0)
+    cache.v_scale.copy_(torch.tensor(448.0))
+    cache.v_codes.fill_(0x77)  # 6 and 6
+    first = bt[:, 0].long()
+    cache.k_codes[first, :, 0] = 0x22  # 1 and 1, the others 0
+    cache.v_codes[first, :, 0] = 0
+    # q . k = less / log2(e) in the first key: D columns of less / 32, scale to match
+    q = torch.full((B, T, Hkv * G, D), less / 32, device="cuda").bfloat16()
+    out = kvcache.attend(q, cache, bt, _i32([held] * B), scale=32 / D * math.log(2.0)).double()
+    n = held + torch.arange(T, device="cuda").double()  # keys with values that a token sees
+    w = 2.0 ** -less
+    want = n * w * 2688.0 / (1 + n * w)
+    # sm_scale * log2(e) and its product with the score round three times: less * 3 * 2^-24 in the exponent
+    floor = 2.0 ** (-40 if T * G <= 16 else -36)
+    err = n * 2688.0 * (floor + w * (2.0 ** -11 + less * 3 * 2.0 ** -24)) + want * 2.0 ** -8
+    assert bool(((out - want[None, :, None, None]).abs() <= err[None, :, None, None]).all()), (out.max(), out.min(), want[:3])
