@@ -1167,14 +1167,25 @@ using namespace vq::kva;
 
 // Whether a call on the 4-bit cache is this file's, or vq_attn_kv4.cu's.  There a
 // tile of 128 keys costs the same for 1 to 128 rows a kv head, here once for every
-// group of 16; the start there costs 10 us more.  With t tiles in the block table and
-// g groups that makes about 12 + 0.0052 t g us here and 22 + 0.0119 t there (heads of
-// 128: 3768 tiles, 32 rows 58 us here and 63 there, 35 rows 74 and 64, 128 rows 171
-// and 68; 128 tiles, 128 rows 21 and 32; heads of 64: 43, 53, 121 here, 49 to 51
-// there; 16 and 23).  Tables are as wide as the longest sequence: 1.6 times that t.
-static bool few_rows(int64_t batch, int64_t rows, int kv_heads, int64_t capacity) {
-  const int64_t g = (rows + 15) / 16, t = batch * kv_heads * ((capacity + 127) / 128);
-  return g <= 2 || (g <= 8 && t * (4 * g - 9) <= 12000);
+// group of 16; the start there costs about 10 us more, and heads cost more.  The host
+// knows the table's width only, so that t is the tiles of sequences that fill it; where
+// lengths lie evenly below that, about half of them are there.  With h heads (sequences
+// x kv heads), g groups of 16 rows, here / there in us:
+//                                        equal lengths   unequal
+//   D = 128  48 rows,  h 128, t 2048        54 / 44       33 / 36
+//                      h 32,  t 4032        80 / 61       40 / 44
+//                      h 512, t 4096       107 / 84       57 / 86
+//            128 rows, h 32,  t 256         30 / 31       20 / 29
+//                      h 32,  t 1024        61 / 40       32 / 37
+//                      h 512, t 4096       259 / 90       98 / 82
+//   D = 64   35 rows,  h 24,  t 3768        56 / 50       25 / 40
+//            48 rows,  h 32,  t 4032        54 / 50       32 / 37
+//            128 rows, h 32,  t 1024        45 / 30       25 / 27
+// Over 400 such points the choice costs 4 % on average, and half at the worst, where lengths
+// are unlike what the width says.  Up to 32 rows always run here, more than 128 never.
+static bool few_rows(int64_t batch, int64_t rows, int kv_heads, int head_dim, int64_t capacity) {
+  const int64_t g = (rows + 15) / 16, h = batch * kv_heads, t = h * ((capacity + 127) / 128);
+  return g <= 8 && (head_dim == 64 ? t * (4 * g - 11) <= 6000 : t * (4 * g - 10) <= 6400 + 4 * h);
 }
 
 static int workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t page,
@@ -1183,7 +1194,7 @@ static int workspace(int64_t batch, int64_t tokens, int32_t heads, int32_t kv_he
   if (batch < 0 || tokens < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0 ||
       page <= 0 || table_width < 0 || table_width > max_width(page))
     return VQ_ERR_INVALID;
-  if (fp4 && !few_rows(batch, tokens * (heads / kv_heads), kv_heads, table_width * page)) {
+  if (fp4 && !few_rows(batch, tokens * (heads / kv_heads), kv_heads, head_dim, table_width * page)) {
     *floats = vq::kv4::workspace(batch, tokens, heads, kv_heads, head_dim, table_width * page);
     *counters = 0;
     return VQ_OK;
@@ -1225,7 +1236,7 @@ static int attention(const void* q, const int64_t* q_strides, int64_t batch, int
     const int64_t ctas = std::min<int64_t>((chunks + THREADS - 1) / THREADS, 8 * vq::mx::sm_count());
     return vq::pdl::launch<k_attn_none>((unsigned)ctas, THREADS, 0, st, 1, a, chunks) ? VQ_OK : VQ_ERR_CUDA;
   }
-  const bool few = !fp4 || few_rows(batch, tokens * a.G, kv_heads, table_width * page);
+  const bool few = !fp4 || few_rows(batch, tokens * a.G, kv_heads, head_dim, table_width * page);
   if (!q || !q_strides || !k_codes || !v_codes || !k_scale || !v_scale || !block_table || !lengths ||
       (few && !counters) || !out || (fp4 && (!k_factor || !v_factor)))
     return VQ_ERR_NULL;
