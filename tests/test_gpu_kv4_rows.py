@@ -348,3 +348,37 @@ def test_rows_empty_plans():
         with pytest.raises(_lib.VqError, match="plan"):
             voyager_b200.check_errors()
         assert count == 11 or not bool(out.any())  # 11 of 10 tokens: all 10
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("bits", [4, 8])
+def test_prompts_captured_and_replayed(bits):
+    """Append and attention of prompts in a graph, whose kernels start under one another: replays with
+    other inputs and another plan write what eager calls write."""
+    from voyager_b200 import kvcache
+
+    B, T, Hkv, G, D, page = 3, 700, 8, 4, 128, 64
+    kind = kvcache.KVCache4 if bits == 4 else kvcache.KVCache
+    table, bt = kvcache.rotary_table(1024, D), _table(B, 16, 1)
+    w = (1 + 0.3 * torch.randn(D, generator=_gen(2), device="cuda")).bfloat16()
+    xs = [torch.randn(B, T, (G + 2) * Hkv, D, generator=_gen(i), device="cuda").bfloat16() for i in range(3)]
+    plans = [([0, 0, 0], [T, T, T]), ([5, 300, 64], [T, 1, 650]), ([0, 63, 0], [0, T, 33])]
+    x, held, new = xs[0].clone(), _i32(plans[0][0]), _i32(plans[0][1])
+
+    def step(cache):
+        q, k, v = x.split([G * Hkv, Hkv, Hkv], 2)
+        q = kvcache.rope_append(q, k, v, table, cache, bt, held, new, q_norm=w, k_norm=w)
+        return kvcache.attend(q, cache, bt, held, new)
+
+    eager, own = (kind.empty(B * 16 + 2, Hkv, D, page) for _ in range(2))
+    step(kind.empty(B * 16 + 2, Hkv, D, page))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(own)
+    for data, (h, n) in zip(xs, plans):
+        x.copy_(data), held.copy_(_i32(h)), new.copy_(_i32(n))
+        want = step(eager)
+        graph.replay()
+        assert torch.equal(out, want)
+        for n in ("k_codes", "v_codes", "k_scale", "v_scale"):
+            assert torch.equal(getattr(own, n).view(torch.uint8), getattr(eager, n).view(torch.uint8))
