@@ -22,7 +22,7 @@
 // into the operand of the second product.
 //
 // Work: the keys of every (sequence, row group, kv head) in units of 128,
-// laid end to end and cut into equal runs, one per CTA (two CTAs per SM), so
+// laid end to end and cut into equal runs, one per CTA (two or three per SM), so
 // that unequal lengths leave no SM idle; a run may span several heads or
 // sequences.  Each of a CTA's 4 warps takes one 32-key tile of every unit and
 // has a ring of its own that TMA fills (K and V, 32 x D bytes each,
@@ -42,19 +42,20 @@
 //  - a tile's codes and scales lie side by side, so that four untiled copies fetch
 //    it; the fragment loads' bank conflicts are avoided by the order of the keys
 //    within the product (key4), which no sum depends on.
-//  - code * scale is exact in f16 (6 significant bits): two PRMTs a word of codes
-//    and a multiplication by the scale make the operands.  A key pair's codes lie in
-//    one word, so that V needs no shuffle.
+//  - code * scale is exact in f16 (6 significant bits): four conversions of E2M1 pairs
+//    and four products with the scale's pair make a word's operands.  A key pair's codes
+//    lie in one word, so that V needs no shuffle.
 //  - no page has a factor of its own, so the weights are relative to m alone, and m
 //    and O move only where some score of the tile passes m (a vote): 2^(15 + s - m).
 //  - a NaN scale makes K's scores NaN as it is.  V's is looked for only in tiles whose
 //    keys some row does not see (0 * NaN); its key is noted, and the rows that see
 //    it get NaN at the end.
-// Bound by instructions: 676 a warp and tile of 32 keys and 8 rows, of which the
-// loads, conversions and products of 4.5 KB are most; HBM has 9/16 of E4M3's bytes.
-// 4 sequences of 131000 keys, 8 x 8 heads of 128: 134 us, 4.5 TB/s (143 over and over,
-// when the power cap takes the clock to 1.82 GHz); 32 sequences to 8192, 8 x 4 heads:
-// 45 us where E4M3 takes 53; 99 keys: 7.7 us.
+// Bound by the latency of a warp's chain at 12 warps an SM (161 registers): 676
+// instructions a warp and tile of 32 keys and 8 rows, of which the loads, conversions
+// and products of 4.5 KB are most, in half of the issue slots; HBM has 9/16 of E4M3's
+// bytes.  4 sequences of 131000 keys, 8 x 8 heads of 128: 144 us over and over, where the
+// power cap takes the clock to 1.82 GHz (4.2 TB/s), 133 in short runs; 32 sequences to
+// 8192, 8 x 4 heads: 45 us where E4M3 takes 53; 99 keys: 7.4 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -107,7 +108,7 @@ struct Args {
 // CTAs per SM.  Three with heads of 64 and one row tile (24 sequences of 28631
 // keys: 130 us against 149 with two, in deeper rings than now); otherwise the third CTA costs more in
 // joins and shallower rings than its warps give (heads of 128, 32 sequences:
-// 66 us against 55).  In 4 bits, bound by instructions, three with one row tile.
+// 66 us against 55).  In 4 bits, where a warp's chain is longer, three with one row tile.
 constexpr int ctas_per_sm(int head_dim, int nt, bool fp4) {
   return (head_dim == 64 || fp4) && nt == 1 ? 3 : 2;
 }
@@ -118,7 +119,6 @@ struct Cfg {
   // a stage holds codes of K, codes of V; in 4 bits then their scales
   static constexpr int TILE_BYTES = FP4 ? TILE * D / 2 : TILE * D, SCALE_BYTES = FP4 ? TILE * D / 16 : 0;
   static constexpr int STAGE = 2 * (TILE_BYTES + SCALE_BYTES);
-  static constexpr int STRIDE = STAGE;
   // Two stages a warp: 128 KB in flight an SM (96 KB at heads of 64) fill HBM, and
   // more only lengthens the queue that every other access waits in (4 sequences
   // of 131000 keys: 168 us, with three 178; heads of 64, 24 sequences of 28631:
@@ -126,7 +126,7 @@ struct Cfg {
   // 128 and three CTAs an SM (108 KB), three at heads of 64 (81 KB).
   static constexpr int PER_SM = ctas_per_sm(D, NT, FP4);
   static constexpr int STAGES = FP4 ? (D == 128 ? 2 : 3) : D == 128 || PER_SM == 3 ? 2 : 3;
-  static constexpr int RING = STAGES * STRIDE;  // per warp
+  static constexpr int RING = STAGES * STAGE;  // per warp
   static constexpr int SMEM_RING = WARPS * RING;
   // the warps' O meet in SUMS buffers, rows LD floats apart
   static constexpr int SUMS = NT == 1 ? 2 : 1, LD = D + 4;
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
     int y = __shfl_sync(FULL, n_row, issued & 31);
     if (FP4 && y < 0) skip |= 1u << wstage, y = 0;
     if (FP4 ? elect_one() : lane == 0) {
-      const uint32_t bar = bar0 + 8 * wstage, dst = ring + wstage * C::STRIDE;
+      const uint32_t bar = bar0 + 8 * wstage, dst = ring + wstage * C::STAGE;
       mbar_expect_tx(bar, C::STAGE);
       if constexpr (!FP4) {
         tma_load_2d(dst, &map_k, 0, y, bar);
@@ -791,7 +791,7 @@ __global__ void __launch_bounds__(THREADS, ctas_per_sm(D, NT, FP4))
       skip &= ~(1u << stage);
       continue;
     }
-    const uint32_t kb = ring + stage * C::STRIDE, vb = kb + C::TILE_BYTES;
+    const uint32_t kb = ring + stage * C::STAGE, vb = kb + C::TILE_BYTES;
     // the key that index r of the products stands for
     auto place = [](int r) { return FP4 ? key4(r) : r; };
     const bool tail = key0 + TILE > free_end;

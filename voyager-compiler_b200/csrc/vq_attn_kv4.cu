@@ -49,12 +49,14 @@
 // there, 420 to read them and their maximum, 1250 for the weights (the exponentials'
 // unit is shared by the streams' warps, 1024 at its rate), 250 to store and hand over;
 // the tensor pipe has 1024 of work in that time (S at N = 64 reads the queries anew for
-// every half, 6 KB an MMA).  Slower were: sixteen warps of softmax at 88 registers
-// (208 us where this takes 190), the next half's scores read under this one's weights
-// (212: spills), weights of the two streams in turn (193), whole tiles.  Pairs of CTAs
-// (cta_group::2) would share the conversion of a tile; not built.  500 tokens x 5 heads
-// on 16011 held, 8 kv heads of 128: 186 us, 895 TFLOP/s; 4 prompts of 2048 tokens, 8 x 4
-// heads: 189 us, 728.  Few tiles: start, ends and joins, about 22 us.
+// every half, 6 KB an MMA).  Slower were, on forms that took 187 to 193 us for the 500
+// tokens below: sixteen warps of softmax at 88 registers (208), the next half's scores
+// read under this one's weights (212: spills), weights of the two streams in turn (193
+// against 187), whole tiles.  Pairs of CTAs (cta_group::2) would share the conversion of a
+// tile; not built.  500 tokens x 5 heads on 16011 held, 8 kv heads of 128: 184 us in short
+// runs, 905 TFLOP/s (193 over and over); 4 prompts of 2048 tokens, 8 x 4 heads: 192 us, 716;
+// 25 tokens x 4 heads on 8 x 16000 (two streams of one row tile): 96 us, 545.  Few tiles:
+// start, ends and joins, about 22 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

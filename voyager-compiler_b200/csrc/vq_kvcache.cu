@@ -21,7 +21,9 @@
 // Bound by HBM for prompts (the projections read once, q and the codes
 // written once) and by latency for single tokens.  A head's norm is a sum over the
 // lanes that hold it, in registers: 8 x 2048 tokens, 8 x 4 heads of 128 in bf16 take
-// 76 us with both norms (floor 58; instructions beside HBM), one token 2.9 us.
+// 76 us with both norms (floor 58; a chain of instructions beside HBM), interleaved 99,
+// in float32 198 (floor 109); one token 2.9 us.  At 80 registers the forms with norms
+// spill 4 to 16 bytes a thread.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -811,9 +813,11 @@ __global__ void __launch_bounds__(FEW_THREADS) k_append4_few(const __grid_consta
 // Many: the keys and values beside k_turn_q, half of the CTAs each; a thread takes
 // its unit of a.hc heads of a token, QH at a time, whose loads travel through a ring.
 // The tokens of a warp are neighbours, so that their codes and scales fill sectors.
-// Bound by instructions, 227 a unit of 16 columns (rotation, maxima, quotients with
-// their correction), issue slots 59 % busy: 8 x 2048 tokens, 32 heads of 128 take 126
-// us with k_turn_q's 39, floor 94.
+// Bound by latency: 227 instructions a unit of 16 columns (rotation, maxima, quotients
+// with their correction), one after the other, a third of an SM's warps, issue slots 50
+// to 59 % busy.  8 x 2048 tokens, 32 heads of 128: 126 us with k_turn_q's 39, floor 94, with
+// norms 146; 8 x 4 heads: 66, floor 55, with norms 74, interleaved 92, in float32 187 (floor
+// 107).  The forms with norms spill 8 to 16 bytes a thread at 80 registers.
 template <typename T, bool IL, int D, bool NORM>
 __global__ void __launch_bounds__(Q_THREADS, 3) k_append4(const __grid_constant__ Args a) {
   using E = typename T::type;

@@ -57,7 +57,9 @@ class CachedDecoder:
                 "q_norm": w.get("q_norm"), "k_norm": w.get("k_norm")})
 
     def caches(self, pages: int) -> List[kvcache.Cache]:
-        """An empty cache of `pages` pages per layer (in 4 bits with factors of 1)."""
+        """An empty cache of `pages` pages per layer, in 4 bits with factors of 1: keys or
+        values of a layer whose blocks stay below 0.094 need smaller ones (``KVCache4``),
+        written to its ``k_factor`` / ``v_factor`` before the first step."""
         kind = kvcache.KVCache if self.cache_bits == 8 else kvcache.KVCache4
         return [kind.empty(pages, self.kv_heads, self.cfg.head_dim, self.page, self.device) for _ in self.layers]
 

@@ -63,9 +63,11 @@ class KVCache4:
     """Codes uint8 [pages, kv_heads, page, head_dim / 2], two E2M1 codes a byte with
     the even column in the low half, scales float8_e4m3fn [pages, kv_heads, page,
     head_dim / 16], factors float32 [kv_heads] within 2^-100 .. 2^100.  A value is code x scale
-    x its head's factor.  Scales reach from 2^-9 to 448, codes to 6: a factor of
-    max|x| / 2688 over a head uses the scales' whole range, and 1 holds values up
-    to 2688 with blocks below 0.01 losing bits."""
+    x its head's factor.  A block's scale is max|x| / (6 factor) as E4M3, with 4 significant
+    bits from 2^-6 to 448; below, it loses bits down to its least, 2^-9.  So blocks
+    up to 2688 x factor fit, those below 0.094 x factor are held more and more coarsely
+    (scales up to a tenth off near 0.05 x factor, a third near 0.02), and below 0.012 x factor their codes
+    shrink too.  A factor of max|x| / 2688 over a head uses the scales' whole range."""
 
     k_codes: torch.Tensor
     v_codes: torch.Tensor
